@@ -10,6 +10,7 @@
 #include <string>
 #include <vector>
 
+#include "mi355x-attention.h"
 #include "mi355x-gemv.h"
 
 struct mi355x_ctx {
@@ -92,6 +93,20 @@ inline bool host_only(const mi355x_ctx *ctx) { return ctx && ctx->device < 0; }
         if (e_ != hipSuccess) return ::mi355x::hip_error(e_, #call); \
     } while (0)
 
+// Makes `dev` current and, at its end, the device that was current before.
+struct DeviceGuard {
+    int prev = -1;
+    explicit DeviceGuard(int dev) {
+        // a host-only context (device < 0) touches no device
+        if (dev < 0 || hipGetDevice(&prev) != hipSuccess) prev = -1;
+        if (dev >= 0 && prev != dev) (void)hipSetDevice(dev);
+    }
+    ~DeviceGuard() {
+        int cur = -1;
+        if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
+    }
+};
+
 struct GemvArgs {
     int type;
     const uint8_t *W;
@@ -171,6 +186,13 @@ int launch_prepack_scatter(mi355x_ctx *ctx, int type, int64_t N, int64_t K, uint
 int launch_prepack_gather(mi355x_ctx *ctx, int type, int64_t N, int64_t K, uint8_t *raw,
                           const uint8_t *packed, size_t offset, size_t size);
 int launch_fill(mi355x_ctx *ctx, void *dst, uint8_t value, size_t bytes);
+
+// The operators of mi355x-attention.h, with arguments that its entry points
+// have checked.
+int launch_kv_plan(mi355x_ctx *ctx, const mi355x_kv_plan_args &a);
+int launch_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_args &a);
+int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &a);
+size_t paged_attention_workspace_bytes(const mi355x_ctx *ctx, int n_heads, int n_kv_heads, int head_dim);
 
 // Resident workgroups per CU of `kernel` at this block size and LDS (cached).
 int occupancy(const void *kernel, int block_threads, size_t lds_bytes);

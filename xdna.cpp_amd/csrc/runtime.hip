@@ -102,19 +102,6 @@ int ensure_staging(mi355x_ctx *ctx, size_t want) {
     return MI355X_OK;
 }
 
-struct DeviceGuard {
-    int prev = -1;
-    explicit DeviceGuard(int dev) {
-        // a host-only context (device < 0) touches no device
-        if (dev < 0 || hipGetDevice(&prev) != hipSuccess) prev = -1;
-        if (dev >= 0 && prev != dev) (void)hipSetDevice(dev);
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
-    }
-};
-
 // gate: false for the calls an entry point makes for itself after passing
 // the device gate once
 int gemv_common(mi355x_ctx *ctx, int type, const void *W, int64_t N, int64_t K, const void *x, bool xbf16,

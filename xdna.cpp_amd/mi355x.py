@@ -1,4 +1,5 @@
-"""ctypes binding of libggml-mi355x.so (the C-ABI in include/mi355x-gemv.h).
+"""ctypes binding of libggml-mi355x.so (the C-ABI in include/mi355x-gemv.h and
+include/mi355x-attention.h).
 
 Python is only the harness language here: tests and bench.py drive the
 library through this module.  Loading fails loudly when the shared library is
@@ -17,6 +18,7 @@ LIB_PATH = os.path.join(HERE, "libggml-mi355x.so")
 OK, EINVAL, EUNSUPPORTED, EHIP, ENOMEM = 0, -1, -2, -3, -4
 
 # ggml type ids
+F16, BF16 = 1, 30
 F32, Q4_0, Q3_K, Q4_K, Q5_K, Q6_K, IQ3_XXS, IQ3_S, IQ2_S, IQ4_XS = 0, 2, 11, 12, 13, 14, 18, 21, 22, 23
 TYPE_NAMES = {Q4_0: "Q4_0", Q3_K: "Q3_K", Q4_K: "Q4_K", Q5_K: "Q5_K", Q6_K: "Q6_K",
               IQ3_XXS: "IQ3_XXS", IQ3_S: "IQ3_S", IQ2_S: "IQ2_S", IQ4_XS: "IQ4_XS"}
@@ -85,9 +87,57 @@ _SIGNATURES = {
                                        _c.c_int64, _c.c_int64]),
     "mi355x_gemv_batched_noalloc": (_c.c_int, [_vp, _c.c_int, _vp, _c.c_int64, _c.c_int64, _vp, _c.c_int64, _vp,
                                                _c.c_int64, _c.c_int64]),
+    "mi355x_kv_plan": (_c.c_int, [_vp, _vp]),
+    "mi355x_qk_norm_rope": (_c.c_int, [_vp, _vp]),
+    "mi355x_paged_attention": (_c.c_int, [_vp, _vp]),
+    "mi355x_paged_attention_workspace": (_c.c_int, [_vp, _c.c_int, _c.c_int, _c.c_int, _c.POINTER(_c.c_size_t)]),
     "mi355x_time_gemv": (_c.c_int, [_vp, _c.c_int, _c.POINTER(_vp), _c.c_int, _c.c_int64, _c.c_int64, _vp,
                                     _vp, _c.c_int, _c.c_int, _c.POINTER(_c.c_double)]),
 }
+
+
+# operators over a paged KV cache (mi355x-attention.h)
+KV_BAD_LENGTH, KV_ROWS, KV_TABLE, KV_PAGES = 1, 2, 4, 8
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+pointer = _c.pointer
+
+
+class KvPool(_c.Structure):
+    """mi355x_kv_pool: one layer's pages of keys and values (strides in values)."""
+    _fields_ = [("type", _c.c_int), ("n_kv_heads", _c.c_int), ("head_dim", _c.c_int), ("page_tokens", _c.c_int),
+                ("n_pages", _c.c_int64), ("k", _vp), ("v", _vp), ("page_stride", _c.c_int64),
+                ("token_stride", _c.c_int64), ("head_stride", _c.c_int64)]
+
+
+class KvPlanArgs(_c.Structure):
+    """mi355x_kv_plan_args (pointers are device addresses)."""
+    _fields_ = [("n_seqs", _c.c_int), ("page_tokens", _c.c_int), ("table_cols", _c.c_int), ("n_free", _c.c_int),
+                ("table_stride", _c.c_int64), ("n_rows", _c.c_int64)] + \
+               [(f, _vp) for f in ("cached", "added", "block_table", "free_pages", "free_head", "free_head_out",
+                                   "row_offsets", "kv_lens", "positions", "slots", "status")]
+
+
+class QkNormRopeArgs(_c.Structure):
+    """mi355x_qk_norm_rope_args (pool: pointer(KvPool) or None)."""
+    _fields_ = [("n_rows", _c.c_int64), ("n_heads", _c.c_int), ("n_kv_heads", _c.c_int), ("head_dim", _c.c_int),
+                ("rot_dim", _c.c_int), ("rope_mode", _c.c_int), ("in_type", _c.c_int), ("out_type", _c.c_int),
+                ("eps", _c.c_float)] + [(f, _vp) for f in ("q", "k", "v")] + \
+               [(f, _c.c_int64) for f in ("q_stride", "k_stride", "v_stride")] + \
+               [(f, _vp) for f in ("q_bias", "k_bias", "v_bias", "q_norm", "k_norm", "positions", "inv_freq",
+                                   "q_out")] + \
+               [("q_out_stride", _c.c_int64), ("pool", _c.POINTER(KvPool)), ("slots", _vp), ("k_out", _vp),
+                ("k_out_stride", _c.c_int64)]
+
+
+class PagedAttentionArgs(_c.Structure):
+    """mi355x_paged_attention_args (pool: pointer(KvPool))."""
+    _fields_ = [("n_rows", _c.c_int64), ("n_seqs", _c.c_int), ("n_heads", _c.c_int), ("max_added", _c.c_int),
+                ("q", _vp), ("q_stride", _c.c_int64), ("pool", _c.POINTER(KvPool)), ("row_offsets", _vp),
+                ("kv_lens", _vp), ("block_table", _vp), ("table_cols", _c.c_int), ("table_stride", _c.c_int64),
+                ("scale", _c.c_float), ("softcap", _c.c_float), ("window", _c.c_int), ("causal", _c.c_int),
+                ("out", _vp), ("out_type", _c.c_int), ("out_stride", _c.c_int64), ("workspace", _vp),
+                ("workspace_bytes", _c.c_size_t)]
+
 
 class GemvJob(_c.Structure):
     """mi355x_gemv_job: {const void *W; int64_t N; float *y;}"""
@@ -375,6 +425,24 @@ class Context:
         finally:
             xb.free()
             yb.free()
+
+    def kv_plan(self, args: KvPlanArgs) -> None:
+        """Block tables, slots and positions of a step from request lengths."""
+        check(self.lib.mi355x_kv_plan(self.h, ctypes.byref(args)))
+
+    def qk_norm_rope(self, args: QkNormRopeArgs) -> None:
+        """Bias, norms, rotation, and keys and values into their pages."""
+        check(self.lib.mi355x_qk_norm_rope(self.h, ctypes.byref(args)))
+
+    def paged_attention(self, args: PagedAttentionArgs) -> None:
+        """Attention of new tokens over the pages."""
+        check(self.lib.mi355x_paged_attention(self.h, ctypes.byref(args)))
+
+    def paged_attention_workspace(self, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+        """Bytes of workspace that paged_attention needs with these heads."""
+        n = ctypes.c_size_t()
+        check(self.lib.mi355x_paged_attention_workspace(self.h, n_heads, n_kv_heads, head_dim, ctypes.byref(n)))
+        return n.value
 
     def gemv(self, w: ResidentWeights, x: np.ndarray) -> np.ndarray:
         """One GEMV with host activations; returns the host output."""
