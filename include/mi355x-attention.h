@@ -168,7 +168,7 @@ MI355X_API int mi355x_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_ar
  * that may run at the same time (two contexts, a graph replayed beside other
  * calls, two graphs) need one each; calls in order on one stream share one. */
 typedef struct mi355x_paged_attention_args {
-    int64_t n_rows;           /* rows of q and out, at most 2^31 - 1 */
+    int64_t n_rows;           /* rows of q and out; times n_heads / n_kv_heads at most 2^31 - 1 */
     int n_seqs;               /* at most 65536 */
     int n_heads;              /* a multiple of the pool's n_kv_heads */
     int max_added;

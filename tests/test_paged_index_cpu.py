@@ -23,6 +23,9 @@ void c_visible(int64_t p, int64_t kv, int64_t reach, int w, int causal, int64_t 
 }
 int c_page(int32_t p, int64_t n) { return page_in_pool(p, n); }
 int c_slot(int64_t s, int64_t n, int shift) { return slot_in_pool(s, n, shift); }
+int32_t c_divided(int32_t n, uint32_t d) { return divided(n, fast_div(d)); }
+int64_t c_stretch(int64_t total, int groups, int64_t g) { return stretch_begin(stretches(total, groups), g); }
+int64_t c_stretch_of(int64_t total, int groups, int64_t u) { return stretch_of(stretches(total, groups), u); }
 int64_t c_pages(int64_t n, int shift) { return pages_of(n, shift); }
 }
 """
@@ -41,6 +44,9 @@ def idx(tmp_path_factory):
     lib.c_visible.argtypes = [i64, i64, i64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
     lib.c_page.argtypes = [ctypes.c_int32, i64]
     lib.c_slot.argtypes = [i64, i64, ctypes.c_int]
+    lib.c_divided.argtypes = [ctypes.c_int32, ctypes.c_uint32]
+    for f in (lib.c_stretch, lib.c_stretch_of):
+        f.argtypes, f.restype = [i64, ctypes.c_int, i64], i64
     lib.c_pages.argtypes, lib.c_pages.restype = [i64, ctypes.c_int], i64
     return lib
 
@@ -99,3 +105,24 @@ def test_pages_and_slots(idx):
             for s in (-2 ** 63, -1, 0, n << shift, (n << shift) - 1, (n << shift) + 1, 2 ** 63 - 1):
                 assert bool(idx.c_slot(s, n, shift)) == (0 <= s < n << shift)
     assert [idx.c_pages(n, 4) for n in (0, 1, 16, 17, 2 ** 31 - 1)] == [0, 1, 1, 2, 2 ** 27]
+
+
+def test_division_by_a_product(idx):
+    rng = np.random.default_rng(2)
+    most = 2 ** 31 - 1
+    for d in [1, 2, 3, 5, 6, 7, 8, 9, 12, 127, 128, 641, 65535, 65536, *map(int, rng.integers(1, 65537, 50))]:
+        ns = {0, 1, d - 1, d, d + 1, most, most - 1, most // d * d, most // d * d - 1, *map(int, rng.integers(0, most, 60))}
+        for n in ns:
+            assert idx.c_divided(n, d) == n // d, (n, d)
+
+
+@pytest.mark.parametrize("groups", [1, 2, 5, 768])
+def test_stretches_cover_the_line(idx, groups):
+    for total in (0, 1, 4, 767, 768, 769, 10 ** 6 + 7, 2 ** 33 + 5):
+        at = [idx.c_stretch(total, groups, g) for g in range(groups + 1)]
+        assert at[0] == 0 and at[-1] == total
+        size = np.diff(at)
+        assert size.min() >= 0 and size.max() - size.min() <= 1 and (np.diff(size) <= 0).all()
+        for g in range(0, groups, max(1, groups // 9)):
+            for u in {at[g], at[g + 1] - 1} if at[g + 1] > at[g] else ():
+                assert idx.c_stretch_of(total, groups, u) == g

@@ -212,6 +212,8 @@ int mi355x_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args *a
     if (!(a.softcap >= 0.0f) || std::isinf(a.softcap)) return invalid(who, "softcap must be finite and not negative");
     if (a.out_type != a.pool->type && a.out_type != MI355X_TYPE_F32)
         return invalid(who, "out_type must be the pool's type or F32 (got " + std::to_string(a.out_type) + ")");
+    if (a.n_rows * (a.n_heads / a.pool->n_kv_heads) > INT32_MAX)
+        return invalid(who, "n_rows times the query heads of a KV head must be below 2^31");
     const int64_t width = static_cast<int64_t>(a.n_heads) * a.pool->head_dim;
     if (int rc = check_row_stride(who, "q_stride", a.n_rows, a.q_stride, width)) return rc;
     if (int rc = check_row_stride(who, "out_stride", a.n_rows, a.out_stride, width)) return rc;

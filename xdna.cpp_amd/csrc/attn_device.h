@@ -1,0 +1,148 @@
+// Device-side building blocks of the attention kernels.
+#pragma once
+
+#include "paged_index.h"
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mi355x-attention.h"
+
+namespace mi355x {
+
+// A call as the kernels see it.
+struct AttnArgs {
+    const void *q, *k, *v;
+    const int32_t *row_offsets, *kv_lens, *table;
+    void *out;
+    float *ws;
+    int64_t q_stride, out_stride, table_stride;
+    int64_t page_stride, token_stride, head_stride;
+    int64_t n_rows;
+    int64_t reach;      // tokens that the table's columns hold
+    int row_limit;      // requests of at most (token form) or more than (chunk form) so many head rows
+    float scale, softcap;
+    FastDiv group;  // query heads of a KV head
+    int n_seqs, n_kv_heads;
+    int n_pages, shift, window, causal, f32_out;
+    int split;  // chunk form: parts of an item's keys
+};
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2_a __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_a __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// The pool's 16-bit type: matrix products, roundings, and the bits of its
+// exponent (all set: infinity or NaN).
+template <int TYPE>
+struct Num;
+template <>
+struct Num<MI355X_TYPE_F16> {
+    typedef _Float16 T;
+    typedef _Float16 V8 __attribute__((ext_vector_type(8)));
+    static constexpr uint32_t kExp = 0x7C00u;
+    static __device__ __forceinline__ f32x4 mfma16(V8 a, V8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(V8 a, V8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Num<MI355X_TYPE_BF16> {
+    typedef __bf16 T;
+    typedef __bf16 V8 __attribute__((ext_vector_type(8)));
+    static constexpr uint32_t kExp = 0x7F80u;
+    static __device__ __forceinline__ f32x4 mfma16(V8 a, V8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(V8 a, V8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+// Whether any of the eight 16-bit values is an infinity or a NaN.
+template <int TYPE>
+__device__ __forceinline__ bool not_finite(u32x4_a v) {
+    constexpr uint32_t e = Num<TYPE>::kExp;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (v[i] & e) == e || ((v[i] >> 16) & e) == e;
+    return bad;
+}
+
+// Four rows of one column each from a 4-row x 16-column block of 16-bit values
+// per 16 lanes: lane c of the 16 passes the address of 4 values of row c / 4
+// from column 4 (c % 4) on, and gets column c of the four rows.
+__device__ __forceinline__ u32x2_a lds_read_transposed(const void *p) {
+    return __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (__attribute__((address_space(3))) s16x4 *)(p)));
+}
+
+// A score in units of ln 2 from q . k; tanh as 1 - 2 / (1 + e^2x), within
+// 2^-23 of 1.
+__device__ __forceinline__ float score2(float dot, const AttnArgs &a) {
+    if (!(a.softcap > 0.0f)) return dot * (a.scale * kLog2e);
+    const float x = dot * (a.scale / a.softcap);
+    const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * (2.0f * kLog2e)));
+    return a.softcap * kLog2e * t;
+}
+
+__device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// Rows and tokens of a request.
+struct SeqGeo {
+    int64_t first;    // its first row
+    int64_t tok_lo;   // its tokens tok_lo .. tok_lo + n_tok - 1 have rows inside the call's
+    int n_tok;
+    int rows;         // n_tok * group: one row per token and query head of a KV head
+    int64_t pos0;     // position of token 0
+    int64_t kv;
+};
+
+__device__ __forceinline__ SeqGeo seq_geo(const AttnArgs &a, int s) {
+    const SeqRows r = seq_rows(a.row_offsets[s], a.row_offsets[s + 1], a.n_rows);
+    SeqGeo g;
+    g.first = r.first;
+    g.tok_lo = r.lo;
+    g.n_tok = static_cast<int>(r.hi - r.lo);
+    g.rows = g.n_tok * static_cast<int>(a.group.d);
+    g.kv = a.kv_lens[s];
+    g.pos0 = g.kv - r.n;
+    return g;
+}
+
+__device__ __forceinline__ KeyRange token_keys(const AttnArgs &a, const SeqGeo &g, int64_t token) {
+    return visible_keys(g.pos0 + token, g.kv, a.reach, a.window, a.causal != 0);
+}
+
+// Exclusive scan of one value per thread over a workgroup of WAVES wavefronts;
+// *total is the sum.  `tmp` holds WAVES values and is free after the call's
+// last barrier.
+template <int WAVES>
+__device__ __forceinline__ int64_t group_scan(int64_t v, int64_t *tmp, int64_t *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t in = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t u = __shfl_up(in, d);
+        if (lane >= d) in += u;
+    }
+    if (lane == 63) tmp[wave] = in;
+    __syncthreads();
+    int64_t before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) before += tmp[w];
+        sum += tmp[w];
+    }
+    __syncthreads();
+    *total = sum;
+    return before + in - v;
+}
+
+}  // namespace mi355x

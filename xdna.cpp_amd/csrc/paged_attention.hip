@@ -1,107 +1,553 @@
-// Attention of new tokens over a paged KV cache.
+// Attention of new tokens over a paged KV cache: the host's choice of form, and
+// the token form, for requests that add one or a few tokens.
 //
 // One pass over a row's keys with the running maximum m and sum l of the
-// softmax: a key's score s moves m to max(m, s), scales what was summed by
-// exp(m_old - m), and adds exp(s - m) v and exp(s - m).
+// softmax: a tile of scores s moves m to max(m, s), scales what was summed by
+// 2^(m_old - m), and adds 2^(s - m) v and 2^(s - m) (scores carry log2 e).
+//
+// Token form.  A token reads its whole cache once and does 4 operations per
+// value and query head, so HBM bounds it.  The query heads of a KV head (and
+// the request's few tokens) are the 16 columns of a matrix product, so that a
+// key read once meets all of them: scores as K q^T, one column per row of q, so
+// that a lane holds 8 scores of one row of a 32-key tile and the softmax needs
+// two exchanges; the weights are then, as they lie, the operand of V^T w, whose
+// V^T comes out of LDS through the transposing read.  Weights go in as two
+// 16-bit planes: the matrix cores idle here, and the second plane makes them as
+// good as f32.
+//
+// Work split.  All requests' keys, heads and row blocks form one line of
+// 128-key units; every workgroup takes an equal stretch of it, whatever the
+// lengths are, finds its place by a scan over the requests' lengths, and
+// writes the output of the rows that lie in its stretch whole.  The two that its ends
+// cut leave (m, l, sum) in the workspace, and a second launch joins them.
+#include "attn_device.h"
 #include "internal.h"
-#include "paged_index.h"
 
 #include <algorithm>
 
 namespace mi355x {
 namespace {
 
-template <int TYPE>
-struct Half;
-template <>
-struct Half<MI355X_TYPE_F16> {
-    typedef _Float16 T;
-};
-template <>
-struct Half<MI355X_TYPE_BF16> {
-    typedef __bf16 T;
+constexpr int kTokenWaves = 4;
+constexpr int kTokenKeys = 32;                            // of a wavefront's tile
+constexpr int kUnitKeys = kTokenWaves * kTokenKeys;       // of a workgroup's unit
+constexpr int kTokenThreads = 64 * kTokenWaves;
+
+// The token form's units of a request: per KV head and block of ROWS head rows
+// one per kUnitKeys keys (one without keys: its rows get zeros).
+struct TokenWork {
+    int64_t units, key_lo;
+    int blocks, tiles;
 };
 
-__device__ __forceinline__ float wave_total(float v) {
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+template <int ROWS>
+__device__ __forceinline__ TokenWork token_work(const AttnArgs &a, const SeqGeo &g) {
+    TokenWork w{0, 0, 0, 1};
+    if (g.rows <= 0 || g.rows > a.row_limit) return w;
+    w.blocks = (g.rows + ROWS - 1) / ROWS;
+    w.key_lo = token_keys(a, g, g.tok_lo).lo;
+    const int64_t hi = token_keys(a, g, g.tok_lo + g.n_tok - 1).hi;
+    w.tiles = static_cast<int>(idx_max(1, (hi - w.key_lo + kUnitKeys - 1) / kUnitKeys));
+    w.units = static_cast<int64_t>(w.blocks) * w.tiles * a.n_kv_heads;
+    return w;
 }
 
-// One wavefront per row and head, key by key; a lane holds values lane + 64 i.
-template <int TYPE, int HD>
-__global__ __launch_bounds__(256) void attention_rows_kernel(mi355x_paged_attention_args a, mi355x_kv_pool pool,
-                                                             int shift) {
-    typedef typename Half<TYPE>::T T;
-    constexpr int kPer = (HD + 63) / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int64_t row = item / a.n_heads;
-    const int h = static_cast<int>(item % a.n_heads);
-    if (row >= a.n_rows) return;
-    const int s = seq_of_row(a.row_offsets, a.n_seqs, row);
-    if (s < 0) return;
-    const int64_t kv = a.kv_lens[s], pos = kv - (a.row_offsets[s + 1] - row);
-    const KeyRange keys =
-        visible_keys(pos, kv, static_cast<int64_t>(a.table_cols) << shift, a.window, a.causal != 0);
-    const int kvh = h / (a.n_heads / pool.n_kv_heads);
-    const int32_t *table = a.block_table + s * a.table_stride;
-    const T *q = static_cast<const T *>(a.q) + row * a.q_stride + static_cast<int64_t>(h) * HD;
-    float qf[kPer], o[kPer];
-    for (int i = 0; i < kPer; ++i) {
-        qf[i] = lane + 64 * i < HD ? static_cast<float>(q[lane + 64 * i]) : 0.0f;
-        o[i] = 0.0f;
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int64_t j = keys.lo; j < keys.hi; ++j) {
-        const int32_t page = table[j >> shift];
-        if (!page_in_pool(page, pool.n_pages)) continue;
-        const int64_t at = page * pool.page_stride + (j & ((int64_t(1) << shift) - 1)) * pool.token_stride +
-                           kvh * pool.head_stride;
-        const T *k = static_cast<const T *>(pool.k) + at, *v = static_cast<const T *>(pool.v) + at;
-        float dot = 0.0f;
-        for (int i = 0; i < kPer; ++i)
-            if (lane + 64 * i < HD) dot = fmaf(qf[i], static_cast<float>(k[lane + 64 * i]), dot);
-        float sc = wave_total(dot) * a.scale;
-        if (a.softcap > 0.0f) sc = a.softcap * tanhf(sc / a.softcap);
-        const float m_new = fmaxf(m, sc), base = m_new == -INFINITY ? 0.0f : m_new;
-        const float keep = expf(m - base), p = expf(sc - base);
-        l = l * keep + p;
-        for (int i = 0; i < kPer; ++i) {
-            const float vi = lane + 64 * i < HD ? static_cast<float>(v[lane + 64 * i]) : 0.0f;
-            o[i] = o[i] * keep + (p == 0.0f ? 0.0f : p * vi);
+// The units before each request, a request per thread: all of them at once, or
+// (more requests than threads) a part at a time.
+template <int ROWS, int WAVES>
+struct Scan {
+    int64_t total;
+    int64_t mine, before;  // of request threadIdx.x
+
+    __device__ __forceinline__ void run(const AttnArgs &a, int64_t *tmp) {
+        total = 0;
+        for (int base = 0; base < a.n_seqs; base += 64 * WAVES) {
+            const int s = base + threadIdx.x;
+            const int64_t n = s < a.n_seqs ? token_work<ROWS>(a, seq_geo(a, s)).units : 0;
+            int64_t sum;
+            const int64_t at = group_scan<WAVES>(n, tmp, &sum);
+            if (base == 0) {
+                mine = n;
+                before = at;
+            }
+            total += sum;
         }
-        m = m_new;
     }
-    const int64_t at = row * a.out_stride + static_cast<int64_t>(h) * HD;
-    for (int i = 0; i < kPer; ++i) {
-        if (lane + 64 * i >= HD) continue;
-        const float v = l == 0.0f ? 0.0f : o[i] / l;
-        if (a.out_type == MI355X_TYPE_F32) static_cast<float *>(a.out)[at + lane + 64 * i] = v;
-        else static_cast<T *>(a.out)[at + lane + 64 * i] = static_cast<T>(v);
+
+    // The request that has unit u < total, and the units before it.
+    __device__ __forceinline__ int find(const AttnArgs &a, int64_t u, int64_t *tmp, int64_t *first) const {
+        int64_t n = mine, at = before, carry = 0;
+        __shared__ int64_t found_at;
+        __shared__ int found;
+        for (int base = 0; base < a.n_seqs; base += 64 * WAVES) {
+            const int s = base + threadIdx.x;
+            if (a.n_seqs > 64 * WAVES) {
+                int64_t sum;
+                n = s < a.n_seqs ? token_work<ROWS>(a, seq_geo(a, s)).units : 0;
+                at = carry + group_scan<WAVES>(n, tmp, &sum);
+                carry += sum;
+            }
+            if (u >= at && u < at + n) {
+                found = s;
+                found_at = at;
+            }
+        }
+        __syncthreads();
+        *first = found_at;
+        return found;
+    }
+};
+
+template <int HD, int MT>
+struct TokenShape {
+    static constexpr int kRows = 16 * MT;
+    static constexpr int kVStride = HD + 16;  // values: rows of V start 8 banks apart
+    static constexpr int kWaveBytes = kTokenKeys * kVStride * 2;
+    static constexpr int kOStride = HD + 4;   // floats of a joined row
+    static_assert(16 * kOStride * 4 <= kWaveBytes, "a wavefront's sums fit where its V tile was");
+    // a part in the workspace: sums of kRows rows, then m, then l
+    static constexpr int kPartFloats = kRows * (HD + 2);
+};
+
+template <int TYPE>
+__device__ __forceinline__ void store4(const AttnArgs &a, int64_t at, f32x4 v) {
+    typedef typename Num<TYPE>::T T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    if (a.f32_out) {
+        *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + at) = v;
+    } else {
+        T4 h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = static_cast<T>(v[i]);
+        *reinterpret_cast<T4 *>(static_cast<T *>(a.out) + at) = h;
     }
 }
 
-template <int TYPE>
-int launch_rows(mi355x_ctx *ctx, const mi355x_paged_attention_args &a, int shift) {
-    const dim3 grid(static_cast<unsigned>((a.n_rows * a.n_heads + 3) / 4));
-    switch (a.pool->head_dim) {
-    case 64: attention_rows_kernel<TYPE, 64><<<grid, 256, 0, ctx->stream>>>(a, *a.pool, shift); break;
-    case 96: attention_rows_kernel<TYPE, 96><<<grid, 256, 0, ctx->stream>>>(a, *a.pool, shift); break;
-    case 128: attention_rows_kernel<TYPE, 128><<<grid, 256, 0, ctx->stream>>>(a, *a.pool, shift); break;
-    default: attention_rows_kernel<TYPE, 256><<<grid, 256, 0, ctx->stream>>>(a, *a.pool, shift); break;
+__device__ __forceinline__ int64_t out_at(const AttnArgs &a, const SeqGeo &g, int kvh, int row, int hd) {
+    const int token = divided(row, a.group), group = static_cast<int>(a.group.d);
+    const int64_t head = static_cast<int64_t>(kvh) * group + (row - token * group);
+    return (g.first + g.tok_lo + token) * a.out_stride + head * hd;
+}
+
+template <int TYPE, int HD, int MT>
+__global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs a) {
+    typedef Num<TYPE> N;
+    typedef typename N::T T;
+    typedef typename N::V8 V8;
+    typedef TokenShape<HD, MT> S;
+    constexpr int kSteps = HD / 32;     // of a 16-key score product
+    constexpr int kBlocks = HD / 16;    // of 16 output values
+    constexpr int kChunks = HD / 8;     // 16-byte chunks of a token's head
+    constexpr int kVLoads = kTokenKeys * kChunks / 64;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kTokenWaves * S::kWaveBytes];
+    __shared__ float lds_m[kTokenWaves][16], lds_l[kTokenWaves][16];
+    __shared__ int64_t tmp[kTokenWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    Scan<S::kRows, kTokenWaves> scan;
+    scan.run(a, tmp);
+    const Stretches line = stretches(scan.total, gridDim.x);
+    const int64_t u0 = stretch_begin(line, blockIdx.x), u1 = stretch_begin(line, blockIdx.x + 1);
+    if (u0 >= u1) return;
+    int64_t before;  // units before request seq
+    int seq = __builtin_amdgcn_readfirstlane(scan.find(a, u0, tmp, &before));
+    T *vt = reinterpret_cast<T *>(lds + wave * S::kWaveBytes);
+    float *ot = reinterpret_cast<float *>(lds + wave * S::kWaveBytes);
+    SeqGeo g = seq_geo(a, seq);
+    TokenWork w = token_work<S::kRows>(a, g);
+    for (int64_t u = u0; u < u1;) {
+        while (u >= before + w.units) {  // the next request with rows
+            before += w.units;
+            ++seq;
+            g = seq_geo(a, seq);
+            w = token_work<S::kRows>(a, g);
+        }
+        const int64_t item = quotient(u - before, w.tiles);
+        const int t0 = static_cast<int>(u - before - item * w.tiles);
+        const int t1 = static_cast<int>(idx_min(w.tiles, t0 + (u1 - u)));
+        const int kvh = static_cast<int>(quotient(item, w.blocks));
+        const int row0 = static_cast<int>(item - static_cast<int64_t>(kvh) * w.blocks) * S::kRows;
+        const int row_last = min(row0 + S::kRows, g.rows) - 1;
+        // tokens that some row of the block sees, and those that all of them see
+        const KeyRange kf = token_keys(a, g, g.tok_lo + divided(row0, a.group));
+        const KeyRange kl = token_keys(a, g, g.tok_lo + divided(row_last, a.group));
+        const int64_t some_lo = kf.lo, some_hi = kl.hi, all_lo = kl.lo, all_hi = kf.hi;
+
+        V8 qf[MT][kSteps];
+        int row_lo[MT], row_hi[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const bool real = row0 + 16 * mt + col < g.rows;
+            const int row = real ? row0 + 16 * mt + col : 0, tok = divided(row, a.group);
+            const int64_t token = g.tok_lo + tok;
+            const KeyRange kr = token_keys(a, g, token);
+            row_lo[mt] = real ? static_cast<int>(kr.lo) : 0;
+            row_hi[mt] = real ? static_cast<int>(kr.hi) : 0;
+            const int64_t head = static_cast<int64_t>(kvh) * a.group.d + (row - tok * static_cast<int>(a.group.d));
+            const T *q = static_cast<const T *>(a.q) + (g.first + token) * a.q_stride + head * HD;
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) {
+                V8 z = {};
+                if (real) z = *reinterpret_cast<const V8 *>(q + 32 * st + 8 * quad);
+                qf[mt][st] = z;
+            }
+        }
+        f32x4 o[MT][kBlocks];
+        float m[MT], l[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt] = -INFINITY;
+            l[mt] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) o[mt][d] = f32x4{0, 0, 0, 0};
+        }
+
+        const int32_t *table = a.table + seq * a.table_stride;
+        u32x4_a kreg[2][kSteps], vreg[kVLoads];
+        uint32_t seen = 0;  // keys of the tile in registers that lie on pages of the pool
+        // the table entry of key (lane & 31) of a tile
+        auto entry = [&](int64_t base) {
+            const int64_t key = base + (lane & 31);
+            return key >= some_lo && key < some_hi ? table[key >> a.shift] : -1;
+        };
+        auto load = [&](int64_t base, int32_t page) {
+            const bool good = page_in_pool(page, a.n_pages);
+            const int64_t key = base + (lane & 31);
+            const int64_t off = good ? page * a.page_stride + (key & ((int64_t(1) << a.shift) - 1)) * a.token_stride +
+                                           kvh * a.head_stride
+                                     : 0;
+            seen = static_cast<uint32_t>(__ballot(good));
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const T *k = static_cast<const T *>(a.k) + __shfl(off, 16 * b + col) + 8 * quad;
+#pragma unroll
+                for (int st = 0; st < kSteps; ++st) kreg[b][st] = *reinterpret_cast<const u32x4_a *>(k + 32 * st);
+            }
+#pragma unroll
+            for (int i = 0; i < kVLoads; ++i) {
+                const int idx = 64 * i + lane;
+                const T *v = static_cast<const T *>(a.v) + __shfl(off, idx / kChunks) + idx % kChunks * 8;
+                vreg[i] = *reinterpret_cast<const u32x4_a *>(v);
+            }
+        };
+        // this wavefront's tiles: every kTokenWaves-th
+        const int64_t first = w.key_lo + t0 * kUnitKeys + wave * kTokenKeys;
+        const int64_t end = idx_min(some_hi, w.key_lo + t1 * kUnitKeys);
+        int32_t next = -1;
+        if (first < end) {
+            load(first, entry(first));
+            next = entry(first + kUnitKeys);
+        }
+        for (int64_t base = first; base < end; base += kUnitKeys) {
+            const uint32_t now = seen;
+            f32x4 s[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    f32x4 c = {0, 0, 0, 0};
+#pragma unroll
+                    for (int st = 0; st < kSteps; ++st)
+                        c = N::mfma16(__builtin_bit_cast(V8, kreg[b][st]), qf[mt][st], c);
+                    s[mt][b] = c;
+                }
+            // every key of the tile seen by every row
+            const bool full = base >= all_lo && base + kTokenKeys <= all_hi && now == 0xFFFFFFFFu;
+            bool odd = false;  // a value that a weight of zero would not take away
+#pragma unroll
+            for (int i = 0; i < kVLoads; ++i) {
+                const int idx = 64 * i + lane, key = idx / kChunks;
+                u32x4_a v = vreg[i];
+                if (!full) {
+                    if (!((now >> key) & 1)) v = u32x4_a{0, 0, 0, 0};
+                    odd |= not_finite<TYPE>(v);
+                }
+                *reinterpret_cast<u32x4_a *>(vt + key * S::kVStride + idx % kChunks * 8) = v;
+            }
+            const int64_t after = base + kUnitKeys;
+            if (after < end) {
+                load(after, next);
+                next = entry(after + kUnitKeys);
+            }
+            V8 hi[MT], lo[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float x = score2(s[mt][b][i], a);
+                        if (!full) {
+                            const int k = 16 * b + 4 * quad + i;
+                            const int64_t key = base + k;
+                            if (!((now >> k) & 1) || key < row_lo[mt] || key >= row_hi[mt]) x = -INFINITY;
+                        }
+                        s[mt][b][i] = x;
+                        top = fmaxf(top, x);
+                    }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float m_new = fmaxf(m[mt], top), ref = finite_base(m_new);
+                if (__any(m_new > m[mt])) {
+                    const float keep = __builtin_amdgcn_exp2f(m[mt] - ref);
+                    l[mt] *= keep;
+#pragma unroll
+                    for (int d = 0; d < kBlocks; ++d) o[mt][d] *= keep;
+                    m[mt] = m_new;
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = __builtin_amdgcn_exp2f(s[mt][b][i] - ref);
+                        l[mt] += p;
+                        const T h = static_cast<T>(p);
+                        hi[mt][4 * b + i] = h;
+                        lo[mt][4 * b + i] = static_cast<T>(p - static_cast<float>(h));
+                    }
+            }
+            auto vcolumn = [&](int d) {
+                const T *p = vt + (4 * quad + col / 4) * S::kVStride + 16 * d + col % 4 * 4;
+                const u32x2_a x = lds_read_transposed(p), y = lds_read_transposed(p + 16 * S::kVStride);
+                return u32x4_a{x[0], x[1], y[0], y[1]};
+            };
+            if (!full && __any(odd)) {
+                // an infinity or NaN under weights of which some are zero because their row
+                // does not see it: row by row, with the values that the row sees
+                for (int r = 0; r < S::kRows; ++r) {
+                    const int mt = r / 16;
+                    uint32_t mask = 0;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        if (t != mt) continue;
+                        const int64_t rl = __shfl(row_lo[t], r % 16) - base, rh = __shfl(row_hi[t], r % 16) - base;
+                        const int klo = static_cast<int>(idx_min(32, idx_max(0, rl)));
+                        const int khi = static_cast<int>(idx_min(32, idx_max(klo, rh)));
+                        mask = static_cast<uint32_t>((uint64_t(1) << khi) - (uint64_t(1) << klo));
+                    }
+#pragma unroll
+                    for (int d = 0; d < kBlocks; ++d) {
+                        u32x4_a v = vcolumn(d);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int k = 16 * (i / 2) + 4 * quad + 2 * (i % 2);
+                            if (!((mask >> k) & 1)) v[i] &= 0xFFFF0000u;
+                            if (!((mask >> (k + 1)) & 1)) v[i] &= 0x0000FFFFu;
+                        }
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) {
+                            f32x4 c = N::mfma16(__builtin_bit_cast(V8, v), hi[t], f32x4{0, 0, 0, 0});
+                            c = N::mfma16(__builtin_bit_cast(V8, v), lo[t], c);
+                            if (t == mt && col == r % 16) o[t][d] += c;
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    const V8 v = __builtin_bit_cast(V8, vcolumn(d));
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        o[mt][d] = N::mfma16(v, hi[mt], o[mt][d]);
+                        o[mt][d] = N::mfma16(v, lo[mt], o[mt][d]);
+                    }
+                }
+            }
+        }
+
+        // join the wavefronts' sums, 16 rows at a time
+        const bool whole = t0 == 0 && t1 == w.tiles;
+        float *part = a.ws + (2 * static_cast<int64_t>(blockIdx.x) + (u != u0)) * S::kPartFloats;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float sum = l[mt];
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (quad == 0) {
+                lds_m[wave][col] = m[mt];
+                lds_l[wave][col] = sum;
+            }
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d)
+                *reinterpret_cast<f32x4 *>(ot + col * S::kOStride + 16 * d + 4 * quad) = o[mt][d];
+            __syncthreads();
+            for (int idx = tid; idx < 16 * (HD / 4); idx += kTokenThreads) {
+                const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
+                const int row = row0 + 16 * mt + r;
+                if (row >= g.rows) break;
+                float top = lds_m[0][r];
+#pragma unroll
+                for (int wv = 1; wv < kTokenWaves; ++wv) top = fmaxf(top, lds_m[wv][r]);
+                const float ref = finite_base(top);
+                float den = 0.0f;
+                f32x4 num = {0, 0, 0, 0};
+#pragma unroll
+                for (int wv = 0; wv < kTokenWaves; ++wv) {
+                    const float f = __builtin_amdgcn_exp2f(lds_m[wv][r] - ref);
+                    den += f * lds_l[wv][r];
+                    num += f * *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(lds + wv * S::kWaveBytes) +
+                                                                 r * S::kOStride + c);
+                }
+                if (whole) {
+                    const f32x4 v = den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den);
+                    store4<TYPE>(a, out_at(a, g, kvh, row, HD) + c, v);
+                } else {
+                    *reinterpret_cast<f32x4 *>(part + (16 * mt + r) * HD + c) = num;
+                    if (c == 0) {
+                        part[S::kRows * HD + 16 * mt + r] = top;
+                        part[S::kRows * (HD + 1) + 16 * mt + r] = den;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        u += t1 - t0;
     }
+}
+
+// Joins the parts of the rows that a boundary between two workgroups' stretches
+// cuts: block b those whose first cut is the start of workgroup b + 1.
+constexpr int kJoinThreads = 512;
+
+template <int TYPE, int HD, int MT>
+__global__ __launch_bounds__(kJoinThreads) void attention_token_join_kernel(AttnArgs a, int groups) {
+    typedef TokenShape<HD, MT> S;
+    constexpr int kWaves = kJoinThreads / 64;
+    __shared__ int64_t tmp[kWaves];
+    __shared__ f32x4 lds_num[kJoinThreads];
+    __shared__ float lds_den[kJoinThreads];
+    const int tid = threadIdx.x;
+    Scan<S::kRows, kWaves> scan;
+    scan.run(a, tmp);
+    const Stretches line = stretches(scan.total, groups);
+    const int64_t u_prev = stretch_begin(line, blockIdx.x), u_cut = stretch_begin(line, blockIdx.x + 1);
+    if (u_prev >= u_cut || u_cut >= line.total) return;
+    int64_t before;
+    const int seq = scan.find(a, u_cut, tmp, &before);
+    const SeqGeo g = seq_geo(a, seq);
+    const TokenWork w = token_work<S::kRows>(a, g);
+    const int64_t item = quotient(u_cut - before, w.tiles);
+    const int64_t begin = before + item * w.tiles, end = begin + w.tiles;
+    if (begin == u_cut || begin < u_prev) return;  // not cut here, or cut before
+    // the stretches blockIdx.x .. that of the last unit have a part each
+    const int n_parts = static_cast<int>(stretch_of(line, end - 1) - blockIdx.x) + 1;
+    const int kvh = static_cast<int>(quotient(item, w.blocks));
+    const int row0 = static_cast<int>(item - static_cast<int64_t>(kvh) * w.blocks) * S::kRows;
+    const int rows = min(S::kRows, g.rows - row0);
+    auto part_of = [&](int i) {  // the first part ends its stretch, the others begin theirs
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x + i) + (i == 0 && begin != u_prev);
+        return a.ws + slot * S::kPartFloats;
+    };
+    // threads: one per row and 4 values, and as many teams as fit share the parts
+    constexpr int kQuads = HD / 4;
+    for (int r0 = 0; r0 < rows; r0 += kJoinThreads / kQuads) {
+        const int n = min(kJoinThreads / kQuads, rows - r0) * kQuads;
+        const int teams = kJoinThreads / n, team = tid / n, r = r0 + tid % n / kQuads, c = tid % kQuads * 4;
+        const bool work = team < teams;
+        float top = -INFINITY;
+        if (work)
+            for (int i = 0; i < n_parts; ++i) top = fmaxf(top, part_of(i)[S::kRows * HD + r]);
+        const float ref = finite_base(top);
+        float den = 0.0f;
+        f32x4 num = {0, 0, 0, 0};
+        if (work)
+#pragma unroll 4
+            for (int i = team; i < n_parts; i += teams) {
+                const float *p = part_of(i);
+                const float f = __builtin_amdgcn_exp2f(p[S::kRows * HD + r] - ref);
+                den += f * p[S::kRows * (HD + 1) + r];
+                num += f * *reinterpret_cast<const f32x4 *>(p + r * HD + c);
+            }
+        lds_num[tid] = num;
+        lds_den[tid] = den;
+        __syncthreads();
+        if (team == 0) {
+            for (int t = 1; t < teams; ++t) {
+                num += lds_num[t * n + tid];
+                den += lds_den[t * n + tid];
+            }
+            const f32x4 v = den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den);
+            store4<TYPE>(a, out_at(a, g, kvh, row0 + r, HD) + c, v);
+        }
+        __syncthreads();
+    }
+}
+
+// Workgroups of the token form that stay on the chip together.
+constexpr int kTokenGroupsPerCu = 3;
+
+int token_groups(const mi355x_ctx *ctx) { return ctx->num_cus * kTokenGroupsPerCu; }
+
+template <int TYPE, int HD, int MT>
+int launch_token(mi355x_ctx *ctx, const AttnArgs &a) {
+    const int groups = token_groups(ctx);
+    attention_token_kernel<TYPE, HD, MT><<<groups, kTokenThreads, 0, ctx->stream>>>(a);
+    MI355X_HIP(hipGetLastError());
+    attention_token_join_kernel<TYPE, HD, MT><<<groups - 1, kJoinThreads, 0, ctx->stream>>>(a, groups);
     MI355X_HIP(hipGetLastError());
     return MI355X_OK;
 }
 
+template <int TYPE, int HD>
+int launch_forms(mi355x_ctx *ctx, const AttnArgs &a, int64_t rows) {
+    if (rows <= 16) return launch_token<TYPE, HD, 1>(ctx, a);
+    if constexpr (HD <= 128)
+        if (rows > 32) return launch_token<TYPE, HD, 4>(ctx, a);
+    return launch_token<TYPE, HD, 2>(ctx, a);
+}
+
+template <int TYPE>
+int launch_sizes(mi355x_ctx *ctx, const AttnArgs &a, int head_dim, int64_t rows) {
+    switch (head_dim) {
+    case 64: return launch_forms<TYPE, 64>(ctx, a, rows);
+    case 96: return launch_forms<TYPE, 96>(ctx, a, rows);
+    case 128: return launch_forms<TYPE, 128>(ctx, a, rows);
+    default: return launch_forms<TYPE, 256>(ctx, a, rows);
+    }
+}
+
 }  // namespace
 
-size_t paged_attention_workspace_bytes(const mi355x_ctx *, int, int, int) { return 256; }
+size_t paged_attention_workspace_bytes(const mi355x_ctx *ctx, int, int, int head_dim) {
+    return static_cast<size_t>(token_groups(ctx)) * 2 * 64 * (head_dim + 2) * 4;
+}
 
-int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &a) {
-    const int shift = __builtin_ctz(static_cast<unsigned>(a.pool->page_tokens));
-    return a.pool->type == MI355X_TYPE_F16 ? launch_rows<MI355X_TYPE_F16>(ctx, a, shift)
-                                           : launch_rows<MI355X_TYPE_BF16>(ctx, a, shift);
+int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &u) {
+    AttnArgs a{};
+    a.q = u.q;
+    a.k = u.pool->k;
+    a.v = u.pool->v;
+    a.row_offsets = u.row_offsets;
+    a.kv_lens = u.kv_lens;
+    a.table = u.block_table;
+    a.out = u.out;
+    a.ws = static_cast<float *>(u.workspace);
+    a.q_stride = u.q_stride;
+    a.out_stride = u.out_stride;
+    a.table_stride = u.table_stride;
+    a.page_stride = u.pool->page_stride;
+    a.token_stride = u.pool->token_stride;
+    a.head_stride = u.pool->head_stride;
+    a.n_rows = u.n_rows;
+    // an empty pool has no address that may be read: no token is seen
+    a.reach = u.pool->n_pages > 0 ? static_cast<int64_t>(u.table_cols) * u.pool->page_tokens : 0;
+    a.scale = u.scale;
+    a.softcap = u.softcap;
+    a.n_seqs = u.n_seqs;
+    a.n_kv_heads = u.pool->n_kv_heads;
+    const int group = u.n_heads / u.pool->n_kv_heads;
+    a.group = fast_div(static_cast<uint32_t>(group));
+    a.n_pages = static_cast<int>(u.pool->n_pages);
+    a.shift = __builtin_ctz(static_cast<unsigned>(u.pool->page_tokens));
+    a.window = u.window;
+    a.causal = u.causal;
+    a.row_limit = INT32_MAX;
+    const int64_t added = u.max_added > 0 ? std::min<int64_t>(u.max_added, u.n_rows) : u.n_rows;
+    a.f32_out = u.out_type == MI355X_TYPE_F32;
+    return u.pool->type == MI355X_TYPE_F16
+               ? launch_sizes<MI355X_TYPE_F16>(ctx, a, u.pool->head_dim, added * group)
+               : launch_sizes<MI355X_TYPE_BF16>(ctx, a, u.pool->head_dim, added * group);
 }
 
 }  // namespace mi355x

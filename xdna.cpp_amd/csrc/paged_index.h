@@ -5,7 +5,7 @@
 #include <stdint.h>
 
 #ifdef __HIPCC__
-#define MI355X_HD __host__ __device__ __forceinline__
+#define MI355X_HD __attribute__((host)) __attribute__((device)) inline __attribute__((always_inline))
 #else
 #define MI355X_HD inline
 #endif
@@ -14,6 +14,47 @@ namespace mi355x {
 
 MI355X_HD int64_t idx_min(int64_t a, int64_t b) { return a < b ? a : b; }
 MI355X_HD int64_t idx_max(int64_t a, int64_t b) { return a > b ? a : b; }
+
+// n / d for 0 <= n < 2^31 as a product and a shift (d >= 1): mul = floor(2^(31 +
+// l) / d) + 1 with l = ceil(log2 d) is above 2^(31 + l) / d by at most 2^l parts
+// of its d, which moves no quotient of n < 2^31.
+struct FastDiv {
+    uint32_t d, mul, shift;
+};
+MI355X_HD FastDiv fast_div(uint32_t d) {
+    FastDiv f{d, 0, 31};
+    while ((uint64_t(1) << (f.shift - 31)) < d) ++f.shift;
+    f.mul = static_cast<uint32_t>((uint64_t(1) << f.shift) / d + 1);
+    return f;
+}
+MI355X_HD int32_t divided(int32_t n, const FastDiv &f) {
+    return static_cast<int32_t>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * f.mul) >> f.shift);
+}
+
+// a / b, by 32-bit division where both fit (64-bit division is long on the GPU).
+MI355X_HD int64_t quotient(int64_t a, int64_t b) {
+    if (((static_cast<uint64_t>(a) | static_cast<uint64_t>(b)) >> 32) == 0)
+        return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
+// `total` units in `groups` stretches of equal length, the first of them one longer.
+struct Stretches {
+    int64_t total, each, longer;
+};
+MI355X_HD Stretches stretches(int64_t total, int groups) {
+    Stretches s;
+    s.total = total;
+    s.each = quotient(total, groups);
+    s.longer = total - s.each * groups;
+    return s;
+}
+MI355X_HD int64_t stretch_begin(const Stretches &s, int64_t g) { return s.each * g + idx_min(g, s.longer); }
+// The stretch that has unit u < total.
+MI355X_HD int64_t stretch_of(const Stretches &s, int64_t u) {
+    const int64_t lead = s.longer * (s.each + 1);
+    return u < lead ? quotient(u, s.each + 1) : s.longer + quotient(u - lead, s.each);
+}
 
 // Pages of 2^shift tokens that hold n >= 0 tokens.
 MI355X_HD int64_t pages_of(int64_t n, int shift) { return (n + (int64_t(1) << shift) - 1) >> shift; }
