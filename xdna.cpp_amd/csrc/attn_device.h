@@ -120,6 +120,28 @@ __device__ __forceinline__ KeyRange token_keys(const AttnArgs &a, const SeqGeo &
     return visible_keys(g.pos0 + token, g.kv, a.reach, a.window, a.causal != 0);
 }
 
+// Four values of a row's output.
+template <int TYPE>
+__device__ __forceinline__ void store_out4(const AttnArgs &a, int64_t at, f32x4 v) {
+    typedef typename Num<TYPE>::T T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    if (a.f32_out) {
+        *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + at) = v;
+    } else {
+        T4 h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = static_cast<T>(v[i]);
+        *reinterpret_cast<T4 *>(static_cast<T *>(a.out) + at) = h;
+    }
+}
+
+// Where the output of head row `row` of KV head kvh begins.
+__device__ __forceinline__ int64_t out_at(const AttnArgs &a, const SeqGeo &g, int kvh, int row, int hd) {
+    const int token = divided(row, a.group), group = static_cast<int>(a.group.d);
+    const int64_t head = static_cast<int64_t>(kvh) * group + (row - token * group);
+    return (g.first + g.tok_lo + token) * a.out_stride + head * hd;
+}
+
 // Exclusive scan of one value per thread over a workgroup of WAVES wavefronts;
 // *total is the sum.  `tmp` holds WAVES values and is free after the call's
 // last barrier.
@@ -144,5 +166,10 @@ __device__ __forceinline__ int64_t group_scan(int64_t v, int64_t *tmp, int64_t *
     *total = sum;
     return before + in - v;
 }
+
+// The chunk form (paged_attention_chunk.hip): requests of more than
+// a.row_limit head rows, and its part of the workspace.
+int launch_attention_chunk(mi355x_ctx *ctx, const AttnArgs &a, int type, int head_dim);
+size_t attention_chunk_workspace(const mi355x_ctx *ctx, int head_dim);
 
 }  // namespace mi355x

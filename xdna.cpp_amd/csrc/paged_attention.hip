@@ -109,26 +109,6 @@ struct TokenShape {
     static constexpr int kPartFloats = kRows * (HD + 2);
 };
 
-template <int TYPE>
-__device__ __forceinline__ void store4(const AttnArgs &a, int64_t at, f32x4 v) {
-    typedef typename Num<TYPE>::T T;
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    if (a.f32_out) {
-        *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + at) = v;
-    } else {
-        T4 h;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = static_cast<T>(v[i]);
-        *reinterpret_cast<T4 *>(static_cast<T *>(a.out) + at) = h;
-    }
-}
-
-__device__ __forceinline__ int64_t out_at(const AttnArgs &a, const SeqGeo &g, int kvh, int row, int hd) {
-    const int token = divided(row, a.group), group = static_cast<int>(a.group.d);
-    const int64_t head = static_cast<int64_t>(kvh) * group + (row - token * group);
-    return (g.first + g.tok_lo + token) * a.out_stride + head * hd;
-}
-
 template <int TYPE, int HD, int MT>
 __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs a) {
     typedef Num<TYPE> N;
@@ -340,6 +320,7 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
                             f32x4 c = N::mfma16(__builtin_bit_cast(V8, v), hi[t], f32x4{0, 0, 0, 0});
                             c = N::mfma16(__builtin_bit_cast(V8, v), lo[t], c);
                             if (t == mt && col == r % 16) o[t][d] += c;
+                            __builtin_amdgcn_sched_barrier(0);  // rare: in few registers
                         }
                     }
                 }
@@ -391,7 +372,7 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
                 }
                 if (whole) {
                     const f32x4 v = den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den);
-                    store4<TYPE>(a, out_at(a, g, kvh, row, HD) + c, v);
+                    store_out4<TYPE>(a, out_at(a, g, kvh, row, HD) + c, v);
                 } else {
                     *reinterpret_cast<f32x4 *>(part + (16 * mt + r) * HD + c) = num;
                     if (c == 0) {
@@ -468,7 +449,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_token_join_kernel(Attn
                 den += lds_den[t * n + tid];
             }
             const f32x4 v = den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den);
-            store4<TYPE>(a, out_at(a, g, kvh, row0 + r, HD) + c, v);
+            store_out4<TYPE>(a, out_at(a, g, kvh, row0 + r, HD) + c, v);
         }
         __syncthreads();
     }
@@ -492,9 +473,15 @@ int launch_token(mi355x_ctx *ctx, const AttnArgs &a) {
 template <int TYPE, int HD>
 int launch_forms(mi355x_ctx *ctx, const AttnArgs &a, int64_t rows) {
     if (rows <= 16) return launch_token<TYPE, HD, 1>(ctx, a);
-    if constexpr (HD <= 128)
-        if (rows > 32) return launch_token<TYPE, HD, 4>(ctx, a);
-    return launch_token<TYPE, HD, 2>(ctx, a);
+    if (rows <= 32) return launch_token<TYPE, HD, 2>(ctx, a);
+    AttnArgs b = a;
+    b.row_limit = 0;
+    if (a.n_seqs > 1) {  // some may add few tokens
+        AttnArgs c = a;
+        c.row_limit = b.row_limit = 16;
+        if (int rc = launch_token<TYPE, HD, 1>(ctx, c)) return rc;
+    }
+    return launch_attention_chunk(ctx, b, TYPE, HD);
 }
 
 template <int TYPE>
@@ -510,7 +497,8 @@ int launch_sizes(mi355x_ctx *ctx, const AttnArgs &a, int head_dim, int64_t rows)
 }  // namespace
 
 size_t paged_attention_workspace_bytes(const mi355x_ctx *ctx, int, int, int head_dim) {
-    return static_cast<size_t>(token_groups(ctx)) * 2 * 64 * (head_dim + 2) * 4;
+    return std::max(static_cast<size_t>(token_groups(ctx)) * 2 * 32 * (head_dim + 2) * 4,
+                    attention_chunk_workspace(ctx, head_dim));
 }
 
 int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &u) {

@@ -1,0 +1,442 @@
+// Attention over a paged KV cache, chunk form: for requests that add many
+// tokens.
+//
+// A workgroup takes 128 head rows (tokens x query heads of one KV head) of a
+// request and walks the keys that they see in tiles of 64; a wavefront owns 32
+// of the rows.  As in the token form a tile's scores are K q^T, so that a lane
+// holds 32 scores of one row, the softmax needs one exchange, and the weights
+// are, as they lie, the operand of V^T w; O^T stays in registers.  The matrix
+// cores bound it, then the exponentials and LDS.
+//
+// K and V tiles travel to LDS directly (global_load_lds), one tile ahead.  Such
+// loads fill LDS in lane order, so rows cannot be padded; instead the 16-byte
+// chunks of a row are permuted by the row's number (the lane that fills a place
+// loads the chunk that belongs there), so that neither the score operands (32
+// rows, one chunk) nor the transposed reads of V (4 rows, two chunks) meet in a
+// bank.
+//
+// Work split.  Blocks of rows are numbered so that a workgroup finds its
+// request from the row offsets alone; the last ones (which see the most keys)
+// start first.  Where they leave CUs idle the keys of each are cut into `split`
+// parts, which leave (m, l, sum) in the workspace for a second launch.
+#include "attn_device.h"
+#include "internal.h"
+
+#include <algorithm>
+
+namespace mi355x {
+namespace {
+
+constexpr int kChunkWaves = 4;
+constexpr int kChunkThreads = 64 * kChunkWaves;
+constexpr int kChunkRows = 32 * kChunkWaves;
+constexpr int kChunkKeys = 64;
+// A row's maximum may grow by this (in factors of 2) before its sums are
+// scaled: weights stay below 2^8, where 16-bit floats are as exact as below 1.
+constexpr float kSlack = 8.0f;
+
+template <int HD>
+struct ChunkShape {
+    static constexpr int kChunks = HD / 8;                            // 16-byte chunks of a token's head
+    static constexpr int kPlaces = HD == 96 ? 16 : kChunks;           // places for them in LDS, a power of two
+    static constexpr int kRowBytes = 16 * kPlaces;
+    static constexpr int kTileBytes = kChunkKeys * kRowBytes;
+    static constexpr int kLoads = kChunkKeys * kPlaces / kChunkThreads;  // of K, and of V, per lane
+    static constexpr int kPartFloats = kChunkRows * (HD + 2);
+    static constexpr int kLds = 4 * kTileBytes;                       // K and V, two tiles each
+};
+
+// The place of chunk c of row r is c ^ k_turn(r) (K) or c ^ v_turn(r) (V).
+__device__ __forceinline__ int k_turn(int r) { return r & 7; }
+__device__ __forceinline__ int v_turn(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+
+// The request whose row blocks include block j, and its first one.
+__device__ __forceinline__ int find_block(const AttnArgs &a, int64_t j, int64_t *first) {
+    auto begin = [&](int s) {  // ascends by at least 1: blocks of 128 rows, one more at every seam
+        return ((static_cast<int64_t>(a.row_offsets[s]) * a.group.d) >> 7) + s;
+    };
+    static_assert(kChunkRows == 128, "the shift above");
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.n_seqs;  // the request is in lo .. lo + n - 1
+    while (n > 1) {
+        const int step = (n + 63) / 64;
+        const int s = lo + lane * step;
+        const uint64_t below = __ballot(lane * step < n && begin(s) <= j);
+        const int k = max(0, 63 - __builtin_clzll(below | 1));
+        n = min(step, n - k * step);
+        lo += k * step;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    *first = begin(lo);
+    return lo;
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+struct ChunkItem {
+    int seq, kvh, row0;
+    SeqGeo g;
+    KeyRange first, last;  // of the block's first and last row
+    int tiles;             // of keys from key_lo on
+    int64_t key_lo;
+};
+
+// False: no rows there.
+__device__ __forceinline__ bool chunk_item(const AttnArgs &a, int64_t j, int kvh, ChunkItem *it) {
+    int64_t begin;
+    it->seq = find_block(a, j, &begin);
+    it->kvh = kvh;
+    it->g = seq_geo(a, it->seq);
+    const int64_t row0 = (j - begin) * kChunkRows;
+    if (row0 < 0 || row0 >= it->g.rows || it->g.rows <= a.row_limit) return false;
+    it->row0 = static_cast<int>(row0);
+    const int row_last = min(it->row0 + kChunkRows, it->g.rows) - 1;
+    it->first = token_keys(a, it->g, it->g.tok_lo + divided(it->row0, a.group));
+    it->last = token_keys(a, it->g, it->g.tok_lo + divided(row_last, a.group));
+    it->key_lo = it->first.lo & ~int64_t(kChunkKeys - 1);
+    it->tiles = static_cast<int>((idx_max(it->last.hi - it->key_lo, 0) + kChunkKeys - 1) / kChunkKeys);
+    return true;
+}
+
+template <int TYPE, int HD, bool CAP, int PLANES>
+__global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chunk_kernel(AttnArgs a) {
+    typedef Num<TYPE> N;
+    typedef typename N::T T;
+    typedef typename N::V8 V8;
+    typedef ChunkShape<HD> S;
+    constexpr int kSteps = HD / 16;   // of a 32-key score product
+    constexpr int kBlocks = HD / 32;  // of 32 output values
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    __shared__ int odd;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    // block = ((j from the last on) * split + part) * KV heads + head
+    const int kvh = static_cast<int>(blockIdx.x % a.n_kv_heads);
+    const int64_t rest = blockIdx.x / a.n_kv_heads;
+    const int part = static_cast<int>(rest % a.split);
+    ChunkItem it;
+    if (!chunk_item(a, gridDim.x / (a.n_kv_heads * a.split) - 1 - rest / a.split, kvh, &it)) return;
+    const SeqGeo g = it.g;
+    const int t0 = static_cast<int>(static_cast<int64_t>(it.tiles) * part / a.split);
+    const int t1 = static_cast<int>(static_cast<int64_t>(it.tiles) * (part + 1) / a.split);
+
+    // this lane's row
+    const int row_raw = it.row0 + 32 * wave + col;
+    const bool real = row_raw < g.rows;
+    const int row = real ? row_raw : 0, tok = divided(row, a.group), group = static_cast<int>(a.group.d);
+    const int64_t head = static_cast<int64_t>(kvh) * group + (row - tok * group);
+    int64_t row_lo = 0, row_hi = 0;
+    if (real) {
+        const KeyRange kr = token_keys(a, g, g.tok_lo + tok);
+        row_lo = kr.lo;
+        row_hi = kr.hi;
+    }
+    V8 qf[kSteps];
+    {
+        const T *q = static_cast<const T *>(a.q) + (g.first + g.tok_lo + tok) * a.q_stride + head * HD;
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+            V8 z = {};
+            if (real) z = *reinterpret_cast<const V8 *>(q + 16 * st + 8 * half);
+            qf[st] = z;
+        }
+    }
+    f32x16 o[kBlocks];
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    const int32_t *table = a.table + it.seq * a.table_stride;
+    // the table entry of key `lane` of tile t
+    auto entry = [&](int t) {
+        const int64_t key = it.key_lo + static_cast<int64_t>(t) * kChunkKeys + lane;
+        return t < t1 && key >= it.first.lo && key < it.last.hi ? table[key >> a.shift] : -1;
+    };
+    uint64_t seen_next = 0;  // keys of the tile on its way that lie on pages of the pool
+    auto load = [&](int t, int32_t page, int buf) {
+        const bool good = page_in_pool(page, a.n_pages);
+        seen_next = __ballot(good);
+        const int64_t key = it.key_lo + static_cast<int64_t>(t) * kChunkKeys + lane;
+        const int64_t off = good ? page * a.page_stride + (key & ((int64_t(1) << a.shift) - 1)) * a.token_stride +
+                                       kvh * a.head_stride
+                                 : 0;
+#pragma unroll
+        for (int i = 0; i < S::kLoads; ++i) {
+            const int at = (i * kChunkWaves + wave) * 64;  // this instruction's first place
+            const int r = (at + lane) / S::kPlaces, place = (at + lane) % S::kPlaces;
+            const int64_t from = __shfl(off, r);
+            int ck = place ^ k_turn(r), cv = place ^ v_turn(r);
+            if (HD == 96) {  // places without a chunk take another's
+                ck = ck < S::kChunks ? ck : ck - 4;
+                cv = cv < S::kChunks ? cv : cv - 4;
+            }
+            const T *k = static_cast<const T *>(a.k) + from + 8 * ck;
+            const T *v = static_cast<const T *>(a.v) + from + 8 * cv;
+            unsigned char *to = lds + 2 * buf * S::kTileBytes + 16 * at;
+            __builtin_amdgcn_global_load_lds(
+                reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(reinterpret_cast<uintptr_t>(k)),
+                (__attribute__((address_space(3))) uint32_t *)(to), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(
+                reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(reinterpret_cast<uintptr_t>(v)),
+                (__attribute__((address_space(3))) uint32_t *)(to + S::kTileBytes), 16, 0, 0);
+        }
+    };
+    // where this lane reads: K row col (+ 32), chunk 2 st + half; V rows 4 half +
+    // (lane % 16) / 4 (+ 8 ..), chunk 4 d + 2 ((lane / 16) % 2) + (lane % 4) / 2
+    const int k_at = col * S::kRowBytes;
+    const int k_low = half ^ k_turn(col);
+    const int v_row = 4 * half + ((lane & 15) >> 2);
+    const int v_at = v_row * S::kRowBytes + (lane & 1) * 8;
+    const int v_low = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_turn(v_row);
+
+    int32_t next = -1;
+    if (t0 < t1) {
+        load(t0, entry(t0), 0);
+        next = entry(t0 + 1);
+    }
+    const float c = a.scale * kLog2e;
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        const uint64_t seen = seen_next;
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this tile's loads
+        __syncthreads();                     // everyone's, and the other buffer is read
+        if (t + 1 < t1) {
+            load(t + 1, next, buf ^ 1);
+            next = entry(t + 2);
+        }
+        unsigned char *kt = lds + 2 * buf * S::kTileBytes, *vt = kt + S::kTileBytes;
+        const int64_t base = it.key_lo + static_cast<int64_t>(t) * kChunkKeys;
+        // every key of the tile seen by every row of the workgroup
+        const bool full = base >= it.last.lo && base + kChunkKeys <= it.first.hi && ~seen == 0;
+        bool by_row = false;
+        if (!full) {
+            // values that no row sees become zero; is any other one not finite?
+            if (tid == 0) odd = 0;
+            __syncthreads();
+            bool bad = false;
+            for (int i = tid; i < kChunkKeys * S::kPlaces; i += kChunkThreads) {
+                u32x4_a *p = reinterpret_cast<u32x4_a *>(vt + 16 * i);
+                if (!((seen >> (i / S::kPlaces)) & 1)) *p = u32x4_a{0, 0, 0, 0};
+                else bad |= not_finite<TYPE>(*p);
+            }
+            if (__any(bad) && lane == 0) odd = 1;
+            __syncthreads();
+            by_row = odd != 0;
+        }
+        f32x16 s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) {
+                const int place = ((2 * (st & 3)) ^ k_low) + 8 * (st >> 2);
+                const V8 k = *reinterpret_cast<const V8 *>(kt + k_at + 32 * kb * S::kRowBytes + 16 * place);
+                s[kb] = N::mfma32(k, qf[st], s[kb]);
+            }
+        }
+        float top = -INFINITY;
+        if (CAP) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[kb][i] = score2(s[kb][i], a);
+        }
+        if (!full) {
+            const int lo = static_cast<int>(idx_max(row_lo - base, 0)), hi = static_cast<int>(idx_min(row_hi - base, 64));
+            uint64_t mine = seen;
+            mine = hi <= 0 || lo >= 64 ? 0 : mine & (hi >= 64 ? ~uint64_t(0) : (uint64_t(1) << hi) - 1) & ~((uint64_t(1) << lo) - 1);
+            mine >>= 4 * half;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!((mine >> (32 * kb + 8 * (i >> 2) + (i & 3))) & 1)) s[kb][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+        top = fmaxf(top, other_half(top));
+        if (!CAP) top *= c;  // c >= 0 here; 0 x infinity gives NaN, which no maximum takes
+        const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
+        if (__any(grows)) {
+            const float m_new = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) o[d] *= keep;
+            m = m_new;
+        }
+        const float ref = finite_base(m);
+        V8 hi[4], lo[PLANES == 2 ? 4 : 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = s[j >> 1][8 * (j & 1) + i];
+                const float p = __builtin_amdgcn_exp2f(CAP ? x - ref : fmaf(x, c, -ref));
+                l += p;
+                const T h = static_cast<T>(p);
+                hi[j][i] = h;
+                if (PLANES == 2) lo[j][i] = static_cast<T>(p - static_cast<float>(h));
+            }
+        auto v_chunk = [&](int j, int d) {  // keys 16 j + {4 half .. + 3, 8 + 4 half .. + 3} of 32 values
+            const int place = ((4 * (d & 1)) ^ v_low) + 8 * (d >> 1);
+            const unsigned char *p = vt + v_at + 16 * j * S::kRowBytes + 16 * place;
+            const u32x2_a x = lds_read_transposed(p), y = lds_read_transposed(p + 8 * S::kRowBytes);
+            return u32x4_a{x[0], x[1], y[0], y[1]};
+        };
+        if (by_row) {
+            // an infinity or NaN under weights of which some are zero because their row
+            // does not see it: row by row, with the values that the row sees
+            for (int r = 0; r < 32; ++r) {
+                const int64_t rl = __shfl(row_lo, r) - base, rh = __shfl(row_hi, r) - base;
+                const int klo = static_cast<int>(idx_min(64, idx_max(0, rl))), khi = static_cast<int>(idx_min(64, idx_max(0, rh)));
+                uint64_t mask = khi <= klo ? 0 : (khi >= 64 ? ~uint64_t(0) : (uint64_t(1) << khi) - 1) & ~((uint64_t(1) << klo) - 1);
+                mask >>= 4 * half;
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    f32x16 x;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        u32x4_a v = v_chunk(j, d);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int k = 16 * j + 8 * (i >> 1) + 2 * (i & 1);
+                            if (!((mask >> k) & 1)) v[i] &= 0xFFFF0000u;
+                            if (!((mask >> (k + 1)) & 1)) v[i] &= 0x0000FFFFu;
+                        }
+                        x = N::mfma32(__builtin_bit_cast(V8, v), hi[j], x);
+                        if (PLANES == 2) x = N::mfma32(__builtin_bit_cast(V8, v), lo[PLANES == 2 ? j : 0], x);
+                        __builtin_amdgcn_sched_barrier(0);  // rare: in few registers
+                    }
+                    if (col == r) o[d] += x;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    const V8 v = __builtin_bit_cast(V8, v_chunk(j, d));
+                    o[d] = N::mfma32(v, hi[j], o[d]);
+                    if (PLANES == 2) o[d] = N::mfma32(v, lo[PLANES == 2 ? j : 0], o[d]);
+                }
+        }
+    }
+
+    l += other_half(l);
+    if (!real) return;
+    if (a.split == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int64_t at = (g.first + g.tok_lo + tok) * a.out_stride + head * HD;
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4 v = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                store_out4<TYPE>(a, at + 32 * d + 8 * i + 4 * half, l == 0.0f ? f32x4{0, 0, 0, 0} : v * inv);
+            }
+    } else {
+        float *w = a.ws + static_cast<int64_t>(blockIdx.x) * S::kPartFloats;
+        const int r = 32 * wave + col;
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4 *>(w + r * HD + 32 * d + 8 * i + 4 * half) =
+                    f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        if (half == 0) {
+            w[kChunkRows * HD + r] = m;
+            w[kChunkRows * (HD + 1) + r] = l;
+        }
+    }
+}
+
+// Joins the parts of each row block and KV head.
+template <int TYPE, int HD>
+__global__ __launch_bounds__(256) void attention_chunk_join_kernel(AttnArgs a) {
+    typedef ChunkShape<HD> S;
+    const int kvh = static_cast<int>(blockIdx.x % a.n_kv_heads);
+    const int64_t rest = blockIdx.x / a.n_kv_heads, blocks = gridDim.x / a.n_kv_heads;
+    ChunkItem it;
+    if (!chunk_item(a, blocks - 1 - rest, kvh, &it)) return;
+    const int rows = min(kChunkRows, it.g.rows - it.row0);
+    constexpr int kQuads = HD / 4;
+    for (int i = threadIdx.x + 256 * blockIdx.y; i < rows * kQuads; i += 256 * gridDim.y) {
+        const int r = i / kQuads, c = i % kQuads * 4;
+        auto part_of = [&](int p) { return a.ws + ((rest * a.split + p) * a.n_kv_heads + kvh) * S::kPartFloats; };
+        float top = -INFINITY;
+        for (int p = 0; p < a.split; ++p) top = fmaxf(top, part_of(p)[kChunkRows * HD + r]);
+        const float ref = finite_base(top);
+        float den = 0.0f;
+        f32x4 num = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int p = 0; p < a.split; ++p) {
+            const float *w = part_of(p);
+            const float f = __builtin_amdgcn_exp2f(w[kChunkRows * HD + r] - ref);
+            den += f * w[kChunkRows * (HD + 1) + r];
+            num += f * *reinterpret_cast<const f32x4 *>(w + r * HD + c);
+        }
+        store_out4<TYPE>(a, out_at(a, it.g, kvh, it.row0 + r, HD) + c,
+                         den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den));
+    }
+}
+
+// Workgroups that a call is split into at most, while that is more than its row blocks.
+int chunk_groups(const mi355x_ctx *ctx) { return 2 * ctx->num_cus; }
+
+template <int TYPE, int HD, bool CAP, int PLANES>
+int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
+    AttnArgs a = args;
+    const int64_t blocks = ((a.n_rows * a.group.d) >> 7) + a.n_seqs, items = blocks * a.n_kv_heads;
+    // parts of no fewer than four tiles where the table allows that many tokens
+    a.split = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>(chunk_groups(ctx) / items, (a.reach + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
+    if (items * a.split > INT32_MAX)
+        return set_error(MI355X_EUNSUPPORTED, "mi355x_paged_attention: more row blocks than a launch takes");
+    attention_chunk_kernel<TYPE, HD, CAP, PLANES>
+        <<<static_cast<unsigned>(items * a.split), kChunkThreads, ChunkShape<HD>::kLds, ctx->stream>>>(a);
+    MI355X_HIP(hipGetLastError());
+    if (a.split > 1) {
+        const dim3 grid(static_cast<unsigned>(items), 4);
+        attention_chunk_join_kernel<TYPE, HD><<<grid, 256, 0, ctx->stream>>>(a);
+        MI355X_HIP(hipGetLastError());
+    }
+    return MI355X_OK;
+}
+
+template <int TYPE, int HD>
+int launch_size(mi355x_ctx *ctx, const AttnArgs &a) {
+    // the common path scales the maximum instead of each score, for which the scale has to be positive
+    const bool cap = a.softcap > 0.0f || a.scale < 0.0f;
+    if (a.f32_out) return cap ? launch_chunk<TYPE, HD, true, 2>(ctx, a) : launch_chunk<TYPE, HD, false, 2>(ctx, a);
+    return cap ? launch_chunk<TYPE, HD, true, 1>(ctx, a) : launch_chunk<TYPE, HD, false, 1>(ctx, a);
+}
+
+template <int TYPE>
+int launch_type(mi355x_ctx *ctx, const AttnArgs &a, int head_dim) {
+    switch (head_dim) {
+    case 64: return launch_size<TYPE, 64>(ctx, a);
+    case 96: return launch_size<TYPE, 96>(ctx, a);
+    case 128: return launch_size<TYPE, 128>(ctx, a);
+    default: return launch_size<TYPE, 256>(ctx, a);
+    }
+}
+
+}  // namespace
+
+size_t attention_chunk_workspace(const mi355x_ctx *ctx, int head_dim) {
+    return static_cast<size_t>(chunk_groups(ctx)) * kChunkRows * (head_dim + 2) * 4;
+}
+
+int launch_attention_chunk(mi355x_ctx *ctx, const AttnArgs &a, int type, int head_dim) {
+    return type == MI355X_TYPE_F16 ? launch_type<MI355X_TYPE_F16>(ctx, a, head_dim)
+                                   : launch_type<MI355X_TYPE_BF16>(ctx, a, head_dim);
+}
+
+}  // namespace mi355x
