@@ -77,6 +77,109 @@ __device__ __forceinline__ TO *out_head(const RopeArgs &a, int64_t row, int whic
            h * a.head_stride;
 }
 
+// Eight values of a head per lane (four pairs of the rotated part, or eight
+// values behind it), LANES lanes per head: head_dim and rot_dim are multiples of
+// 8 and rows, strides and pages of 16 bytes.  A lane's place within the head is
+// the same for every head that it takes, so it forms its sines and cosines once
+// per row, and every lane's loads are two of 8 or 16 bytes.
+template <int TYPE>
+struct Four {
+    typedef typename Elem<TYPE>::T V __attribute__((ext_vector_type(4)));
+};
+typedef float f32x4_r __attribute__((ext_vector_type(4)));
+
+template <int IN, int OUT, bool PAIRS, int LANES>
+__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int heads, int rows_per_group) {
+    typedef typename Elem<IN>::T TI;
+    typedef typename Elem<OUT>::T TO;
+    typedef typename Four<IN>::V VI;
+    typedef typename Four<OUT>::V VO;
+    constexpr int kHeadsAtOnce = 256 / LANES;
+    const int u = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+    const int hd = a.head_dim, rot = a.rot_dim;
+    const bool on = 8 * u < hd, turned = 8 * u < rot;
+    // the lane's two runs of four values
+    const int i0 = !on ? 0 : turned && !PAIRS ? 4 * u : 8 * u;
+    const int i1 = !on ? 4 : turned && !PAIRS ? rot / 2 + 4 * u : 8 * u + 4;
+    const int first_head = blockIdx.y * kHeadsAtOnce, step = gridDim.y * kHeadsAtOnce;
+    f32x4_r freq = {0, 0, 0, 0};
+    if (turned) freq = *reinterpret_cast<const f32x4_r *>(a.inv_freq + 4 * u);
+    const int64_t row_end = min(a.n_rows, (static_cast<int64_t>(blockIdx.x) + 1) * rows_per_group);
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_group; row < row_end; ++row) {
+        float c[4], s[4];
+        if (turned) {
+            const int32_t pos = a.positions[row];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) turn(pos, freq[i], &c[i], &s[i]);
+        }
+        for (int hh = first_head + slot; hh < heads; hh += step) {
+            const int which = hh < a.n_heads ? 0 : hh < a.n_heads + a.n_kv_heads ? 1 : 2;
+            const int h = hh - (which == 0 ? 0 : which == 1 ? a.n_heads : a.n_heads + a.n_kv_heads);
+            const TI *src = static_cast<const TI *>(which == 0 ? a.in[0] : which == 1 ? a.in[1] : a.in[2]) +
+                            row * (which == 0 ? a.in_stride[0] : which == 1 ? a.in_stride[1] : a.in_stride[2]) +
+                            static_cast<int64_t>(h) * hd;
+            const float *bias = which == 0 ? a.bias[0] : which == 1 ? a.bias[1] : a.bias[2];
+            const float *norm = which == 0 ? a.norm[0] : which == 1 ? a.norm[1] : nullptr;
+            const int j0 = which == 2 ? 8 * u : i0, j1 = which == 2 ? 8 * u + 4 : i1;
+            float x[8];
+            if (on) {
+                const VI p = *reinterpret_cast<const VI *>(src + j0), q = *reinterpret_cast<const VI *>(src + j1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = Elem<IN>::up(p[i]);
+                    x[4 + i] = Elem<IN>::up(q[i]);
+                }
+                if (bias) {
+                    const float *b = bias + static_cast<int64_t>(h) * hd;
+                    const f32x4_r p1 = *reinterpret_cast<const f32x4_r *>(b + j0),
+                                  q1 = *reinterpret_cast<const f32x4_r *>(b + j1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[i] += p1[i];
+                        x[4 + i] += q1[i];
+                    }
+                }
+            }
+            if (norm) {  // the same for all lanes of a head
+                float ss = 0.0f;
+                if (on)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+                const float scale = 1.0f / sqrtf(group_sum(ss, LANES) / static_cast<float>(hd) + a.eps);
+                if (on) {
+                    const f32x4_r p1 = *reinterpret_cast<const f32x4_r *>(norm + j0),
+                                  q1 = *reinterpret_cast<const f32x4_r *>(norm + j1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[i] = x[i] * scale * p1[i];
+                        x[4 + i] = x[4 + i] * scale * q1[i];
+                    }
+                }
+            }
+            if (turned && which != 2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int m = PAIRS ? 2 * i : i, n = PAIRS ? 2 * i + 1 : 4 + i;
+                    const float v = x[m], w = x[n];
+                    x[m] = v * c[i] - w * s[i];
+                    x[n] = w * c[i] + v * s[i];
+                }
+            }
+            TO *dst = on ? out_head<TO>(a, row, which, h) : nullptr;
+            if (dst) {
+                VO p, q;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[i] = Elem<OUT>::down(x[i]);
+                    q[i] = Elem<OUT>::down(x[4 + i]);
+                }
+                *reinterpret_cast<VO *>(dst + j0) = p;
+                *reinterpret_cast<VO *>(dst + j1) = q;
+            }
+        }
+    }
+}
+
 // Any sizes and alignments: one wavefront per row and head, value by value.
 template <int IN, int OUT, bool PAIRS>
 __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int heads, int64_t items) {
@@ -117,30 +220,63 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int heads, in
     for (int i = rot + lane; i < hd; i += 64) dst[i] = Elem<OUT>::down(normed(i));
 }
 
-template <int IN, int OUT>
-int launch_rope(mi355x_ctx *ctx, const RopeArgs &a, bool pairs) {
+template <int IN, int OUT, bool PAIRS, int LANES>
+int launch_rope_lanes(mi355x_ctx *ctx, const RopeArgs &a) {
     const int heads = a.n_heads + (a.slots ? 2 : 1) * a.n_kv_heads;
-    const int64_t items = a.n_rows * heads;
-    // HIP takes up to 2^32 - 1 threads of a launch in x
-    constexpr int64_t kMostItems = int64_t(1) << 25;
+    const int64_t at_once = 256 / LANES, passes = (heads + at_once - 1) / at_once;
+    // few rows: a workgroup per row and pass over its heads; many: one per row
+    const int64_t split = std::max<int64_t>(1, std::min<int64_t>(passes, 4 * ctx->num_cus / std::max<int64_t>(1, a.n_rows)));
+    constexpr int64_t kMostGroups = int64_t(1) << 22;
+    const int rows_per_group = static_cast<int>((a.n_rows + kMostGroups - 1) / kMostGroups);
+    const dim3 grid(static_cast<unsigned>((a.n_rows + rows_per_group - 1) / rows_per_group), static_cast<unsigned>(split));
+    rope_kernel<IN, OUT, PAIRS, LANES><<<grid, 256, 0, ctx->stream>>>(a, heads, rows_per_group);
+    MI355X_HIP(hipGetLastError());
+    return MI355X_OK;
+}
+
+template <int IN, int OUT, bool PAIRS>
+int launch_rope_any(mi355x_ctx *ctx, const RopeArgs &a) {
+    const int heads = a.n_heads + (a.slots ? 2 : 1) * a.n_kv_heads;
+    constexpr int64_t kMostItems = int64_t(1) << 25;  // wavefronts of a launch
     for (int64_t row = 0; row < a.n_rows;) {
         const int64_t rows = std::min(a.n_rows - row, std::max<int64_t>(1, kMostItems / heads));
         RopeArgs b = a;
-        b.n_rows = rows;
         for (int i = 0; i < 3; ++i)
             if (b.in[i]) b.in[i] = static_cast<const typename Elem<IN>::T *>(a.in[i]) + row * a.in_stride[i];
         b.q_out = static_cast<typename Elem<OUT>::T *>(a.q_out) + row * a.q_out_stride;
         if (a.positions) b.positions = a.positions + row;
         if (a.slots) b.slots = a.slots + row;
         else b.k_dst = static_cast<typename Elem<OUT>::T *>(a.k_dst) + row * a.k_row_stride;
-        const unsigned grid = static_cast<unsigned>((rows * heads + 3) / 4);
-        if (pairs) rope_any_kernel<IN, OUT, true><<<grid, 256, 0, ctx->stream>>>(b, heads, rows * heads);
-        else rope_any_kernel<IN, OUT, false><<<grid, 256, 0, ctx->stream>>>(b, heads, rows * heads);
+        rope_any_kernel<IN, OUT, PAIRS>
+            <<<static_cast<unsigned>((rows * heads + 3) / 4), 256, 0, ctx->stream>>>(b, heads, rows * heads);
         MI355X_HIP(hipGetLastError());
         row += rows;
     }
-    (void)items;
     return MI355X_OK;
+}
+
+bool whole_chunks(const void *p, int64_t stride, int64_t bytes) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * bytes % 16 == 0;
+}
+
+template <int IN, int OUT, bool PAIRS>
+int launch_rope_pairs(mi355x_ctx *ctx, const RopeArgs &a) {
+    constexpr int64_t ib = sizeof(typename Elem<IN>::T), ob = sizeof(typename Elem<OUT>::T);
+    bool fast = a.head_dim % 8 == 0 && a.rot_dim % 8 == 0 && a.head_dim <= 512 &&
+                whole_chunks(a.q_out, a.q_out_stride, ob) && whole_chunks(a.inv_freq, 0, 4);
+    for (int i = 0; i < 3; ++i) fast = fast && whole_chunks(a.in[i], a.in_stride[i], ib) && whole_chunks(a.bias[i], 0, 4);
+    for (int i = 0; i < 2; ++i) fast = fast && whole_chunks(a.norm[i], 0, 4);
+    if (!a.slots) fast = fast && whole_chunks(a.k_dst, a.k_row_stride, ob);
+    if (!fast) return launch_rope_any<IN, OUT, PAIRS>(ctx, a);
+    if (a.head_dim <= 64) return launch_rope_lanes<IN, OUT, PAIRS, 8>(ctx, a);
+    if (a.head_dim <= 128) return launch_rope_lanes<IN, OUT, PAIRS, 16>(ctx, a);
+    if (a.head_dim <= 256) return launch_rope_lanes<IN, OUT, PAIRS, 32>(ctx, a);
+    return launch_rope_lanes<IN, OUT, PAIRS, 64>(ctx, a);
+}
+
+template <int IN, int OUT>
+int launch_rope(mi355x_ctx *ctx, const RopeArgs &a, bool pairs) {
+    return pairs ? launch_rope_pairs<IN, OUT, true>(ctx, a) : launch_rope_pairs<IN, OUT, false>(ctx, a);
 }
 
 template <int OUT>
