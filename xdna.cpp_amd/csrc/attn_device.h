@@ -21,7 +21,8 @@ struct AttnArgs {
     int64_t n_rows;
     int64_t reach;      // tokens that the table's columns hold
     int row_limit;      // requests of at most (token form) or more than (chunk form) so many head rows
-    float scale, softcap;
+    float scale2;            // scale log2 e: scores are in factors of 2
+    float cap_in, cap_out;   // 2 scale log2 e / softcap and softcap log2 e; 0: no cap
     FastDiv group;  // query heads of a KV head
     int n_seqs, n_kv_heads;
     int n_pages, shift, window, causal, f32_out;
@@ -78,18 +79,37 @@ __device__ __forceinline__ bool not_finite(u32x4_a v) {
 // Four rows of one column each from a 4-row x 16-column block of 16-bit values
 // per 16 lanes: lane c of the 16 passes the address of 4 values of row c / 4
 // from column 4 (c % 4) on, and gets column c of the four rows.
-__device__ __forceinline__ u32x2_a lds_read_transposed(const void *p) {
-    return __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                           (__attribute__((address_space(3))) s16x4 *)(p)));
+// __restrict__ keeps the compiler from taking every LDS load that is on its way
+// (global_load_lds) for a write to the same place, and waiting for it: the
+// kernels' barriers order those.
+__device__ __forceinline__ u32x2_a lds_read_transposed(const s16x4 *__restrict__ p) {
+    return __builtin_bit_cast(
+        u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p)));
 }
 
-// A score in units of ln 2 from q . k; tanh as 1 - 2 / (1 + e^2x), within
-// 2^-23 of 1.
+// A score from q . k; tanh x as 1 - 2 / (1 + e^2x), within 2^-23 of 1.
 __device__ __forceinline__ float score2(float dot, const AttnArgs &a) {
-    if (!(a.softcap > 0.0f)) return dot * (a.scale * kLog2e);
-    const float x = dot * (a.scale / a.softcap);
-    const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * (2.0f * kLog2e)));
-    return a.softcap * kLog2e * t;
+    if (a.cap_out == 0.0f) return dot * a.scale2;
+    return fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(dot * a.cap_in)), a.cap_out);
+}
+
+// Maximum and sum over a lane and the one 32 lanes on.
+__device__ __forceinline__ void both_halves(float v, float *a, float *b) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+    const uint32_t x = r[0], y = r[1];
+    *a = __builtin_bit_cast(float, x);
+    *b = __builtin_bit_cast(float, y);
+}
+__device__ __forceinline__ float half_max(float v) {
+    float a, b;
+    both_halves(v, &a, &b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float v) {
+    float a, b;
+    both_halves(v, &a, &b);
+    return a + b;
 }
 
 __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.0f : m; }

@@ -110,7 +110,7 @@ struct TokenShape {
 };
 
 template <int TYPE, int HD, int MT>
-__global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 ? 2 : 1) void attention_token_kernel(AttnArgs a) {
     typedef Num<TYPE> N;
     typedef typename N::T T;
     typedef typename N::V8 V8;
@@ -121,6 +121,7 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
     constexpr int kVLoads = kTokenKeys * kChunks / 64;
     __shared__ __attribute__((aligned(16))) unsigned char lds[kTokenWaves * S::kWaveBytes];
     __shared__ float lds_m[kTokenWaves][16], lds_l[kTokenWaves][16];
+    __shared__ int lds_odd[kTokenWaves];
     __shared__ int64_t tmp[kTokenWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, quad = lane >> 4;
@@ -151,7 +152,8 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
         // tokens that some row of the block sees, and those that all of them see
         const KeyRange kf = token_keys(a, g, g.tok_lo + divided(row0, a.group));
         const KeyRange kl = token_keys(a, g, g.tok_lo + divided(row_last, a.group));
-        const int64_t some_lo = kf.lo, some_hi = kl.hi, all_lo = kl.lo, all_hi = kf.hi;
+        const int64_t all_lo = kl.lo, all_hi = kf.hi;
+        const bool whole = t0 == 0 && t1 == w.tiles;
 
         V8 qf[MT][kSteps];
         int row_lo[MT], row_hi[MT];
@@ -172,6 +174,23 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
                 qf[mt][st] = z;
             }
         }
+        const int32_t *table = a.table + seq * a.table_stride;
+        const T *kp = static_cast<const T *>(a.k) + kvh * a.head_stride + 8 * quad;
+        const T *vp = static_cast<const T *>(a.v) + kvh * a.head_stride;
+
+        // Tokens [some_lo, some_hi) are seen by some row; the others' values count as
+        // zero.  Where a value that only some of the rows see is not finite (a weight of
+        // zero would not take it away), the rows are done again one by one.
+        int64_t some_lo = kf.lo, some_hi = kl.hi;
+        bool odd = false;
+        for (int only = -1; only < S::kRows; ++only) {
+        if (only >= 0) {
+            if (!odd || row0 + only >= g.rows) break;
+            const KeyRange kr = token_keys(a, g, g.tok_lo + divided(row0 + only, a.group));
+            some_lo = kr.lo;
+            some_hi = kr.hi;
+        }
+        bool odd_lane = false;
         f32x4 o[MT][kBlocks];
         float m[MT], l[MT];
 #pragma unroll
@@ -182,7 +201,6 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
             for (int d = 0; d < kBlocks; ++d) o[mt][d] = f32x4{0, 0, 0, 0};
         }
 
-        const int32_t *table = a.table + seq * a.table_stride;
         u32x4_a kreg[2][kSteps], vreg[kVLoads];
         uint32_t seen = 0;  // keys of the tile in registers that lie on pages of the pool
         // the table entry of key (lane & 31) of a tile
@@ -193,20 +211,19 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
         auto load = [&](int64_t base, int32_t page) {
             const bool good = page_in_pool(page, a.n_pages);
             const int64_t key = base + (lane & 31);
-            const int64_t off = good ? page * a.page_stride + (key & ((int64_t(1) << a.shift) - 1)) * a.token_stride +
-                                           kvh * a.head_stride
+            const int64_t off = good ? page * a.page_stride + (key & ((int64_t(1) << a.shift) - 1)) * a.token_stride
                                      : 0;
             seen = static_cast<uint32_t>(__ballot(good));
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const T *k = static_cast<const T *>(a.k) + __shfl(off, 16 * b + col) + 8 * quad;
+                const T *k = kp + __shfl(off, 16 * b + col);
 #pragma unroll
                 for (int st = 0; st < kSteps; ++st) kreg[b][st] = *reinterpret_cast<const u32x4_a *>(k + 32 * st);
             }
 #pragma unroll
             for (int i = 0; i < kVLoads; ++i) {
                 const int idx = 64 * i + lane;
-                const T *v = static_cast<const T *>(a.v) + __shfl(off, idx / kChunks) + idx % kChunks * 8;
+                const T *v = vp + __shfl(off, idx / kChunks) + idx % kChunks * 8;
                 vreg[i] = *reinterpret_cast<const u32x4_a *>(v);
             }
         };
@@ -233,14 +250,13 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
                 }
             // every key of the tile seen by every row
             const bool full = base >= all_lo && base + kTokenKeys <= all_hi && now == 0xFFFFFFFFu;
-            bool odd = false;  // a value that a weight of zero would not take away
 #pragma unroll
             for (int i = 0; i < kVLoads; ++i) {
                 const int idx = 64 * i + lane, key = idx / kChunks;
                 u32x4_a v = vreg[i];
                 if (!full) {
                     if (!((now >> key) & 1)) v = u32x4_a{0, 0, 0, 0};
-                    odd |= not_finite<TYPE>(v);
+                    odd_lane |= not_finite<TYPE>(v);
                 }
                 *reinterpret_cast<u32x4_a *>(vt + key * S::kVStride + idx % kChunks * 8) = v;
             }
@@ -289,56 +305,22 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
             }
             auto vcolumn = [&](int d) {
                 const T *p = vt + (4 * quad + col / 4) * S::kVStride + 16 * d + col % 4 * 4;
-                const u32x2_a x = lds_read_transposed(p), y = lds_read_transposed(p + 16 * S::kVStride);
+                const u32x2_a x = lds_read_transposed(reinterpret_cast<const s16x4 *>(p)),
+                              y = lds_read_transposed(reinterpret_cast<const s16x4 *>(p + 16 * S::kVStride));
                 return u32x4_a{x[0], x[1], y[0], y[1]};
             };
-            if (!full && __any(odd)) {
-                // an infinity or NaN under weights of which some are zero because their row
-                // does not see it: row by row, with the values that the row sees
-                for (int r = 0; r < S::kRows; ++r) {
-                    const int mt = r / 16;
-                    uint32_t mask = 0;
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        if (t != mt) continue;
-                        const int64_t rl = __shfl(row_lo[t], r % 16) - base, rh = __shfl(row_hi[t], r % 16) - base;
-                        const int klo = static_cast<int>(idx_min(32, idx_max(0, rl)));
-                        const int khi = static_cast<int>(idx_min(32, idx_max(klo, rh)));
-                        mask = static_cast<uint32_t>((uint64_t(1) << khi) - (uint64_t(1) << klo));
-                    }
+            for (int d = 0; d < kBlocks; ++d) {
+                const V8 v = __builtin_bit_cast(V8, vcolumn(d));
 #pragma unroll
-                    for (int d = 0; d < kBlocks; ++d) {
-                        u32x4_a v = vcolumn(d);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int k = 16 * (i / 2) + 4 * quad + 2 * (i % 2);
-                            if (!((mask >> k) & 1)) v[i] &= 0xFFFF0000u;
-                            if (!((mask >> (k + 1)) & 1)) v[i] &= 0x0000FFFFu;
-                        }
-#pragma unroll
-                        for (int t = 0; t < MT; ++t) {
-                            f32x4 c = N::mfma16(__builtin_bit_cast(V8, v), hi[t], f32x4{0, 0, 0, 0});
-                            c = N::mfma16(__builtin_bit_cast(V8, v), lo[t], c);
-                            if (t == mt && col == r % 16) o[t][d] += c;
-                            __builtin_amdgcn_sched_barrier(0);  // rare: in few registers
-                        }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    const V8 v = __builtin_bit_cast(V8, vcolumn(d));
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        o[mt][d] = N::mfma16(v, hi[mt], o[mt][d]);
-                        o[mt][d] = N::mfma16(v, lo[mt], o[mt][d]);
-                    }
+                for (int mt = 0; mt < MT; ++mt) {
+                    o[mt][d] = N::mfma16(v, hi[mt], o[mt][d]);
+                    o[mt][d] = N::mfma16(v, lo[mt], o[mt][d]);
                 }
             }
         }
 
         // join the wavefronts' sums, 16 rows at a time
-        const bool whole = t0 == 0 && t1 == w.tiles;
         float *part = a.ws + (2 * static_cast<int64_t>(blockIdx.x) + (u != u0)) * S::kPartFloats;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -349,14 +331,23 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
                 lds_m[wave][col] = m[mt];
                 lds_l[wave][col] = sum;
             }
+            if (mt == 0 && only < 0) {
+                const bool any = __any(odd_lane);
+                if (lane == 0) lds_odd[wave] = any;
+            }
 #pragma unroll
             for (int d = 0; d < kBlocks; ++d)
                 *reinterpret_cast<f32x4 *>(ot + col * S::kOStride + 16 * d + 4 * quad) = o[mt][d];
             __syncthreads();
-            for (int idx = tid; idx < 16 * (HD / 4); idx += kTokenThreads) {
+            if (mt == 0 && only < 0)
+                for (int wv = 0; wv < kTokenWaves; ++wv) odd |= lds_odd[wv] != 0;
+            int start = tid;
+            asm volatile("" : "+v"(start));  // the addresses below are formed here, not kept through the loops
+            for (int idx = start; idx < 16 * (HD / 4); idx += kTokenThreads) {
                 const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
                 const int row = row0 + 16 * mt + r;
                 if (row >= g.rows) break;
+                if (only >= 0 && row != row0 + only) continue;
                 float top = lds_m[0][r];
 #pragma unroll
                 for (int wv = 1; wv < kTokenWaves; ++wv) top = fmaxf(top, lds_m[wv][r]);
@@ -382,6 +373,7 @@ __global__ __launch_bounds__(kTokenThreads) void attention_token_kernel(AttnArgs
                 }
             }
             __syncthreads();
+        }
         }
         u += t1 - t0;
     }
@@ -520,8 +512,11 @@ int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &u
     a.n_rows = u.n_rows;
     // an empty pool has no address that may be read: no token is seen
     a.reach = u.pool->n_pages > 0 ? static_cast<int64_t>(u.table_cols) * u.pool->page_tokens : 0;
-    a.scale = u.scale;
-    a.softcap = u.softcap;
+    a.scale2 = u.scale * kLog2e;
+    if (u.softcap > 0.0f) {
+        a.cap_in = u.scale / u.softcap * (2.0f * kLog2e);
+        a.cap_out = u.softcap * kLog2e;
+    }
     a.n_seqs = u.n_seqs;
     a.n_kv_heads = u.pool->n_kv_heads;
     const int group = u.n_heads / u.pool->n_kv_heads;

@@ -71,8 +71,6 @@ __device__ __forceinline__ int find_block(const AttnArgs &a, int64_t j, int64_t 
     return lo;
 }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
-
 struct ChunkItem {
     int seq, kvh, row0;
     SeqGeo g;
@@ -141,218 +139,198 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
             qf[st] = z;
         }
     }
-    f32x16 o[kBlocks];
-#pragma unroll
-    for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-
-    const int32_t *table = a.table + it.seq * a.table_stride;
-    // the table entry of key `lane` of tile t
-    auto entry = [&](int t) {
-        const int64_t key = it.key_lo + static_cast<int64_t>(t) * kChunkKeys + lane;
-        return t < t1 && key >= it.first.lo && key < it.last.hi ? table[key >> a.shift] : -1;
-    };
-    uint64_t seen_next = 0;  // keys of the tile on its way that lie on pages of the pool
-    auto load = [&](int t, int32_t page, int buf) {
-        const bool good = page_in_pool(page, a.n_pages);
-        seen_next = __ballot(good);
-        const int64_t key = it.key_lo + static_cast<int64_t>(t) * kChunkKeys + lane;
-        const int64_t off = good ? page * a.page_stride + (key & ((int64_t(1) << a.shift) - 1)) * a.token_stride +
-                                       kvh * a.head_stride
-                                 : 0;
-#pragma unroll
-        for (int i = 0; i < S::kLoads; ++i) {
-            const int at = (i * kChunkWaves + wave) * 64;  // this instruction's first place
-            const int r = (at + lane) / S::kPlaces, place = (at + lane) % S::kPlaces;
-            const int64_t from = __shfl(off, r);
-            int ck = place ^ k_turn(r), cv = place ^ v_turn(r);
-            if (HD == 96) {  // places without a chunk take another's
-                ck = ck < S::kChunks ? ck : ck - 4;
-                cv = cv < S::kChunks ? cv : cv - 4;
-            }
-            const T *k = static_cast<const T *>(a.k) + from + 8 * ck;
-            const T *v = static_cast<const T *>(a.v) + from + 8 * cv;
-            unsigned char *to = lds + 2 * buf * S::kTileBytes + 16 * at;
-            __builtin_amdgcn_global_load_lds(
-                reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(reinterpret_cast<uintptr_t>(k)),
-                (__attribute__((address_space(3))) uint32_t *)(to), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds(
-                reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(reinterpret_cast<uintptr_t>(v)),
-                (__attribute__((address_space(3))) uint32_t *)(to + S::kTileBytes), 16, 0, 0);
-        }
-    };
-    // where this lane reads: K row col (+ 32), chunk 2 st + half; V rows 4 half +
-    // (lane % 16) / 4 (+ 8 ..), chunk 4 d + 2 ((lane / 16) % 2) + (lane % 4) / 2
+    // where this lane's loads come from: its chunk of a token's head (the row that
+    // it fills, modulo 8, is the same in all of its loads), and where it reads: K row
+    // col (+ 32), chunk 2 st + half; V rows 4 half + (lane % 16) / 4 (+ 8 ..), chunk
+    // 4 d + 2 ((lane / 16) % 2) + (lane % 4) / 2
+    const int fill_row = (wave * 64 + lane) / S::kPlaces;
+    static_assert(kChunkThreads / S::kPlaces % 8 == 0, "rows of one lane's loads, modulo 8");
+    int ck = lane % S::kPlaces ^ k_turn(fill_row), cv = lane % S::kPlaces ^ v_turn(fill_row);
+    if (HD == 96) {  // places without a chunk take another's
+        ck = ck < S::kChunks ? ck : ck - 4;
+        cv = cv < S::kChunks ? cv : cv - 4;
+    }
+    const T *kp = static_cast<const T *>(a.k) + kvh * a.head_stride + 8 * ck;
+    const T *vp = static_cast<const T *>(a.v) + kvh * a.head_stride + 8 * cv;
     const int k_at = col * S::kRowBytes;
     const int k_low = half ^ k_turn(col);
     const int v_row = 4 * half + ((lane & 15) >> 2);
     const int v_at = v_row * S::kRowBytes + (lane & 1) * 8;
     const int v_low = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_turn(v_row);
+    const int32_t *table = a.table + it.seq * a.table_stride;
+    const float c = a.scale2;
 
-    int32_t next = -1;
-    if (t0 < t1) {
-        load(t0, entry(t0), 0);
-        next = entry(t0 + 1);
-    }
-    const float c = a.scale * kLog2e;
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        const uint64_t seen = seen_next;
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this tile's loads
-        __syncthreads();                     // everyone's, and the other buffer is read
-        if (t + 1 < t1) {
-            load(t + 1, next, buf ^ 1);
-            next = entry(t + 2);
-        }
-        unsigned char *kt = lds + 2 * buf * S::kTileBytes, *vt = kt + S::kTileBytes;
-        const int64_t base = it.key_lo + static_cast<int64_t>(t) * kChunkKeys;
-        // every key of the tile seen by every row of the workgroup
-        const bool full = base >= it.last.lo && base + kChunkKeys <= it.first.hi && ~seen == 0;
-        bool by_row = false;
-        if (!full) {
-            // values that no row sees become zero; is any other one not finite?
-            if (tid == 0) odd = 0;
+    // Tokens [some_lo, some_hi) are seen by some row; the others' values count as
+    // zero.  Where a value that only some of the rows see is not finite (a weight of
+    // zero would not take it away), the rows are done again one by one.
+    int64_t some_lo = it.first.lo, some_hi = it.last.hi;
+    if (tid == 0) odd = 0;
+    for (int only = -1; only < kChunkRows; ++only) {
+        if (only >= 0) {
             __syncthreads();
-            bool bad = false;
-            for (int i = tid; i < kChunkKeys * S::kPlaces; i += kChunkThreads) {
-                u32x4_a *p = reinterpret_cast<u32x4_a *>(vt + 16 * i);
-                if (!((seen >> (i / S::kPlaces)) & 1)) *p = u32x4_a{0, 0, 0, 0};
-                else bad |= not_finite<TYPE>(*p);
-            }
-            if (__any(bad) && lane == 0) odd = 1;
-            __syncthreads();
-            by_row = odd != 0;
+            if (odd == 0 || it.row0 + only >= g.rows) break;
+            const KeyRange kr = token_keys(a, g, g.tok_lo + divided(it.row0 + only, a.group));
+            some_lo = kr.lo;
+            some_hi = kr.hi;
         }
-        f32x16 s[2];
+        f32x16 o[kBlocks];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
-#pragma unroll
-            for (int st = 0; st < kSteps; ++st) {
-                const int place = ((2 * (st & 3)) ^ k_low) + 8 * (st >> 2);
-                const V8 k = *reinterpret_cast<const V8 *>(kt + k_at + 32 * kb * S::kRowBytes + 16 * place);
-                s[kb] = N::mfma32(k, qf[st], s[kb]);
-            }
-        }
-        float top = -INFINITY;
-        if (CAP) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[kb][i] = score2(s[kb][i], a);
-        }
-        if (!full) {
-            const int lo = static_cast<int>(idx_max(row_lo - base, 0)), hi = static_cast<int>(idx_min(row_hi - base, 64));
-            uint64_t mine = seen;
-            mine = hi <= 0 || lo >= 64 ? 0 : mine & (hi >= 64 ? ~uint64_t(0) : (uint64_t(1) << hi) - 1) & ~((uint64_t(1) << lo) - 1);
-            mine >>= 4 * half;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!((mine >> (32 * kb + 8 * (i >> 2) + (i & 3))) & 1)) s[kb][i] = -INFINITY;
-        }
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
-        top = fmaxf(top, other_half(top));
-        if (!CAP) top *= c;  // c >= 0 here; 0 x infinity gives NaN, which no maximum takes
-        const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
-        if (__any(grows)) {
-            const float m_new = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
-            l *= keep;
-#pragma unroll
-            for (int d = 0; d < kBlocks; ++d) o[d] *= keep;
-            m = m_new;
-        }
-        const float ref = finite_base(m);
-        V8 hi[4], lo[PLANES == 2 ? 4 : 1];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = s[j >> 1][8 * (j & 1) + i];
-                const float p = __builtin_amdgcn_exp2f(CAP ? x - ref : fmaf(x, c, -ref));
-                l += p;
-                const T h = static_cast<T>(p);
-                hi[j][i] = h;
-                if (PLANES == 2) lo[j][i] = static_cast<T>(p - static_cast<float>(h));
-            }
-        auto v_chunk = [&](int j, int d) {  // keys 16 j + {4 half .. + 3, 8 + 4 half .. + 3} of 32 values
-            const int place = ((4 * (d & 1)) ^ v_low) + 8 * (d >> 1);
-            const unsigned char *p = vt + v_at + 16 * j * S::kRowBytes + 16 * place;
-            const u32x2_a x = lds_read_transposed(p), y = lds_read_transposed(p + 8 * S::kRowBytes);
-            return u32x4_a{x[0], x[1], y[0], y[1]};
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+        // the table entry of key `lane` of tile t
+        auto entry = [&](int t) {
+            const int64_t key = it.key_lo + static_cast<int64_t>(t) * kChunkKeys + lane;
+            return t < t1 && key >= some_lo && key < some_hi ? table[key >> a.shift] : -1;
         };
-        if (by_row) {
-            // an infinity or NaN under weights of which some are zero because their row
-            // does not see it: row by row, with the values that the row sees
-            for (int r = 0; r < 32; ++r) {
-                const int64_t rl = __shfl(row_lo, r) - base, rh = __shfl(row_hi, r) - base;
-                const int klo = static_cast<int>(idx_min(64, idx_max(0, rl))), khi = static_cast<int>(idx_min(64, idx_max(0, rh)));
-                uint64_t mask = khi <= klo ? 0 : (khi >= 64 ? ~uint64_t(0) : (uint64_t(1) << khi) - 1) & ~((uint64_t(1) << klo) - 1);
-                mask >>= 4 * half;
+        uint64_t seen_next = 0;  // keys of the tile on its way that lie on pages of the pool
+        auto load = [&](int t, int32_t page, int buf) {
+            const bool good = page_in_pool(page, a.n_pages);
+            seen_next = __ballot(good);
+            const int64_t key = it.key_lo + static_cast<int64_t>(t) * kChunkKeys + lane;
+            const int64_t off =
+                good ? page * a.page_stride + (key & ((int64_t(1) << a.shift) - 1)) * a.token_stride : 0;
+            unsigned char *to = lds + 2 * buf * S::kTileBytes + 1024 * wave;
 #pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    f32x16 x;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        u32x4_a v = v_chunk(j, d);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int k = 16 * j + 8 * (i >> 1) + 2 * (i & 1);
-                            if (!((mask >> k) & 1)) v[i] &= 0xFFFF0000u;
-                            if (!((mask >> (k + 1)) & 1)) v[i] &= 0x0000FFFFu;
-                        }
-                        x = N::mfma32(__builtin_bit_cast(V8, v), hi[j], x);
-                        if (PLANES == 2) x = N::mfma32(__builtin_bit_cast(V8, v), lo[PLANES == 2 ? j : 0], x);
-                        __builtin_amdgcn_sched_barrier(0);  // rare: in few registers
-                    }
-                    if (col == r) o[d] += x;
-                }
+            for (int i = 0; i < S::kLoads; ++i) {
+                const int64_t from = __shfl(off, fill_row + i * (kChunkThreads / S::kPlaces));
+                __builtin_amdgcn_global_load_lds(
+                    reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(
+                        reinterpret_cast<uintptr_t>(kp + from)),
+                    (__attribute__((address_space(3))) uint32_t *)(to + 16 * kChunkThreads * i), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds(
+                    reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(
+                        reinterpret_cast<uintptr_t>(vp + from)),
+                    (__attribute__((address_space(3))) uint32_t *)(to + S::kTileBytes + 16 * kChunkThreads * i), 16,
+                    0, 0);
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    const V8 v = __builtin_bit_cast(V8, v_chunk(j, d));
-                    o[d] = N::mfma32(v, hi[j], o[d]);
-                    if (PLANES == 2) o[d] = N::mfma32(v, lo[PLANES == 2 ? j : 0], o[d]);
-                }
+        };
+        int32_t next = -1;
+        if (t0 < t1) {
+            load(t0, entry(t0), 0);
+            next = entry(t0 + 1);
         }
-    }
-
-    l += other_half(l);
-    if (!real) return;
-    if (a.split == 1) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int64_t at = (g.first + g.tok_lo + tok) * a.out_stride + head * HD;
-#pragma unroll
-        for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f32x4 v = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-                store_out4<TYPE>(a, at + 32 * d + 8 * i + 4 * half, l == 0.0f ? f32x4{0, 0, 0, 0} : v * inv);
+        for (int t = t0; t < t1; ++t) {
+            const int buf = (t - t0) & 1;
+            const uint64_t seen = seen_next;
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this tile's loads
+            __syncthreads();                     // everyone's, and the other buffer is read
+            if (t + 1 < t1) {
+                load(t + 1, next, buf ^ 1);
+                next = entry(t + 2);
             }
-    } else {
-        float *w = a.ws + static_cast<int64_t>(blockIdx.x) * S::kPartFloats;
-        const int r = 32 * wave + col;
+            unsigned char *kt = lds + 2 * buf * S::kTileBytes, *vt = kt + S::kTileBytes;
+            const int64_t base = it.key_lo + static_cast<int64_t>(t) * kChunkKeys;
+            // every key of the tile seen by every row of the workgroup
+            const bool full = base >= it.last.lo && base + kChunkKeys <= it.first.hi && ~seen == 0;
+            if (!full) {
+                bool bad = false;
+                for (int i = tid; i < kChunkKeys * S::kPlaces; i += kChunkThreads) {
+                    u32x4_a *p = reinterpret_cast<u32x4_a *>(vt + 16 * i);
+                    if (!((seen >> (i / S::kPlaces)) & 1)) *p = u32x4_a{0, 0, 0, 0};
+                    else bad |= not_finite<TYPE>(*p);
+                }
+                if (__any(bad) && lane == 0) odd = 1;
+                __syncthreads();
+            }
+            f32x16 s[2];
 #pragma unroll
-        for (int d = 0; d < kBlocks; ++d)
+            for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<f32x4 *>(w + r * HD + 32 * d + 8 * i + 4 * half) =
-                    f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-        if (half == 0) {
-            w[kChunkRows * HD + r] = m;
-            w[kChunkRows * (HD + 1) + r] = l;
+                for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+#pragma unroll
+                for (int st = 0; st < kSteps; ++st) {
+                    const int place = ((2 * (st & 3)) ^ k_low) + 8 * (st >> 2);
+                    const V8 k = *reinterpret_cast<const V8 *>(kt + k_at + 32 * kb * S::kRowBytes + 16 * place);
+                    s[kb] = N::mfma32(k, qf[st], s[kb]);
+                }
+            }
+            if (CAP) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[kb][i] = score2(s[kb][i], a);
+            }
+            if (!full) {
+                const int lo = static_cast<int>(idx_max(row_lo - base, 0));
+                const int hi = static_cast<int>(idx_min(row_hi - base, 64));
+                uint64_t mine = 0;
+                if (hi > lo) mine = seen & (~uint64_t(0) >> (64 - hi)) & ~((uint64_t(1) << lo) - 1);
+                mine >>= 4 * half;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!((mine >> (32 * kb + 8 * (i >> 2) + (i & 3))) & 1)) s[kb][i] = -INFINITY;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+            top = half_max(top);
+            if (!CAP) top *= c;  // c >= 0 here; 0 x infinity gives NaN, which no maximum takes
+            const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
+            if (__any(grows)) {
+                const float m_new = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
+                l *= keep;
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) o[d] *= keep;
+                m = m_new;
+            }
+            const float ref = finite_base(m);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                V8 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = s[j >> 1][8 * (j & 1) + i];
+                    const float p = __builtin_amdgcn_exp2f(CAP ? x - ref : fmaf(x, c, -ref));
+                    l += p;
+                    const T h = static_cast<T>(p);
+                    hi[i] = h;
+                    if (PLANES == 2) lo[i] = static_cast<T>(p - static_cast<float>(h));
+                }
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    // keys 16 j + {4 half .. + 3, 8 + 4 half .. + 3} of 32 values
+                    const int place = ((4 * (d & 1)) ^ v_low) + 8 * (d >> 1);
+                    const s16x4 *p = reinterpret_cast<const s16x4 *>(vt + v_at + 16 * j * S::kRowBytes + 16 * place);
+                    const u32x2_a x = lds_read_transposed(p), y = lds_read_transposed(p + S::kRowBytes);
+                    const V8 v = __builtin_bit_cast(V8, u32x4_a{x[0], x[1], y[0], y[1]});
+                    o[d] = N::mfma32(v, hi, o[d]);
+                    if (PLANES == 2) o[d] = N::mfma32(v, lo, o[d]);
+                }
+            }
+        }
+
+        l = half_sum(l);
+        int r = 32 * wave + col;
+        if (!real || (only >= 0 && r != only)) continue;
+        asm volatile("" : "+v"(r));  // the addresses below are formed here, not kept through the loops
+        if (a.split == 1) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t at = out_at(a, g, kvh, it.row0 + r, HD);
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 v = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                    store_out4<TYPE>(a, at + 32 * d + 8 * i + 4 * half, l == 0.0f ? f32x4{0, 0, 0, 0} : v * inv);
+                }
+        } else {
+            float *w = a.ws + static_cast<int64_t>(blockIdx.x) * S::kPartFloats;
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4 *>(w + r * HD + 32 * d + 8 * i + 4 * half) =
+                        f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+            if (half == 0) {
+                w[kChunkRows * HD + r] = m;
+                w[kChunkRows * (HD + 1) + r] = l;
+            }
         }
     }
 }
@@ -413,7 +391,7 @@ int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
 template <int TYPE, int HD>
 int launch_size(mi355x_ctx *ctx, const AttnArgs &a) {
     // the common path scales the maximum instead of each score, for which the scale has to be positive
-    const bool cap = a.softcap > 0.0f || a.scale < 0.0f;
+    const bool cap = a.cap_out > 0.0f || a.scale2 < 0.0f;
     if (a.f32_out) return cap ? launch_chunk<TYPE, HD, true, 2>(ctx, a) : launch_chunk<TYPE, HD, false, 2>(ctx, a);
     return cap ? launch_chunk<TYPE, HD, true, 1>(ctx, a) : launch_chunk<TYPE, HD, false, 1>(ctx, a);
 }
