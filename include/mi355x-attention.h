@@ -40,7 +40,8 @@ extern "C" {
  *   k + p * page_stride + (t % page_tokens) * token_stride + h * head_stride
  * (strides in values) for head h, head_dim values side by side; so do the
  * values, from v.  [page][token][head] and [page][head][token] are both
- * strides of this kind.  k, v: 16-byte aligned; strides: multiples of 8. */
+ * strides of this kind.  k, v: 16-byte aligned; strides: multiples of 8, at most
+ * 2^31. */
 typedef struct mi355x_kv_pool {
     int type;        /* MI355X_TYPE_F16 or MI355X_TYPE_BF16 */
     int n_kv_heads;
@@ -178,7 +179,7 @@ typedef struct mi355x_paged_attention_args {
     const int32_t *row_offsets; /* n_seqs + 1 */
     const int32_t *kv_lens;     /* n_seqs */
     const int32_t *block_table;
-    int table_cols;
+    int table_cols;           /* times page_tokens at most 2^30 */
     int64_t table_stride;
     float scale;
     float softcap;            /* 0: none */

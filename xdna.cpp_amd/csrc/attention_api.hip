@@ -42,7 +42,7 @@ int check_pool(const char *who, const mi355x_kv_pool *p) {
         return invalid(who, "n_pages must be 0 to 2^31 - 1 (got " + std::to_string(p->n_pages) + ")");
     if (p->n_pages > 0 && (!p->k || !p->v)) return invalid(who, "null pool");
     if (!aligned(p->k, 16) || !aligned(p->v, 16)) return invalid(who, "the pool must be 16-byte aligned");
-    constexpr int64_t kMostStride = int64_t(1) << 31;
+    constexpr int64_t kMostStride = int64_t(1) << 31;  // the kernels form products of 32-bit numbers
     for (int64_t s : {p->page_stride, p->token_stride, p->head_stride})
         if (s < 0 || s % 8 != 0 || s > kMostStride)
             return invalid(who, "pool strides must be multiples of 8 values, 0 to 2^31 (got " + std::to_string(s) + ")");
@@ -205,8 +205,8 @@ int mi355x_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args *a
         (a.n_seqs > 1 && a.table_stride < a.table_cols))
         return invalid(who, "table_stride must be at least table_cols and at most 2^31 - 1 (got " +
                                 std::to_string(a.table_stride) + ")");
-    if (static_cast<int64_t>(a.table_cols) * a.pool->page_tokens > INT32_MAX)
-        return invalid(who, "table_cols pages must hold fewer than 2^31 tokens");
+    if (static_cast<int64_t>(a.table_cols) * a.pool->page_tokens > (1 << 30))
+        return invalid(who, "table_cols pages must hold at most 2^30 tokens");
     if (a.window < 0) return invalid(who, "negative window");
     if (!std::isfinite(a.scale)) return invalid(who, "scale must be finite");
     if (!(a.softcap >= 0.0f) || std::isinf(a.softcap)) return invalid(who, "softcap must be finite and not negative");

@@ -17,9 +17,10 @@ struct AttnArgs {
     void *out;
     float *ws;
     int64_t q_stride, out_stride, table_stride;
-    int64_t page_stride, token_stride, head_stride;
+    int64_t head_stride;
     int64_t n_rows;
-    int64_t reach;      // tokens that the table's columns hold
+    uint32_t page_stride, token_stride;
+    int reach;          // tokens that the table's columns hold, at most 2^30
     int row_limit;      // requests of at most (token form) or more than (chunk form) so many head rows
     float scale2;            // scale log2 e: scores are in factors of 2
     float cap_in, cap_out;   // 2 scale log2 e / softcap and softcap log2 e; 0: no cap
@@ -87,10 +88,18 @@ __device__ __forceinline__ u32x2_a lds_read_transposed(const s16x4 *__restrict__
         u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p)));
 }
 
-// A score from q . k; tanh x as 1 - 2 / (1 + e^2x), within 2^-23 of 1.
-__device__ __forceinline__ float score2(float dot, const AttnArgs &a) {
-    if (a.cap_out == 0.0f) return dot * a.scale2;
-    return fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(dot * a.cap_in)), a.cap_out);
+// Scores of n values of q . k; tanh x as 1 - 2 / (1 + e^2x), within 2^-23 of 1.
+template <int N>
+__device__ __forceinline__ void scores2(float (&x)[N], const AttnArgs &a) {
+    if (a.cap_out == 0.0f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] *= a.scale2;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            x[i] = fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i] * a.cap_in)),
+                        a.cap_out);
+    }
 }
 
 // Maximum and sum over a lane and the one 32 lanes on.
@@ -111,6 +120,29 @@ __device__ __forceinline__ float half_sum(float v) {
     both_halves(v, &a, &b);
     return a + b;
 }
+
+// Maximum and sum over the four lanes with the same number modulo 16.
+__device__ __forceinline__ void both_rows(float v, float *a, float *b) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+    const uint32_t x = r[0], y = r[1];
+    *a = __builtin_bit_cast(float, x);
+    *b = __builtin_bit_cast(float, y);
+}
+__device__ __forceinline__ float quad_max(float v) {
+    float a, b;
+    both_rows(v, &a, &b);
+    return half_max(fmaxf(a, b));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    float a, b;
+    both_rows(v, &a, &b);
+    return half_sum(a + b);
+}
+
+// A row's maximum may grow by this (in factors of 2) before its sums are
+// scaled: weights stay below 2^8, where 16-bit floats are as exact as below 1.
+constexpr float kSlack = 8.0f;
 
 __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.0f : m; }
 
@@ -136,8 +168,28 @@ __device__ __forceinline__ SeqGeo seq_geo(const AttnArgs &a, int s) {
     return g;
 }
 
-__device__ __forceinline__ KeyRange token_keys(const AttnArgs &a, const SeqGeo &g, int64_t token) {
-    return visible_keys(g.pos0 + token, g.kv, a.reach, a.window, a.causal != 0);
+// Tokens lo .. hi - 1 (at most 2^30) that a token of the request sees.
+struct Keys {
+    int lo, hi;
+};
+__device__ __forceinline__ Keys token_keys(const AttnArgs &a, const SeqGeo &g, int64_t token) {
+    const KeyRange r = visible_keys(g.pos0 + token, g.kv, a.reach, a.window, a.causal != 0);
+    return Keys{static_cast<int>(r.lo), static_cast<int>(r.hi)};
+}
+
+// Where a token lies behind its KV head's first value; page in the pool.
+__device__ __forceinline__ int64_t token_at(const AttnArgs &a, int page, int key) {
+    const uint32_t in_page = static_cast<uint32_t>(key) & ((1u << a.shift) - 1);
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(page)) * a.page_stride +
+                                static_cast<uint64_t>(in_page) * a.token_stride);
+}
+
+// Which of the BITS keys from `base` on lie in [lo, hi), a bit each.
+template <typename MASK>
+__device__ __forceinline__ MASK range_mask(int lo, int hi, int base) {
+    constexpr int kBits = 8 * sizeof(MASK);
+    const int l = max(lo - base, 0), h = min(hi - base, kBits);
+    return h > l ? static_cast<MASK>(static_cast<MASK>(~MASK(0) >> (kBits - h)) & ~((MASK(1) << l) - 1)) : MASK(0);
 }
 
 // Four values of a row's output.

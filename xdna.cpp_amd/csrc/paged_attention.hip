@@ -36,18 +36,17 @@ constexpr int kTokenThreads = 64 * kTokenWaves;
 // The token form's units of a request: per KV head and block of ROWS head rows
 // one per kUnitKeys keys (one without keys: its rows get zeros).
 struct TokenWork {
-    int64_t units, key_lo;
-    int blocks, tiles;
+    int64_t units;
+    int blocks, tiles, key_lo;
 };
 
 template <int ROWS>
 __device__ __forceinline__ TokenWork token_work(const AttnArgs &a, const SeqGeo &g) {
-    TokenWork w{0, 0, 0, 1};
+    TokenWork w{0, 0, 1, 0};
     if (g.rows <= 0 || g.rows > a.row_limit) return w;
     w.blocks = (g.rows + ROWS - 1) / ROWS;
     w.key_lo = token_keys(a, g, g.tok_lo).lo;
-    const int64_t hi = token_keys(a, g, g.tok_lo + g.n_tok - 1).hi;
-    w.tiles = static_cast<int>(idx_max(1, (hi - w.key_lo + kUnitKeys - 1) / kUnitKeys));
+    w.tiles = max(1, (token_keys(a, g, g.tok_lo + g.n_tok - 1).hi - w.key_lo + kUnitKeys - 1) / kUnitKeys);
     w.units = static_cast<int64_t>(w.blocks) * w.tiles * a.n_kv_heads;
     return w;
 }
@@ -110,7 +109,7 @@ struct TokenShape {
 };
 
 template <int TYPE, int HD, int MT>
-__global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 ? 2 : 1) void attention_token_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD <= 128 ? 2 : 1) void attention_token_kernel(AttnArgs a) {
     typedef Num<TYPE> N;
     typedef typename N::T T;
     typedef typename N::V8 V8;
@@ -150,9 +149,9 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 
         const int row0 = static_cast<int>(item - static_cast<int64_t>(kvh) * w.blocks) * S::kRows;
         const int row_last = min(row0 + S::kRows, g.rows) - 1;
         // tokens that some row of the block sees, and those that all of them see
-        const KeyRange kf = token_keys(a, g, g.tok_lo + divided(row0, a.group));
-        const KeyRange kl = token_keys(a, g, g.tok_lo + divided(row_last, a.group));
-        const int64_t all_lo = kl.lo, all_hi = kf.hi;
+        const Keys kf = token_keys(a, g, g.tok_lo + divided(row0, a.group));
+        const Keys kl = token_keys(a, g, g.tok_lo + divided(row_last, a.group));
+        const int all_lo = kl.lo, all_hi = kf.hi;
         const bool whole = t0 == 0 && t1 == w.tiles;
 
         V8 qf[MT][kSteps];
@@ -162,9 +161,9 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 
             const bool real = row0 + 16 * mt + col < g.rows;
             const int row = real ? row0 + 16 * mt + col : 0, tok = divided(row, a.group);
             const int64_t token = g.tok_lo + tok;
-            const KeyRange kr = token_keys(a, g, token);
-            row_lo[mt] = real ? static_cast<int>(kr.lo) : 0;
-            row_hi[mt] = real ? static_cast<int>(kr.hi) : 0;
+            const Keys kr = token_keys(a, g, token);
+            row_lo[mt] = kr.lo;
+            row_hi[mt] = real ? kr.hi : 0;
             const int64_t head = static_cast<int64_t>(kvh) * a.group.d + (row - tok * static_cast<int>(a.group.d));
             const T *q = static_cast<const T *>(a.q) + (g.first + token) * a.q_stride + head * HD;
 #pragma unroll
@@ -181,12 +180,12 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 
         // Tokens [some_lo, some_hi) are seen by some row; the others' values count as
         // zero.  Where a value that only some of the rows see is not finite (a weight of
         // zero would not take it away), the rows are done again one by one.
-        int64_t some_lo = kf.lo, some_hi = kl.hi;
+        int some_lo = kf.lo, some_hi = kl.hi;
         bool odd = false;
         for (int only = -1; only < S::kRows; ++only) {
         if (only >= 0) {
             if (!odd || row0 + only >= g.rows) break;
-            const KeyRange kr = token_keys(a, g, g.tok_lo + divided(row0 + only, a.group));
+            const Keys kr = token_keys(a, g, g.tok_lo + divided(row0 + only, a.group));
             some_lo = kr.lo;
             some_hi = kr.hi;
         }
@@ -204,15 +203,13 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 
         u32x4_a kreg[2][kSteps], vreg[kVLoads];
         uint32_t seen = 0;  // keys of the tile in registers that lie on pages of the pool
         // the table entry of key (lane & 31) of a tile
-        auto entry = [&](int64_t base) {
-            const int64_t key = base + (lane & 31);
+        auto entry = [&](int base) {
+            const int key = base + (lane & 31);
             return key >= some_lo && key < some_hi ? table[key >> a.shift] : -1;
         };
-        auto load = [&](int64_t base, int32_t page) {
+        auto load = [&](int base, int32_t page) {
             const bool good = page_in_pool(page, a.n_pages);
-            const int64_t key = base + (lane & 31);
-            const int64_t off = good ? page * a.page_stride + (key & ((int64_t(1) << a.shift) - 1)) * a.token_stride
-                                     : 0;
+            const int64_t off = good ? token_at(a, page, base + (lane & 31)) : 0;
             seen = static_cast<uint32_t>(__ballot(good));
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -228,16 +225,16 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 
             }
         };
         // this wavefront's tiles: every kTokenWaves-th
-        const int64_t first = w.key_lo + t0 * kUnitKeys + wave * kTokenKeys;
-        const int64_t end = idx_min(some_hi, w.key_lo + t1 * kUnitKeys);
+        const int first = w.key_lo + t0 * kUnitKeys + wave * kTokenKeys;
+        const int end = min(some_hi, w.key_lo + t1 * kUnitKeys);
         int32_t next = -1;
         if (first < end) {
             load(first, entry(first));
             next = entry(first + kUnitKeys);
         }
-        for (int64_t base = first; base < end; base += kUnitKeys) {
+        for (int base = first; base < end; base += kUnitKeys) {
             const uint32_t now = seen;
-            f32x4 s[MT][2];
+            float s[MT][8];  // keys 16 (i / 4) + 4 quad + i % 4
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -246,7 +243,8 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 
 #pragma unroll
                     for (int st = 0; st < kSteps; ++st)
                         c = N::mfma16(__builtin_bit_cast(V8, kreg[b][st]), qf[mt][st], c);
-                    s[mt][b] = c;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[mt][4 * b + i] = c[i];
                 }
             // every key of the tile seen by every row
             const bool full = base >= all_lo && base + kTokenKeys <= all_hi && now == 0xFFFFFFFFu;
@@ -260,7 +258,7 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 
                 }
                 *reinterpret_cast<u32x4_a *>(vt + key * S::kVStride + idx % kChunks * 8) = v;
             }
-            const int64_t after = base + kUnitKeys;
+            const int after = base + kUnitKeys;
             if (after < end) {
                 load(after, next);
                 next = entry(after + kUnitKeys);
@@ -268,40 +266,33 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 
             V8 hi[MT], lo[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                float top = -INFINITY;
+                scores2(s[mt], a);
+                if (!full) {
+                    const uint32_t see = (now & range_mask<uint32_t>(row_lo[mt], row_hi[mt], base)) >> (4 * quad);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                    for (int i = 0; i < 8; ++i)
+                        if (!((see >> (16 * (i >> 2) + (i & 3))) & 1)) s[mt][i] = -INFINITY;
+                }
+                float top = s[mt][0];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float x = score2(s[mt][b][i], a);
-                        if (!full) {
-                            const int k = 16 * b + 4 * quad + i;
-                            const int64_t key = base + k;
-                            if (!((now >> k) & 1) || key < row_lo[mt] || key >= row_hi[mt]) x = -INFINITY;
-                        }
-                        s[mt][b][i] = x;
-                        top = fmaxf(top, x);
-                    }
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float m_new = fmaxf(m[mt], top), ref = finite_base(m_new);
-                if (__any(m_new > m[mt])) {
-                    const float keep = __builtin_amdgcn_exp2f(m[mt] - ref);
+                for (int i = 1; i < 8; ++i) top = fmaxf(top, s[mt][i]);
+                top = quad_max(top);
+                if (__any(top > m[mt] + kSlack || (m[mt] == -INFINITY && top > m[mt]))) {
+                    const float m_new = fmaxf(m[mt], top), keep = __builtin_amdgcn_exp2f(m[mt] - finite_base(m_new));
                     l[mt] *= keep;
 #pragma unroll
                     for (int d = 0; d < kBlocks; ++d) o[mt][d] *= keep;
                     m[mt] = m_new;
                 }
+                const float ref = finite_base(m[mt]);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = __builtin_amdgcn_exp2f(s[mt][b][i] - ref);
-                        l[mt] += p;
-                        const T h = static_cast<T>(p);
-                        hi[mt][4 * b + i] = h;
-                        lo[mt][4 * b + i] = static_cast<T>(p - static_cast<float>(h));
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(s[mt][i] - ref);
+                    l[mt] += p;
+                    const T h = static_cast<T>(p);
+                    hi[mt][i] = h;
+                    lo[mt][i] = static_cast<T>(p - static_cast<float>(h));
+                }
             }
             auto vcolumn = [&](int d) {
                 const T *p = vt + (4 * quad + col / 4) * S::kVStride + 16 * d + col % 4 * 4;
@@ -324,9 +315,7 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 128 ? 3 : HD * MT <= 256 
         float *part = a.ws + (2 * static_cast<int64_t>(blockIdx.x) + (u != u0)) * S::kPartFloats;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            float sum = l[mt];
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
+            const float sum = quad_sum(l[mt]);
             if (quad == 0) {
                 lds_m[wave][col] = m[mt];
                 lds_l[wave][col] = sum;
@@ -447,14 +436,13 @@ __global__ __launch_bounds__(kJoinThreads) void attention_token_join_kernel(Attn
     }
 }
 
-// Workgroups of the token form that stay on the chip together.
-constexpr int kTokenGroupsPerCu = 3;
-
-int token_groups(const mi355x_ctx *ctx) { return ctx->num_cus * kTokenGroupsPerCu; }
+// The token form runs as many workgroups as stay on the chip together.
+constexpr int kTokenGroupsPerCu = 4;
 
 template <int TYPE, int HD, int MT>
 int launch_token(mi355x_ctx *ctx, const AttnArgs &a) {
-    const int groups = token_groups(ctx);
+    const void *kernel = reinterpret_cast<const void *>(attention_token_kernel<TYPE, HD, MT>);
+    const int groups = ctx->num_cus * std::max(1, std::min(kTokenGroupsPerCu, occupancy(kernel, kTokenThreads, 0)));
     attention_token_kernel<TYPE, HD, MT><<<groups, kTokenThreads, 0, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
     attention_token_join_kernel<TYPE, HD, MT><<<groups - 1, kJoinThreads, 0, ctx->stream>>>(a, groups);
@@ -489,7 +477,7 @@ int launch_sizes(mi355x_ctx *ctx, const AttnArgs &a, int head_dim, int64_t rows)
 }  // namespace
 
 size_t paged_attention_workspace_bytes(const mi355x_ctx *ctx, int, int, int head_dim) {
-    return std::max(static_cast<size_t>(token_groups(ctx)) * 2 * 32 * (head_dim + 2) * 4,
+    return std::max(static_cast<size_t>(ctx->num_cus * kTokenGroupsPerCu) * 2 * 32 * (head_dim + 2) * 4,
                     attention_chunk_workspace(ctx, head_dim));
 }
 
@@ -506,12 +494,12 @@ int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &u
     a.q_stride = u.q_stride;
     a.out_stride = u.out_stride;
     a.table_stride = u.table_stride;
-    a.page_stride = u.pool->page_stride;
-    a.token_stride = u.pool->token_stride;
+    a.page_stride = static_cast<uint32_t>(u.pool->page_stride);
+    a.token_stride = static_cast<uint32_t>(u.pool->token_stride);
     a.head_stride = u.pool->head_stride;
     a.n_rows = u.n_rows;
     // an empty pool has no address that may be read: no token is seen
-    a.reach = u.pool->n_pages > 0 ? static_cast<int64_t>(u.table_cols) * u.pool->page_tokens : 0;
+    a.reach = u.pool->n_pages > 0 ? u.table_cols * u.pool->page_tokens : 0;
     a.scale2 = u.scale * kLog2e;
     if (u.softcap > 0.0f) {
         a.cap_in = u.scale / u.softcap * (2.0f * kLog2e);

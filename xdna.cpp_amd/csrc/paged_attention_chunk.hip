@@ -31,10 +31,6 @@ constexpr int kChunkWaves = 4;
 constexpr int kChunkThreads = 64 * kChunkWaves;
 constexpr int kChunkRows = 32 * kChunkWaves;
 constexpr int kChunkKeys = 64;
-// A row's maximum may grow by this (in factors of 2) before its sums are
-// scaled: weights stay below 2^8, where 16-bit floats are as exact as below 1.
-constexpr float kSlack = 8.0f;
-
 template <int HD>
 struct ChunkShape {
     static constexpr int kChunks = HD / 8;                            // 16-byte chunks of a token's head
@@ -74,9 +70,9 @@ __device__ __forceinline__ int find_block(const AttnArgs &a, int64_t j, int64_t 
 struct ChunkItem {
     int seq, kvh, row0;
     SeqGeo g;
-    KeyRange first, last;  // of the block's first and last row
-    int tiles;             // of keys from key_lo on
-    int64_t key_lo;
+    Keys first, last;  // of the block's first and last row
+    int tiles;         // of keys from key_lo on
+    int key_lo;
 };
 
 // False: no rows there.
@@ -91,8 +87,8 @@ __device__ __forceinline__ bool chunk_item(const AttnArgs &a, int64_t j, int kvh
     const int row_last = min(it->row0 + kChunkRows, it->g.rows) - 1;
     it->first = token_keys(a, it->g, it->g.tok_lo + divided(it->row0, a.group));
     it->last = token_keys(a, it->g, it->g.tok_lo + divided(row_last, a.group));
-    it->key_lo = it->first.lo & ~int64_t(kChunkKeys - 1);
-    it->tiles = static_cast<int>((idx_max(it->last.hi - it->key_lo, 0) + kChunkKeys - 1) / kChunkKeys);
+    it->key_lo = it->first.lo & ~(kChunkKeys - 1);
+    it->tiles = (max(it->last.hi - it->key_lo, 0) + kChunkKeys - 1) / kChunkKeys;
     return true;
 }
 
@@ -123,12 +119,8 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
     const bool real = row_raw < g.rows;
     const int row = real ? row_raw : 0, tok = divided(row, a.group), group = static_cast<int>(a.group.d);
     const int64_t head = static_cast<int64_t>(kvh) * group + (row - tok * group);
-    int64_t row_lo = 0, row_hi = 0;
-    if (real) {
-        const KeyRange kr = token_keys(a, g, g.tok_lo + tok);
-        row_lo = kr.lo;
-        row_hi = kr.hi;
-    }
+    const Keys mine = token_keys(a, g, g.tok_lo + tok);
+    const int row_lo = mine.lo, row_hi = real ? mine.hi : 0;
     V8 qf[kSteps];
     {
         const T *q = static_cast<const T *>(a.q) + (g.first + g.tok_lo + tok) * a.q_stride + head * HD;
@@ -163,13 +155,13 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
     // Tokens [some_lo, some_hi) are seen by some row; the others' values count as
     // zero.  Where a value that only some of the rows see is not finite (a weight of
     // zero would not take it away), the rows are done again one by one.
-    int64_t some_lo = it.first.lo, some_hi = it.last.hi;
+    int some_lo = it.first.lo, some_hi = it.last.hi;
     if (tid == 0) odd = 0;
     for (int only = -1; only < kChunkRows; ++only) {
         if (only >= 0) {
             __syncthreads();
             if (odd == 0 || it.row0 + only >= g.rows) break;
-            const KeyRange kr = token_keys(a, g, g.tok_lo + divided(it.row0 + only, a.group));
+            const Keys kr = token_keys(a, g, g.tok_lo + divided(it.row0 + only, a.group));
             some_lo = kr.lo;
             some_hi = kr.hi;
         }
@@ -181,16 +173,14 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
         float m = -INFINITY, l = 0.0f;
         // the table entry of key `lane` of tile t
         auto entry = [&](int t) {
-            const int64_t key = it.key_lo + static_cast<int64_t>(t) * kChunkKeys + lane;
+            const int key = it.key_lo + t * kChunkKeys + lane;
             return t < t1 && key >= some_lo && key < some_hi ? table[key >> a.shift] : -1;
         };
         uint64_t seen_next = 0;  // keys of the tile on its way that lie on pages of the pool
         auto load = [&](int t, int32_t page, int buf) {
             const bool good = page_in_pool(page, a.n_pages);
             seen_next = __ballot(good);
-            const int64_t key = it.key_lo + static_cast<int64_t>(t) * kChunkKeys + lane;
-            const int64_t off =
-                good ? page * a.page_stride + (key & ((int64_t(1) << a.shift) - 1)) * a.token_stride : 0;
+            const int64_t off = good ? token_at(a, page, it.key_lo + t * kChunkKeys + lane) : 0;
             unsigned char *to = lds + 2 * buf * S::kTileBytes + 1024 * wave;
 #pragma unroll
             for (int i = 0; i < S::kLoads; ++i) {
@@ -221,7 +211,7 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
                 next = entry(t + 2);
             }
             unsigned char *kt = lds + 2 * buf * S::kTileBytes, *vt = kt + S::kTileBytes;
-            const int64_t base = it.key_lo + static_cast<int64_t>(t) * kChunkKeys;
+            const int base = it.key_lo + t * kChunkKeys;
             // every key of the tile seen by every row of the workgroup
             const bool full = base >= it.last.lo && base + kChunkKeys <= it.first.hi && ~seen == 0;
             if (!full) {
@@ -234,41 +224,31 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
                 if (__any(bad) && lane == 0) odd = 1;
                 __syncthreads();
             }
-            f32x16 s[2];
+            float s[32];  // keys 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
+                f32x16 x;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+                for (int i = 0; i < 16; ++i) x[i] = 0.0f;
 #pragma unroll
                 for (int st = 0; st < kSteps; ++st) {
                     const int place = ((2 * (st & 3)) ^ k_low) + 8 * (st >> 2);
                     const V8 k = *reinterpret_cast<const V8 *>(kt + k_at + 32 * kb * S::kRowBytes + 16 * place);
-                    s[kb] = N::mfma32(k, qf[st], s[kb]);
+                    x = N::mfma32(k, qf[st], x);
                 }
-            }
-            if (CAP) {
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[kb][i] = score2(s[kb][i], a);
+                for (int i = 0; i < 16; ++i) s[16 * kb + i] = x[i];
             }
+            if (CAP) scores2(s, a);
             if (!full) {
-                const int lo = static_cast<int>(idx_max(row_lo - base, 0));
-                const int hi = static_cast<int>(idx_min(row_hi - base, 64));
-                uint64_t mine = 0;
-                if (hi > lo) mine = seen & (~uint64_t(0) >> (64 - hi)) & ~((uint64_t(1) << lo) - 1);
-                mine >>= 4 * half;
+                const uint64_t see = (seen & range_mask<uint64_t>(row_lo, row_hi, base)) >> (4 * half);
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (!((mine >> (32 * kb + 8 * (i >> 2) + (i & 3))) & 1)) s[kb][i] = -INFINITY;
+                for (int i = 0; i < 32; ++i)
+                    if (!((see >> (32 * (i >> 4) + 8 * ((i >> 2) & 3) + (i & 3))) & 1)) s[i] = -INFINITY;
             }
             float top = -INFINITY;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
             top = half_max(top);
             if (!CAP) top *= c;  // c >= 0 here; 0 x infinity gives NaN, which no maximum takes
             const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
@@ -285,7 +265,7 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
                 V8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float x = s[j >> 1][8 * (j & 1) + i];
+                    const float x = s[8 * j + i];
                     const float p = __builtin_amdgcn_exp2f(CAP ? x - ref : fmaf(x, c, -ref));
                     l += p;
                     const T h = static_cast<T>(p);
@@ -374,7 +354,7 @@ int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
     const int64_t blocks = ((a.n_rows * a.group.d) >> 7) + a.n_seqs, items = blocks * a.n_kv_heads;
     // parts of no fewer than four tiles where the table allows that many tokens
     a.split = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>(chunk_groups(ctx) / items, (a.reach + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
+        1, std::min<int64_t>(chunk_groups(ctx) / items, (int64_t(a.reach) + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
     if (items * a.split > INT32_MAX)
         return set_error(MI355X_EUNSUPPORTED, "mi355x_paged_attention: more row blocks than a launch takes");
     attention_chunk_kernel<TYPE, HD, CAP, PLANES>
