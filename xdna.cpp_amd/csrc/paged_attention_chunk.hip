@@ -31,6 +31,9 @@ constexpr int kChunkWaves = 4;
 constexpr int kChunkThreads = 64 * kChunkWaves;
 constexpr int kChunkRows = 32 * kChunkWaves;
 constexpr int kChunkKeys = 64;
+// Instruction kinds of __builtin_amdgcn_sched_group_barrier.
+constexpr int kMfma = 0x8, kDsRead = 0x100;
+
 template <int HD>
 struct ChunkShape {
     static constexpr int kChunks = HD / 8;                            // 16-byte chunks of a token's head
@@ -225,19 +228,30 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
                 __syncthreads();
             }
             float s[32];  // keys 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
+            f32x16 x[2];
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                f32x16 x;
+            for (int i = 0; i < 16; ++i) x[0][i] = x[1][i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+            for (int st = 0; st < kSteps; ++st)
 #pragma unroll
-                for (int st = 0; st < kSteps; ++st) {
+                for (int kb = 0; kb < 2; ++kb) {
                     const int place = ((2 * (st & 3)) ^ k_low) + 8 * (st >> 2);
                     const V8 k = *reinterpret_cast<const V8 *>(kt + k_at + 32 * kb * S::kRowBytes + 16 * place);
-                    x = N::mfma32(k, qf[st], x);
+                    x[kb] = N::mfma32(k, qf[st], x[kb]);
                 }
+            // operands kAhead reads ahead of their products: left alone, each waits for its own
+            constexpr int kAhead = 6;
+            __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[16 * kb + i] = x[i];
+            for (int i = 0; i < 2 * kSteps - kAhead; ++i) {
+                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[i] = x[0][i];
+                s[16 + i] = x[1][i];
             }
             if (CAP) scores2(s, a);
             if (!full) {
@@ -260,28 +274,39 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
                 m = m_new;
             }
             const float ref = finite_base(m);
+            auto v_chunk = [&](int j, int d) {  // keys 16 j + {4 half .. + 3, 8 + 4 half .. + 3} of 32 values
+                const int place = ((4 * (d & 1)) ^ v_low) + 8 * (d >> 1);
+                const s16x4 *p = reinterpret_cast<const s16x4 *>(vt + v_at + 16 * j * S::kRowBytes + 16 * place);
+                const u32x2_a x = lds_read_transposed(p), y = lds_read_transposed(p + S::kRowBytes);
+                return __builtin_bit_cast(V8, u32x4_a{x[0], x[1], y[0], y[1]});
+            };
+            // the next 16 keys' reads go out before this 16 keys' weights are formed (the
+            // fences keep that order: left alone, each product waits for its own read)
+            V8 v[2][kBlocks];
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) v[0][d] = v_chunk(0, d);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                if (j < 3)
+#pragma unroll
+                    for (int d = 0; d < kBlocks; ++d) v[(j + 1) & 1][d] = v_chunk(j + 1, d);
+                __builtin_amdgcn_sched_barrier(0);
                 V8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float x = s[8 * j + i];
-                    const float p = __builtin_amdgcn_exp2f(CAP ? x - ref : fmaf(x, c, -ref));
+                    const float y = s[8 * j + i], p = __builtin_amdgcn_exp2f(CAP ? y - ref : fmaf(y, c, -ref));
                     l += p;
                     const T h = static_cast<T>(p);
                     hi[i] = h;
                     if (PLANES == 2) lo[i] = static_cast<T>(p - static_cast<float>(h));
                 }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) {
-                    // keys 16 j + {4 half .. + 3, 8 + 4 half .. + 3} of 32 values
-                    const int place = ((4 * (d & 1)) ^ v_low) + 8 * (d >> 1);
-                    const s16x4 *p = reinterpret_cast<const s16x4 *>(vt + v_at + 16 * j * S::kRowBytes + 16 * place);
-                    const u32x2_a x = lds_read_transposed(p), y = lds_read_transposed(p + S::kRowBytes);
-                    const V8 v = __builtin_bit_cast(V8, u32x4_a{x[0], x[1], y[0], y[1]});
-                    o[d] = N::mfma32(v, hi, o[d]);
-                    if (PLANES == 2) o[d] = N::mfma32(v, lo, o[d]);
+                    o[d] = N::mfma32(v[j & 1][d], hi, o[d]);
+                    if (PLANES == 2) o[d] = N::mfma32(v[j & 1][d], lo, o[d]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
 
