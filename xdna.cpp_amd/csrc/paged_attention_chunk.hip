@@ -45,9 +45,18 @@ struct ChunkShape {
     static constexpr int kLds = 4 * kTileBytes;                       // K and V, two tiles each
 };
 
-// The place of chunk c of row r is c ^ k_turn(r) (K) or c ^ v_turn(r) (V).
-__device__ __forceinline__ int k_turn(int r) { return r & 7; }
-__device__ __forceinline__ int v_turn(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+// The place of chunk c of row r is c ^ turn: 16 consecutive rows' chunk c (K), or
+// 4 chunks of 4 consecutive rows (V), lie in the 16 places that make up LDS's 64
+// banks.  (Rows of 32 places: 8 of them for K, so that a lane fills the same
+// chunk of all its rows.)
+template <int PLACES>
+__device__ __forceinline__ int k_turn(int r) {
+    return PLACES == 8 ? (r >> 1) & 7 : PLACES == 16 ? r & 15 : r & 7;
+}
+template <int PLACES>
+__device__ __forceinline__ int v_turn(int r) {
+    return PLACES == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
+}
 
 // The request whose row blocks include block j, and its first one.
 __device__ __forceinline__ int find_block(const AttnArgs &a, int64_t j, int64_t *first) {
@@ -134,13 +143,13 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
             qf[st] = z;
         }
     }
-    // where this lane's loads come from: its chunk of a token's head (the row that
-    // it fills, modulo 8, is the same in all of its loads), and where it reads: K row
+    // where this lane's loads come from: its chunk of a token's head (the turn of the
+    // rows that it fills is the same), and where it reads: K row
     // col (+ 32), chunk 2 st + half; V rows 4 half + (lane % 16) / 4 (+ 8 ..), chunk
     // 4 d + 2 ((lane / 16) % 2) + (lane % 4) / 2
     const int fill_row = (wave * 64 + lane) / S::kPlaces;
-    static_assert(kChunkThreads / S::kPlaces % 8 == 0, "rows of one lane's loads, modulo 8");
-    int ck = lane % S::kPlaces ^ k_turn(fill_row), cv = lane % S::kPlaces ^ v_turn(fill_row);
+    static_assert(kChunkThreads / S::kPlaces % (S::kPlaces == 32 ? 8 : 16) == 0, "one turn for all of a lane's rows");
+    int ck = lane % S::kPlaces ^ k_turn<S::kPlaces>(fill_row), cv = lane % S::kPlaces ^ v_turn<S::kPlaces>(fill_row);
     if (HD == 96) {  // places without a chunk take another's
         ck = ck < S::kChunks ? ck : ck - 4;
         cv = cv < S::kChunks ? cv : cv - 4;
@@ -148,10 +157,10 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
     const T *kp = static_cast<const T *>(a.k) + kvh * a.head_stride + 8 * ck;
     const T *vp = static_cast<const T *>(a.v) + kvh * a.head_stride + 8 * cv;
     const int k_at = col * S::kRowBytes;
-    const int k_low = half ^ k_turn(col);
+    const int k_low = half ^ k_turn<S::kPlaces>(col);
     const int v_row = 4 * half + ((lane & 15) >> 2);
     const int v_at = v_row * S::kRowBytes + (lane & 1) * 8;
-    const int v_low = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_turn(v_row);
+    const int v_low = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_turn<S::kPlaces>(v_row);
     const int32_t *table = a.table + it.seq * a.table_stride;
     const float c = a.scale2;
 
@@ -235,7 +244,7 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
             for (int st = 0; st < kSteps; ++st)
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
-                    const int place = ((2 * (st & 3)) ^ k_low) + 8 * (st >> 2);
+                    const int place = (2 * st) ^ k_low;
                     const V8 k = *reinterpret_cast<const V8 *>(kt + k_at + 32 * kb * S::kRowBytes + 16 * place);
                     x[kb] = N::mfma32(k, qf[st], x[kb]);
                 }
@@ -275,7 +284,7 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
             }
             const float ref = finite_base(m);
             auto v_chunk = [&](int j, int d) {  // keys 16 j + {4 half .. + 3, 8 + 4 half .. + 3} of 32 values
-                const int place = ((4 * (d & 1)) ^ v_low) + 8 * (d >> 1);
+                const int place = (4 * d) ^ v_low;
                 const s16x4 *p = reinterpret_cast<const s16x4 *>(vt + v_at + 16 * j * S::kRowBytes + 16 * place);
                 const u32x2_a x = lds_read_transposed(p), y = lds_read_transposed(p + S::kRowBytes);
                 return __builtin_bit_cast(V8, u32x4_a{x[0], x[1], y[0], y[1]});
