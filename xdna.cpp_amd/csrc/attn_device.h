@@ -27,7 +27,8 @@ struct AttnArgs {
     FastDiv group;  // query heads of a KV head
     int n_seqs, n_kv_heads;
     int n_pages, shift, window, causal, f32_out;
-    int split;  // chunk form: parts of an item's keys
+    int split;    // chunk form: parts of an item's keys
+    int by_page;  // chunk form: the rows of a load share a page, 32-bit offsets within it
 };
 
 constexpr float kLog2e = 1.44269504088896341f;

@@ -79,6 +79,13 @@ __device__ __forceinline__ int find_block(const AttnArgs &a, int64_t j, int64_t 
     return lo;
 }
 
+// 16 bytes per lane from memory to LDS, lane after lane from `to` on.
+__device__ __forceinline__ void load_lds16(const void *from, unsigned char *to) {
+    __builtin_amdgcn_global_load_lds(
+        reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(reinterpret_cast<uintptr_t>(from)),
+        (__attribute__((address_space(3))) uint32_t *)(to), 16, 0, 0);
+}
+
 struct ChunkItem {
     int seq, kvh, row0;
     SeqGeo g;
@@ -154,8 +161,12 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
         ck = ck < S::kChunks ? ck : ck - 4;
         cv = cv < S::kChunks ? cv : cv - 4;
     }
-    const T *kp = static_cast<const T *>(a.k) + kvh * a.head_stride + 8 * ck;
-    const T *vp = static_cast<const T *>(a.v) + kvh * a.head_stride + 8 * cv;
+    // a wavefront's load covers kFillRows consecutive rows; where those share a page
+    // (a.by_page) its address is one scalar and an offset per lane
+    constexpr int kFillRows = 64 / S::kPlaces, kFillStep = kChunkThreads / S::kPlaces;
+    const T *kp = static_cast<const T *>(a.k) + kvh * a.head_stride, *vp = static_cast<const T *>(a.v) + kvh * a.head_stride;
+    const uint32_t k_off = 2 * ((lane / S::kPlaces) * a.token_stride + 8 * ck);  // bytes
+    const uint32_t v_off = 2 * ((lane / S::kPlaces) * a.token_stride + 8 * cv);
     const int k_at = col * S::kRowBytes;
     const int k_low = half ^ k_turn<S::kPlaces>(col);
     const int v_row = 4 * half + ((lane & 15) >> 2);
@@ -183,29 +194,36 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
         float m = -INFINITY, l = 0.0f;
-        // the table entry of key `lane` of tile t
+        const int col_lo = some_lo >> a.shift, col_hi = (some_hi - 1) >> a.shift;
+        // the table entry of key `lane` of tile t, if some row sees a token on its page
         auto entry = [&](int t) {
-            const int key = it.key_lo + t * kChunkKeys + lane;
-            return t < t1 && key >= some_lo && key < some_hi ? table[key >> a.shift] : -1;
+            const int column = (it.key_lo + t * kChunkKeys + lane) >> a.shift;
+            return t < t1 && column >= col_lo && column <= col_hi ? table[column] : -1;
         };
-        uint64_t seen_next = 0;  // keys of the tile on its way that lie on pages of the pool
-        auto load = [&](int t, int32_t page, int buf) {
-            const bool good = page_in_pool(page, a.n_pages);
-            seen_next = __ballot(good);
-            const int64_t off = good ? token_at(a, page, it.key_lo + t * kChunkKeys + lane) : 0;
+        uint64_t seen_next = 0;  // keys of the tile on its way that some row sees, on pages of the pool
+        auto load = [&](int t, int32_t entry, int buf) {
+            const bool good = page_in_pool(entry, a.n_pages);
+            const int base = it.key_lo + t * kChunkKeys, page = good ? entry : 0;
+            seen_next = __ballot(good) & range_mask<uint64_t>(some_lo, some_hi, base);
             unsigned char *to = lds + 2 * buf * S::kTileBytes + 1024 * wave;
+            // the load's first row: kFillRows wave + kFillStep i
+            if (a.by_page) {
 #pragma unroll
-            for (int i = 0; i < S::kLoads; ++i) {
-                const int64_t from = __shfl(off, fill_row + i * (kChunkThreads / S::kPlaces));
-                __builtin_amdgcn_global_load_lds(
-                    reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(
-                        reinterpret_cast<uintptr_t>(kp + from)),
-                    (__attribute__((address_space(3))) uint32_t *)(to + 16 * kChunkThreads * i), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds(
-                    reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(
-                        reinterpret_cast<uintptr_t>(vp + from)),
-                    (__attribute__((address_space(3))) uint32_t *)(to + S::kTileBytes + 16 * kChunkThreads * i), 16,
-                    0, 0);
+                for (int i = 0; i < S::kLoads; ++i) {
+                    const int row = kFillRows * wave + i * kFillStep;
+                    const int64_t from = token_at(a, __builtin_amdgcn_readlane(page, row), base + row);
+                    load_lds16(reinterpret_cast<const char *>(kp + from) + k_off, to + 16 * kChunkThreads * i);
+                    load_lds16(reinterpret_cast<const char *>(vp + from) + v_off,
+                               to + S::kTileBytes + 16 * kChunkThreads * i);
+                }
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < S::kLoads; ++i) {
+                    const int row = kFillRows * wave + i * kFillStep + lane / S::kPlaces;
+                    const int64_t from = token_at(a, __shfl(page, row), base + row);
+                    load_lds16(kp + from + 8 * ck, to + 16 * kChunkThreads * i);
+                    load_lds16(vp + from + 8 * cv, to + S::kTileBytes + 16 * kChunkThreads * i);
+                }
             }
         };
         int32_t next = -1;
@@ -385,6 +403,7 @@ int chunk_groups(const mi355x_ctx *ctx) { return 2 * ctx->num_cus; }
 template <int TYPE, int HD, bool CAP, int PLANES>
 int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
     AttnArgs a = args;
+    a.by_page = a.shift >= __builtin_ctz(64 / ChunkShape<HD>::kPlaces) && a.token_stride < (1u << 26);
     const int64_t blocks = ((a.n_rows * a.group.d) >> 7) + a.n_seqs, items = blocks * a.n_kv_heads;
     // parts of no fewer than four tiles where the table allows that many tokens
     a.split = static_cast<int>(std::max<int64_t>(
