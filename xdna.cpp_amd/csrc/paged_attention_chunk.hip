@@ -27,21 +27,20 @@
 namespace mi355x {
 namespace {
 
-constexpr int kChunkWaves = 4;
-constexpr int kChunkThreads = 64 * kChunkWaves;
-constexpr int kChunkRows = 32 * kChunkWaves;
 constexpr int kChunkKeys = 64;
 // Instruction kinds of __builtin_amdgcn_sched_group_barrier.
 constexpr int kMfma = 0x8, kDsRead = 0x100;
 
-template <int HD>
+template <int HD, int WAVES>
 struct ChunkShape {
+    static constexpr int kThreads = 64 * WAVES;
+    static constexpr int kRows = 32 * WAVES;
     static constexpr int kChunks = HD / 8;                            // 16-byte chunks of a token's head
     static constexpr int kPlaces = HD == 96 ? 16 : kChunks;           // places for them in LDS, a power of two
     static constexpr int kRowBytes = 16 * kPlaces;
     static constexpr int kTileBytes = kChunkKeys * kRowBytes;
-    static constexpr int kLoads = kChunkKeys * kPlaces / kChunkThreads;  // of K, and of V, per lane
-    static constexpr int kPartFloats = kChunkRows * (HD + 2);
+    static constexpr int kLoads = kChunkKeys * kPlaces / kThreads;  // of K, and of V, per lane
+    static constexpr int kPartFloats = kRows * (HD + 2);
     static constexpr int kLds = 4 * kTileBytes;                       // K and V, two tiles each
 };
 
@@ -58,12 +57,12 @@ __device__ __forceinline__ int v_turn(int r) {
     return PLACES == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
 }
 
-// The request whose row blocks include block j, and its first one.
+// The request whose blocks of 2^SHIFT rows include block j, and its first one.
+template <int SHIFT>
 __device__ __forceinline__ int find_block(const AttnArgs &a, int64_t j, int64_t *first) {
-    auto begin = [&](int s) {  // ascends by at least 1: blocks of 128 rows, one more at every seam
-        return ((static_cast<int64_t>(a.row_offsets[s]) * a.group.d) >> 7) + s;
+    auto begin = [&](int s) {  // ascends by at least 1: one block more at every seam
+        return ((static_cast<int64_t>(a.row_offsets[s]) * a.group.d) >> SHIFT) + s;
     };
-    static_assert(kChunkRows == 128, "the shift above");
     const int lane = threadIdx.x & 63;
     int lo = 0, n = a.n_seqs;  // the request is in lo .. lo + n - 1
     while (n > 1) {
@@ -94,16 +93,21 @@ struct ChunkItem {
     int key_lo;
 };
 
+constexpr int row_shift(int waves) { return waves == 8 ? 8 : 7; }
+
 // False: no rows there.
+template <int WAVES>
 __device__ __forceinline__ bool chunk_item(const AttnArgs &a, int64_t j, int kvh, ChunkItem *it) {
     int64_t begin;
-    it->seq = find_block(a, j, &begin);
+    constexpr int kRows = 32 * WAVES;
+    static_assert(kRows == 1 << row_shift(WAVES), "blocks of rows");
+    it->seq = find_block<row_shift(WAVES)>(a, j, &begin);
     it->kvh = kvh;
     it->g = seq_geo(a, it->seq);
-    const int64_t row0 = (j - begin) * kChunkRows;
+    const int64_t row0 = (j - begin) * kRows;
     if (row0 < 0 || row0 >= it->g.rows || it->g.rows <= a.row_limit) return false;
     it->row0 = static_cast<int>(row0);
-    const int row_last = min(it->row0 + kChunkRows, it->g.rows) - 1;
+    const int row_last = min(it->row0 + kRows, it->g.rows) - 1;
     it->first = token_keys(a, it->g, it->g.tok_lo + divided(it->row0, a.group));
     it->last = token_keys(a, it->g, it->g.tok_lo + divided(row_last, a.group));
     it->key_lo = it->first.lo & ~(kChunkKeys - 1);
@@ -111,12 +115,13 @@ __device__ __forceinline__ bool chunk_item(const AttnArgs &a, int64_t j, int kvh
     return true;
 }
 
-template <int TYPE, int HD, bool CAP, int PLANES>
-__global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chunk_kernel(AttnArgs a) {
+template <int TYPE, int HD, bool CAP, int PLANES, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_kernel(AttnArgs a) {
     typedef Num<TYPE> N;
     typedef typename N::T T;
     typedef typename N::V8 V8;
-    typedef ChunkShape<HD> S;
+    typedef ChunkShape<HD, WAVES> S;
+    constexpr int kThreads = S::kThreads, kRows = S::kRows;
     constexpr int kSteps = HD / 16;   // of a 32-key score product
     constexpr int kBlocks = HD / 32;  // of 32 output values
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
@@ -128,7 +133,7 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
     const int64_t rest = blockIdx.x / a.n_kv_heads;
     const int part = static_cast<int>(rest % a.split);
     ChunkItem it;
-    if (!chunk_item(a, gridDim.x / (a.n_kv_heads * a.split) - 1 - rest / a.split, kvh, &it)) return;
+    if (!chunk_item<WAVES>(a, gridDim.x / (a.n_kv_heads * a.split) - 1 - rest / a.split, kvh, &it)) return;
     const SeqGeo g = it.g;
     const int t0 = static_cast<int>(static_cast<int64_t>(it.tiles) * part / a.split);
     const int t1 = static_cast<int>(static_cast<int64_t>(it.tiles) * (part + 1) / a.split);
@@ -155,7 +160,7 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
     // col (+ 32), chunk 2 st + half; V rows 4 half + (lane % 16) / 4 (+ 8 ..), chunk
     // 4 d + 2 ((lane / 16) % 2) + (lane % 4) / 2
     const int fill_row = (wave * 64 + lane) / S::kPlaces;
-    static_assert(kChunkThreads / S::kPlaces % (S::kPlaces == 32 ? 8 : 16) == 0, "one turn for all of a lane's rows");
+    static_assert(kThreads / S::kPlaces % (S::kPlaces == 32 ? 8 : 16) == 0, "one turn for all of a lane's rows");
     int ck = lane % S::kPlaces ^ k_turn<S::kPlaces>(fill_row), cv = lane % S::kPlaces ^ v_turn<S::kPlaces>(fill_row);
     if (HD == 96) {  // places without a chunk take another's
         ck = ck < S::kChunks ? ck : ck - 4;
@@ -163,7 +168,7 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
     }
     // a wavefront's load covers kFillRows consecutive rows; where those share a page
     // (a.by_page) its address is one scalar and an offset per lane
-    constexpr int kFillRows = 64 / S::kPlaces, kFillStep = kChunkThreads / S::kPlaces;
+    constexpr int kFillRows = 64 / S::kPlaces, kFillStep = kThreads / S::kPlaces;
     const T *kp = static_cast<const T *>(a.k) + kvh * a.head_stride, *vp = static_cast<const T *>(a.v) + kvh * a.head_stride;
     const uint32_t k_off = 2 * ((lane / S::kPlaces) * a.token_stride + 8 * ck);  // bytes
     const uint32_t v_off = 2 * ((lane / S::kPlaces) * a.token_stride + 8 * cv);
@@ -180,7 +185,7 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
     // zero would not take it away), the rows are done again one by one.
     int some_lo = it.first.lo, some_hi = it.last.hi;
     if (tid == 0) odd = 0;
-    for (int only = -1; only < kChunkRows; ++only) {
+    for (int only = -1; only < kRows; ++only) {
         if (only >= 0) {
             __syncthreads();
             if (odd == 0 || it.row0 + only >= g.rows) break;
@@ -212,17 +217,17 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
                 for (int i = 0; i < S::kLoads; ++i) {
                     const int row = kFillRows * wave + i * kFillStep;
                     const int64_t from = token_at(a, __builtin_amdgcn_readlane(page, row), base + row);
-                    load_lds16(reinterpret_cast<const char *>(kp + from) + k_off, to + 16 * kChunkThreads * i);
+                    load_lds16(reinterpret_cast<const char *>(kp + from) + k_off, to + 16 * kThreads * i);
                     load_lds16(reinterpret_cast<const char *>(vp + from) + v_off,
-                               to + S::kTileBytes + 16 * kChunkThreads * i);
+                               to + S::kTileBytes + 16 * kThreads * i);
                 }
             } else {
 #pragma unroll 1
                 for (int i = 0; i < S::kLoads; ++i) {
                     const int row = kFillRows * wave + i * kFillStep + lane / S::kPlaces;
                     const int64_t from = token_at(a, __shfl(page, row), base + row);
-                    load_lds16(kp + from + 8 * ck, to + 16 * kChunkThreads * i);
-                    load_lds16(vp + from + 8 * cv, to + S::kTileBytes + 16 * kChunkThreads * i);
+                    load_lds16(kp + from + 8 * ck, to + 16 * kThreads * i);
+                    load_lds16(vp + from + 8 * cv, to + S::kTileBytes + 16 * kThreads * i);
                 }
             }
         };
@@ -246,7 +251,7 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
             const bool full = base >= it.last.lo && base + kChunkKeys <= it.first.hi && ~seen == 0;
             if (!full) {
                 bool bad = false;
-                for (int i = tid; i < kChunkKeys * S::kPlaces; i += kChunkThreads) {
+                for (int i = tid; i < kChunkKeys * S::kPlaces; i += kThreads) {
                     u32x4_a *p = reinterpret_cast<u32x4_a *>(vt + 16 * i);
                     if (!((seen >> (i / S::kPlaces)) & 1)) *p = u32x4_a{0, 0, 0, 0};
                     else bad |= not_finite<TYPE>(*p);
@@ -360,8 +365,8 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
                     *reinterpret_cast<f32x4 *>(w + r * HD + 32 * d + 8 * i + 4 * half) =
                         f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
             if (half == 0) {
-                w[kChunkRows * HD + r] = m;
-                w[kChunkRows * (HD + 1) + r] = l;
+                w[kRows * HD + r] = m;
+                w[kRows * (HD + 1) + r] = l;
             }
         }
     }
@@ -370,26 +375,27 @@ __global__ __launch_bounds__(kChunkThreads, HD > 128 ? 1 : 2) void attention_chu
 // Joins the parts of each row block and KV head.
 template <int TYPE, int HD>
 __global__ __launch_bounds__(256) void attention_chunk_join_kernel(AttnArgs a) {
-    typedef ChunkShape<HD> S;
+    typedef ChunkShape<HD, 4> S;
+    constexpr int kRows = S::kRows;
     const int kvh = static_cast<int>(blockIdx.x % a.n_kv_heads);
     const int64_t rest = blockIdx.x / a.n_kv_heads, blocks = gridDim.x / a.n_kv_heads;
     ChunkItem it;
-    if (!chunk_item(a, blocks - 1 - rest, kvh, &it)) return;
-    const int rows = min(kChunkRows, it.g.rows - it.row0);
+    if (!chunk_item<4>(a, blocks - 1 - rest, kvh, &it)) return;
+    const int rows = min(kRows, it.g.rows - it.row0);
     constexpr int kQuads = HD / 4;
     for (int i = threadIdx.x + 256 * blockIdx.y; i < rows * kQuads; i += 256 * gridDim.y) {
         const int r = i / kQuads, c = i % kQuads * 4;
         auto part_of = [&](int p) { return a.ws + ((rest * a.split + p) * a.n_kv_heads + kvh) * S::kPartFloats; };
         float top = -INFINITY;
-        for (int p = 0; p < a.split; ++p) top = fmaxf(top, part_of(p)[kChunkRows * HD + r]);
+        for (int p = 0; p < a.split; ++p) top = fmaxf(top, part_of(p)[kRows * HD + r]);
         const float ref = finite_base(top);
         float den = 0.0f;
         f32x4 num = {0, 0, 0, 0};
 #pragma unroll 4
         for (int p = 0; p < a.split; ++p) {
             const float *w = part_of(p);
-            const float f = __builtin_amdgcn_exp2f(w[kChunkRows * HD + r] - ref);
-            den += f * w[kChunkRows * (HD + 1) + r];
+            const float f = __builtin_amdgcn_exp2f(w[kRows * HD + r] - ref);
+            den += f * w[kRows * (HD + 1) + r];
             num += f * *reinterpret_cast<const f32x4 *>(w + r * HD + c);
         }
         store_out4<TYPE>(a, out_at(a, it.g, kvh, it.row0 + r, HD) + c,
@@ -400,18 +406,33 @@ __global__ __launch_bounds__(256) void attention_chunk_join_kernel(AttnArgs a) {
 // Workgroups that a call is split into at most, while that is more than its row blocks.
 int chunk_groups(const mi355x_ctx *ctx) { return 2 * ctx->num_cus; }
 
+// Workgroups of 256 rows where there are enough of them for all CUs: they load
+// half as much into LDS per row (prompt of 8192 tokens: 586 us with 128 rows, 556 with
+// 256).  Else 128, and more of them.  Heads of 256 values leave registers for four
+// wavefronts.
 template <int TYPE, int HD, bool CAP, int PLANES>
 int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
     AttnArgs a = args;
-    a.by_page = a.shift >= __builtin_ctz(64 / ChunkShape<HD>::kPlaces) && a.token_stride < (1u << 26);
-    const int64_t blocks = ((a.n_rows * a.group.d) >> 7) + a.n_seqs, items = blocks * a.n_kv_heads;
+    a.by_page = a.shift >= __builtin_ctz(64 / ChunkShape<HD, 4>::kPlaces) && a.token_stride < (1u << 26);
+    a.split = 1;
+    const int64_t rows = a.n_rows * a.group.d;
+    if constexpr (HD <= 128) {
+        const int64_t items = ((rows >> row_shift(8)) + a.n_seqs) * a.n_kv_heads;
+        if ((rows >> row_shift(8)) * a.n_kv_heads >= ctx->num_cus && items <= INT32_MAX) {
+            attention_chunk_kernel<TYPE, HD, CAP, PLANES, 8>
+                <<<static_cast<unsigned>(items), 512, ChunkShape<HD, 8>::kLds, ctx->stream>>>(a);
+            MI355X_HIP(hipGetLastError());
+            return MI355X_OK;
+        }
+    }
+    const int64_t items = ((rows >> row_shift(4)) + a.n_seqs) * a.n_kv_heads;
     // parts of no fewer than four tiles where the table allows that many tokens
     a.split = static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>(chunk_groups(ctx) / items, (int64_t(a.reach) + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
     if (items * a.split > INT32_MAX)
         return set_error(MI355X_EUNSUPPORTED, "mi355x_paged_attention: more row blocks than a launch takes");
-    attention_chunk_kernel<TYPE, HD, CAP, PLANES>
-        <<<static_cast<unsigned>(items * a.split), kChunkThreads, ChunkShape<HD>::kLds, ctx->stream>>>(a);
+    attention_chunk_kernel<TYPE, HD, CAP, PLANES, 4>
+        <<<static_cast<unsigned>(items * a.split), 256, ChunkShape<HD, 4>::kLds, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
     if (a.split > 1) {
         const dim3 grid(static_cast<unsigned>(items), 4);
@@ -442,7 +463,7 @@ int launch_type(mi355x_ctx *ctx, const AttnArgs &a, int head_dim) {
 }  // namespace
 
 size_t attention_chunk_workspace(const mi355x_ctx *ctx, int head_dim) {
-    return static_cast<size_t>(chunk_groups(ctx)) * kChunkRows * (head_dim + 2) * 4;
+    return static_cast<size_t>(chunk_groups(ctx)) * 128 * (head_dim + 2) * 4;
 }
 
 int launch_attention_chunk(mi355x_ctx *ctx, const AttnArgs &a, int type, int head_dim) {
