@@ -165,9 +165,10 @@ MI355X_API int mi355x_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_ar
  * a request's new tokens; it picks the form and nothing else (0: unknown).
  *
  * workspace: mi355x_paged_attention_workspace bytes for parts of long rows,
- * 16-byte aligned; its contents before and after a call mean nothing.  Calls
- * that may run at the same time (two contexts, a graph replayed beside other
- * calls, two graphs) need one each; calls in order on one stream share one. */
+ * 16-byte aligned.  Zero it once, before its first call (mi355x_fill): it
+ * begins with counters that every call finds and leaves at 0.  Calls that may
+ * run at the same time (two contexts, a graph replayed beside other calls, two
+ * graphs) need one each; calls in order on one stream share one. */
 typedef struct mi355x_paged_attention_args {
     int64_t n_rows;           /* rows of q and out; times n_heads / n_kv_heads at most 2^31 - 1 */
     int n_seqs;               /* at most 65536 */

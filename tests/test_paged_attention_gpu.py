@@ -67,7 +67,7 @@ class Case:
                 self.bufs[k] = d(v)
         if "out" not in self.bufs:
             self.bufs["out"] = d(encode(np.full(max(self.T, 1) * self.os, 7.0), self.out_t))
-            self.bufs["ws"] = d(np.full(self.ws_bytes // 4, np.nan, np.float32))
+            self.bufs["ws"] = d(np.zeros(self.ws_bytes, np.uint8))
 
     def outputs(self):
         o = decode(self.bufs["out"].download(storage(self.out_t), self.T * self.os), self.out_t).reshape(self.T, -1)

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "device_common.h"
 #include "mi355x-attention.h"
 
 namespace mi355x {
@@ -15,7 +16,8 @@ struct AttnArgs {
     const void *q, *k, *v;
     const int32_t *row_offsets, *kv_lens, *table;
     void *out;
-    float *ws;
+    float *ws;      // parts
+    int *counters;  // 0 before and after a call
     int64_t q_stride, out_stride, table_stride;
     int64_t head_stride;
     int64_t n_rows;
@@ -213,6 +215,97 @@ __device__ __forceinline__ int64_t out_at(const AttnArgs &a, const SeqGeo &g, in
     const int token = divided(row, a.group), group = static_cast<int>(a.group.d);
     const int64_t head = static_cast<int64_t>(kvh) * group + (row - token * group);
     return (g.first + g.tok_lo + token) * a.out_stride + head * hd;
+}
+
+// Parts of a row's sums that travel between workgroups of one launch, whose dies'
+// L2s do not see each other: stored and read past them, so that no L2 has to be
+// written back or emptied (fences that do so made 64 ragged requests 454 us
+// instead of 196).  A workgroup that has waited for its stores and met a barrier
+// may then count itself in.
+constexpr int kPastL2 = 16;  // the sc1 bit of a buffer operation
+struct FarParts {
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ __forceinline__ explicit FarParts(float *base)
+        : rsrc(__builtin_amdgcn_make_buffer_rsrc(base, 0, 0xFFFFFFFFu, kBufferWord3)) {}
+    __device__ __forceinline__ void store(int at, float v) const {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rsrc, 4 * at, 0, kPastL2);
+    }
+    __device__ __forceinline__ void store4(int at, f32x4 v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_a, v), rsrc, 4 * at, 0, kPastL2);
+    }
+    __device__ __forceinline__ float load(int at) const {
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, 4 * at, 0, kPastL2));
+    }
+    __device__ __forceinline__ f32x4 load4(int at) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, 4 * at, 0, kPastL2));
+    }
+};
+// The same of an earlier launch.
+struct NearParts {
+    const float *base;
+    __device__ __forceinline__ explicit NearParts(const float *b) : base(b) {}
+    __device__ __forceinline__ float load(int at) const { return base[at]; }
+    __device__ __forceinline__ f32x4 load4(int at) const { return *reinterpret_cast<const f32x4 *>(base + at); }
+};
+
+// Counts this workgroup in at *counter, which `n` of them do; true for the last
+// one, which finds the others' parts complete and leaves the counter at 0.
+// Called by all threads; `flag` is LDS.
+__device__ __forceinline__ bool last_of(int *counter, int n, int *flag) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's stores
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == n - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = before == n - 1;
+    }
+    __syncthreads();
+    return *flag != 0;
+}
+
+// Sums of 4 values of a row over some of its parts.
+struct Joined {
+    float top = -INFINITY, den = 0.0f;
+    f32x4 num = {0, 0, 0, 0};
+    __device__ __forceinline__ void add(float m, float l, f32x4 x) {
+        const float t = fmaxf(top, m), ref = finite_base(t);
+        const float f = __builtin_amdgcn_exp2f(top - ref), h = __builtin_amdgcn_exp2f(m - ref);
+        num = num * f + x * h;
+        den = den * f + l * h;
+        top = t;
+    }
+    __device__ __forceinline__ f32x4 value() const {
+        return den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den);
+    }
+};
+
+// Adds parts first, first + step, .. below n: part i has the row's 4 values at
+// values(i), its maximum at maximum(i) and its sum at total(i) of `parts`.  The
+// loads of eight parts go out together.
+template <typename P, typename V, typename M, typename L>
+__device__ __forceinline__ void join_parts(Joined &j, const P &parts, int n, int first, int step, V values, M maximum,
+                                           L total) {
+    for (int i = first; i < n; i += 8 * step) {
+        f32x4 x[8];
+        float m[8], l[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int p = min(i + k * step, n - 1);
+            x[k] = parts.load4(values(p));
+            m[k] = parts.load(maximum(p));
+            l[k] = parts.load(total(p));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (i + k * step < n) j.add(m[k], l[k], x[k]);
+    }
+}
+
+// A value that all lanes share, told to the compiler as such.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // Exclusive scan of one value per thread over a workgroup of WAVES wavefronts;

@@ -18,8 +18,9 @@
 // Work split.  All requests' keys, heads and row blocks form one line of
 // 128-key units; every workgroup takes an equal stretch of it, whatever the
 // lengths are, finds its place by a scan over the requests' lengths, and
-// writes the output of the rows that lie in its stretch whole.  The two that its ends
-// cut leave (m, l, sum) in the workspace, and a second launch joins them.
+// writes the output of the rows that lie in its stretch whole.  Of rows that the
+// ends of stretches cut each workgroup leaves (m, l, sum) in the workspace, and
+// the last of them to get there joins the parts.
 #include "attn_device.h"
 #include "internal.h"
 
@@ -51,14 +52,29 @@ __device__ __forceinline__ TokenWork token_work(const AttnArgs &a, const SeqGeo 
     return w;
 }
 
-// The units before each request, a request per thread: all of them at once, or
-// (more requests than threads) a part at a time.
+// The units before each request, a request per thread.  Up to 64 requests: every
+// wavefront scans them by itself.  More: the workgroup does, all of them at once
+// or a part at a time.
 template <int ROWS, int WAVES>
 struct Scan {
     int64_t total;
-    int64_t mine, before;  // of request threadIdx.x
+    int64_t mine, before;  // of request threadIdx.x (% 64)
 
     __device__ __forceinline__ void run(const AttnArgs &a, int64_t *tmp) {
+        if (a.n_seqs <= 64) {
+            const int lane = threadIdx.x & 63;
+            mine = lane < a.n_seqs ? token_work<ROWS>(a, seq_geo(a, lane)).units : 0;
+            int64_t in = mine;
+            if (a.n_seqs > 1)
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int64_t u = __shfl_up(in, d);
+                    if (lane >= d) in += u;
+                }
+            before = in - mine;
+            total = uniform(__shfl(in, a.n_seqs - 1));
+            return;
+        }
         total = 0;
         for (int base = 0; base < a.n_seqs; base += 64 * WAVES) {
             const int s = base + threadIdx.x;
@@ -71,10 +87,17 @@ struct Scan {
             }
             total += sum;
         }
+        total = uniform(total);
     }
 
     // The request that has unit u < total, and the units before it.
     __device__ __forceinline__ int find(const AttnArgs &a, int64_t u, int64_t *tmp, int64_t *first) const {
+        if (a.n_seqs <= 64) {
+            const uint64_t here = __ballot(u >= before && u < before + mine);
+            const int s = __builtin_ctzll(here | (uint64_t(1) << 63));
+            *first = uniform(__shfl(before, s));
+            return s;
+        }
         int64_t n = mine, at = before, carry = 0;
         __shared__ int64_t found_at;
         __shared__ int found;
@@ -92,8 +115,8 @@ struct Scan {
             }
         }
         __syncthreads();
-        *first = found_at;
-        return found;
+        *first = uniform(found_at);
+        return __builtin_amdgcn_readfirstlane(found);
     }
 };
 
@@ -109,7 +132,7 @@ struct TokenShape {
 };
 
 template <int TYPE, int HD, int MT>
-__global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD <= 128 ? 2 : 1) void attention_token_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD * MT <= 256 && HD <= 128 ? 2 : 1) void attention_token_kernel(AttnArgs a) {
     typedef Num<TYPE> N;
     typedef typename N::T T;
     typedef typename N::V8 V8;
@@ -130,7 +153,7 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD <= 128 ? 2 : 
     const int64_t u0 = stretch_begin(line, blockIdx.x), u1 = stretch_begin(line, blockIdx.x + 1);
     if (u0 >= u1) return;
     int64_t before;  // units before request seq
-    int seq = __builtin_amdgcn_readfirstlane(scan.find(a, u0, tmp, &before));
+    int seq = scan.find(a, u0, tmp, &before);
     T *vt = reinterpret_cast<T *>(lds + wave * S::kWaveBytes);
     float *ot = reinterpret_cast<float *>(lds + wave * S::kWaveBytes);
     SeqGeo g = seq_geo(a, seq);
@@ -312,7 +335,8 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD <= 128 ? 2 : 
         }
 
         // join the wavefronts' sums, 16 rows at a time
-        float *part = a.ws + (2 * static_cast<int64_t>(blockIdx.x) + (u != u0)) * S::kPartFloats;
+        const FarParts parts(a.ws);
+        const int part = (2 * blockIdx.x + (u != u0)) * S::kPartFloats;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const float sum = quad_sum(l[mt]);
@@ -354,85 +378,59 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD <= 128 ? 2 : 
                     const f32x4 v = den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den);
                     store_out4<TYPE>(a, out_at(a, g, kvh, row, HD) + c, v);
                 } else {
-                    *reinterpret_cast<f32x4 *>(part + (16 * mt + r) * HD + c) = num;
+                    parts.store4(part + (16 * mt + r) * HD + c, num);
                     if (c == 0) {
-                        part[S::kRows * HD + 16 * mt + r] = top;
-                        part[S::kRows * (HD + 1) + 16 * mt + r] = den;
+                        parts.store(part + S::kRows * HD + 16 * mt + r, top);
+                        parts.store(part + S::kRows * (HD + 1) + 16 * mt + r, den);
                     }
                 }
             }
             __syncthreads();
         }
         }
-        u += t1 - t0;
-    }
-}
-
-// Joins the parts of the rows that a boundary between two workgroups' stretches
-// cuts: block b those whose first cut is the start of workgroup b + 1.
-constexpr int kJoinThreads = 512;
-
-template <int TYPE, int HD, int MT>
-__global__ __launch_bounds__(kJoinThreads) void attention_token_join_kernel(AttnArgs a, int groups) {
-    typedef TokenShape<HD, MT> S;
-    constexpr int kWaves = kJoinThreads / 64;
-    __shared__ int64_t tmp[kWaves];
-    __shared__ f32x4 lds_num[kJoinThreads];
-    __shared__ float lds_den[kJoinThreads];
-    const int tid = threadIdx.x;
-    Scan<S::kRows, kWaves> scan;
-    scan.run(a, tmp);
-    const Stretches line = stretches(scan.total, groups);
-    const int64_t u_prev = stretch_begin(line, blockIdx.x), u_cut = stretch_begin(line, blockIdx.x + 1);
-    if (u_prev >= u_cut || u_cut >= line.total) return;
-    int64_t before;
-    const int seq = scan.find(a, u_cut, tmp, &before);
-    const SeqGeo g = seq_geo(a, seq);
-    const TokenWork w = token_work<S::kRows>(a, g);
-    const int64_t item = quotient(u_cut - before, w.tiles);
-    const int64_t begin = before + item * w.tiles, end = begin + w.tiles;
-    if (begin == u_cut || begin < u_prev) return;  // not cut here, or cut before
-    // the stretches blockIdx.x .. that of the last unit have a part each
-    const int n_parts = static_cast<int>(stretch_of(line, end - 1) - blockIdx.x) + 1;
-    const int kvh = static_cast<int>(quotient(item, w.blocks));
-    const int row0 = static_cast<int>(item - static_cast<int64_t>(kvh) * w.blocks) * S::kRows;
-    const int rows = min(S::kRows, g.rows - row0);
-    auto part_of = [&](int i) {  // the first part ends its stretch, the others begin theirs
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x + i) + (i == 0 && begin != u_prev);
-        return a.ws + slot * S::kPartFloats;
-    };
-    // threads: one per row and 4 values, and as many teams as fit share the parts
-    constexpr int kQuads = HD / 4;
-    for (int r0 = 0; r0 < rows; r0 += kJoinThreads / kQuads) {
-        const int n = min(kJoinThreads / kQuads, rows - r0) * kQuads;
-        const int teams = kJoinThreads / n, team = tid / n, r = r0 + tid % n / kQuads, c = tid % kQuads * 4;
-        const bool work = team < teams;
-        float top = -INFINITY;
-        if (work)
-            for (int i = 0; i < n_parts; ++i) top = fmaxf(top, part_of(i)[S::kRows * HD + r]);
-        const float ref = finite_base(top);
-        float den = 0.0f;
-        f32x4 num = {0, 0, 0, 0};
-        if (work)
-#pragma unroll 4
-            for (int i = team; i < n_parts; i += teams) {
-                const float *p = part_of(i);
-                const float f = __builtin_amdgcn_exp2f(p[S::kRows * HD + r] - ref);
-                den += f * p[S::kRows * (HD + 1) + r];
-                num += f * *reinterpret_cast<const f32x4 *>(p + r * HD + c);
+        if (!whole) {
+            const int64_t begin = u - t0, end = begin + w.tiles;
+            const int64_t from = stretch_of(line, begin);
+            const int n_parts = static_cast<int>(stretch_of(line, end - 1) - from) + 1;
+            if (last_of(a.counters + from, n_parts, &lds_odd[0])) {
+                // the first part ends its stretch (unless it is all of it), the others begin theirs
+                const FarParts parts(a.ws);
+                const int second = begin != stretch_begin(line, from);
+                auto part_of = [&](int i) {
+                    return (2 * (static_cast<int>(from) + i) + (i == 0 ? second : 0)) * S::kPartFloats;
+                };
+                // a thread per row and 4 values, and as many teams of them as fit share the parts
+                constexpr int kQuads = HD / 4;
+                f32x4 *nums = reinterpret_cast<f32x4 *>(lds);
+                float *dens = reinterpret_cast<float *>(nums + kTokenThreads), *tops = dens + kTokenThreads;
+                const int rows = row_last - row0 + 1;
+                int id = tid;
+                asm volatile("" : "+v"(id));  // as above
+                for (int r0 = 0; r0 < rows; r0 += kTokenThreads / kQuads) {
+                    const int n = min(kTokenThreads / kQuads, rows - r0) * kQuads;
+                    const int teams = min(n_parts, kTokenThreads / n), team = id / n;
+                    const int r = r0 + id % n / kQuads, c = id % kQuads * 4;
+                    Joined j;
+                    if (team < teams)
+                        join_parts(
+                            j, parts, n_parts, team, teams, [&](int i) { return part_of(i) + r * HD + c; },
+                            [&](int i) { return part_of(i) + S::kRows * HD + r; },
+                            [&](int i) { return part_of(i) + S::kRows * (HD + 1) + r; });
+                    if (teams > 1) {
+                        nums[id] = j.num;
+                        dens[id] = j.den;
+                        tops[id] = j.top;
+                        __syncthreads();
+                        if (team == 0)
+                            for (int t = 1; t < teams; ++t) j.add(tops[t * n + id], dens[t * n + id], nums[t * n + id]);
+                    }
+                    if (team == 0) store_out4<TYPE>(a, out_at(a, g, kvh, row0 + r, HD) + c, j.value());
+                    if (teams > 1) __syncthreads();
+                }
             }
-        lds_num[tid] = num;
-        lds_den[tid] = den;
-        __syncthreads();
-        if (team == 0) {
-            for (int t = 1; t < teams; ++t) {
-                num += lds_num[t * n + tid];
-                den += lds_den[t * n + tid];
-            }
-            const f32x4 v = den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den);
-            store_out4<TYPE>(a, out_at(a, g, kvh, row0 + r, HD) + c, v);
+            __syncthreads();  // lds_odd, lds
         }
-        __syncthreads();
+        u += t1 - t0;
     }
 }
 
@@ -440,26 +438,33 @@ __global__ __launch_bounds__(kJoinThreads) void attention_token_join_kernel(Attn
 constexpr int kTokenGroupsPerCu = 4;
 
 template <int TYPE, int HD, int MT>
-int launch_token(mi355x_ctx *ctx, const AttnArgs &a) {
+int launch_token(mi355x_ctx *ctx, const AttnArgs &a, int64_t rows) {
     const void *kernel = reinterpret_cast<const void *>(attention_token_kernel<TYPE, HD, MT>);
-    const int groups = ctx->num_cus * std::max(1, std::min(kTokenGroupsPerCu, occupancy(kernel, kTokenThreads, 0)));
-    attention_token_kernel<TYPE, HD, MT><<<groups, kTokenThreads, 0, ctx->stream>>>(a);
-    MI355X_HIP(hipGetLastError());
-    attention_token_join_kernel<TYPE, HD, MT><<<groups - 1, kJoinThreads, 0, ctx->stream>>>(a, groups);
+    const int64_t fit = ctx->num_cus * std::max(1, std::min(kTokenGroupsPerCu, occupancy(kernel, kTokenThreads, 0)));
+    // no more than the units that the table and the rows allow
+    const int64_t heads = static_cast<int64_t>(a.n_seqs) * a.n_kv_heads, tiles = a.reach / kUnitKeys + 1;
+    const int64_t blocks = std::max<int64_t>(1, rows / (16 * MT));
+    const int64_t units = heads > fit ? fit : heads * std::min(fit, tiles * std::min(fit, blocks));
+    attention_token_kernel<TYPE, HD, MT>
+        <<<static_cast<unsigned>(std::min(fit, units)), kTokenThreads, 0, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
     return MI355X_OK;
 }
 
 template <int TYPE, int HD>
 int launch_forms(mi355x_ctx *ctx, const AttnArgs &a, int64_t rows) {
-    if (rows <= 16) return launch_token<TYPE, HD, 1>(ctx, a);
-    if (rows <= 32) return launch_token<TYPE, HD, 2>(ctx, a);
+    if (rows <= 16) return launch_token<TYPE, HD, 1>(ctx, a, rows);
+    if (rows <= 32) return launch_token<TYPE, HD, 2>(ctx, a, rows);
+    if constexpr (HD <= 128) {
+        if (rows <= 48) return launch_token<TYPE, HD, 3>(ctx, a, rows);
+        if (rows <= 64) return launch_token<TYPE, HD, 4>(ctx, a, rows);
+    }
     AttnArgs b = a;
     b.row_limit = 0;
     if (a.n_seqs > 1) {  // some may add few tokens
         AttnArgs c = a;
         c.row_limit = b.row_limit = 16;
-        if (int rc = launch_token<TYPE, HD, 1>(ctx, c)) return rc;
+        if (int rc = launch_token<TYPE, HD, 1>(ctx, c, 16)) return rc;
     }
     return launch_attention_chunk(ctx, b, TYPE, HD);
 }
@@ -476,9 +481,14 @@ int launch_sizes(mi355x_ctx *ctx, const AttnArgs &a, int head_dim, int64_t rows)
 
 }  // namespace
 
+// One counter per workgroup of the token form (and per row block of a split chunk form, which are fewer).
+static size_t counter_bytes(const mi355x_ctx *ctx) {
+    return (static_cast<size_t>(ctx->num_cus) * kTokenGroupsPerCu * 4 + 255) / 256 * 256;
+}
+
 size_t paged_attention_workspace_bytes(const mi355x_ctx *ctx, int, int, int head_dim) {
-    return std::max(static_cast<size_t>(ctx->num_cus * kTokenGroupsPerCu) * 2 * 32 * (head_dim + 2) * 4,
-                    attention_chunk_workspace(ctx, head_dim));
+    return counter_bytes(ctx) + std::max(static_cast<size_t>(ctx->num_cus * kTokenGroupsPerCu) * 2 * 64 * (head_dim + 2) * 4,
+                                         attention_chunk_workspace(ctx, head_dim));
 }
 
 int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &u) {
@@ -490,7 +500,8 @@ int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &u
     a.kv_lens = u.kv_lens;
     a.table = u.block_table;
     a.out = u.out;
-    a.ws = static_cast<float *>(u.workspace);
+    a.counters = static_cast<int *>(u.workspace);
+    a.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(u.workspace) + counter_bytes(ctx));
     a.q_stride = u.q_stride;
     a.out_stride = u.out_stride;
     a.table_stride = u.table_stride;

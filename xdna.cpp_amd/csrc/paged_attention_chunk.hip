@@ -344,63 +344,57 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
 
         l = half_sum(l);
         int r = 32 * wave + col;
-        if (!real || (only >= 0 && r != only)) continue;
         asm volatile("" : "+v"(r));  // the addresses below are formed here, not kept through the loops
-        if (a.split == 1) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const int64_t at = out_at(a, g, kvh, it.row0 + r, HD);
+        if (real && (only < 0 || r == only)) {
+            if (a.split == 1) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const int64_t at = out_at(a, g, kvh, it.row0 + r, HD);
 #pragma unroll
-            for (int d = 0; d < kBlocks; ++d)
+                for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4 v = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-                    store_out4<TYPE>(a, at + 32 * d + 8 * i + 4 * half, l == 0.0f ? f32x4{0, 0, 0, 0} : v * inv);
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 v = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                        store_out4<TYPE>(a, at + 32 * d + 8 * i + 4 * half, l == 0.0f ? f32x4{0, 0, 0, 0} : v * inv);
+                    }
+            } else {
+                float *w = a.ws + static_cast<int64_t>(blockIdx.x) * S::kPartFloats;
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<f32x4 *>(w + r * HD + 32 * d + 8 * i + 4 * half) =
+                            f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                if (half == 0) {
+                    w[kRows * HD + r] = m;
+                    w[kRows * (HD + 1) + r] = l;
                 }
-        } else {
-            float *w = a.ws + static_cast<int64_t>(blockIdx.x) * S::kPartFloats;
-#pragma unroll
-            for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<f32x4 *>(w + r * HD + 32 * d + 8 * i + 4 * half) =
-                        f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-            if (half == 0) {
-                w[kRows * HD + r] = m;
-                w[kRows * (HD + 1) + r] = l;
             }
         }
     }
 }
 
-// Joins the parts of each row block and KV head.
+// Joins the parts of each row block and KV head: a workgroup kJoinRows of its
+// rows, a thread 4 values.  (In the kernel above, by the last of a block's
+// workgroups, the parts of a chunk of 512 tokens cost 40 us instead of JJ: one CU
+// reads what 16 do here.)
+constexpr int kJoinThreads = 256;
+
 template <int TYPE, int HD>
-__global__ __launch_bounds__(256) void attention_chunk_join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kJoinThreads) void attention_chunk_join_kernel(AttnArgs a) {
     typedef ChunkShape<HD, 4> S;
-    constexpr int kRows = S::kRows;
+    constexpr int kRows = S::kRows, kQuads = HD / 4;
     const int kvh = static_cast<int>(blockIdx.x % a.n_kv_heads);
-    const int64_t rest = blockIdx.x / a.n_kv_heads, blocks = gridDim.x / a.n_kv_heads;
+    const int rest = static_cast<int>(blockIdx.x / a.n_kv_heads), blocks = static_cast<int>(gridDim.x / a.n_kv_heads);
     ChunkItem it;
     if (!chunk_item<4>(a, blocks - 1 - rest, kvh, &it)) return;
-    const int rows = min(kRows, it.g.rows - it.row0);
-    constexpr int kQuads = HD / 4;
-    for (int i = threadIdx.x + 256 * blockIdx.y; i < rows * kQuads; i += 256 * gridDim.y) {
-        const int r = i / kQuads, c = i % kQuads * 4;
-        auto part_of = [&](int p) { return a.ws + ((rest * a.split + p) * a.n_kv_heads + kvh) * S::kPartFloats; };
-        float top = -INFINITY;
-        for (int p = 0; p < a.split; ++p) top = fmaxf(top, part_of(p)[kRows * HD + r]);
-        const float ref = finite_base(top);
-        float den = 0.0f;
-        f32x4 num = {0, 0, 0, 0};
-#pragma unroll 4
-        for (int p = 0; p < a.split; ++p) {
-            const float *w = part_of(p);
-            const float f = __builtin_amdgcn_exp2f(w[kRows * HD + r] - ref);
-            den += f * w[kRows * (HD + 1) + r];
-            num += f * *reinterpret_cast<const f32x4 *>(w + r * HD + c);
-        }
-        store_out4<TYPE>(a, out_at(a, it.g, kvh, it.row0 + r, HD) + c,
-                         den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den));
-    }
+    const int i = threadIdx.x + kJoinThreads * blockIdx.y, r = i / kQuads, c = i % kQuads * 4;
+    if (r >= kRows || r >= it.g.rows - it.row0) return;
+    Joined j;
+    auto part_of = [&](int p) { return ((rest * a.split + p) * a.n_kv_heads + kvh) * S::kPartFloats; };
+    join_parts(
+        j, NearParts(a.ws), a.split, 0, 1, [&](int p) { return part_of(p) + r * HD + c; },
+        [&](int p) { return part_of(p) + kRows * HD + r; }, [&](int p) { return part_of(p) + kRows * (HD + 1) + r; });
+    store_out4<TYPE>(a, out_at(a, it.g, kvh, it.row0 + r, HD) + c, j.value());
 }
 
 // Workgroups that a call is split into at most, while that is more than its row blocks.
@@ -435,8 +429,8 @@ int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
         <<<static_cast<unsigned>(items * a.split), 256, ChunkShape<HD, 4>::kLds, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
     if (a.split > 1) {
-        const dim3 grid(static_cast<unsigned>(items), 4);
-        attention_chunk_join_kernel<TYPE, HD><<<grid, 256, 0, ctx->stream>>>(a);
+        const dim3 grid(static_cast<unsigned>(items), (128 * HD / 4 + kJoinThreads - 1) / kJoinThreads);
+        attention_chunk_join_kernel<TYPE, HD><<<grid, kJoinThreads, 0, ctx->stream>>>(a);
         MI355X_HIP(hipGetLastError());
     }
     return MI355X_OK;
