@@ -138,24 +138,26 @@ def attention(q, pool, offsets, kv_lens, table, scale, softcap=0.0, window=0, ca
         j = np.arange(max(0, min(kv, reach)))
         pg = table[s][j // pool.page]
         good = (pg >= 0) & (pg < pool.n_pages)
-        for i in range(n):
-            r, p = int(offsets[s]) + i, kv - n + i
-            if r >= T:
-                continue
-            see = good & ((j <= p) if causal else True)
-            if window:
-                see = see & (j > p - window)
-            jj, pp = j[see], pg[see]
-            if not jj.size:
-                continue
-            k, v = pool.k[pp, jj % pool.page], pool.v[pp, jj % pool.page]  # [n, kv heads, hd]
-            for h in range(H):
-                kh, vh = k[:, h // G], v[:, h // G]
-                sc = scale * (kh @ q[r, h])
-                size[r, h] = np.abs(scale) * (np.abs(kh) @ np.abs(q[r, h])).max()
-                if softcap:
-                    sc = softcap * np.tanh(sc / softcap)
-                w = np.exp(sc - sc.max())
-                w /= w.sum()
-                out[r, h], mag[r, h] = w @ vh, w @ np.abs(vh)
+        r0, i = int(offsets[s]), np.arange(n)
+        i = i[r0 + i < T]
+        if not j.size or not i.size:
+            continue
+        p = (kv - n + i)[:, None]
+        see = np.broadcast_to(good, (i.size, j.size)) & ((j <= p) if causal else True)
+        if window:
+            see = see & (j > p - window)
+        pp = np.where(good, pg, 0)
+        k, v = pool.k[pp, j % pool.page], pool.v[pp, j % pool.page]  # [keys, kv heads, hd]
+        some = see.any(0)
+        k, v = np.where(some[:, None, None], k, 0.0), np.where(some[:, None, None], v, 0.0)
+        for h in range(H):
+            kh, vh, qh = k[:, h // G], v[:, h // G], q[r0 + i, h]
+            sc = scale * (qh @ kh.T)
+            size[r0 + i, h] = np.where(see, np.abs(scale) * (np.abs(qh) @ np.abs(kh).T), 0.0).max(1)
+            if softcap:
+                sc = softcap * np.tanh(sc / softcap)
+            sc = np.where(see, sc, -np.inf)
+            w = np.exp(sc - np.where(see.any(1), sc.max(1), 0.0)[:, None])
+            w /= np.maximum(w.sum(1, keepdims=True), 1e-300)
+            out[r0 + i, h], mag[r0 + i, h] = w @ vh, w @ np.abs(vh)
     return out, mag, size

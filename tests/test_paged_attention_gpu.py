@@ -132,6 +132,24 @@ def test_chunks(ctx, hq, hk, hd, t, out):
     go(ctx, [37, 1, 150, 5], [37, 200, 333, 64], hq, hk, hd, t, out)
 
 
+@pytest.mark.parametrize("t,out", [(F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)])
+@pytest.mark.parametrize("hd,hq,hk,softcap", [(64, 8, 1, 0.0), (96, 16, 2, 25.0), (128, 14, 2, 0.0), (256, 8, 1, 0.0)])
+def test_many_rows(ctx, hd, hq, hk, softcap, t, out):
+    """Enough head rows for workgroups of 256 of them on every CU, and few ones among them."""
+    go(ctx, [700] * 6 + [1, 3] + [997] * 5, [700] * 6 + [900, 50] + [1000] * 5, hq, hk, hd, t, out, softcap=softcap)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+@pytest.mark.parametrize("q_lens", [[1, 2], [40, 100]])
+def test_scales_of_any_sign(ctx, q_lens, scale):
+    c = Case(ctx, q_lens, [300, 130], 4, 2, 64, F16, F32)
+    try:
+        c.scale = c.args.scale = scale
+        c.run().verify(scale)
+    finally:
+        c.free()
+
+
 @pytest.mark.parametrize("kv", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 1000, 4097])
 def test_every_length(ctx, kv):
     go(ctx, [1], [kv], 4, 2, 64, F16, F32, page=8)

@@ -30,7 +30,7 @@ struct AttnArgs {
     int n_seqs, n_kv_heads;
     int n_pages, shift, window, causal, f32_out;
     int split;    // chunk form: parts of an item's keys
-    int by_page;  // chunk form: the rows of a load share a page, 32-bit offsets within it
+    int by_page;  // the rows of a load into LDS share a page, with 32-bit offsets in it
 };
 
 constexpr float kLog2e = 1.44269504088896341f;
@@ -89,6 +89,13 @@ __device__ __forceinline__ bool not_finite(u32x4_a v) {
 __device__ __forceinline__ u32x2_a lds_read_transposed(const s16x4 *__restrict__ p) {
     return __builtin_bit_cast(
         u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p)));
+}
+
+// 16 bytes per lane from memory to LDS, lane after lane from `to` on.
+__device__ __forceinline__ void load_lds16(const void *from, unsigned char *to) {
+    __builtin_amdgcn_global_load_lds(
+        reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(reinterpret_cast<uintptr_t>(from)),
+        (__attribute__((address_space(3))) uint32_t *)(to), 16, 0, 0);
 }
 
 // Scores of n values of q . k; tanh x as 1 - 2 / (1 + e^2x), within 2^-23 of 1.
@@ -159,16 +166,20 @@ struct SeqGeo {
     int64_t kv;
 };
 
-__device__ __forceinline__ SeqGeo seq_geo(const AttnArgs &a, int s) {
-    const SeqRows r = seq_rows(a.row_offsets[s], a.row_offsets[s + 1], a.n_rows);
+__device__ __forceinline__ SeqGeo seq_geo(const AttnArgs &a, int32_t begin, int32_t end, int32_t kv) {
+    const SeqRows r = seq_rows(begin, end, a.n_rows);
     SeqGeo g;
     g.first = r.first;
     g.tok_lo = r.lo;
     g.n_tok = static_cast<int>(r.hi - r.lo);
     g.rows = g.n_tok * static_cast<int>(a.group.d);
-    g.kv = a.kv_lens[s];
+    g.kv = kv;
     g.pos0 = g.kv - r.n;
     return g;
+}
+
+__device__ __forceinline__ SeqGeo seq_geo(const AttnArgs &a, int s) {
+    return seq_geo(a, a.row_offsets[s], a.row_offsets[s + 1], a.kv_lens[s]);
 }
 
 // Tokens lo .. hi - 1 (at most 2^30) that a token of the request sees.

@@ -33,19 +33,19 @@ constexpr int kTokenWaves = 4;
 constexpr int kTokenKeys = 32;                            // of a wavefront's tile
 constexpr int kUnitKeys = kTokenWaves * kTokenKeys;       // of a workgroup's unit
 constexpr int kTokenThreads = 64 * kTokenWaves;
+constexpr int kTokenRows = 16;                            // head rows of a workgroup: columns of a product
 
-// The token form's units of a request: per KV head and block of ROWS head rows
+// The token form's units of a request: per KV head and block of kTokenRows head rows
 // one per kUnitKeys keys (one without keys: its rows get zeros).
 struct TokenWork {
     int64_t units;
     int blocks, tiles, key_lo;
 };
 
-template <int ROWS>
 __device__ __forceinline__ TokenWork token_work(const AttnArgs &a, const SeqGeo &g) {
     TokenWork w{0, 0, 1, 0};
     if (g.rows <= 0 || g.rows > a.row_limit) return w;
-    w.blocks = (g.rows + ROWS - 1) / ROWS;
+    w.blocks = (g.rows + kTokenRows - 1) / kTokenRows;
     w.key_lo = token_keys(a, g, g.tok_lo).lo;
     w.tiles = max(1, (token_keys(a, g, g.tok_lo + g.n_tok - 1).hi - w.key_lo + kUnitKeys - 1) / kUnitKeys);
     w.units = static_cast<int64_t>(w.blocks) * w.tiles * a.n_kv_heads;
@@ -55,15 +55,29 @@ __device__ __forceinline__ TokenWork token_work(const AttnArgs &a, const SeqGeo 
 // The units before each request, a request per thread.  Up to 64 requests: every
 // wavefront scans them by itself.  More: the workgroup does, all of them at once
 // or a part at a time.
-template <int ROWS, int WAVES>
+template <int WAVES>
 struct Scan {
     int64_t total;
     int64_t mine, before;  // of request threadIdx.x (% 64)
+    int32_t row_begin, row_end, kv;  // up to 64 requests: its offsets and length
+
+    // Request s's rows and tokens, which up to 64 requests' lanes have.
+    __device__ __forceinline__ SeqGeo geo(const AttnArgs &a, int s) const {
+        if (a.n_seqs > 64) return seq_geo(a, s);
+        return seq_geo(a, __builtin_amdgcn_readlane(row_begin, s), __builtin_amdgcn_readlane(row_end, s),
+                       __builtin_amdgcn_readlane(kv, s));
+    }
 
     __device__ __forceinline__ void run(const AttnArgs &a, int64_t *tmp) {
         if (a.n_seqs <= 64) {
             const int lane = threadIdx.x & 63;
-            mine = lane < a.n_seqs ? token_work<ROWS>(a, seq_geo(a, lane)).units : 0;
+            row_begin = row_end = kv = 0;
+            if (lane < a.n_seqs) {
+                row_begin = a.row_offsets[lane];
+                row_end = a.row_offsets[lane + 1];
+                kv = a.kv_lens[lane];
+            }
+            mine = lane < a.n_seqs ? token_work(a, seq_geo(a, row_begin, row_end, kv)).units : 0;
             int64_t in = mine;
             if (a.n_seqs > 1)
 #pragma unroll
@@ -78,7 +92,7 @@ struct Scan {
         total = 0;
         for (int base = 0; base < a.n_seqs; base += 64 * WAVES) {
             const int s = base + threadIdx.x;
-            const int64_t n = s < a.n_seqs ? token_work<ROWS>(a, seq_geo(a, s)).units : 0;
+            const int64_t n = s < a.n_seqs ? token_work(a, seq_geo(a, s)).units : 0;
             int64_t sum;
             const int64_t at = group_scan<WAVES>(n, tmp, &sum);
             if (base == 0) {
@@ -105,7 +119,7 @@ struct Scan {
             const int s = base + threadIdx.x;
             if (a.n_seqs > 64 * WAVES) {
                 int64_t sum;
-                n = s < a.n_seqs ? token_work<ROWS>(a, seq_geo(a, s)).units : 0;
+                n = s < a.n_seqs ? token_work(a, seq_geo(a, s)).units : 0;
                 at = carry + group_scan<WAVES>(n, tmp, &sum);
                 carry += sum;
             }
@@ -116,27 +130,28 @@ struct Scan {
         }
         __syncthreads();
         *first = uniform(found_at);
-        return __builtin_amdgcn_readfirstlane(found);
+        const int s = __builtin_amdgcn_readfirstlane(found);
+        __syncthreads();
+        return s;
     }
 };
 
-template <int HD, int MT>
+template <int HD>
 struct TokenShape {
-    static constexpr int kRows = 16 * MT;
     static constexpr int kVStride = HD + 16;  // values: rows of V start 8 banks apart
     static constexpr int kWaveBytes = kTokenKeys * kVStride * 2;
     static constexpr int kOStride = HD + 4;   // floats of a joined row
     static_assert(16 * kOStride * 4 <= kWaveBytes, "a wavefront's sums fit where its V tile was");
-    // a part in the workspace: sums of kRows rows, then m, then l
-    static constexpr int kPartFloats = kRows * (HD + 2);
+    // a part in the workspace: sums of kTokenRows rows, then m, then l
+    static constexpr int kPartFloats = kTokenRows * (HD + 2);
 };
 
-template <int TYPE, int HD, int MT>
-__global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD * MT <= 256 && HD <= 128 ? 2 : 1) void attention_token_kernel(AttnArgs a) {
+template <int TYPE, int HD>
+__global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) void attention_token_kernel(AttnArgs a) {
     typedef Num<TYPE> N;
     typedef typename N::T T;
     typedef typename N::V8 V8;
-    typedef TokenShape<HD, MT> S;
+    typedef TokenShape<HD> S;
     constexpr int kSteps = HD / 32;     // of a 16-key score product
     constexpr int kBlocks = HD / 16;    // of 16 output values
     constexpr int kChunks = HD / 8;     // 16-byte chunks of a token's head
@@ -147,7 +162,7 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD * MT <= 256 &
     __shared__ int64_t tmp[kTokenWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, quad = lane >> 4;
-    Scan<S::kRows, kTokenWaves> scan;
+    Scan<kTokenWaves> scan;
     scan.run(a, tmp);
     const Stretches line = stretches(scan.total, gridDim.x);
     const int64_t u0 = stretch_begin(line, blockIdx.x), u1 = stretch_begin(line, blockIdx.x + 1);
@@ -156,44 +171,40 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD * MT <= 256 &
     int seq = scan.find(a, u0, tmp, &before);
     T *vt = reinterpret_cast<T *>(lds + wave * S::kWaveBytes);
     float *ot = reinterpret_cast<float *>(lds + wave * S::kWaveBytes);
-    SeqGeo g = seq_geo(a, seq);
-    TokenWork w = token_work<S::kRows>(a, g);
+    SeqGeo g = scan.geo(a, seq);
+    TokenWork w = token_work(a, g);
     for (int64_t u = u0; u < u1;) {
         while (u >= before + w.units) {  // the next request with rows
             before += w.units;
             ++seq;
-            g = seq_geo(a, seq);
-            w = token_work<S::kRows>(a, g);
+            g = scan.geo(a, seq);
+            w = token_work(a, g);
         }
         const int64_t item = quotient(u - before, w.tiles);
         const int t0 = static_cast<int>(u - before - item * w.tiles);
         const int t1 = static_cast<int>(idx_min(w.tiles, t0 + (u1 - u)));
         const int kvh = static_cast<int>(quotient(item, w.blocks));
-        const int row0 = static_cast<int>(item - static_cast<int64_t>(kvh) * w.blocks) * S::kRows;
-        const int row_last = min(row0 + S::kRows, g.rows) - 1;
+        const int row0 = static_cast<int>(item - static_cast<int64_t>(kvh) * w.blocks) * kTokenRows;
+        const int row_last = min(row0 + kTokenRows, g.rows) - 1;
         // tokens that some row of the block sees, and those that all of them see
         const Keys kf = token_keys(a, g, g.tok_lo + divided(row0, a.group));
         const Keys kl = token_keys(a, g, g.tok_lo + divided(row_last, a.group));
         const int all_lo = kl.lo, all_hi = kf.hi;
         const bool whole = t0 == 0 && t1 == w.tiles;
 
-        V8 qf[MT][kSteps];
-        int row_lo[MT], row_hi[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const bool real = row0 + 16 * mt + col < g.rows;
-            const int row = real ? row0 + 16 * mt + col : 0, tok = divided(row, a.group);
-            const int64_t token = g.tok_lo + tok;
-            const Keys kr = token_keys(a, g, token);
-            row_lo[mt] = kr.lo;
-            row_hi[mt] = real ? kr.hi : 0;
+        V8 qf[kSteps];
+        const bool real = row0 + col < g.rows;
+        const int row = real ? row0 + col : 0, tok = divided(row, a.group);
+        const Keys mine = token_keys(a, g, g.tok_lo + tok);
+        const int row_lo = mine.lo, row_hi = real ? mine.hi : 0;
+        {
             const int64_t head = static_cast<int64_t>(kvh) * a.group.d + (row - tok * static_cast<int>(a.group.d));
-            const T *q = static_cast<const T *>(a.q) + (g.first + token) * a.q_stride + head * HD;
+            const T *q = static_cast<const T *>(a.q) + (g.first + g.tok_lo + tok) * a.q_stride + head * HD;
 #pragma unroll
             for (int st = 0; st < kSteps; ++st) {
                 V8 z = {};
                 if (real) z = *reinterpret_cast<const V8 *>(q + 32 * st + 8 * quad);
-                qf[mt][st] = z;
+                qf[st] = z;
             }
         }
         const int32_t *table = a.table + seq * a.table_stride;
@@ -205,188 +216,159 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD * MT <= 256 &
         // zero would not take it away), the rows are done again one by one.
         int some_lo = kf.lo, some_hi = kl.hi;
         bool odd = false;
-        for (int only = -1; only < S::kRows; ++only) {
-        if (only >= 0) {
-            if (!odd || row0 + only >= g.rows) break;
-            const Keys kr = token_keys(a, g, g.tok_lo + divided(row0 + only, a.group));
-            some_lo = kr.lo;
-            some_hi = kr.hi;
-        }
-        bool odd_lane = false;
-        f32x4 o[MT][kBlocks];
-        float m[MT], l[MT];
+        for (int only = -1; only < kTokenRows; ++only) {
+            if (only >= 0) {
+                if (!odd || row0 + only >= g.rows) break;
+                const Keys kr = token_keys(a, g, g.tok_lo + divided(row0 + only, a.group));
+                some_lo = kr.lo;
+                some_hi = kr.hi;
+            }
+            bool odd_lane = false;
+            f32x4 o[kBlocks];
+            float m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            m[mt] = -INFINITY;
-            l[mt] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < kBlocks; ++d) o[mt][d] = f32x4{0, 0, 0, 0};
-        }
+            for (int d = 0; d < kBlocks; ++d) o[d] = f32x4{0, 0, 0, 0};
 
-        u32x4_a kreg[2][kSteps], vreg[kVLoads];
-        uint32_t seen = 0;  // keys of the tile in registers that lie on pages of the pool
-        // the table entry of key (lane & 31) of a tile
-        auto entry = [&](int base) {
-            const int key = base + (lane & 31);
-            return key >= some_lo && key < some_hi ? table[key >> a.shift] : -1;
-        };
-        auto load = [&](int base, int32_t page) {
-            const bool good = page_in_pool(page, a.n_pages);
-            const int64_t off = good ? token_at(a, page, base + (lane & 31)) : 0;
-            seen = static_cast<uint32_t>(__ballot(good));
+            u32x4_a kreg[2][kSteps], vreg[kVLoads];
+            uint32_t seen = 0;  // keys of the tile in registers that lie on pages of the pool
+            // the table entry of key (lane & 31) of a tile
+            auto entry = [&](int base) {
+                const int key = base + (lane & 31);
+                return key >= some_lo && key < some_hi ? table[key >> a.shift] : -1;
+            };
+            auto load = [&](int base, int32_t page) {
+                const bool good = page_in_pool(page, a.n_pages);
+                const int64_t off = good ? token_at(a, page, base + (lane & 31)) : 0;
+                seen = static_cast<uint32_t>(__ballot(good));
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const T *k = kp + __shfl(off, 16 * b + col);
+                for (int b = 0; b < 2; ++b) {
+                    const T *k = kp + __shfl(off, 16 * b + col);
 #pragma unroll
-                for (int st = 0; st < kSteps; ++st) kreg[b][st] = *reinterpret_cast<const u32x4_a *>(k + 32 * st);
+                    for (int st = 0; st < kSteps; ++st) kreg[b][st] = *reinterpret_cast<const u32x4_a *>(k + 32 * st);
+                }
+#pragma unroll
+                for (int i = 0; i < kVLoads; ++i) {
+                    const int idx = 64 * i + lane;
+                    const T *v = vp + __shfl(off, idx / kChunks) + idx % kChunks * 8;
+                    vreg[i] = *reinterpret_cast<const u32x4_a *>(v);
+                }
+            };
+            // this wavefront's tiles: every kTokenWaves-th
+            const int first = w.key_lo + t0 * kUnitKeys + wave * kTokenKeys;
+            const int end = min(some_hi, w.key_lo + t1 * kUnitKeys);
+            int32_t next = -1;
+            if (first < end) {
+                load(first, entry(first));
+                next = entry(first + kUnitKeys);
             }
-#pragma unroll
-            for (int i = 0; i < kVLoads; ++i) {
-                const int idx = 64 * i + lane;
-                const T *v = vp + __shfl(off, idx / kChunks) + idx % kChunks * 8;
-                vreg[i] = *reinterpret_cast<const u32x4_a *>(v);
-            }
-        };
-        // this wavefront's tiles: every kTokenWaves-th
-        const int first = w.key_lo + t0 * kUnitKeys + wave * kTokenKeys;
-        const int end = min(some_hi, w.key_lo + t1 * kUnitKeys);
-        int32_t next = -1;
-        if (first < end) {
-            load(first, entry(first));
-            next = entry(first + kUnitKeys);
-        }
-        for (int base = first; base < end; base += kUnitKeys) {
-            const uint32_t now = seen;
-            float s[MT][8];  // keys 16 (i / 4) + 4 quad + i % 4
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int base = first; base < end; base += kUnitKeys) {
+                const uint32_t now = seen;
+                float s[8];  // keys 16 (i / 4) + 4 quad + i % 4
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     f32x4 c = {0, 0, 0, 0};
 #pragma unroll
-                    for (int st = 0; st < kSteps; ++st)
-                        c = N::mfma16(__builtin_bit_cast(V8, kreg[b][st]), qf[mt][st], c);
+                    for (int st = 0; st < kSteps; ++st) c = N::mfma16(__builtin_bit_cast(V8, kreg[b][st]), qf[st], c);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[mt][4 * b + i] = c[i];
+                    for (int i = 0; i < 4; ++i) s[4 * b + i] = c[i];
                 }
-            // every key of the tile seen by every row
-            const bool full = base >= all_lo && base + kTokenKeys <= all_hi && now == 0xFFFFFFFFu;
+                // every key of the tile seen by every row
+                const bool full = base >= all_lo && base + kTokenKeys <= all_hi && now == 0xFFFFFFFFu;
 #pragma unroll
-            for (int i = 0; i < kVLoads; ++i) {
-                const int idx = 64 * i + lane, key = idx / kChunks;
-                u32x4_a v = vreg[i];
-                if (!full) {
-                    if (!((now >> key) & 1)) v = u32x4_a{0, 0, 0, 0};
-                    odd_lane |= not_finite<TYPE>(v);
+                for (int i = 0; i < kVLoads; ++i) {
+                    const int idx = 64 * i + lane, key = idx / kChunks;
+                    u32x4_a v = vreg[i];
+                    if (!full) {
+                        if (!((now >> key) & 1)) v = u32x4_a{0, 0, 0, 0};
+                        odd_lane |= not_finite<TYPE>(v);
+                    }
+                    *reinterpret_cast<u32x4_a *>(vt + key * S::kVStride + idx % kChunks * 8) = v;
                 }
-                *reinterpret_cast<u32x4_a *>(vt + key * S::kVStride + idx % kChunks * 8) = v;
-            }
-            const int after = base + kUnitKeys;
-            if (after < end) {
-                load(after, next);
-                next = entry(after + kUnitKeys);
-            }
-            V8 hi[MT], lo[MT];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                scores2(s[mt], a);
+                const int after = base + kUnitKeys;
+                if (after < end) {
+                    load(after, next);
+                    next = entry(after + kUnitKeys);
+                }
+                scores2(s, a);
                 if (!full) {
-                    const uint32_t see = (now & range_mask<uint32_t>(row_lo[mt], row_hi[mt], base)) >> (4 * quad);
+                    const uint32_t see = (now & range_mask<uint32_t>(row_lo, row_hi, base)) >> (4 * quad);
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (!((see >> (16 * (i >> 2) + (i & 3))) & 1)) s[mt][i] = -INFINITY;
+                        if (!((see >> (16 * (i >> 2) + (i & 3))) & 1)) s[i] = -INFINITY;
                 }
-                float top = s[mt][0];
+                float top = s[0];
 #pragma unroll
-                for (int i = 1; i < 8; ++i) top = fmaxf(top, s[mt][i]);
+                for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
                 top = quad_max(top);
-                if (__any(top > m[mt] + kSlack || (m[mt] == -INFINITY && top > m[mt]))) {
-                    const float m_new = fmaxf(m[mt], top), keep = __builtin_amdgcn_exp2f(m[mt] - finite_base(m_new));
-                    l[mt] *= keep;
+                if (__any(top > m + kSlack || (m == -INFINITY && top > m))) {
+                    const float m_new = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
+                    l *= keep;
 #pragma unroll
-                    for (int d = 0; d < kBlocks; ++d) o[mt][d] *= keep;
-                    m[mt] = m_new;
+                    for (int d = 0; d < kBlocks; ++d) o[d] *= keep;
+                    m = m_new;
                 }
-                const float ref = finite_base(m[mt]);
+                const float ref = finite_base(m);
+                V8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(s[mt][i] - ref);
-                    l[mt] += p;
+                    const float p = __builtin_amdgcn_exp2f(s[i] - ref);
+                    l += p;
                     const T h = static_cast<T>(p);
-                    hi[mt][i] = h;
-                    lo[mt][i] = static_cast<T>(p - static_cast<float>(h));
+                    hi[i] = h;
+                    lo[i] = static_cast<T>(p - static_cast<float>(h));
+                }
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    const T *p = vt + (4 * quad + col / 4) * S::kVStride + 16 * d + col % 4 * 4;
+                    const u32x2_a x = lds_read_transposed(reinterpret_cast<const s16x4 *>(p)),
+                                  y = lds_read_transposed(reinterpret_cast<const s16x4 *>(p + 16 * S::kVStride));
+                    const V8 v = __builtin_bit_cast(V8, u32x4_a{x[0], x[1], y[0], y[1]});
+                    o[d] = N::mfma16(v, hi, o[d]);
+                    o[d] = N::mfma16(v, lo, o[d]);
                 }
             }
-            auto vcolumn = [&](int d) {
-                const T *p = vt + (4 * quad + col / 4) * S::kVStride + 16 * d + col % 4 * 4;
-                const u32x2_a x = lds_read_transposed(reinterpret_cast<const s16x4 *>(p)),
-                              y = lds_read_transposed(reinterpret_cast<const s16x4 *>(p + 16 * S::kVStride));
-                return u32x4_a{x[0], x[1], y[0], y[1]};
-            };
-#pragma unroll
-            for (int d = 0; d < kBlocks; ++d) {
-                const V8 v = __builtin_bit_cast(V8, vcolumn(d));
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    o[mt][d] = N::mfma16(v, hi[mt], o[mt][d]);
-                    o[mt][d] = N::mfma16(v, lo[mt], o[mt][d]);
-                }
-            }
-        }
 
-        // join the wavefronts' sums, 16 rows at a time
-        const FarParts parts(a.ws);
-        const int part = (2 * blockIdx.x + (u != u0)) * S::kPartFloats;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const float sum = quad_sum(l[mt]);
+            // join the wavefronts' sums
+            const FarParts parts(a.ws);
+            const int part = (2 * blockIdx.x + (u != u0)) * S::kPartFloats;
+            const float sum = quad_sum(l);
             if (quad == 0) {
-                lds_m[wave][col] = m[mt];
+                lds_m[wave][col] = m;
                 lds_l[wave][col] = sum;
             }
-            if (mt == 0 && only < 0) {
+            if (only < 0) {
                 const bool any = __any(odd_lane);
                 if (lane == 0) lds_odd[wave] = any;
             }
 #pragma unroll
             for (int d = 0; d < kBlocks; ++d)
-                *reinterpret_cast<f32x4 *>(ot + col * S::kOStride + 16 * d + 4 * quad) = o[mt][d];
+                *reinterpret_cast<f32x4 *>(ot + col * S::kOStride + 16 * d + 4 * quad) = o[d];
             __syncthreads();
-            if (mt == 0 && only < 0)
+            if (only < 0)
                 for (int wv = 0; wv < kTokenWaves; ++wv) odd |= lds_odd[wv] != 0;
             int start = tid;
             asm volatile("" : "+v"(start));  // the addresses below are formed here, not kept through the loops
-            for (int idx = start; idx < 16 * (HD / 4); idx += kTokenThreads) {
+            for (int idx = start; idx < kTokenRows * (HD / 4); idx += kTokenThreads) {
                 const int r = idx / (HD / 4), c = idx % (HD / 4) * 4;
-                const int row = row0 + 16 * mt + r;
-                if (row >= g.rows) break;
-                if (only >= 0 && row != row0 + only) continue;
-                float top = lds_m[0][r];
+                if (row0 + r >= g.rows) break;
+                if (only >= 0 && r != only) continue;
+                Joined j;
 #pragma unroll
-                for (int wv = 1; wv < kTokenWaves; ++wv) top = fmaxf(top, lds_m[wv][r]);
-                const float ref = finite_base(top);
-                float den = 0.0f;
-                f32x4 num = {0, 0, 0, 0};
-#pragma unroll
-                for (int wv = 0; wv < kTokenWaves; ++wv) {
-                    const float f = __builtin_amdgcn_exp2f(lds_m[wv][r] - ref);
-                    den += f * lds_l[wv][r];
-                    num += f * *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(lds + wv * S::kWaveBytes) +
-                                                                 r * S::kOStride + c);
-                }
+                for (int wv = 0; wv < kTokenWaves; ++wv)
+                    j.add(lds_m[wv][r], lds_l[wv][r],
+                          *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(lds + wv * S::kWaveBytes) +
+                                                           r * S::kOStride + c));
                 if (whole) {
-                    const f32x4 v = den == 0.0f ? f32x4{0, 0, 0, 0} : num * (1.0f / den);
-                    store_out4<TYPE>(a, out_at(a, g, kvh, row, HD) + c, v);
+                    store_out4<TYPE>(a, out_at(a, g, kvh, row0 + r, HD) + c, j.value());
                 } else {
-                    parts.store4(part + (16 * mt + r) * HD + c, num);
+                    parts.store4(part + r * HD + c, j.num);
                     if (c == 0) {
-                        parts.store(part + S::kRows * HD + 16 * mt + r, top);
-                        parts.store(part + S::kRows * (HD + 1) + 16 * mt + r, den);
+                        parts.store(part + kTokenRows * HD + r, j.top);
+                        parts.store(part + kTokenRows * (HD + 1) + r, j.den);
                     }
                 }
             }
             __syncthreads();
-        }
         }
         if (!whole) {
             const int64_t begin = u - t0, end = begin + w.tiles;
@@ -414,18 +396,17 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD * MT <= 256 &
                     if (team < teams)
                         join_parts(
                             j, parts, n_parts, team, teams, [&](int i) { return part_of(i) + r * HD + c; },
-                            [&](int i) { return part_of(i) + S::kRows * HD + r; },
-                            [&](int i) { return part_of(i) + S::kRows * (HD + 1) + r; });
-                    if (teams > 1) {
-                        nums[id] = j.num;
-                        dens[id] = j.den;
-                        tops[id] = j.top;
-                        __syncthreads();
-                        if (team == 0)
-                            for (int t = 1; t < teams; ++t) j.add(tops[t * n + id], dens[t * n + id], nums[t * n + id]);
+                            [&](int i) { return part_of(i) + kTokenRows * HD + r; },
+                            [&](int i) { return part_of(i) + kTokenRows * (HD + 1) + r; });
+                    nums[id] = j.num;
+                    dens[id] = j.den;
+                    tops[id] = j.top;
+                    __syncthreads();
+                    if (team == 0) {
+                        for (int t = 1; t < teams; ++t) j.add(tops[t * n + id], dens[t * n + id], nums[t * n + id]);
+                        store_out4<TYPE>(a, out_at(a, g, kvh, row0 + r, HD) + c, j.value());
                     }
-                    if (team == 0) store_out4<TYPE>(a, out_at(a, g, kvh, row0 + r, HD) + c, j.value());
-                    if (teams > 1) __syncthreads();
+                    __syncthreads();
                 }
             }
             __syncthreads();  // lds_odd, lds
@@ -437,34 +418,34 @@ __global__ __launch_bounds__(kTokenThreads, HD * MT <= 64 ? 3 : HD * MT <= 256 &
 // The token form runs as many workgroups as stay on the chip together.
 constexpr int kTokenGroupsPerCu = 4;
 
-template <int TYPE, int HD, int MT>
-int launch_token(mi355x_ctx *ctx, const AttnArgs &a, int64_t rows) {
-    const void *kernel = reinterpret_cast<const void *>(attention_token_kernel<TYPE, HD, MT>);
+template <int TYPE, int HD>
+int launch_token(mi355x_ctx *ctx, const AttnArgs &a) {
+    const void *kernel = reinterpret_cast<const void *>(attention_token_kernel<TYPE, HD>);
     const int64_t fit = ctx->num_cus * std::max(1, std::min(kTokenGroupsPerCu, occupancy(kernel, kTokenThreads, 0)));
-    // no more than the units that the table and the rows allow
-    const int64_t heads = static_cast<int64_t>(a.n_seqs) * a.n_kv_heads, tiles = a.reach / kUnitKeys + 1;
-    const int64_t blocks = std::max<int64_t>(1, rows / (16 * MT));
-    const int64_t units = heads > fit ? fit : heads * std::min(fit, tiles * std::min(fit, blocks));
-    attention_token_kernel<TYPE, HD, MT>
+    // no more than the units that the table allows
+    const int64_t heads = static_cast<int64_t>(a.n_seqs) * a.n_kv_heads;
+    const int64_t units = heads * (a.reach / kUnitKeys + 1);
+    attention_token_kernel<TYPE, HD>
         <<<static_cast<unsigned>(std::min(fit, units)), kTokenThreads, 0, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
     return MI355X_OK;
 }
 
+// rows: the host's bound on a request's head rows.  Up to kTokenRows the token
+// form; else the chunk form, behind the token form for the requests that add
+// few (one request alone takes the chunk form at once).  With 17 to 64 rows the
+// chunk form is the faster one too: 16 requests of 5 tokens and 8 heads 28.9 us
+// against 39.3 for a token form of three row blocks, one of 4 tokens on 30000 36
+// against 211; 16 of 8 tokens and 4 heads 77 against 68.
 template <int TYPE, int HD>
 int launch_forms(mi355x_ctx *ctx, const AttnArgs &a, int64_t rows) {
-    if (rows <= 16) return launch_token<TYPE, HD, 1>(ctx, a, rows);
-    if (rows <= 32) return launch_token<TYPE, HD, 2>(ctx, a, rows);
-    if constexpr (HD <= 128) {
-        if (rows <= 48) return launch_token<TYPE, HD, 3>(ctx, a, rows);
-        if (rows <= 64) return launch_token<TYPE, HD, 4>(ctx, a, rows);
-    }
+    if (rows <= kTokenRows) return launch_token<TYPE, HD>(ctx, a);
     AttnArgs b = a;
     b.row_limit = 0;
-    if (a.n_seqs > 1) {  // some may add few tokens
+    if (a.n_seqs > 1) {
         AttnArgs c = a;
-        c.row_limit = b.row_limit = 16;
-        if (int rc = launch_token<TYPE, HD, 1>(ctx, c, 16)) return rc;
+        c.row_limit = b.row_limit = kTokenRows;
+        if (int rc = launch_token<TYPE, HD>(ctx, c)) return rc;
     }
     return launch_attention_chunk(ctx, b, TYPE, HD);
 }
@@ -481,13 +462,13 @@ int launch_sizes(mi355x_ctx *ctx, const AttnArgs &a, int head_dim, int64_t rows)
 
 }  // namespace
 
-// One counter per workgroup of the token form (and per row block of a split chunk form, which are fewer).
+// One counter per workgroup of the token form.
 static size_t counter_bytes(const mi355x_ctx *ctx) {
     return (static_cast<size_t>(ctx->num_cus) * kTokenGroupsPerCu * 4 + 255) / 256 * 256;
 }
 
 size_t paged_attention_workspace_bytes(const mi355x_ctx *ctx, int, int, int head_dim) {
-    return counter_bytes(ctx) + std::max(static_cast<size_t>(ctx->num_cus * kTokenGroupsPerCu) * 2 * 64 * (head_dim + 2) * 4,
+    return counter_bytes(ctx) + std::max(static_cast<size_t>(ctx->num_cus * kTokenGroupsPerCu) * 2 * kTokenRows * (head_dim + 2) * 4,
                                          attention_chunk_workspace(ctx, head_dim));
 }
 

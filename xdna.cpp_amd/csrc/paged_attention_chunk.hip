@@ -78,13 +78,6 @@ __device__ __forceinline__ int find_block(const AttnArgs &a, int64_t j, int64_t 
     return lo;
 }
 
-// 16 bytes per lane from memory to LDS, lane after lane from `to` on.
-__device__ __forceinline__ void load_lds16(const void *from, unsigned char *to) {
-    __builtin_amdgcn_global_load_lds(
-        reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(reinterpret_cast<uintptr_t>(from)),
-        (__attribute__((address_space(3))) uint32_t *)(to), 16, 0, 0);
-}
-
 struct ChunkItem {
     int seq, kvh, row0;
     SeqGeo g;
@@ -143,6 +136,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
     const bool real = row_raw < g.rows;
     const int row = real ? row_raw : 0, tok = divided(row, a.group), group = static_cast<int>(a.group.d);
     const int64_t head = static_cast<int64_t>(kvh) * group + (row - tok * group);
+    const bool busy = it.row0 + 32 * wave < g.rows;  // a wavefront without rows only loads
     const Keys mine = token_keys(a, g, g.tok_lo + tok);
     const int row_lo = mine.lo, row_hi = real ? mine.hi : 0;
     V8 qf[kSteps];
@@ -259,6 +253,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
                 if (__any(bad) && lane == 0) odd = 1;
                 __syncthreads();
             }
+            if (!busy) continue;
             float s[32];  // keys 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
             f32x16 x[2];
 #pragma unroll
@@ -296,7 +291,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
 #pragma unroll
             for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
             top = half_max(top);
-            if (!CAP) top *= c;  // c >= 0 here; 0 x infinity gives NaN, which no maximum takes
+            if (!CAP) top *= c;  // c > 0 here
             const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
             if (__any(grows)) {
                 const float m_new = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
@@ -438,8 +433,8 @@ int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
 
 template <int TYPE, int HD>
 int launch_size(mi355x_ctx *ctx, const AttnArgs &a) {
-    // the common path scales the maximum instead of each score, for which the scale has to be positive
-    const bool cap = a.cap_out > 0.0f || a.scale2 < 0.0f;
+    // the common path masks and takes the maximum before it scales, for which the scale has to be positive
+    const bool cap = a.cap_out > 0.0f || !(a.scale2 > 0.0f);
     if (a.f32_out) return cap ? launch_chunk<TYPE, HD, true, 2>(ctx, a) : launch_chunk<TYPE, HD, false, 2>(ctx, a);
     return cap ? launch_chunk<TYPE, HD, true, 1>(ctx, a) : launch_chunk<TYPE, HD, false, 1>(ctx, a);
 }

@@ -41,10 +41,12 @@ MI355X_HD int64_t quotient(int64_t a, int64_t b) {
 // `total` units in `groups` stretches of equal length, the first of them one longer.
 struct Stretches {
     int64_t total, each, longer;
+    int groups;
 };
 MI355X_HD Stretches stretches(int64_t total, int groups) {
     Stretches s;
     s.total = total;
+    s.groups = groups;
     s.each = quotient(total, groups);
     s.longer = total - s.each * groups;
     return s;
