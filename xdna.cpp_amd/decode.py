@@ -64,6 +64,8 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     lib.qd_set_io.argtypes = [C.c_void_p, C.c_int]
     lib.qd_set_wait.restype = C.c_int
     lib.qd_set_wait.argtypes = [C.c_void_p, C.c_int]
+    lib.qd_set_attention.restype = C.c_int
+    lib.qd_set_attention.argtypes = [C.c_void_p, C.c_int]
     lib.qd_last_wait.restype = C.c_int
     lib.qd_last_wait.argtypes = [C.c_void_p]
     lib.qd_last_launches.restype = C.c_int64
@@ -192,6 +194,15 @@ class Model:
         ggml plugin (weights as tensors in its buffer, activation in, one
         graph_compute per group, outputs out, synchronize)."""
         if self.lib.qd_set_wait(self.h, mode) != 0:
+            raise RuntimeError(self.lib.qd_last_error().decode())
+
+    ATTENTION_HOST, ATTENTION_GPU = 0, 1
+
+    def set_attention(self, mode: int) -> None:
+        """ATTENTION_HOST (default): attention on the host, a prompt token at a
+        time; ATTENTION_GPU: biases, RoPE and attention on the GPU over f16
+        pages, the prompt in chunks of up to 512 tokens."""
+        if self.lib.qd_set_attention(self.h, mode) != 0:
             raise RuntimeError(self.lib.qd_last_error().decode())
 
     PLUGIN_GROUPS_SERVER, PLUGIN_GROUPS_LAUNCH = 0, 1

@@ -7,6 +7,7 @@
 
 #include "ggml-mi355x.h"
 #include "ggml_abi.h"
+#include "mi355x-attention.h"
 #include "mi355x-gemv.h"
 
 #include <hip/hip_runtime_api.h>
@@ -218,6 +219,7 @@ struct qd_model {
     int wait_mode = QD_WAIT_SERVER;
     int variant = MI355X_VARIANT_AUTO;
     int last_wait = QD_WAIT_FENCE;  // the mode the last GPU decode used
+    int attention = QD_ATTENTION_HOST;
 
     mi355x_server *server = nullptr;
     std::unique_ptr<PluginDecode> plugin;
@@ -566,6 +568,16 @@ int qd_set_wait(qd_model *m, int mode) {
     return 0;
 }
 
+int qd_set_attention(qd_model *m, int mode) {
+    if (!m) return fail("qd_set_attention: null model");
+    if (mode != QD_ATTENTION_HOST && mode != QD_ATTENTION_GPU) return fail("qd_set_attention: unknown mode");
+    if (mode == QD_ATTENTION_GPU && m->c.head_dim != 64 && m->c.head_dim != 96 && m->c.head_dim != 128 &&
+        m->c.head_dim != 256)
+        return fail("qd_set_attention: attention on the GPU needs a head_dim of 64, 96, 128 or 256");
+    m->attention = mode;
+    return 0;
+}
+
 int64_t qd_last_launches(const qd_model *m) { return m ? m->last_launches : 0; }
 
 int qd_last_wait(const qd_model *m) { return m ? m->last_wait : -1; }
@@ -718,6 +730,291 @@ int attach_plugin(qd_model *m) {
     return 0;
 }
 
+// A decode with attention on the GPU (QD_ATTENTION_GPU).  Buffers belong to the
+// call; destroyed in any state.
+struct GpuDecode {
+    qd_model *m;
+    mi355x_ctx *ctx;
+    const int H, QD, KVD, hd, F, L, T, rows;  // rows: of the largest pass
+    std::vector<void *> device, host;
+    // device: activations in, GEMV outputs, attention's in- and output, pages
+    float *x = nullptr, *y = nullptr, *qkv = nullptr, *att = nullptr, *bias = nullptr, *inv_freq = nullptr;
+    uint16_t *q = nullptr, *pages = nullptr;
+    int32_t *ints = nullptr;
+    int64_t *slots = nullptr;
+    void *workspace = nullptr;
+    size_t workspace_bytes = 0, y_floats = 0;
+    float *hx = nullptr, *hy = nullptr;  // page-locked
+    int32_t *h_added = nullptr;
+    int n_pages = 0;
+    int64_t launches = 0;
+    double t_gpu = 0.0;
+
+    GpuDecode(qd_model *model, int tokens, int most_rows)
+        : m(model), ctx(model->ctx), H(model->c.hidden), QD(model->q_dim()), KVD(model->kv_dim()),
+          hd(model->c.head_dim), F(model->c.ffn), L(model->c.n_layers), T(tokens), rows(most_rows) {}
+    GpuDecode(const GpuDecode &) = delete;
+    GpuDecode &operator=(const GpuDecode &) = delete;
+    ~GpuDecode() {
+        (void)mi355x_ctx_sync(ctx);
+        for (void *p : device) (void)mi355x_free(ctx, p);
+        for (void *p : host) (void)mi355x_host_free(p);
+    }
+
+    bool alloc(void *p, size_t bytes) {  // p: where the pointer goes
+        void *v = nullptr;
+        if (mi355x_malloc(ctx, bytes, &v) != MI355X_OK) return false;
+        device.push_back(v);
+        std::memcpy(p, &v, sizeof(v));
+        return true;
+    }
+    bool alloc_host(void *p, size_t bytes) {
+        void *v = nullptr;
+        if (mi355x_host_malloc(bytes, &v) != MI355X_OK) return false;
+        host.push_back(v);
+        std::memcpy(p, &v, sizeof(v));
+        return true;
+    }
+
+    // integers on the device: added, lengths (in place), the free list's head,
+    // the two row offsets, the status, positions, the free list, the block table
+    int32_t *added() { return ints; }
+    int32_t *kv_len() { return ints + 1; }
+    int32_t *head() { return ints + 2; }
+    int32_t *offsets() { return ints + 3; }
+    int32_t *status() { return ints + 5; }
+    int32_t *positions() { return ints + 6; }
+    int32_t *free_pages() { return positions() + rows; }
+    int32_t *table() { return free_pages() + n_pages; }
+
+    int init() {
+        n_pages = (T + QD_PAGE_TOKENS - 1) / QD_PAGE_TOKENS;
+        const size_t R = static_cast<size_t>(rows), wide = static_cast<size_t>(std::max(2 * F, std::max(H, QD)));
+        y_floats = std::max(R * wide, static_cast<size_t>(m->c.vocab));
+        const size_t pool = static_cast<size_t>(n_pages) * QD_PAGE_TOKENS * KVD;  // values of one layer's keys
+        if (mi355x_paged_attention_workspace(ctx, m->c.n_heads, m->c.n_kv_heads, hd, &workspace_bytes) != MI355X_OK)
+            return -1;
+        if (!alloc(&x, 4 * R * std::max(F, std::max(H, QD))) || !alloc(&y, 4 * y_floats) ||
+            !alloc(&qkv, 4 * R * (QD + 2 * KVD)) || !alloc(&att, 4 * R * QD) || !alloc(&q, 2 * R * QD) ||
+            !alloc(&bias, 4 * static_cast<size_t>(L) * (QD + 2 * KVD)) || !alloc(&inv_freq, 2 * static_cast<size_t>(hd)) ||
+            !alloc(&pages, 4 * pool * static_cast<size_t>(L)) ||
+            !alloc(&ints, 4 * (6 + R + 2 * static_cast<size_t>(n_pages))) || !alloc(&slots, 8 * R) ||
+            !alloc(&workspace, workspace_bytes) || !alloc_host(&hx, 4 * R * std::max(F, std::max(H, QD))) ||
+            !alloc_host(&hy, 4 * y_floats) || !alloc_host(&h_added, 4))
+            return -1;
+        std::vector<int32_t> start(6 + R + 2 * static_cast<size_t>(n_pages), 0);
+        for (int p = 0; p < n_pages; ++p) start[6 + R + static_cast<size_t>(p)] = p;
+        std::vector<float> b, f(static_cast<size_t>(hd / 2));
+        for (int l = 0; l < L; ++l) {
+            b.insert(b.end(), m->bq[l].begin(), m->bq[l].end());
+            b.insert(b.end(), m->bk[l].begin(), m->bk[l].end());
+            b.insert(b.end(), m->bv[l].begin(), m->bv[l].end());
+        }
+        for (int i = 0; i < hd / 2; ++i)
+            f[i] = std::pow(m->c.rope_theta, -2.0f * static_cast<float>(i) / static_cast<float>(hd));
+        if (mi355x_memcpy_h2d(ctx, ints, start.data(), 4 * start.size()) != MI355X_OK ||
+            mi355x_memcpy_h2d(ctx, bias, b.data(), 4 * b.size()) != MI355X_OK ||
+            mi355x_memcpy_h2d(ctx, inv_freq, f.data(), 4 * f.size()) != MI355X_OK ||
+            mi355x_fill(ctx, workspace, 0, workspace_bytes) != MI355X_OK ||
+            mi355x_fill(ctx, pages, 0, 4 * pool * static_cast<size_t>(L)) != MI355X_OK)
+            return -1;
+        return 0;
+    }
+
+    int wait() {
+        return m->wait_mode == QD_WAIT_STREAM ? mi355x_ctx_sync(ctx) : mi355x_ctx_fence(ctx);
+    }
+
+    // y (n rows, `stride` floats apart) = W_id x (n rows of the matrix's K)
+    int product(int id, const float *in, float *out, int64_t stride, int n) {
+        const Matrix &w = m->mats[id];
+        ++launches;
+        if (n == 1) return mi355x_gemv(ctx, MI355X_TYPE_Q4_0, w.dev, w.N, w.K, in, out);
+        return mi355x_gemv_batched(ctx, MI355X_TYPE_Q4_0, w.dev, w.N, w.K, in, w.K, out, stride, n);
+    }
+
+    int upload(int64_t floats) { return mi355x_memcpy_h2d_async(ctx, x, hx, 4 * static_cast<size_t>(floats)); }
+
+    int download(int64_t floats) {
+        if (mi355x_memcpy_d2h_async(ctx, hy, y, 4 * static_cast<size_t>(floats)) != MI355X_OK) return -1;
+        return wait();
+    }
+
+    // one more pass of n tokens: their places in the pages
+    int plan(int n) {
+        *h_added = n;
+        mi355x_kv_plan_args a{};
+        a.n_seqs = 1;
+        a.page_tokens = QD_PAGE_TOKENS;
+        a.table_cols = n_pages;
+        a.table_stride = n_pages;
+        a.n_free = n_pages;
+        a.n_rows = n;
+        a.cached = kv_len();  // in place, as is the head
+        a.kv_lens = kv_len();
+        a.added = added();
+        a.block_table = table();
+        a.free_pages = free_pages();
+        a.free_head = head();
+        a.free_head_out = head();
+        a.row_offsets = offsets();
+        a.positions = positions();
+        a.slots = slots;
+        a.status = status();
+        if (mi355x_memcpy_h2d_async(ctx, added(), h_added, 4) != MI355X_OK) return -1;
+        return mi355x_kv_plan(ctx, &a);
+    }
+
+    // attention's output (n rows of QD) from the q|k|v rows of layer l
+    int attention(int l, int n) {
+        const size_t pool_values = static_cast<size_t>(n_pages) * QD_PAGE_TOKENS * KVD;
+        mi355x_kv_pool pool{};
+        pool.type = MI355X_TYPE_F16;
+        pool.n_kv_heads = m->c.n_kv_heads;
+        pool.head_dim = hd;
+        pool.page_tokens = QD_PAGE_TOKENS;
+        pool.n_pages = n_pages;
+        pool.k = pages + 2 * static_cast<size_t>(l) * pool_values;
+        pool.v = pages + (2 * static_cast<size_t>(l) + 1) * pool_values;
+        pool.page_stride = static_cast<int64_t>(QD_PAGE_TOKENS) * KVD;
+        pool.token_stride = KVD;
+        pool.head_stride = hd;
+        const int64_t width = QD + 2 * KVD;
+        const float *b = bias + static_cast<size_t>(l) * static_cast<size_t>(width);
+        mi355x_qk_norm_rope_args r{};
+        r.n_rows = n;
+        r.n_heads = m->c.n_heads;
+        r.n_kv_heads = m->c.n_kv_heads;
+        r.head_dim = r.rot_dim = hd;
+        r.rope_mode = MI355X_ROPE_HALVES;
+        r.in_type = MI355X_TYPE_F32;
+        r.out_type = MI355X_TYPE_F16;
+        r.q = qkv;
+        r.k = qkv + QD;
+        r.v = qkv + QD + KVD;
+        r.q_stride = r.k_stride = r.v_stride = width;
+        r.q_bias = b;
+        r.k_bias = b + QD;
+        r.v_bias = b + QD + KVD;
+        r.positions = positions();
+        r.inv_freq = inv_freq;
+        r.q_out = q;
+        r.q_out_stride = QD;
+        r.pool = &pool;
+        r.slots = slots;
+        if (mi355x_qk_norm_rope(ctx, &r) != MI355X_OK) return -1;
+        mi355x_paged_attention_args a{};
+        a.n_rows = n;
+        a.n_seqs = 1;
+        a.n_heads = m->c.n_heads;
+        a.max_added = n;
+        a.q = q;
+        a.q_stride = QD;
+        a.pool = &pool;
+        a.row_offsets = offsets();
+        a.kv_lens = kv_len();
+        a.block_table = table();
+        a.table_cols = n_pages;
+        a.table_stride = n_pages;
+        a.scale = 1.0f / std::sqrt(static_cast<float>(hd));
+        a.causal = 1;
+        a.out = att;
+        a.out_type = MI355X_TYPE_F32;
+        a.out_stride = QD;
+        a.workspace = workspace;
+        a.workspace_bytes = workspace_bytes;
+        return mi355x_paged_attention(ctx, &a);
+    }
+
+    // The pass of n tokens; with logits, those behind the last one.
+    int pass(const int32_t *tokens, int n, float *logits) {
+        const int64_t width = QD + 2 * KVD;
+        std::vector<float> h(static_cast<size_t>(n) * H), out(static_cast<size_t>(H));
+        for (int i = 0; i < n; ++i)
+            dequant_q4_0_row(m->mats[7 * L].q.data() + static_cast<int64_t>(tokens[i]) * (H / 32) * 18, H,
+                             h.data() + static_cast<size_t>(i) * H);
+        auto normed = [&](const std::vector<float> &w) {
+            for (int i = 0; i < n; ++i)
+                rmsnorm(h.data() + static_cast<size_t>(i) * H, w.data(), hx + static_cast<size_t>(i) * H, H, m->c.norm_eps);
+        };
+        auto residual = [&] {
+            for (size_t i = 0; i < h.size(); ++i) h[i] += hy[i];
+        };
+        double t0 = now();
+        if (plan(n)) return -1;
+        t_gpu += now() - t0;
+        for (int l = 0; l < L; ++l) {
+            normed(m->attn_norm[l]);
+            t0 = now();
+            if (upload(static_cast<int64_t>(n) * H) || product(7 * l + QD_Q, x, qkv, width, n) ||
+                product(7 * l + QD_K, x, qkv + QD, width, n) || product(7 * l + QD_V, x, qkv + QD + KVD, width, n) ||
+                attention(l, n) || product(7 * l + QD_O, att, y, H, n) || download(static_cast<int64_t>(n) * H))
+                return -1;
+            t_gpu += now() - t0;
+            residual();
+            normed(m->ffn_norm[l]);
+            t0 = now();
+            if (upload(static_cast<int64_t>(n) * H) || product(7 * l + QD_GATE, x, y, 2 * F, n) ||
+                product(7 * l + QD_UP, x, y + F, 2 * F, n) || download(static_cast<int64_t>(n) * 2 * F))
+                return -1;
+            t_gpu += now() - t0;
+#pragma omp parallel for if (n > 1)
+            for (int i = 0; i < n; ++i) {
+                float *g = hy + static_cast<size_t>(i) * 2 * F;
+                silu_mul(g, g + F, F);
+                std::memcpy(hx + static_cast<size_t>(i) * F, g, static_cast<size_t>(F) * 4);
+            }
+            t0 = now();
+            if (upload(static_cast<int64_t>(n) * F) || product(7 * l + QD_DOWN, x, y, H, n) ||
+                download(static_cast<int64_t>(n) * H))
+                return -1;
+            t_gpu += now() - t0;
+            residual();
+        }
+        if (!logits) return 0;
+        rmsnorm(h.data() + static_cast<size_t>(n - 1) * H, m->out_norm.data(), hx, H, m->c.norm_eps);
+        t0 = now();
+        if (upload(H) || product(7 * L, x, y, 0, 1) || download(m->c.vocab)) return -1;
+        t_gpu += now() - t0;
+        std::memcpy(logits, hy, static_cast<size_t>(m->c.vocab) * 4);
+        return 0;
+    }
+};
+
+// qd_generate with attention on the GPU.
+int generate_gpu_attention(qd_model *m, const int32_t *prompt, int n_prompt, int n_gen, int32_t *out_tokens,
+                           double *timings) {
+    GpuDecode d(m, n_prompt + std::max(n_gen, 1), std::min(n_prompt, QD_CHUNK_ROWS));
+    auto failed = [&] { return fail(std::string("qd_generate: ") + mi355x_last_error()); };
+    if (d.init()) return failed();
+    std::vector<float> logits(static_cast<size_t>(m->c.vocab));
+    const double t_start = now();
+    for (int at = 0; at < n_prompt; at += QD_CHUNK_ROWS) {
+        const int n = std::min(QD_CHUNK_ROWS, n_prompt - at);
+        if (d.pass(prompt + at, n, at + n == n_prompt && n_gen > 0 ? logits.data() : nullptr)) return failed();
+    }
+    int32_t tok = 0;
+    if (n_gen > 0) out_tokens[0] = tok = argmax(logits.data(), m->c.vocab);
+    const double t_gen0 = now();
+    d.t_gpu = 0.0;
+    d.launches = 0;
+    for (int i = 1; i < n_gen; ++i) {
+        if (d.pass(&tok, 1, logits.data())) return failed();
+        out_tokens[i] = tok = argmax(logits.data(), m->c.vocab);
+    }
+    const double t_end = now();
+    if (n_gen > 0) m->last_logits = logits;
+    m->last_launches = d.launches;
+    m->last_wait = m->wait_mode == QD_WAIT_STREAM ? QD_WAIT_STREAM : QD_WAIT_FENCE;
+    if (timings) {
+        timings[0] = t_gen0 - t_start;
+        timings[1] = t_end - t_gen0;
+        timings[2] = d.t_gpu;
+        timings[3] = t_end - t_gen0 - d.t_gpu;
+    }
+    return 0;
+}
+
 }  // namespace
 
 int qd_generate(qd_model *m, int backend, qd_gemv_fn cpu_gemv, void *user, const int32_t *prompt, int n_prompt,
@@ -726,6 +1023,10 @@ int qd_generate(qd_model *m, int backend, qd_gemv_fn cpu_gemv, void *user, const
         return fail("qd_generate: bad arguments");
     if (backend == 0 && !m->ctx) return fail("qd_generate: qd_attach_gpu first");
     if (backend == 1 && !cpu_gemv) return fail("qd_generate: no CPU GEMV");
+    if (backend == 0 && m->attention == QD_ATTENTION_GPU) {
+        omp_set_num_threads(m->threads);
+        return generate_gpu_attention(m, prompt, n_prompt, n_gen, out_tokens, timings);
+    }
     const qd_config &c = m->c;
     const int H = c.hidden, QD = m->q_dim(), KVD = m->kv_dim(), hd = c.head_dim;
     const int L = c.n_layers, T = n_prompt + std::max(n_gen, 1);

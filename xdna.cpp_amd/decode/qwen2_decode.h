@@ -2,7 +2,8 @@
  * qwen2_decode.h -- batch-1 greedy decoder of a Qwen2-shaped model with Q4_0
  * weights, for end-to-end measurement of the decode GEMV path.
  *
- * Everything except the matrix-vector products runs on the host in C++
+ * Everything except the matrix-vector products (and, if asked for, attention)
+ * runs on the host in C++
  * (RMSNorm, RoPE, grouped-query attention over a f32 KV cache, SwiGLU,
  * residuals, embedding lookup, argmax).  Every weight matrix -- per layer
  * q, k, v, o, gate, up, down, plus the tied output projection -- is a Q4_0
@@ -127,6 +128,22 @@ QD_API int qd_set_wait(qd_model *m, int mode);
  * ggml-mi355x.h). */
 QD_API int qd_set_plugin_groups(qd_model *m, int mode);
 QD_API int qd_last_wait(const qd_model *m);
+/* Where attention runs on the GPU path (backend 0):
+ * QD_ATTENTION_HOST (default): on the host, over an f32 cache, a prompt token at
+ * a time;
+ * QD_ATTENTION_GPU: biases, RoPE and attention on the GPU with the operators of
+ * mi355x-attention.h, over f16 pages of QD_PAGE_TOKENS tokens: one
+ * mi355x_kv_plan per pass, then per layer the q|k|v GEMVs into device memory,
+ * mi355x_qk_norm_rope, mi355x_paged_attention and the o GEMV on its output.  The
+ * prompt goes through in chunks of up to QD_CHUNK_ROWS tokens
+ * (mi355x_gemv_batched); norms, SiLU, residuals, embedding and argmax stay on the
+ * host.  One launch per GEMV: the wait mode is QD_WAIT_STREAM if that is set,
+ * else QD_WAIT_FENCE.  head_dim 64, 96, 128 or 256. */
+#define QD_ATTENTION_HOST 0
+#define QD_ATTENTION_GPU 1
+#define QD_PAGE_TOKENS 64
+#define QD_CHUNK_ROWS 512
+QD_API int qd_set_attention(qd_model *m, int mode);
 /* Kernel variant of the GPU GEMVs (MI355X_OPT_VARIANT of mi355x-gemv.h):
  * MI355X_VARIANT_GGML_Q8 gives ggml-cpu's Q8_0-activation arithmetic. */
 QD_API int qd_set_variant(qd_model *m, int variant);
