@@ -1,9 +1,9 @@
 // Block tables, slots and positions of a serving step, built on the GPU from
 // the requests' lengths.
 //
-// Two exclusive scans over the requests (new tokens, new pages) give every
-// request its rows and its entries of the free list; a row then finds its
-// request by a binary search of the offsets.  The work is tens of bytes per
+// Sums over the requests (new tokens, new pages) give every request its rows and
+// its entries of the free list; a row then finds its request by a binary search of
+// the offsets.  The work is tens of bytes per
 // request and 12 per row, so latency bounds it.
 #include "internal.h"
 #include "paged_index.h"
@@ -15,10 +15,12 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
-// Requests whose offsets the one-launch form keeps in LDS.
-constexpr int kPlanLdsSeqs = 1024;
-// Rows up to which one workgroup writes them itself.
-constexpr int64_t kPlanOneLaunchRows = 4096;
+// Requests up to which one launch does it all, a request per thread.
+constexpr int kPlanOneLaunchSeqs = kPlanThreads;
+// Rows of a thread there, at least.
+constexpr int kPlanThreadRows = 4;
+// Rows up to which one workgroup writes those of a step in place.
+constexpr int64_t kPlanInPlaceRows = 4096;
 
 struct PlanSeq {
     int64_t cached, added, held, fresh;
@@ -42,108 +44,150 @@ __device__ __forceinline__ PlanSeq plan_seq(const mi355x_kv_plan_args &a, int sh
     return q;
 }
 
-__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t u = __shfl_up(v, d);
-        if (lane >= d) v += u;
-    }
-    return v;
+// Inclusive sums over a wavefront, held at 2^32 - 1: a total of 2^31 or more does
+// not fit anyway, and then no sum is used.
+template <int CTRL, int ROW_MASK = 0xF>
+__device__ __forceinline__ uint32_t sum_step(uint32_t v) {
+    const uint32_t u = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROW_MASK, 0xF, false);
+    return __builtin_elementwise_add_sat(v, u);
+}
+__device__ __forceinline__ uint32_t wave_sums(uint32_t v) {
+    v = sum_step<0x111>(v);       // row_shr:1
+    v = sum_step<0x112>(v);       // row_shr:2
+    v = sum_step<0x114>(v);       // row_shr:4
+    v = sum_step<0x118>(v);       // row_shr:8
+    v = sum_step<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    return sum_step<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
-// One workgroup: scans, tables, and (rows) the rows themselves.
-__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(mi355x_kv_plan_args a, int shift, int rows) {
-    __shared__ int64_t sums[2][kPlanWaves];
+// The sums before this thread's values over the workgroup, and the totals.
+struct PlanSums {
+    uint32_t rows, pages, all_rows, all_pages;
+};
+__device__ __forceinline__ PlanSums group_sums(uint32_t rows, uint32_t pages, uint32_t (*tmp)[kPlanWaves]) {
+    const int wave = threadIdx.x >> 6, n = blockDim.x >> 6;
+    const uint32_t in_rows = wave_sums(rows), in_pages = wave_sums(pages);
+    if ((threadIdx.x & 63) == 63) {
+        tmp[0][wave] = in_rows;
+        tmp[1][wave] = in_pages;
+    }
+    __syncthreads();
+    PlanSums s{in_rows - rows, in_pages - pages, 0, 0};
+    for (int w = 0; w < n; ++w) {
+        if (w < wave) {
+            s.rows = __builtin_elementwise_add_sat(s.rows, tmp[0][w]);
+            s.pages = __builtin_elementwise_add_sat(s.pages, tmp[1][w]);
+        }
+        s.all_rows = __builtin_elementwise_add_sat(s.all_rows, tmp[0][w]);
+        s.all_pages = __builtin_elementwise_add_sat(s.all_pages, tmp[1][w]);
+    }
+    return s;
+}
+
+__device__ __forceinline__ int plan_flags(const mi355x_kv_plan_args &a, int flags, const PlanSums &s, int64_t head) {
+    if (s.all_rows > a.n_rows) flags |= MI355X_KV_ROWS;
+    if (head < 0 || head > a.n_free || s.all_pages > a.n_free - head) flags |= MI355X_KV_PAGES;
+    return flags;
+}
+
+// What belongs to request s, and (s = 0) to the step.
+__device__ __forceinline__ void write_seq(const mi355x_kv_plan_args &a, int s, const PlanSeq &q, int64_t row,
+                                          int64_t first, bool ok) {
+    a.row_offsets[s] = ok ? static_cast<int32_t>(row) : 0;
+    a.kv_lens[s] = static_cast<int32_t>(ok ? q.cached + q.added : q.cached);
+    if (ok)
+        for (int64_t i = 0; i < q.fresh; ++i) a.block_table[s * a.table_stride + q.held + i] = a.free_pages[first + i];
+}
+__device__ __forceinline__ void write_step(const mi355x_kv_plan_args &a, int64_t rows, int64_t head, int flags) {
+    a.row_offsets[a.n_seqs] = static_cast<int32_t>(rows);
+    *a.free_head_out = static_cast<int32_t>(head);
+    if (a.status) *a.status = flags;
+}
+
+// Up to kPlanOneLaunchSeqs requests: sums, tables and rows in one launch.  Each of
+// several workgroups takes a part of the rows and sums over all requests for
+// itself, which costs less than a second launch (65 thousand rows of 256 requests
+// PP us against 9.4); the first one writes what belongs to the requests.
+__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(mi355x_kv_plan_args a, int shift, int group_rows) {
+    __shared__ uint32_t sums[2][kPlanWaves];
     __shared__ int all_flags;
-    __shared__ int32_t off_lds[kPlanLdsSeqs + 1], kv_lds[kPlanLdsSeqs], held_lds[kPlanLdsSeqs], first_lds[kPlanLdsSeqs];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nthr = blockDim.x, nwave = nthr >> 6;
+    __shared__ int32_t off[kPlanOneLaunchSeqs + 1], kv_len[kPlanOneLaunchSeqs], held[kPlanOneLaunchSeqs],
+        fresh_at[kPlanOneLaunchSeqs];
+    const int tid = threadIdx.x, nthr = blockDim.x;
+    const int64_t head = *a.free_head;
+    PlanSeq q{};
+    if (tid < a.n_seqs) q = plan_seq(a, shift, tid);
     if (tid == 0) all_flags = 0;
     __syncthreads();
-    // totals first: a step that does not fit takes nothing
-    int64_t n_new = 0, n_fresh = 0;
-    int flags = 0;
-    for (int s = tid; s < a.n_seqs; s += nthr) {
-        const PlanSeq q = plan_seq(a, shift, s);
-        n_new += q.added;
-        n_fresh += q.fresh;
-        flags |= q.flags;
-    }
-    n_new = __shfl(wave_scan(n_new, lane), 63);
-    n_fresh = __shfl(wave_scan(n_fresh, lane), 63);
-    if (flags) atomicOr(&all_flags, flags);
-    if (lane == 0) {
-        sums[0][wave] = n_new;
-        sums[1][wave] = n_fresh;
-    }
-    __syncthreads();
-    n_new = n_fresh = 0;
-    for (int w = 0; w < nwave; ++w) {
-        n_new += sums[0][w];
-        n_fresh += sums[1][w];
-    }
-    const int64_t head = *a.free_head;
-    flags = all_flags;
-    if (n_new > a.n_rows) flags |= MI355X_KV_ROWS;
-    if (head < 0 || head > a.n_free || n_fresh > a.n_free - head) flags |= MI355X_KV_PAGES;
-    __syncthreads();  // every thread has read free_head, which free_head_out may be
+    if (q.flags) atomicOr(&all_flags, q.flags);
+    const PlanSums s = group_sums(static_cast<uint32_t>(q.added), static_cast<uint32_t>(q.fresh), sums);
+    // every thread of a workgroup has read what the first one may write in place
+    const int flags = plan_flags(a, all_flags, s, head);
     const bool ok = flags == 0;
-    if (tid == 0) {
-        *a.free_head_out = static_cast<int32_t>(ok ? head + n_fresh : head);
-        if (a.status) *a.status = flags;
-        a.row_offsets[a.n_seqs] = ok ? static_cast<int32_t>(n_new) : 0;
-        if (rows) off_lds[a.n_seqs] = ok ? static_cast<int32_t>(n_new) : 0;
+    const int64_t rows = ok ? s.all_rows : 0;
+    if (blockIdx.x == 0) {
+        if (tid < a.n_seqs) write_seq(a, tid, q, s.rows, head + s.pages, ok);
+        if (tid == 0) write_step(a, rows, ok ? head + s.all_pages : head, flags);
     }
-    int64_t carry_new = 0, carry_fresh = 0;
-    for (int base = 0; base < a.n_seqs; base += nthr) {
-        const int s = base + tid;
-        PlanSeq q{};
-        if (s < a.n_seqs) q = plan_seq(a, shift, s);
-        const int64_t in_new = wave_scan(q.added, lane), in_fresh = wave_scan(q.fresh, lane);
-        if (lane == 63) {
-            sums[0][wave] = in_new;
-            sums[1][wave] = in_fresh;
-        }
-        __syncthreads();
-        int64_t at = carry_new + in_new - q.added, first = head + carry_fresh + in_fresh - q.fresh;
-        for (int w = 0; w < nwave; ++w) {
-            if (w < wave) {
-                at += sums[0][w];
-                first += sums[1][w];
-            }
-            carry_new += sums[0][w];
-            carry_fresh += sums[1][w];
-        }
-        if (s < a.n_seqs) {
-            const int64_t kv = ok ? q.cached + q.added : q.cached;
-            a.row_offsets[s] = ok ? static_cast<int32_t>(at) : 0;
-            a.kv_lens[s] = static_cast<int32_t>(kv);
-            if (ok)
-                for (int64_t i = 0; i < q.fresh; ++i)
-                    a.block_table[s * a.table_stride + q.held + i] = a.free_pages[first + i];
-            if (rows) {
-                off_lds[s] = ok ? static_cast<int32_t>(at) : 0;
-                kv_lds[s] = static_cast<int32_t>(kv);
-                held_lds[s] = static_cast<int32_t>(q.held);
-                first_lds[s] = static_cast<int32_t>(first);
-            }
-        }
-        __syncthreads();
+    if (tid < a.n_seqs) {
+        off[tid] = ok ? static_cast<int32_t>(s.rows) : 0;
+        kv_len[tid] = static_cast<int32_t>(q.cached + q.added);
+        held[tid] = static_cast<int32_t>(q.held);
+        fresh_at[tid] = static_cast<int32_t>(head + s.pages);
     }
-    if (!rows) return;
-    const int64_t real = ok ? n_new : 0;
-    for (int64_t r = tid; r < a.n_rows; r += nthr) {
+    if (tid == 0) off[a.n_seqs] = static_cast<int32_t>(rows);
+    __syncthreads();
+    const int64_t row_end = idx_min(a.n_rows, (static_cast<int64_t>(blockIdx.x) + 1) * group_rows);
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * group_rows + tid; r < row_end; r += nthr) {
         int32_t pos = 0;
         int64_t slot = -1;
-        if (r < real) {
-            const int s = seq_of_row(off_lds, a.n_seqs, r);
-            pos = static_cast<int32_t>(kv_lds[s] - (off_lds[s + 1] - r));
+        if (r < rows) {
+            const int t = seq_of_row(off, a.n_seqs, r);
+            pos = static_cast<int32_t>(kv_len[t] - (off[t + 1] - r));
             const int32_t col = pos >> shift;
-            const int32_t page = col < held_lds[s] ? a.block_table[s * a.table_stride + col]
-                                                   : a.free_pages[first_lds[s] + (col - held_lds[s])];
+            // its own entry, or the one that the first workgroup is about to make it
+            const int32_t page = col < held[t] ? a.block_table[t * a.table_stride + col]
+                                               : a.free_pages[fresh_at[t] + (col - held[t])];
             if (page >= 0) slot = (static_cast<int64_t>(page) << shift) + (pos & ((1 << shift) - 1));
         }
         a.positions[r] = pos;
         a.slots[r] = slot;
     }
+}
+
+// More requests: one workgroup sums, a part of the requests at a time.
+__global__ __launch_bounds__(kPlanThreads) void kv_plan_seqs_kernel(mi355x_kv_plan_args a, int shift) {
+    __shared__ uint32_t sums[2][kPlanWaves];
+    __shared__ int all_flags;
+    const int tid = threadIdx.x;
+    const int64_t head = *a.free_head;
+    if (tid == 0) all_flags = 0;
+    PlanSums all{};
+    // totals first: a step that does not fit takes nothing
+    for (int base = 0; base < a.n_seqs; base += kPlanThreads) {
+        __syncthreads();
+        PlanSeq q{};
+        if (base + tid < a.n_seqs) q = plan_seq(a, shift, base + tid);
+        if (q.flags) atomicOr(&all_flags, q.flags);
+        const PlanSums s = group_sums(static_cast<uint32_t>(q.added), static_cast<uint32_t>(q.fresh), sums);
+        all.all_rows = __builtin_elementwise_add_sat(all.all_rows, s.all_rows);
+        all.all_pages = __builtin_elementwise_add_sat(all.all_pages, s.all_pages);
+    }
+    __syncthreads();
+    const int flags = plan_flags(a, all_flags, all, head);
+    const bool ok = flags == 0;
+    uint32_t rows = 0, pages = 0;
+    for (int base = 0; base < a.n_seqs; base += kPlanThreads) {
+        __syncthreads();
+        PlanSeq q{};
+        if (base + tid < a.n_seqs) q = plan_seq(a, shift, base + tid);
+        const PlanSums s = group_sums(static_cast<uint32_t>(q.added), static_cast<uint32_t>(q.fresh), sums);
+        if (base + tid < a.n_seqs)
+            write_seq(a, base + tid, q, int64_t(rows) + s.rows, head + pages + s.pages, ok);
+        rows = __builtin_elementwise_add_sat(rows, s.all_rows);
+        pages = __builtin_elementwise_add_sat(pages, s.all_pages);
+    }
+    if (tid == 0) write_step(a, ok ? all.all_rows : 0, ok ? head + all.all_pages : head, flags);
 }
 
 // Rows of a step whose offsets, lengths and tables stand already.
@@ -166,12 +210,22 @@ __global__ __launch_bounds__(256) void kv_plan_rows_kernel(mi355x_kv_plan_args a
 
 int launch_kv_plan(mi355x_ctx *ctx, const mi355x_kv_plan_args &a) {
     const int shift = __builtin_ctz(static_cast<unsigned>(a.page_tokens));
-    const bool one = a.n_seqs <= kPlanLdsSeqs && a.n_rows <= kPlanOneLaunchRows;
-    const int64_t work = std::max<int64_t>(a.n_seqs, one ? a.n_rows : 0);
-    const int threads = static_cast<int>(std::min<int64_t>(kPlanThreads, std::max<int64_t>(64, (work + 63) / 64 * 64)));
-    kv_plan_kernel<<<1, threads, 0, ctx->stream>>>(a, shift, one ? 1 : 0);
+    // a request per thread, and enough threads for the rows of a small step
+    const int64_t most = std::max<int64_t>(a.n_seqs, std::min<int64_t>(a.n_rows, 256));
+    const int threads = static_cast<int>(std::min<int64_t>(kPlanThreads, std::max<int64_t>(64, (most + 63) / 64 * 64)));
+    // several workgroups may not read what the first one writes in place
+    const bool in_place = a.kv_lens == a.cached || a.free_head_out == a.free_head;
+    const int64_t group_rows = int64_t(threads) * kPlanThreadRows;
+    if (a.n_seqs <= kPlanOneLaunchSeqs && (!in_place || a.n_rows <= kPlanInPlaceRows)) {
+        const int64_t groups = in_place ? 1 : std::max<int64_t>(1, std::min<int64_t>(1024, (a.n_rows + group_rows - 1) / group_rows));
+        const int64_t rows = (std::max<int64_t>(a.n_rows, 1) + groups - 1) / groups;
+        kv_plan_kernel<<<static_cast<unsigned>(groups), threads, 0, ctx->stream>>>(a, shift, static_cast<int>(rows));
+        MI355X_HIP(hipGetLastError());
+        return MI355X_OK;
+    }
+    kv_plan_seqs_kernel<<<1, kPlanThreads, 0, ctx->stream>>>(a, shift);
     MI355X_HIP(hipGetLastError());
-    if (!one && a.n_rows > 0) {
+    if (a.n_rows > 0) {
         kv_plan_rows_kernel<<<static_cast<unsigned>((a.n_rows + 255) / 256), 256, 0, ctx->stream>>>(a, shift);
         MI355X_HIP(hipGetLastError());
     }

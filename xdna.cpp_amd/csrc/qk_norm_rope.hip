@@ -77,40 +77,41 @@ __device__ __forceinline__ TO *out_head(const RopeArgs &a, int64_t row, int whic
            h * a.head_stride;
 }
 
-// Eight values of a head per lane (four pairs of the rotated part, or eight
-// values behind it), LANES lanes per head: head_dim and rot_dim are multiples of
-// 8 and rows, strides and pages of 16 bytes.  A lane's place within the head is
-// the same for every head that it takes, so it forms its sines and cosines once
-// per row, and every lane's loads are two of 8 or 16 bytes.
-template <int TYPE>
-struct Four {
-    typedef typename Elem<TYPE>::T V __attribute__((ext_vector_type(4)));
+// Two runs of W values of a head per lane -- W pairs of the rotated part, or 2 W
+// values behind it --, LANES lanes per head: head_dim and rot_dim are multiples
+// of 2 W, and rows, strides and pages of 16 bytes.  A lane's place within the head
+// is the same for every head that it takes, so it forms its sines and cosines
+// once per row.  W = 8 (16-byte loads of 16-bit values) where the sizes allow it:
+// 8192 rows of 32 + 2 x 8 heads of 128 RR us, 52 with W = 4.
+template <int TYPE, int W>
+struct Run {
+    typedef typename Elem<TYPE>::T V __attribute__((ext_vector_type(W)));
 };
-typedef float f32x4_r __attribute__((ext_vector_type(4)));
 
-template <int IN, int OUT, bool PAIRS, int LANES>
+template <int IN, int OUT, bool PAIRS, int W, int LANES>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int heads, int rows_per_group) {
     typedef typename Elem<IN>::T TI;
     typedef typename Elem<OUT>::T TO;
-    typedef typename Four<IN>::V VI;
-    typedef typename Four<OUT>::V VO;
+    typedef typename Run<IN, W>::V VI;
+    typedef typename Run<OUT, W>::V VO;
+    typedef typename Run<MI355X_TYPE_F32, W>::V VF;
     constexpr int kHeadsAtOnce = 256 / LANES;
     const int u = threadIdx.x % LANES, slot = threadIdx.x / LANES;
     const int hd = a.head_dim, rot = a.rot_dim;
-    const bool on = 8 * u < hd, turned = 8 * u < rot;
-    // the lane's two runs of four values
-    const int i0 = !on ? 0 : turned && !PAIRS ? 4 * u : 8 * u;
-    const int i1 = !on ? 4 : turned && !PAIRS ? rot / 2 + 4 * u : 8 * u + 4;
+    const bool on = 2 * W * u < hd, turned = 2 * W * u < rot;
+    // the lane's two runs
+    const int i0 = !on ? 0 : turned && !PAIRS ? W * u : 2 * W * u;
+    const int i1 = !on ? W : turned && !PAIRS ? rot / 2 + W * u : 2 * W * u + W;
     const int first_head = blockIdx.y * kHeadsAtOnce, step = gridDim.y * kHeadsAtOnce;
-    f32x4_r freq = {0, 0, 0, 0};
-    if (turned) freq = *reinterpret_cast<const f32x4_r *>(a.inv_freq + 4 * u);
+    VF freq;
+    if (turned) freq = *reinterpret_cast<const VF *>(a.inv_freq + W * u);
     const int64_t row_end = min(a.n_rows, (static_cast<int64_t>(blockIdx.x) + 1) * rows_per_group);
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_group; row < row_end; ++row) {
-        float c[4], s[4];
+        float c[W], s[W];
         if (turned) {
             const int32_t pos = a.positions[row];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) turn(pos, freq[i], &c[i], &s[i]);
+            for (int i = 0; i < W; ++i) turn(pos, freq[i], &c[i], &s[i]);
         }
         for (int hh = first_head + slot; hh < heads; hh += step) {
             const int which = hh < a.n_heads ? 0 : hh < a.n_heads + a.n_kv_heads ? 1 : 2;
@@ -120,23 +121,22 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int heads, int ro
                             static_cast<int64_t>(h) * hd;
             const float *bias = which == 0 ? a.bias[0] : which == 1 ? a.bias[1] : a.bias[2];
             const float *norm = which == 0 ? a.norm[0] : which == 1 ? a.norm[1] : nullptr;
-            const int j0 = which == 2 ? 8 * u : i0, j1 = which == 2 ? 8 * u + 4 : i1;
-            float x[8];
+            const int j0 = which == 2 ? 2 * W * u : i0, j1 = which == 2 ? 2 * W * u + W : i1;
+            float x[2 * W];
             if (on) {
                 const VI p = *reinterpret_cast<const VI *>(src + j0), q = *reinterpret_cast<const VI *>(src + j1);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < W; ++i) {
                     x[i] = Elem<IN>::up(p[i]);
-                    x[4 + i] = Elem<IN>::up(q[i]);
+                    x[W + i] = Elem<IN>::up(q[i]);
                 }
                 if (bias) {
                     const float *b = bias + static_cast<int64_t>(h) * hd;
-                    const f32x4_r p1 = *reinterpret_cast<const f32x4_r *>(b + j0),
-                                  q1 = *reinterpret_cast<const f32x4_r *>(b + j1);
+                    const VF p1 = *reinterpret_cast<const VF *>(b + j0), q1 = *reinterpret_cast<const VF *>(b + j1);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < W; ++i) {
                         x[i] += p1[i];
-                        x[4 + i] += q1[i];
+                        x[W + i] += q1[i];
                     }
                 }
             }
@@ -144,22 +144,21 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int heads, int ro
                 float ss = 0.0f;
                 if (on)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+                    for (int i = 0; i < 2 * W; ++i) ss = fmaf(x[i], x[i], ss);
                 const float scale = 1.0f / sqrtf(group_sum(ss, LANES) / static_cast<float>(hd) + a.eps);
                 if (on) {
-                    const f32x4_r p1 = *reinterpret_cast<const f32x4_r *>(norm + j0),
-                                  q1 = *reinterpret_cast<const f32x4_r *>(norm + j1);
+                    const VF p1 = *reinterpret_cast<const VF *>(norm + j0), q1 = *reinterpret_cast<const VF *>(norm + j1);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < W; ++i) {
                         x[i] = x[i] * scale * p1[i];
-                        x[4 + i] = x[4 + i] * scale * q1[i];
+                        x[W + i] = x[W + i] * scale * q1[i];
                     }
                 }
             }
             if (turned && which != 2) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int m = PAIRS ? 2 * i : i, n = PAIRS ? 2 * i + 1 : 4 + i;
+                for (int i = 0; i < W; ++i) {
+                    const int m = PAIRS ? 2 * i : i, n = PAIRS ? 2 * i + 1 : W + i;
                     const float v = x[m], w = x[n];
                     x[m] = v * c[i] - w * s[i];
                     x[n] = w * c[i] + v * s[i];
@@ -169,9 +168,9 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int heads, int ro
             if (dst) {
                 VO p, q;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < W; ++i) {
                     p[i] = Elem<OUT>::down(x[i]);
-                    q[i] = Elem<OUT>::down(x[4 + i]);
+                    q[i] = Elem<OUT>::down(x[W + i]);
                 }
                 *reinterpret_cast<VO *>(dst + j0) = p;
                 *reinterpret_cast<VO *>(dst + j1) = q;
@@ -220,7 +219,7 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int heads, in
     for (int i = rot + lane; i < hd; i += 64) dst[i] = Elem<OUT>::down(normed(i));
 }
 
-template <int IN, int OUT, bool PAIRS, int LANES>
+template <int IN, int OUT, bool PAIRS, int W, int LANES>
 int launch_rope_lanes(mi355x_ctx *ctx, const RopeArgs &a) {
     const int heads = a.n_heads + (a.slots ? 2 : 1) * a.n_kv_heads;
     const int64_t at_once = 256 / LANES, passes = (heads + at_once - 1) / at_once;
@@ -229,7 +228,7 @@ int launch_rope_lanes(mi355x_ctx *ctx, const RopeArgs &a) {
     constexpr int64_t kMostGroups = int64_t(1) << 22;
     const int rows_per_group = static_cast<int>((a.n_rows + kMostGroups - 1) / kMostGroups);
     const dim3 grid(static_cast<unsigned>((a.n_rows + rows_per_group - 1) / rows_per_group), static_cast<unsigned>(split));
-    rope_kernel<IN, OUT, PAIRS, LANES><<<grid, 256, 0, ctx->stream>>>(a, heads, rows_per_group);
+    rope_kernel<IN, OUT, PAIRS, W, LANES><<<grid, 256, 0, ctx->stream>>>(a, heads, rows_per_group);
     MI355X_HIP(hipGetLastError());
     return MI355X_OK;
 }
@@ -268,10 +267,16 @@ int launch_rope_pairs(mi355x_ctx *ctx, const RopeArgs &a) {
     for (int i = 0; i < 2; ++i) fast = fast && whole_chunks(a.norm[i], 0, 4);
     if (!a.slots) fast = fast && whole_chunks(a.k_dst, a.k_row_stride, ob);
     if (!fast) return launch_rope_any<IN, OUT, PAIRS>(ctx, a);
-    if (a.head_dim <= 64) return launch_rope_lanes<IN, OUT, PAIRS, 8>(ctx, a);
-    if (a.head_dim <= 128) return launch_rope_lanes<IN, OUT, PAIRS, 16>(ctx, a);
-    if (a.head_dim <= 256) return launch_rope_lanes<IN, OUT, PAIRS, 32>(ctx, a);
-    return launch_rope_lanes<IN, OUT, PAIRS, 64>(ctx, a);
+    if (a.head_dim % 16 == 0 && a.rot_dim % 16 == 0) {
+        if (a.head_dim <= 64) return launch_rope_lanes<IN, OUT, PAIRS, 8, 4>(ctx, a);
+        if (a.head_dim <= 128) return launch_rope_lanes<IN, OUT, PAIRS, 8, 8>(ctx, a);
+        if (a.head_dim <= 256) return launch_rope_lanes<IN, OUT, PAIRS, 8, 16>(ctx, a);
+        return launch_rope_lanes<IN, OUT, PAIRS, 8, 32>(ctx, a);
+    }
+    if (a.head_dim <= 64) return launch_rope_lanes<IN, OUT, PAIRS, 4, 8>(ctx, a);
+    if (a.head_dim <= 128) return launch_rope_lanes<IN, OUT, PAIRS, 4, 16>(ctx, a);
+    if (a.head_dim <= 256) return launch_rope_lanes<IN, OUT, PAIRS, 4, 32>(ctx, a);
+    return launch_rope_lanes<IN, OUT, PAIRS, 4, 64>(ctx, a);
 }
 
 template <int IN, int OUT>
