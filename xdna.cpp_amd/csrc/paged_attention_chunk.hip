@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
 
 // Joins the parts of each row block and KV head: a workgroup kJoinRows of its
 // rows, a thread 4 values.  (In the kernel above, by the last of a block's
-// workgroups, the parts of a chunk of 512 tokens cost 40 us instead of JJ: one CU
+// workgroups, the parts of a chunk of 512 tokens cost 40 us instead of 7.6: one CU
 // reads what 16 do here.)
 constexpr int kJoinThreads = 256;
 
