@@ -172,6 +172,14 @@ def test_windows_and_caps(ctx, window, softcap):
     go(ctx, [1, 90, 4, 300], [700, 90, 333, 301], 4, 2, 64, F16, F32, window=window, softcap=softcap, sharp=3.0)
 
 
+@pytest.mark.parametrize("q_lens,kv", [([1, 2], [300, 130]), ([40, 100], [300, 130])])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cap", [1e-40, 1e-3, 0.5, 40.0, 50.0, 1000.0, 1e9, 3e38])
+def test_caps_of_any_size(ctx, cap, hd, q_lens, kv):
+    """Scores far below the cap are as exact as without one."""
+    go(ctx, q_lens, kv, 4, 2, hd, F16, F32, softcap=cap)
+
+
 @pytest.mark.parametrize("window", [0, 30])
 def test_not_causal(ctx, window):
     go(ctx, [1, 50, 200], [40, 50, 260], 4, 2, 64, window=window, causal=False)
@@ -181,6 +189,12 @@ def test_many_requests_of_all_lengths(ctx):
     rng = np.random.default_rng(1)
     q = rng.integers(0, 4, 300)
     go(ctx, list(q), list(q + rng.integers(0, 200, 300)), 4, 1, 64, F16, F16, page=8)
+
+
+def test_thousands_of_requests(ctx):
+    rng = np.random.default_rng(2)
+    q = rng.integers(0, 3, 3000)
+    go(ctx, list(q), list(q + rng.integers(0, 40, 3000)), 2, 1, 64, BF16, F32, page=4)
 
 
 def test_one_long_request_among_short_ones(ctx):
@@ -204,7 +218,8 @@ def test_rows_that_see_nothing_and_requests_of_no_length(ctx):
         c.free()
 
 
-@pytest.mark.parametrize("q_lens,kv", [([1, 1], [40, 77]), ([30, 64], [130, 200]), ([6, 200], [90, 200])])
+@pytest.mark.parametrize("q_lens,kv", [([1, 1], [40, 77]), ([30, 64], [130, 200]), ([6, 200], [90, 200]),
+                                       ([130] * 260, [130] * 259 + [150])])
 @pytest.mark.parametrize("poison", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("window", [0, 20])
 def test_tokens_not_seen_do_not_reach_a_row(ctx, q_lens, kv, poison, window):

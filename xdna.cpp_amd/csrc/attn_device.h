@@ -25,7 +25,7 @@ struct AttnArgs {
     int reach;          // tokens that the table's columns hold, at most 2^30
     int row_limit;      // requests of at most (token form) or more than (chunk form) so many head rows
     float scale2;            // scale log2 e: scores are in factors of 2
-    float cap_in, cap_out;   // 2 scale log2 e / softcap and softcap log2 e; 0: no cap
+    float cap_in, cap_out;   // 2 scale log2 e / softcap (finite) and softcap log2 e; 0: no cap
     FastDiv group;  // query heads of a KV head
     int n_seqs, n_kv_heads;
     int n_pages, shift, window, causal, f32_out;
@@ -98,7 +98,9 @@ __device__ __forceinline__ void load_lds16(const void *from, unsigned char *to) 
         (__attribute__((address_space(3))) uint32_t *)(to), 16, 0, 0);
 }
 
-// Scores of n values of q . k; tanh x as 1 - 2 / (1 + e^2x), within 2^-23 of 1.
+// Scores of N values x of q . k, in factors of 2.  tanh y as 1 - 2 / (1 + e^2y),
+// within 2^-23 of 1, and below 1/8, where that is too coarse for a small score,
+// by its series (the next term is 62/2835 y^8: 2^-29).
 template <int N>
 __device__ __forceinline__ void scores2(float (&x)[N], const AttnArgs &a) {
     if (a.cap_out == 0.0f) {
@@ -106,9 +108,13 @@ __device__ __forceinline__ void scores2(float (&x)[N], const AttnArgs &a) {
         for (int i = 0; i < N; ++i) x[i] *= a.scale2;
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            x[i] = fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i] * a.cap_in)),
-                        a.cap_out);
+        for (int i = 0; i < N; ++i) {
+            const float e = x[i] * a.cap_in, y = e * (0.5f / kLog2e), y2 = y * y;
+            const float small = x[i] * a.scale2 *
+                                fmaf(y2, fmaf(y2, fmaf(y2, -17.0f / 315, 2.0f / 15), -1.0f / 3), 1.0f);
+            const float big = fmaf(-2.0f * a.cap_out, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(e)), a.cap_out);
+            x[i] = fabsf(y) < 0.125f ? small : big;
+        }
     }
 }
 

@@ -25,6 +25,7 @@
 #include "internal.h"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace mi355x {
 namespace {
@@ -494,7 +495,7 @@ int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &u
     a.reach = u.pool->n_pages > 0 ? u.table_cols * u.pool->page_tokens : 0;
     a.scale2 = u.scale * kLog2e;
     if (u.softcap > 0.0f) {
-        a.cap_in = u.scale / u.softcap * (2.0f * kLog2e);
+        a.cap_in = std::max(-FLT_MAX, std::min(FLT_MAX, u.scale / u.softcap * (2.0f * kLog2e)));
         a.cap_out = u.softcap * kLog2e;
     }
     a.n_seqs = u.n_seqs;

@@ -28,6 +28,9 @@ namespace mi355x {
 namespace {
 
 constexpr int kChunkKeys = 64;
+// Softcaps (times log2 e) up to which 1 - 2 / (1 + e^2y) is near enough to tanh y, to
+// 2^-23 of the cap.
+constexpr float kNearCap = 64.0f;
 // Instruction kinds of __builtin_amdgcn_sched_group_barrier.
 constexpr int kMfma = 0x8, kDsRead = 0x100;
 
@@ -136,7 +139,6 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
     const bool real = row_raw < g.rows;
     const int row = real ? row_raw : 0, tok = divided(row, a.group), group = static_cast<int>(a.group.d);
     const int64_t head = static_cast<int64_t>(kvh) * group + (row - tok * group);
-    const bool busy = it.row0 + 32 * wave < g.rows;  // a wavefront without rows only loads
     const Keys mine = token_keys(a, g, g.tok_lo + tok);
     const int row_lo = mine.lo, row_hi = real ? mine.hi : 0;
     V8 qf[kSteps];
@@ -172,7 +174,11 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
     const int v_at = v_row * S::kRowBytes + (lane & 1) * 8;
     const int v_low = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_turn<S::kPlaces>(v_row);
     const int32_t *table = a.table + it.seq * a.table_stride;
-    const float c = a.scale2;
+    // A row's scores are c1 y + c0, c1 > 0, of the values y that the loop below keeps
+    // and compares: of q . k, of -1 / (1 + e^2y) under a cap (a weight then costs one
+    // operation less), or of the scores themselves.
+    const bool near_cap = CAP && a.cap_out > 0.0f && a.cap_out <= kNearCap;
+    const float c1 = CAP ? near_cap ? 2.0f * a.cap_out : 1.0f : a.scale2, c0 = near_cap ? a.cap_out : 0.0f;
 
     // Tokens [some_lo, some_hi) are seen by some row; the others' values count as
     // zero.  Where a value that only some of the rows see is not finite (a weight of
@@ -253,7 +259,8 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
                 if (__any(bad) && lane == 0) odd = 1;
                 __syncthreads();
             }
-            if (!busy) continue;
+            // keys that no row of this wavefront sees
+            if (!__any(row_lo < base + kChunkKeys && row_hi > base)) continue;
             float s[32];  // keys 32 (i / 16) + 8 (i / 4 % 4) + 4 half + i % 4
             f32x16 x[2];
 #pragma unroll
@@ -280,8 +287,14 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
                 s[i] = x[0][i];
                 s[16 + i] = x[1][i];
             }
-            if (CAP) scores2(s, a);
-            if (!full) {
+            if (near_cap) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) s[i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[i] * a.cap_in));
+            } else if (CAP) {
+                scores2(s, a);
+            }
+            // every key seen by every row of this wavefront
+            if (!full && !__all(row_lo <= base && base + kChunkKeys <= row_hi && ~seen == 0)) {
                 const uint64_t see = (seen & range_mask<uint64_t>(row_lo, row_hi, base)) >> (4 * half);
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
@@ -291,7 +304,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
 #pragma unroll
             for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
             top = half_max(top);
-            if (!CAP) top *= c;  // c > 0 here
+            top = fmaf(top, c1, c0);
             const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
             if (__any(grows)) {
                 const float m_new = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
@@ -300,7 +313,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
                 for (int d = 0; d < kBlocks; ++d) o[d] *= keep;
                 m = m_new;
             }
-            const float ref = finite_base(m);
+            const float base2 = c0 - finite_base(m);
             auto v_chunk = [&](int j, int d) {  // keys 16 j + {4 half .. + 3, 8 + 4 half .. + 3} of 32 values
                 const int place = (4 * d) ^ v_low;
                 const s16x4 *p = reinterpret_cast<const s16x4 *>(vt + v_at + 16 * j * S::kRowBytes + 16 * place);
@@ -321,7 +334,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
                 V8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float y = s[8 * j + i], p = __builtin_amdgcn_exp2f(CAP ? y - ref : fmaf(y, c, -ref));
+                    const float y = s[8 * j + i], p = __builtin_amdgcn_exp2f(fmaf(y, c1, base2));
                     l += p;
                     const T h = static_cast<T>(p);
                     hi[i] = h;
