@@ -69,7 +69,7 @@ def equal(got, ref):
 @pytest.mark.parametrize("n,cached_hi,added_hi,page,pad", [
     (1, 0, 1, 16, 0), (1, 100, 1, 1, 0), (3, 0, 70, 8, 5), (64, 900, 1, 16, 0), (65, 50, 9, 64, 1),
     (257, 300, 40, 32, 3), (1024, 40, 3, 8, 0), (1025, 40, 3, 8, 2), (2500, 33, 5, 4, 700), (7, 3000, 4000, 256, 11),
-    (40, 0, 0, 16, 6)])
+    (40, 0, 0, 16, 6), (2, 5, 90000, 1, 4), (1100, 9, 300, 2, 1)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_plan(ctx, n, cached_hi, added_hi, page, pad, in_place):
     rng = np.random.default_rng([n, page])

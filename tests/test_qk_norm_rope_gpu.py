@@ -195,3 +195,25 @@ def test_zero_rows_of_a_norm_and_non_finite_values(ctx):
         assert np.all(np.isfinite(q))
     finally:
         c.free()
+
+
+def test_more_rows_than_workgroups(ctx):
+    """Past 2^22 rows a workgroup takes several: the first and the last ones."""
+    T, hd = 2 ** 22 + 2 ** 20 + 3, 8
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((T, hd), dtype=np.float32)
+    pos = np.arange(T, dtype=np.int32)
+    freq = (1e4 ** (-2.0 * np.arange(hd // 2) / hd)).astype(np.float32)
+    bufs = [ctx.to_device(a) for a in (x, pos, freq, np.zeros(T * hd, np.float32))]
+    try:
+        ctx.qk_norm_rope(mi355x.QkNormRopeArgs(
+            n_rows=T, n_heads=1, n_kv_heads=0, head_dim=hd, rot_dim=hd, rope_mode=mi355x.ROPE_HALVES, in_type=F32,
+            out_type=F32, eps=1e-6, q=bufs[0].ptr, q_stride=hd, positions=bufs[1].ptr, inv_freq=bufs[2].ptr,
+            q_out=bufs[3].ptr, q_out_stride=hd))
+        ctx.sync()
+        got = bufs[3].download(np.float32, T * hd).reshape(T, 1, hd)
+        for part in (slice(0, 5000), slice(T // 2, T // 2 + 5000), slice(T - 5000, T)):
+            check(got[part], *paged_ref.rope(x[part, None], None, None, 1e-6, pos[part], freq, hd, False), F32, part)
+    finally:
+        for b in bufs:
+            b.free()

@@ -88,13 +88,10 @@ __device__ __forceinline__ int plan_flags(const mi355x_kv_plan_args &a, int flag
     return flags;
 }
 
-// What belongs to request s, and (s = 0) to the step.
-__device__ __forceinline__ void write_seq(const mi355x_kv_plan_args &a, int s, const PlanSeq &q, int64_t row,
-                                          int64_t first, bool ok) {
+// What belongs to request s but its table, and what belongs to the step.
+__device__ __forceinline__ void write_seq(const mi355x_kv_plan_args &a, int s, const PlanSeq &q, int64_t row, bool ok) {
     a.row_offsets[s] = ok ? static_cast<int32_t>(row) : 0;
     a.kv_lens[s] = static_cast<int32_t>(ok ? q.cached + q.added : q.cached);
-    if (ok)
-        for (int64_t i = 0; i < q.fresh; ++i) a.block_table[s * a.table_stride + q.held + i] = a.free_pages[first + i];
 }
 __device__ __forceinline__ void write_step(const mi355x_kv_plan_args &a, int64_t rows, int64_t head, int flags) {
     a.row_offsets[a.n_seqs] = static_cast<int32_t>(rows);
@@ -124,7 +121,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(mi355x_kv_plan_ar
     const bool ok = flags == 0;
     const int64_t rows = ok ? s.all_rows : 0;
     if (blockIdx.x == 0) {
-        if (tid < a.n_seqs) write_seq(a, tid, q, s.rows, head + s.pages, ok);
+        if (tid < a.n_seqs) write_seq(a, tid, q, s.rows, ok);
         if (tid == 0) write_step(a, rows, ok ? head + s.all_pages : head, flags);
     }
     if (tid < a.n_seqs) {
@@ -143,9 +140,15 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(mi355x_kv_plan_ar
             const int t = seq_of_row(off, a.n_seqs, r);
             pos = static_cast<int32_t>(kv_len[t] - (off[t + 1] - r));
             const int32_t col = pos >> shift;
-            // its own entry, or the one that the first workgroup is about to make it
-            const int32_t page = col < held[t] ? a.block_table[t * a.table_stride + col]
-                                               : a.free_pages[fresh_at[t] + (col - held[t])];
+            // an entry that stands, or a new one, which its page's first row writes
+            int32_t *entry = a.block_table + t * a.table_stride + col;
+            int32_t page;
+            if (col < held[t]) {
+                page = *entry;
+            } else {
+                page = a.free_pages[fresh_at[t] + (col - held[t])];
+                if ((pos & ((1 << shift) - 1)) == 0) *entry = page;
+            }
             if (page >= 0) slot = (static_cast<int64_t>(page) << shift) + (pos & ((1 << shift) - 1));
         }
         a.positions[r] = pos;
@@ -157,6 +160,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(mi355x_kv_plan_ar
 __global__ __launch_bounds__(kPlanThreads) void kv_plan_seqs_kernel(mi355x_kv_plan_args a, int shift) {
     __shared__ uint32_t sums[2][kPlanWaves];
     __shared__ int all_flags;
+    __shared__ int32_t fresh_at[kPlanThreads + 1], held[kPlanThreads];
     const int tid = threadIdx.x;
     const int64_t head = *a.free_head;
     if (tid == 0) all_flags = 0;
@@ -180,8 +184,18 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_seqs_kernel(mi355x_kv_pl
         PlanSeq q{};
         if (base + tid < a.n_seqs) q = plan_seq(a, shift, base + tid);
         const PlanSums s = group_sums(static_cast<uint32_t>(q.added), static_cast<uint32_t>(q.fresh), sums);
-        if (base + tid < a.n_seqs)
-            write_seq(a, base + tid, q, int64_t(rows) + s.rows, head + pages + s.pages, ok);
+        if (base + tid < a.n_seqs) write_seq(a, base + tid, q, int64_t(rows) + s.rows, ok);
+        if (ok) {
+            // the part's new pages, side by side in the free list, a thread each
+            fresh_at[tid] = static_cast<int32_t>(s.pages);
+            held[tid] = static_cast<int32_t>(q.held);
+            if (tid == 0) fresh_at[kPlanThreads] = static_cast<int32_t>(s.all_pages);
+            __syncthreads();
+            for (int64_t i = tid; i < s.all_pages; i += kPlanThreads) {
+                const int t = seq_of_row(fresh_at, kPlanThreads, i);
+                a.block_table[(base + t) * a.table_stride + held[t] + (i - fresh_at[t])] = a.free_pages[head + pages + i];
+            }
+        }
         rows = __builtin_elementwise_add_sat(rows, s.all_rows);
         pages = __builtin_elementwise_add_sat(pages, s.all_pages);
     }

@@ -405,6 +405,9 @@ __global__ __launch_bounds__(kJoinThreads) void attention_chunk_join_kernel(Attn
     store_out4<TYPE>(a, out_at(a, it.g, kvh, it.row0 + r, HD) + c, j.value());
 }
 
+// Threads of a launch.
+constexpr int64_t kMostThreads = UINT32_MAX;
+
 // Workgroups that a call is split into at most, while that is more than its row blocks.
 int chunk_groups(const mi355x_ctx *ctx) { return 2 * ctx->num_cus; }
 
@@ -420,7 +423,7 @@ int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
     const int64_t rows = a.n_rows * a.group.d;
     if constexpr (HD <= 128) {
         const int64_t items = ((rows >> row_shift(8)) + a.n_seqs) * a.n_kv_heads;
-        if ((rows >> row_shift(8)) * a.n_kv_heads >= ctx->num_cus && items <= INT32_MAX) {
+        if ((rows >> row_shift(8)) * a.n_kv_heads >= ctx->num_cus && items <= kMostThreads / 512) {
             attention_chunk_kernel<TYPE, HD, CAP, PLANES, 8>
                 <<<static_cast<unsigned>(items), 512, ChunkShape<HD, 8>::kLds, ctx->stream>>>(a);
             MI355X_HIP(hipGetLastError());
@@ -431,7 +434,7 @@ int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
     // parts of no fewer than four tiles where the table allows that many tokens
     a.split = static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>(chunk_groups(ctx) / items, (int64_t(a.reach) + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
-    if (items * a.split > INT32_MAX)
+    if (items * a.split > kMostThreads / 256)
         return set_error(MI355X_EUNSUPPORTED, "mi355x_paged_attention: more row blocks than a launch takes");
     attention_chunk_kernel<TYPE, HD, CAP, PLANES, 4>
         <<<static_cast<unsigned>(items * a.split), 256, ChunkShape<HD, 4>::kLds, ctx->stream>>>(a);
