@@ -13,7 +13,10 @@
 // two exchanges; the weights are then, as they lie, the operand of V^T w, whose
 // V^T comes out of LDS through the transposing read.  Weights go in as two
 // 16-bit planes: the matrix cores idle here, and the second plane makes them as
-// good as f32.
+// good as f32.  64 requests of up to 8192 tokens, 32 query and 8 KV heads of 128:
+// 1.0 GB in 190 us, 5.2 TB/s, as fast as a copy; one of 131072 tokens 113 us, 4.8
+// TB/s.  Short calls are bound by latency: lengths, table, keys, parts and their
+// join each wait for the one before (640 tokens, 2 KV heads: 9.7 us).
 //
 // Work split.  All requests' keys, heads and row blocks form one line of
 // 128-key units; every workgroup takes an equal stretch of it, whatever the
@@ -54,8 +57,9 @@ __device__ __forceinline__ TokenWork token_work(const AttnArgs &a, const SeqGeo 
 }
 
 // The units before each request, a request per thread.  Up to 64 requests: every
-// wavefront scans them by itself.  More: the workgroup does, all of them at once
-// or a part at a time.
+// wavefront scans them by itself (one request of 640 tokens 9.8 us against 10.1, 64
+// ragged ones 194 against 196).  More: the workgroup does, all of them at once or a
+// part at a time.
 template <int WAVES>
 struct Scan {
     int64_t total;

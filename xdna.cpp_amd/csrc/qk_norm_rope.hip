@@ -230,7 +230,8 @@ template <int IN, int OUT, bool PAIRS, int W, int LANES>
 int launch_rope_lanes(mi355x_ctx *ctx, const RopeArgs &a) {
     const int heads = a.n_heads + (a.slots ? 2 : 1) * a.n_kv_heads;
     const int64_t at_once = 256 / LANES, passes = (heads + at_once - 1) / at_once;
-    // few rows: a workgroup per row and pass over its heads; many: one per row
+    // few rows: a workgroup per row and pass over its heads (one row of 20 heads of 128:
+    // 3.9 us against 4.1); many: one per row
     const int64_t split = std::max<int64_t>(1, std::min<int64_t>(passes, 4 * ctx->num_cus / std::max<int64_t>(1, a.n_rows)));
     constexpr int64_t kMostGroups = int64_t(1) << 22;
     const int rows_per_group = static_cast<int>((a.n_rows + kMostGroups - 1) / kMostGroups);
