@@ -139,6 +139,15 @@ def test_many_rows(ctx, hd, hq, hk, softcap, t, out):
     go(ctx, [700] * 6 + [1, 3] + [997] * 5, [700] * 6 + [900, 50] + [1000] * 5, hq, hk, hd, t, out, softcap=softcap)
 
 
+@pytest.mark.parametrize("t,out", [(F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("hd,hq,hk", [(96, 2, 1), (128, 14, 2), (128, 4, 4), (256, 2, 1)])
+@pytest.mark.parametrize("window,causal", [(0, True), (300, True), (0, False)])
+def test_long_chunks_alone(ctx, hd, hq, hk, window, causal, t, out):
+    """Many rows of one request: workgroups of 256, their keys in parts."""
+    q = -(-2050 * hk // hq)
+    go(ctx, [q], [q + 1000], hq, hk, hd, t, out, window=window, causal=causal)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3])
 @pytest.mark.parametrize("q_lens", [[1, 2], [40, 100]])
 def test_scales_of_any_sign(ctx, q_lens, scale):
@@ -219,13 +228,13 @@ def test_rows_that_see_nothing_and_requests_of_no_length(ctx):
 
 
 @pytest.mark.parametrize("q_lens,kv", [([1, 1], [40, 77]), ([30, 64], [130, 200]), ([6, 200], [90, 200]),
-                                       ([130] * 260, [130] * 259 + [150])])
+                                       ([130] * 260, [130] * 259 + [150]), ([1100, 1300], [1100, 1400])])
 @pytest.mark.parametrize("poison", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("window", [0, 20])
 def test_tokens_not_seen_do_not_reach_a_row(ctx, q_lens, kv, poison, window):
     """Every slot that no row sees is poisoned, and tokens that some rows see:
     the others' outputs stay as they were, bit for bit."""
-    c = Case(ctx, q_lens, kv, 4, 2, 64, F16, F16, window=window)
+    c = Case(ctx, q_lens, kv, 4, 2, 96 if q_lens[0] > 1000 else 64, F16, F16, window=window)
     try:
         clean = c.run().outputs()
         c.verify()

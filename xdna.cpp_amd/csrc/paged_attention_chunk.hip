@@ -1,7 +1,7 @@
 // Attention over a paged KV cache, chunk form: for requests that add many
 // tokens.
 //
-// A workgroup takes 128 head rows (tokens x query heads of one KV head) of a
+// A workgroup takes 128 or 256 head rows (tokens x query heads of one KV head) of a
 // request and walks the keys that they see in tiles of 64; a wavefront owns 32
 // of the rows.  As in the token form a tile's scores are K q^T, so that a lane
 // holds 32 scores of one row, the softmax needs one exchange, and the weights
@@ -393,14 +393,14 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
 // reads what 16 do here.)
 constexpr int kJoinThreads = 256;
 
-template <int TYPE, int HD>
+template <int TYPE, int HD, int WAVES>
 __global__ __launch_bounds__(kJoinThreads) void attention_chunk_join_kernel(AttnArgs a) {
-    typedef ChunkShape<HD, 4> S;
+    typedef ChunkShape<HD, WAVES> S;
     constexpr int kRows = S::kRows, kQuads = HD / 4;
     const int kvh = static_cast<int>(blockIdx.x % a.n_kv_heads);
     const int rest = static_cast<int>(blockIdx.x / a.n_kv_heads), blocks = static_cast<int>(gridDim.x / a.n_kv_heads);
     ChunkItem it;
-    if (!chunk_item<4>(a, blocks - 1 - rest, kvh, &it)) return;
+    if (!chunk_item<WAVES>(a, blocks - 1 - rest, kvh, &it)) return;
     const int i = threadIdx.x + kJoinThreads * blockIdx.y, r = i / kQuads, c = i % kQuads * 4;
     if (r >= kRows || r >= it.g.rows - it.row0) return;
     Joined j;
@@ -411,48 +411,56 @@ __global__ __launch_bounds__(kJoinThreads) void attention_chunk_join_kernel(Attn
     store_out4<TYPE>(a, out_at(a, it.g, kvh, it.row0 + r, HD) + c, j.value());
 }
 
+// Blocks of 2^shift rows as find_block numbers them: request s begins at
+// floor(offset_s / 2^shift) + s and takes ceil(rows_s / 2^shift) of them, so the
+// last one ends at ceil(rows / 2^shift) + n_seqs - 1 at most.
+int64_t row_blocks(int64_t rows, int shift, int n_seqs) {
+    return ((rows + (int64_t(1) << shift) - 1) >> shift) + n_seqs - 1;
+}
+
 // Threads of a launch.
 constexpr int64_t kMostThreads = UINT32_MAX;
 
-// Workgroups that a call is split into at most, while that is more than its row blocks.
-int chunk_groups(const mi355x_ctx *ctx) { return 2 * ctx->num_cus; }
+// Workgroups that a call is split into at most, while that is more than its row blocks:
+// as many as run at once.
+template <int WAVES>
+int chunk_groups(const mi355x_ctx *ctx) { return 8 / WAVES * ctx->num_cus; }
 
-// Workgroups of 256 rows where there are enough of them for all CUs: they load
-// half as much into LDS per row (prompt of 8192 tokens: 586 us with 128 rows, 556 with
-// 256).  Else 128, and more of them.  Heads of 256 values leave registers for four
-// wavefronts.
+template <int TYPE, int HD, bool CAP, int PLANES, int WAVES>
+int launch_blocks(mi355x_ctx *ctx, AttnArgs a) {
+    const int64_t items = row_blocks(a.n_rows * a.group.d, row_shift(WAVES), a.n_seqs) * a.n_kv_heads;
+    // few blocks: parts of their keys, for the tiles of all CUs (a chunk of 512 tokens on
+    // 4096, 64 blocks: 46 us, 141 unsplit; 53 with half as many again), of no fewer than
+    // four tiles where the table allows that many tokens
+    a.split = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>(chunk_groups<WAVES>(ctx) / items, (int64_t(a.reach) + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
+    if (items * a.split > kMostThreads / (64 * WAVES))
+        return set_error(MI355X_EUNSUPPORTED, "mi355x_paged_attention: more row blocks than a launch takes");
+    attention_chunk_kernel<TYPE, HD, CAP, PLANES, WAVES>
+        <<<static_cast<unsigned>(items * a.split), 64 * WAVES, ChunkShape<HD, WAVES>::kLds, ctx->stream>>>(a);
+    MI355X_HIP(hipGetLastError());
+    if (a.split > 1) {
+        const dim3 grid(static_cast<unsigned>(items), (32 * WAVES * HD / 4 + kJoinThreads - 1) / kJoinThreads);
+        attention_chunk_join_kernel<TYPE, HD, WAVES><<<grid, kJoinThreads, 0, ctx->stream>>>(a);
+        MI355X_HIP(hipGetLastError());
+    }
+    return MI355X_OK;
+}
+
+// Workgroups of 256 rows load half as much into LDS per row, but a request's last
+// one leaves more wavefronts without rows: they are for requests of 2048 rows and
+// more on average (us with 128 -> 256 rows: a prompt of 8192 tokens and 4 heads 586
+// -> 556; one request of 4096 rows 46.2 -> 43.8, 8 of them 81 -> 76; 8 of 2048 70 ->
+// 68; one of 1024 20.7 -> 23.2; 64 of 132 129 -> 153, of 800 407 -> 426).  Heads of 64
+// values leave registers for three workgroups of 128 rows on a CU (4096 tokens
+// and 4 heads 96 us, 101 with 256 rows), heads of 256 none for 256 rows.
 template <int TYPE, int HD, bool CAP, int PLANES>
 int launch_chunk(mi355x_ctx *ctx, const AttnArgs &args) {
     AttnArgs a = args;
     a.by_page = a.shift >= __builtin_ctz(64 / ChunkShape<HD, 4>::kPlaces) && a.token_stride < (1u << 26);
-    a.split = 1;
-    const int64_t rows = a.n_rows * a.group.d;
-    if constexpr (HD <= 128) {
-        const int64_t items = ((rows >> row_shift(8)) + a.n_seqs) * a.n_kv_heads;
-        if ((rows >> row_shift(8)) * a.n_kv_heads >= ctx->num_cus && items <= kMostThreads / 512) {
-            attention_chunk_kernel<TYPE, HD, CAP, PLANES, 8>
-                <<<static_cast<unsigned>(items), 512, ChunkShape<HD, 8>::kLds, ctx->stream>>>(a);
-            MI355X_HIP(hipGetLastError());
-            return MI355X_OK;
-        }
-    }
-    const int64_t items = ((rows >> row_shift(4)) + a.n_seqs) * a.n_kv_heads;
-    // few blocks: parts of their keys, for the tiles of all CUs (a chunk of 512 tokens on
-    // 4096, 66 blocks: 47 us, 141 unsplit), of no fewer than four tiles where the
-    // table allows that many tokens
-    a.split = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>(chunk_groups(ctx) / items, (int64_t(a.reach) + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
-    if (items * a.split > kMostThreads / 256)
-        return set_error(MI355X_EUNSUPPORTED, "mi355x_paged_attention: more row blocks than a launch takes");
-    attention_chunk_kernel<TYPE, HD, CAP, PLANES, 4>
-        <<<static_cast<unsigned>(items * a.split), 256, ChunkShape<HD, 4>::kLds, ctx->stream>>>(a);
-    MI355X_HIP(hipGetLastError());
-    if (a.split > 1) {
-        const dim3 grid(static_cast<unsigned>(items), (128 * HD / 4 + kJoinThreads - 1) / kJoinThreads);
-        attention_chunk_join_kernel<TYPE, HD><<<grid, kJoinThreads, 0, ctx->stream>>>(a);
-        MI355X_HIP(hipGetLastError());
-    }
-    return MI355X_OK;
+    if constexpr (HD == 96 || HD == 128)
+        if (a.n_rows * a.group.d >= 2048 * int64_t(a.n_seqs)) return launch_blocks<TYPE, HD, CAP, PLANES, 8>(ctx, a);
+    return launch_blocks<TYPE, HD, CAP, PLANES, 4>(ctx, a);
 }
 
 template <int TYPE, int HD>
@@ -476,7 +484,7 @@ int launch_type(mi355x_ctx *ctx, const AttnArgs &a, int head_dim) {
 }  // namespace
 
 size_t attention_chunk_workspace(const mi355x_ctx *ctx, int head_dim) {
-    return static_cast<size_t>(chunk_groups(ctx)) * 128 * (head_dim + 2) * 4;
+    return static_cast<size_t>(chunk_groups<4>(ctx)) * 128 * (head_dim + 2) * 4;
 }
 
 int launch_attention_chunk(mi355x_ctx *ctx, const AttnArgs &a, int type, int head_dim) {
