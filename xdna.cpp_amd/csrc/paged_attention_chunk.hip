@@ -65,24 +65,36 @@ __device__ __forceinline__ int v_turn(int r) {
     return PLACES == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
 }
 
-// The request whose blocks of 2^SHIFT rows include block j, and its first one.
+// The request whose blocks of 2^SHIFT rows include block j, its first one, and its
+// rows and tokens.  Up to 64 requests: a lane has loaded what belongs to each, so
+// that no load waits for the search.
 template <int SHIFT>
-__device__ __forceinline__ int find_block(const AttnArgs &a, int64_t j, int64_t *first) {
-    auto begin = [&](int s) {  // ascends by at least 1: one block more at every seam
-        return ((static_cast<int64_t>(a.row_offsets[s]) * a.group.d) >> SHIFT) + s;
-    };
+__device__ __forceinline__ int find_block(const AttnArgs &a, int64_t j, int64_t *first, SeqGeo *g) {
+    // ascends by at least 1: one block more at every seam
+    auto begin = [&](int32_t offset, int s) { return ((static_cast<int64_t>(offset) * a.group.d) >> SHIFT) + s; };
     const int lane = threadIdx.x & 63;
+    if (a.n_seqs <= 64) {
+        const int s = min(lane, a.n_seqs - 1);
+        const int32_t from = a.row_offsets[s], to = a.row_offsets[s + 1], kv = a.kv_lens[s];
+        const uint64_t below = __ballot(lane < a.n_seqs && begin(from, s) <= j);
+        const int found = 63 - __builtin_clzll(below | 1);
+        const int32_t offset = __builtin_amdgcn_readlane(from, found);
+        *first = begin(offset, found);
+        *g = seq_geo(a, offset, __builtin_amdgcn_readlane(to, found), __builtin_amdgcn_readlane(kv, found));
+        return found;
+    }
     int lo = 0, n = a.n_seqs;  // the request is in lo .. lo + n - 1
     while (n > 1) {
         const int step = (n + 63) / 64;
         const int s = lo + lane * step;
-        const uint64_t below = __ballot(lane * step < n && begin(s) <= j);
+        const uint64_t below = __ballot(lane * step < n && begin(a.row_offsets[s], s) <= j);
         const int k = max(0, 63 - __builtin_clzll(below | 1));
         n = min(step, n - k * step);
         lo += k * step;
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
-    *first = begin(lo);
+    *g = seq_geo(a, lo);
+    *first = begin(a.row_offsets[lo], lo);
     return lo;
 }
 
@@ -102,9 +114,8 @@ __device__ __forceinline__ bool chunk_item(const AttnArgs &a, int64_t j, int kvh
     int64_t begin;
     constexpr int kRows = 32 * WAVES;
     static_assert(kRows == 1 << row_shift(WAVES), "blocks of rows");
-    it->seq = find_block<row_shift(WAVES)>(a, j, &begin);
+    it->seq = find_block<row_shift(WAVES)>(a, j, &begin, &it->g);
     it->kvh = kvh;
-    it->g = seq_geo(a, it->seq);
     const int64_t row0 = (j - begin) * kRows;
     if (row0 < 0 || row0 >= it->g.rows || it->g.rows <= a.row_limit) return false;
     it->row0 = static_cast<int>(row0);
