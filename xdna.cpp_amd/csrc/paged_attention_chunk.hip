@@ -433,9 +433,10 @@ int64_t row_blocks(int64_t rows, int shift, int n_seqs) {
 constexpr int64_t kMostThreads = UINT32_MAX;
 
 // Workgroups that a call is split into at most, while that is more than its row blocks:
-// as many as run at once.
-template <int WAVES>
-int chunk_groups(const mi355x_ctx *ctx) { return 8 / WAVES * ctx->num_cus; }
+// as many as run at once (heads of 256: one on a CU; 512 tokens on 4096 73 us, 87
+// with twice as many).
+template <int HD, int WAVES>
+int chunk_groups(const mi355x_ctx *ctx) { return (HD > 128 ? 1 : 8 / WAVES) * ctx->num_cus; }
 
 template <int TYPE, int HD, bool CAP, int PLANES, int WAVES>
 int launch_blocks(mi355x_ctx *ctx, AttnArgs a) {
@@ -444,7 +445,7 @@ int launch_blocks(mi355x_ctx *ctx, AttnArgs a) {
     // 4096, 64 blocks: 46 us, 141 unsplit; 53 with half as many again), of no fewer than
     // four tiles where the table allows that many tokens
     a.split = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>(chunk_groups<WAVES>(ctx) / items, (int64_t(a.reach) + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
+        1, std::min<int64_t>(chunk_groups<HD, WAVES>(ctx) / items, (int64_t(a.reach) + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
     if (items * a.split > kMostThreads / (64 * WAVES))
         return set_error(MI355X_EUNSUPPORTED, "mi355x_paged_attention: more row blocks than a launch takes");
     attention_chunk_kernel<TYPE, HD, CAP, PLANES, WAVES>
@@ -495,7 +496,9 @@ int launch_type(mi355x_ctx *ctx, const AttnArgs &a, int head_dim) {
 }  // namespace
 
 size_t attention_chunk_workspace(const mi355x_ctx *ctx, int head_dim) {
-    return static_cast<size_t>(chunk_groups<4>(ctx)) * 128 * (head_dim + 2) * 4;
+    // the same floats for workgroups of 128 and of 256 rows
+    const int groups = head_dim > 128 ? chunk_groups<256, 4>(ctx) : chunk_groups<128, 4>(ctx);
+    return static_cast<size_t>(groups) * 128 * (head_dim + 2) * 4;
 }
 
 int launch_attention_chunk(mi355x_ctx *ctx, const AttnArgs &a, int type, int head_dim) {
