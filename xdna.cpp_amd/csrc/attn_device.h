@@ -26,6 +26,7 @@ struct AttnArgs {
     int row_limit;      // requests of at most (token form) or more than (chunk form) so many head rows
     float scale2;            // scale log2 e: scores are in factors of 2
     float cap_in, cap_out;   // 2 scale log2 e / softcap (finite) and softcap log2 e; 0: no cap
+    float line_share;  // token form: 1 / (12 teams of a join x requests x KV heads)
     FastDiv group;  // query heads of a KV head
     int n_seqs, n_kv_heads;
     int n_pages, shift, window, causal, f32_out;

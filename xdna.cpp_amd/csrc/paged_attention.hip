@@ -141,6 +141,21 @@ struct Scan {
     }
 };
 
+// How the units are shared out.  A stretch of u units takes about u steps, and the
+// join of N / u parts, eight of which each of its teams loads at a time, N / (8 u
+// teams) and more: u = sqrt(N / (12 teams)) of the average N, where there are
+// workgroups to spare (16 heads of 128, 2 KV heads: one request of 16000 tokens 21
+// us, 26 with a unit each; of 64000 31, 54; 4 of 5000 14.9, 18.0).
+__device__ __forceinline__ Stretches token_line(const AttnArgs &a, int64_t total) {
+    const float wanted = sqrtf(static_cast<float>(total) * a.line_share) + 0.5f;
+    int64_t groups = gridDim.x;
+    if (wanted >= 2.0f) {
+        const int64_t u = static_cast<int64_t>(wanted);
+        groups = idx_min(groups, quotient(total + u - 1, u));
+    }
+    return stretches(total, static_cast<int>(groups));
+}
+
 template <int HD>
 struct TokenShape {
     static constexpr int kVStride = HD + 16;  // values: rows of V start 8 banks apart
@@ -169,7 +184,8 @@ __global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) vo
     const int col = lane & 15, quad = lane >> 4;
     Scan<kTokenWaves> scan;
     scan.run(a, tmp);
-    const Stretches line = stretches(scan.total, gridDim.x);
+    const Stretches line = token_line(a, scan.total);
+    if (static_cast<int>(blockIdx.x) >= line.groups) return;
     const int64_t u0 = stretch_begin(line, blockIdx.x), u1 = stretch_begin(line, blockIdx.x + 1);
     if (u0 >= u1) return;
     int64_t before;  // units before request seq
@@ -512,6 +528,9 @@ int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &u
     a.causal = u.causal;
     a.row_limit = INT32_MAX;
     const int64_t added = u.max_added > 0 ? std::min<int64_t>(u.max_added, u.n_rows) : u.n_rows;
+    const int join_threads = static_cast<int>(std::min<int64_t>(kTokenRows, added * group)) * (u.pool->head_dim / 4);
+    a.line_share = 1.0f / (12.0f * static_cast<float>(std::max(1, kTokenThreads / join_threads)) *
+                           static_cast<float>(u.n_seqs) * static_cast<float>(u.pool->n_kv_heads));
     a.f32_out = u.out_type == MI355X_TYPE_F32;
     return u.pool->type == MI355X_TYPE_F16
                ? launch_sizes<MI355X_TYPE_F16>(ctx, a, u.pool->head_dim, added * group)
