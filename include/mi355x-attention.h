@@ -159,7 +159,7 @@ MI355X_API int mi355x_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_ar
  * table's last column or of a negative length count as not seen.  Rows of out
  * behind row_offsets[n_seqs], and rows that offsets past n_rows name, are not
  * written.  row_offsets ascend from 0.
- * head_dim 64, 96, 128 or 256 (others: MI355X_EUNSUPPORTED, and so are 2^24
+ * head_dim 64, 96, 128 or 256 (others: MI355X_EUNSUPPORTED, and so are 2^23
  * blocks of rows: (n_rows * group / 128 + n_seqs) * n_kv_heads); q, out: 16-byte
  * aligned rows (q_stride a multiple of 8, out_stride of 8), head h at
  * h * head_dim; out may not overlap an input.  max_added is the host's bound on

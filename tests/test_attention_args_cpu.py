@@ -143,6 +143,15 @@ def test_head_sizes_that_are_not_computed(host, hd):
     assert host.lib.mi355x_paged_attention_workspace(host.h, 4, 2, 64, ctypes.byref(n)) == EHIP
 
 
+@pytest.mark.parametrize("rows,seqs,heads,kv,code", [
+    (65536, 65536, 128, 128, EUNSUPPORTED), (65536, 65536, 127, 127, EHIP), (2 ** 30 - 128, 1, 2, 1, EUNSUPPORTED),
+    (2 ** 30 - 256, 1, 1, 1, EHIP), (2 ** 26, 1, 16, 16, EUNSUPPORTED)])
+def test_as_many_blocks_as_a_launch_takes(host, rows, seqs, heads, kv, code):
+    p = pool(n_kv_heads=kv, token_stride=64 * kv, page_stride=1024 * kv)
+    a = attn(p, n_rows=rows, n_seqs=seqs, n_heads=heads, q_stride=64 * heads, out_stride=64 * heads)
+    assert rc(host, "mi355x_paged_attention", a) == code
+
+
 def test_attention_of_no_rows_is_done(host):
     assert rc(host, "mi355x_paged_attention", attn(n_rows=0, q=None, out=None)) == OK
     assert rc(host, "mi355x_paged_attention", attn(n_seqs=0, row_offsets=None)) == OK

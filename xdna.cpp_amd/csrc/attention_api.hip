@@ -214,6 +214,11 @@ int mi355x_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args *a
         return invalid(who, "out_type must be the pool's type or F32 (got " + std::to_string(a.out_type) + ")");
     if (a.n_rows * (a.n_heads / a.pool->n_kv_heads) > INT32_MAX)
         return invalid(who, "n_rows times the query heads of a KV head must be below 2^31");
+    // a launch's threads are counted in 32 bits
+    const int64_t blocks = (a.n_rows * (a.n_heads / a.pool->n_kv_heads) / 128 + a.n_seqs) * a.pool->n_kv_heads;
+    if (blocks >= (1 << 23))
+        return set_error(MI355X_EUNSUPPORTED, std::string(who) + ": " + std::to_string(blocks) +
+                                                  " blocks of rows, 2^23 or more");
     const int64_t width = static_cast<int64_t>(a.n_heads) * a.pool->head_dim;
     if (int rc = check_row_stride(who, "q_stride", a.n_rows, a.q_stride, width)) return rc;
     if (int rc = check_row_stride(who, "out_stride", a.n_rows, a.out_stride, width)) return rc;

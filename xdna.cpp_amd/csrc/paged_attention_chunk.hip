@@ -429,9 +429,6 @@ int64_t row_blocks(int64_t rows, int shift, int n_seqs) {
     return ((rows + (int64_t(1) << shift) - 1) >> shift) + n_seqs - 1;
 }
 
-// Threads of a launch.
-constexpr int64_t kMostThreads = UINT32_MAX;
-
 // Workgroups that a call is split into at most, while that is more than its row blocks:
 // as many as run at once (heads of 256: one on a CU; 512 tokens on 4096 73 us, 87
 // with twice as many).
@@ -446,8 +443,6 @@ int launch_blocks(mi355x_ctx *ctx, AttnArgs a) {
     // four tiles where the table allows that many tokens
     a.split = static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>(chunk_groups<HD, WAVES>(ctx) / items, (int64_t(a.reach) + 4 * kChunkKeys - 1) / (4 * kChunkKeys))));
-    if (items * a.split > kMostThreads / (64 * WAVES))
-        return set_error(MI355X_EUNSUPPORTED, "mi355x_paged_attention: more row blocks than a launch takes");
     attention_chunk_kernel<TYPE, HD, CAP, PLANES, WAVES>
         <<<static_cast<unsigned>(items * a.split), 64 * WAVES, ChunkShape<HD, WAVES>::kLds, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
