@@ -159,6 +159,8 @@ __device__ __forceinline__ float quad_sum(float v) {
 
 // A row's maximum may grow by this (in factors of 2) before its sums are
 // scaled: weights stay below 2^8, where 16-bit floats are as exact as below 1.
+// Each row takes a new maximum by its own scores alone, also where another row of its
+// wavefront asks for one: tokens that it does not see leave its roundings as they are.
 constexpr float kSlack = 8.0f;
 
 __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.0f : m; }

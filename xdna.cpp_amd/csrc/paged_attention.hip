@@ -321,8 +321,9 @@ __global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) vo
 #pragma unroll
                 for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
                 top = quad_max(top);
-                if (__any(top > m + kSlack || (m == -INFINITY && top > m))) {
-                    const float m_new = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
+                const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
+                if (__any(grows)) {
+                    const float m_new = grows ? top : m, keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
                     l *= keep;
 #pragma unroll
                     for (int d = 0; d < kBlocks; ++d) o[d] *= keep;

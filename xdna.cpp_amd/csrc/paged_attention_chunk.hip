@@ -324,7 +324,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
             top = fmaf(top, c1, c0);
             const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
             if (__any(grows)) {
-                const float m_new = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
+                const float m_new = grows ? top : m, keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
                 l *= keep;
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) o[d] *= keep;
