@@ -150,8 +150,10 @@ MI355X_API int mi355x_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_ar
  * Scores, weights and sums are f32, products of 16-bit values on the matrix
  * cores.  The weights meet v as 16-bit values of the pool's type (half a step,
  * 2^-8 or 2^-11 of a weight: as much as the rounding of a 16-bit output), or
- * as two such planes where the output is f32 or a request's rows are few (no
- * more than 2^-16 of a weight then).
+ * as two such planes where the output is f32 or the form for few rows runs (no
+ * more than 2^-16 of a weight then).  F16 has steps of 2^-24 besides: weights are
+ * off by up to 2^-24 of the largest one among the 32 or 64 tokens that they are
+ * taken with, and by more below 2^-40 of the row's largest.
  * A row that sees nothing gives zeros.  Tokens that a row does not see do not
  * reach its output, whatever their bits are (NaN and infinities too), and
  * columns of the table that no row of the request sees are not read.  Tokens on

@@ -246,7 +246,8 @@ __global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) vo
             }
             bool odd_lane = false;
             f32x4 o[kBlocks];
-            float m = -INFINITY, l = 0.0f;
+            Reference<TYPE> ref;
+            float l = 0.0f;
 #pragma unroll
             for (int d = 0; d < kBlocks; ++d) o[d] = f32x4{0, 0, 0, 0};
 
@@ -321,19 +322,18 @@ __global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) vo
 #pragma unroll
                 for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
                 top = quad_max(top);
-                const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
-                if (__any(grows)) {
-                    const float m_new = grows ? top : m, keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
+                const bool moves = ref.moves(top);
+                const float keep = ref.move(moves, top);
+                if (__any(moves)) {
                     l *= keep;
 #pragma unroll
                     for (int d = 0; d < kBlocks; ++d) o[d] *= keep;
-                    m = m_new;
                 }
-                const float ref = finite_base(m);
+                const float zero = ref.base();
                 V8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(s[i] - ref);
+                    const float p = __builtin_amdgcn_exp2f(s[i] - zero);
                     l += p;
                     const T h = static_cast<T>(p);
                     hi[i] = h;
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) vo
             const int part = (2 * blockIdx.x + (u != u0)) * S::kPartFloats;
             const float sum = quad_sum(l);
             if (quad == 0) {
-                lds_m[wave][col] = m;
+                lds_m[wave][col] = ref.m;
                 lds_l[wave][col] = sum;
             }
             if (only < 0) {

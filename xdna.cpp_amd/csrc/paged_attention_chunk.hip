@@ -215,7 +215,8 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
         for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-        float m = -INFINITY, l = 0.0f;
+        Reference<TYPE> ref;
+        float l = 0.0f;
         const int col_lo = some_lo >> a.shift, col_hi = (some_hi - 1) >> a.shift;
         // the table entry of key `lane` of tile t, if some row sees a token on its page
         auto entry = [&](int t) {
@@ -322,15 +323,14 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
             for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
             top = half_max(top);
             top = fmaf(top, c1, c0);
-            const bool grows = top > m + kSlack || (m == -INFINITY && top > m);
-            if (__any(grows)) {
-                const float m_new = grows ? top : m, keep = __builtin_amdgcn_exp2f(m - finite_base(m_new));
+            const bool moves = ref.moves(top);
+            if (__any(moves)) {
+                const float keep = ref.move(moves, top);
                 l *= keep;
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) o[d] *= keep;
-                m = m_new;
             }
-            const float base2 = c0 - finite_base(m);
+            const float base2 = c0 - ref.base();
             auto v_chunk = [&](int j, int d) {  // keys 16 j + {4 half .. + 3, 8 + 4 half .. + 3} of 32 values
                 const int place = (4 * d) ^ v_low;
                 const s16x4 *p = reinterpret_cast<const s16x4 *>(vt + v_at + 16 * j * S::kRowBytes + 16 * place);
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
                         *reinterpret_cast<f32x4 *>(w + r * HD + 32 * d + 8 * i + 4 * half) =
                             f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
                 if (half == 0) {
-                    w[kRows * HD + r] = m;
+                    w[kRows * HD + r] = ref.m;
                     w[kRows * (HD + 1) + r] = l;
                 }
             }
