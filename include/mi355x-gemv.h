@@ -84,7 +84,9 @@ MI355X_API const char *mi355x_last_error(void);
  * [injected]".  One fault at a time, process-wide, disarmed once it fired;
  * entry NULL disarms.  The name "mi355x_ctx_workspace" (not reached by "*")
  * instead makes mi355x_ctx_create find no room for the workspace of batched
- * calls, which is no error.  The environment variable
+ * calls, which is no error, and "mi355x_kv_plan_pages" makes a mi355x_kv_plan
+ * (mi355x-attention.h) refuse its step for want of pages, in its status.  The
+ * environment variable
  * MI355X_INJECT_FAULT="<entry>:<hip_error>[:<skip>]" arms one at first use
  * of the library. */
 MI355X_API int mi355x_inject_fault(const char *entry, int hip_error, int skip);

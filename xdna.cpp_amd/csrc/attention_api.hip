@@ -101,6 +101,11 @@ int mi355x_kv_plan(mi355x_ctx *ctx, const mi355x_kv_plan_args *args) {
     if (int rc = device_gate(ctx, who)) return rc;
     DeviceGuard dg(ctx->device);
     if (int rc = ov_join(ctx)) return rc;
+    if (take_fault("mi355x_kv_plan_pages")) {
+        mi355x_kv_plan_args none = a;
+        none.n_free = -1;  // no head lies in 0 .. -1: refused, whatever the step needs
+        return launch_kv_plan(ctx, none);
+    }
     return launch_kv_plan(ctx, a);
 }
 

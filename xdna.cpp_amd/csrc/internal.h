@@ -85,6 +85,9 @@ void clear_error();
 // a host-only context (device MI355X_DEVICE_HOST_ONLY), hipErrorNoDevice.
 // Nothing here touches the device.
 int device_gate(const mi355x_ctx *ctx, const char *entry);
+// Whether a fault is armed under exactly this name ("*" means entry points);
+// disarms it.
+bool take_fault(const char *name);
 inline bool host_only(const mi355x_ctx *ctx) { return ctx && ctx->device < 0; }
 
 #define MI355X_HIP(call)                                \

@@ -195,8 +195,8 @@ void read_fault_env() {
     arm_fault(spec.substr(0, c1).c_str(), error, skip);
 }
 
-// Whether a fault is armed under exactly this name ("*" means entry points);
-// disarms it.
+}  // namespace
+
 bool take_fault(const char *name) {
     std::call_once(g_fault_env_once, read_fault_env);
     if (!g_fault.armed.load(std::memory_order_relaxed)) return false;
@@ -209,8 +209,6 @@ bool take_fault(const char *name) {
     g_fault.armed.store(false);
     return true;
 }
-
-}  // namespace
 
 int device_gate(const mi355x_ctx *ctx, const char *entry) {
     std::call_once(g_fault_env_once, read_fault_env);

@@ -746,6 +746,9 @@ struct GpuDecode {
     size_t workspace_bytes = 0, y_floats = 0;
     float *hx = nullptr, *hy = nullptr;  // page-locked
     int32_t *h_added = nullptr;
+    volatile int32_t *h_status = nullptr;  // of the pass's plan, which writes it there
+    int32_t *status = nullptr;             // its device address
+    std::string refused;                   // the error of a plan that does not fit
     int n_pages = 0;
     int64_t launches = 0;
     double t_gpu = 0.0;
@@ -777,13 +780,12 @@ struct GpuDecode {
     }
 
     // integers on the device: added, lengths (in place), the free list's head,
-    // the two row offsets, the status, positions, the free list, the block table
+    // the two row offsets, positions, the free list, the block table
     int32_t *added() { return ints; }
     int32_t *kv_len() { return ints + 1; }
     int32_t *head() { return ints + 2; }
     int32_t *offsets() { return ints + 3; }
-    int32_t *status() { return ints + 5; }
-    int32_t *positions() { return ints + 6; }
+    int32_t *positions() { return ints + 5; }
     int32_t *free_pages() { return positions() + rows; }
     int32_t *table() { return free_pages() + n_pages; }
 
@@ -798,12 +800,16 @@ struct GpuDecode {
             !alloc(&qkv, 4 * R * (QD + 2 * KVD)) || !alloc(&att, 4 * R * QD) || !alloc(&q, 2 * R * QD) ||
             !alloc(&bias, 4 * static_cast<size_t>(L) * (QD + 2 * KVD)) || !alloc(&inv_freq, 2 * static_cast<size_t>(hd)) ||
             !alloc(&pages, 4 * pool * static_cast<size_t>(L)) ||
-            !alloc(&ints, 4 * (6 + R + 2 * static_cast<size_t>(n_pages))) || !alloc(&slots, 8 * R) ||
+            !alloc(&ints, 4 * (5 + R + 2 * static_cast<size_t>(n_pages))) || !alloc(&slots, 8 * R) ||
             !alloc(&workspace, workspace_bytes) || !alloc_host(&hx, 4 * R * std::max(F, std::max(H, QD))) ||
-            !alloc_host(&hy, 4 * y_floats) || !alloc_host(&h_added, 4))
+            !alloc_host(&hy, 4 * y_floats) || !alloc_host(&h_added, 8))
             return -1;
-        std::vector<int32_t> start(6 + R + 2 * static_cast<size_t>(n_pages), 0);
-        for (int p = 0; p < n_pages; ++p) start[6 + R + static_cast<size_t>(p)] = p;
+        h_status = h_added + 1;
+        void *dev = nullptr;
+        if (mi355x_host_device_ptr(h_added, &dev) != MI355X_OK) return -1;
+        status = static_cast<int32_t *>(dev) + 1;
+        std::vector<int32_t> start(5 + R + 2 * static_cast<size_t>(n_pages), 0);
+        for (int p = 0; p < n_pages; ++p) start[5 + R + static_cast<size_t>(p)] = p;
         std::vector<float> b, f(static_cast<size_t>(hd / 2));
         for (int l = 0; l < L; ++l) {
             b.insert(b.end(), m->bq[l].begin(), m->bq[l].end());
@@ -843,6 +849,7 @@ struct GpuDecode {
     // one more pass of n tokens: their places in the pages
     int plan(int n) {
         *h_added = n;
+        *h_status = -1;
         mi355x_kv_plan_args a{};
         a.n_seqs = 1;
         a.page_tokens = QD_PAGE_TOKENS;
@@ -860,7 +867,7 @@ struct GpuDecode {
         a.row_offsets = offsets();
         a.positions = positions();
         a.slots = slots;
-        a.status = status();
+        a.status = status;
         if (mi355x_memcpy_h2d_async(ctx, added(), h_added, 4) != MI355X_OK) return -1;
         return mi355x_kv_plan(ctx, &a);
     }
@@ -950,6 +957,10 @@ struct GpuDecode {
                 product(7 * l + QD_K, x, qkv + QD, width, n) || product(7 * l + QD_V, x, qkv + QD + KVD, width, n) ||
                 attention(l, n) || product(7 * l + QD_O, att, y, H, n) || download(static_cast<int64_t>(n) * H))
                 return -1;
+            if (l == 0 && *h_status != 0) {  // written before what was waited for
+                refused = "no place for the pass's tokens (the plan's status " + std::to_string(*h_status) + ")";
+                return -1;
+            }
             t_gpu += now() - t0;
             residual();
             normed(m->ffn_norm[l]);
@@ -985,7 +996,7 @@ struct GpuDecode {
 int generate_gpu_attention(qd_model *m, const int32_t *prompt, int n_prompt, int n_gen, int32_t *out_tokens,
                            double *timings) {
     GpuDecode d(m, n_prompt + std::max(n_gen, 1), std::min(n_prompt, QD_CHUNK_ROWS));
-    auto failed = [&] { return fail(std::string("qd_generate: ") + mi355x_last_error()); };
+    auto failed = [&] { return fail("qd_generate: " + (d.refused.empty() ? mi355x_last_error() : d.refused)); };
     if (d.init()) return failed();
     std::vector<float> logits(static_cast<size_t>(m->c.vocab));
     const double t_start = now();
