@@ -936,7 +936,7 @@ struct GpuDecode {
     // The pass of n tokens; with logits, those behind the last one.
     int pass(const int32_t *tokens, int n, float *logits) {
         const int64_t width = QD + 2 * KVD;
-        std::vector<float> h(static_cast<size_t>(n) * H), out(static_cast<size_t>(H));
+        std::vector<float> h(static_cast<size_t>(n) * H);
         for (int i = 0; i < n; ++i)
             dequant_q4_0_row(m->mats[7 * L].q.data() + static_cast<int64_t>(tokens[i]) * (H / 32) * 18, H,
                              h.data() + static_cast<size_t>(i) * H);
