@@ -152,14 +152,15 @@ MI355X_API int mi355x_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_ar
  * 2^-8 or 2^-11 of a weight: as much as the rounding of a 16-bit output), or
  * as two such planes (no more than 2^-16 of a weight then) where the output is f32
  * or the request takes the form for few rows: at most 16 of them times query heads
- * of a KV head, by max_added or, in a call of several requests, its own.  F16 has steps of 2^-24 besides: weights are
- * off by up to 2^-24 of the largest one among the 32 or 64 tokens that they are
+ * of a KV head, by max_added or, in a call of several requests, its own.  That form
+ * with an f32 output has them to 2^-22.  F16 has steps of 2^-24 besides: weights
+ * are off by up to 2^-24 of the largest one among the 32 or 64 tokens that they are
  * taken with, and by more below 2^-40 of the row's largest.
  * A row that sees nothing gives zeros.  Tokens that a row does not see do not
  * reach its output, whatever their bits are (NaN and infinities too), and
  * columns of the table that no row of the request sees are not read.  An infinite
- * value of v that a row sees makes that value of its output infinite or NaN (with two
- * planes NaN also where every such value has one sign), and no other.  Tokens on
+ * value of v that a row sees makes that value of its output infinite or NaN (with more
+ * than one plane NaN also where all such have one sign), and no other.  Tokens on
  * a page outside the pool (a table entry not in 0 .. n_pages - 1), behind the
  * table's last column or of a negative length count as not seen.  Rows of out
  * behind row_offsets[n_seqs], and rows that offsets past n_rows name, are not
@@ -168,8 +169,8 @@ MI355X_API int mi355x_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_ar
  * blocks of rows: (n_rows * group / 128 + n_seqs) * n_kv_heads); q, out: 16-byte
  * aligned rows (q_stride a multiple of 8, out_stride of 8), head h at
  * h * head_dim; out may not overlap an input.  max_added is the host's bound on
- * a request's new tokens (0: unknown); it picks the form, and with it one plane or
- * two for a 16-bit output, and never which rows are computed.
+ * a request's new tokens (0: unknown); it picks the form, and with it the number of
+ * planes, and never which rows are computed.
  *
  * workspace: mi355x_paged_attention_workspace bytes for parts of long rows,
  * 16-byte aligned.  Zero it once, before its first call (mi355x_fill): it

@@ -11,12 +11,11 @@
 // key read once meets all of them: scores as K q^T, one column per row of q, so
 // that a lane holds 8 scores of one row of a 32-key tile and the softmax needs
 // two exchanges; the weights are then, as they lie, the operand of V^T w, whose
-// V^T comes out of LDS through the transposing read.  Weights go in as two
-// 16-bit planes: the matrix cores idle here, and the second plane makes them as
-// good as f32.  64 requests of up to 8192 tokens, 32 query and 8 KV heads of 128:
-// 1.0 GB in 190 us, 5.2 TB/s, as fast as a copy; one of 131072 tokens 113 us, 4.8
-// TB/s.  Short calls are bound by latency: lengths, table, keys, parts and their
-// join each wait for the one before (640 tokens, 2 KV heads: 9.7 us).
+// V^T comes out of LDS through the transposing read.  64 requests of up to 8192
+// tokens, 32 query and 8 KV heads of 128: 1.0 GB in 190-197 us, 5.1-5.3 TB/s, as fast as
+// a copy; one of 131072 tokens 113 us, 4.8 TB/s.  Short calls are bound by latency:
+// lengths, table, keys, parts and their join each wait for the one before (640
+// tokens, 2 KV heads: 9.6 us).
 //
 // Work split.  All requests' keys, heads and row blocks form one line of
 // 128-key units; every workgroup takes an equal stretch of it, whatever the
@@ -166,7 +165,7 @@ struct TokenShape {
     static constexpr int kPartFloats = kTokenRows * (HD + 2);
 };
 
-template <int TYPE, int HD>
+template <int TYPE, int HD, int PLANES>
 __global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) void attention_token_kernel(AttnArgs a) {
     typedef Num<TYPE> N;
     typedef typename N::T T;
@@ -330,14 +329,12 @@ __global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) vo
                     for (int d = 0; d < kBlocks; ++d) o[d] *= keep;
                 }
                 const float zero = ref.base();
-                V8 hi, lo;
+                V8 w[PLANES];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float p = __builtin_amdgcn_exp2f(s[i] - zero);
                     l += p;
-                    const T h = static_cast<T>(p);
-                    hi[i] = h;
-                    lo[i] = static_cast<T>(p - static_cast<float>(h));
+                    split_weight<TYPE, PLANES>(p, w, i);
                 }
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) {
@@ -345,8 +342,8 @@ __global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) vo
                     const u32x2_a x = lds_read_transposed(reinterpret_cast<const s16x4 *>(p)),
                                   y = lds_read_transposed(reinterpret_cast<const s16x4 *>(p + 16 * S::kVStride));
                     const V8 v = __builtin_bit_cast(V8, u32x4_a{x[0], x[1], y[0], y[1]});
-                    o[d] = N::mfma16(v, hi, o[d]);
-                    o[d] = N::mfma16(v, lo, o[d]);
+#pragma unroll
+                    for (int i = 0; i < PLANES; ++i) o[d] = N::mfma16(v, w[i], o[d]);
                 }
             }
 
@@ -440,17 +437,24 @@ __global__ __launch_bounds__(kTokenThreads, HD <= 64 ? 3 : HD <= 128 ? 2 : 1) vo
 // The token form runs as many workgroups as stay on the chip together.
 constexpr int kTokenGroupsPerCu = 4;
 
-template <int TYPE, int HD>
-int launch_token(mi355x_ctx *ctx, const AttnArgs &a) {
-    const void *kernel = reinterpret_cast<const void *>(attention_token_kernel<TYPE, HD>);
+template <int TYPE, int HD, int PLANES>
+int launch_planes(mi355x_ctx *ctx, const AttnArgs &a) {
+    const void *kernel = reinterpret_cast<const void *>(attention_token_kernel<TYPE, HD, PLANES>);
     const int64_t fit = ctx->num_cus * std::max(1, std::min(kTokenGroupsPerCu, occupancy(kernel, kTokenThreads, 0)));
     // no more than the units that the table allows
     const int64_t heads = static_cast<int64_t>(a.n_seqs) * a.n_kv_heads;
     const int64_t units = heads * (a.reach / kUnitKeys + 1);
-    attention_token_kernel<TYPE, HD>
+    attention_token_kernel<TYPE, HD, PLANES>
         <<<static_cast<unsigned>(std::min(fit, units)), kTokenThreads, 0, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
     return MI355X_OK;
+}
+
+template <int TYPE, int HD>
+int launch_token(mi355x_ctx *ctx, const AttnArgs &a) {
+    if constexpr (TYPE == MI355X_TYPE_BF16)
+        if (a.f32_out) return launch_planes<TYPE, HD, 3>(ctx, a);
+    return launch_planes<TYPE, HD, 2>(ctx, a);
 }
 
 // rows: the host's bound on a request's head rows.  Up to kTokenRows the token

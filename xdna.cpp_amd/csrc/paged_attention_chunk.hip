@@ -351,21 +351,18 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
 #pragma unroll
                     for (int d = 0; d < kBlocks; ++d) v[(j + 1) & 1][d] = v_chunk(j + 1, d);
                 __builtin_amdgcn_sched_barrier(0);
-                V8 hi, lo;
+                V8 w[PLANES];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float y = s[8 * j + i], p = __builtin_amdgcn_exp2f(fmaf(y, c1, base2));
                     l += p;
-                    const T h = static_cast<T>(p);
-                    hi[i] = h;
-                    if (PLANES == 2) lo[i] = static_cast<T>(p - static_cast<float>(h));
+                    split_weight<TYPE, PLANES>(p, w, i);
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    o[d] = N::mfma32(v[j & 1][d], hi, o[d]);
-                    if (PLANES == 2) o[d] = N::mfma32(v[j & 1][d], lo, o[d]);
-                }
+                for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                    for (int i = 0; i < PLANES; ++i) o[d] = N::mfma32(v[j & 1][d], w[i], o[d]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
