@@ -459,10 +459,12 @@ int launch_token(mi355x_ctx *ctx, const AttnArgs &a) {
 
 // rows: the host's bound on a request's head rows.  Up to kTokenRows the token
 // form; else the chunk form, behind the token form for the requests that add
-// few (one request alone takes the chunk form at once).  With 17 to 64 rows the
-// chunk form is the faster one too: 16 requests of 5 tokens and 8 heads 28.9 us
-// against 39.3 for a token form of three row blocks, one of 4 tokens on 30000 36
-// against 211; 16 of 8 tokens and 4 heads 77 against 68.
+// few (one request alone takes the chunk form at once).  With more rows the token form
+// reads the keys again for every kTokenRows of them; the chunk form is as fast or
+// faster from 17 on (us, chunk form against token form; contexts of 500 to 6000
+// tokens): 16 requests of 5 tokens and 8 heads 29.7, 38.0; of 5 and 4 71.6, 85.4; of 8
+// and 4 71.7, 87.1; of 17 and 1 70.9, 85.5; of 1 and 32 21.9, 21.8; 64 of 3 tokens and 8
+// heads 71.8, 84.7, of 16 and 4 214, 672; one of 4 and 8 on 30000 tokens 32.8, 33.2.
 template <int TYPE, int HD>
 int launch_forms(mi355x_ctx *ctx, const AttnArgs &a, int64_t rows) {
     if (rows <= kTokenRows) return launch_token<TYPE, HD>(ctx, a);

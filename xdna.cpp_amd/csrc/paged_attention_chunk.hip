@@ -5,13 +5,13 @@
 // request and walks the keys that they see in tiles of 64; a wavefront owns 32
 // of the rows.  As in the token form a tile's scores are K q^T, so that a lane
 // holds 32 scores of one row, the softmax needs one exchange, and the weights
-// are, as they lie, the operand of V^T w; O^T stays in registers.  The matrix
-// cores bound it: a prompt of 8192 tokens, 32 query and 8 KV heads of 128, is 0.55
-// Tflop at 548 us, 1.00 Pflop/s, where a product of two 8192 x 8192 matrices
-// reaches 1.22 on the card.  Without its exponentials it takes 500 us, without
-// its loads 493, with a quarter of the second product 426: nothing but the matrix
-// cores weighs much, and neither priorities nor products between the
-// exponentials move it.
+// are, as they lie, the operand of V^T w; O^T stays in registers.  Matrix cores and
+// vector units bound it, one after the other: a prompt of 8192 tokens, 32 query and 8 KV
+// heads of 128, is 0.55 Tflop at 540-608 us, 0.9-1.0 Pflop/s, with the matrix cores
+// busy in 43% of the cycles and vector instructions in 47%, where products of 8192 x
+// 8192 matrices reach 1.39 on the card with 69% and 10%.  Without its exponentials
+// it takes 40 us less, without its loads 48, with a quarter of the second product 115;
+// neither priorities nor products between the exponentials move it.
 //
 // K and V tiles travel to LDS directly (global_load_lds), one tile ahead.  Such
 // loads fill LDS in lane order, so rows cannot be padded; instead the 16-byte
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(64 * WAVES, HD > 128 ? 1 : 2) void attention_chunk_
     }
     // a wavefront's load covers kFillRows consecutive rows; where those share a page
     // (a.by_page) its address is one scalar and an offset per lane (prompt of 8192
-    // tokens: 548 us, 556 otherwise)
+    // tokens 8 us of 556)
     constexpr int kFillRows = 64 / S::kPlaces, kFillStep = kThreads / S::kPlaces;
     const T *kp = static_cast<const T *>(a.k) + kvh * a.head_stride, *vp = static_cast<const T *>(a.v) + kvh * a.head_stride;
     const uint32_t k_off = 2 * ((lane / S::kPlaces) * a.token_stride + 8 * ck);  // bytes
