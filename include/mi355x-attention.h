@@ -147,8 +147,8 @@ MI355X_API int mi355x_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_ar
  *   j <= p (causal != 0; else every j < kv_lens[s]),  and j > p - window (window > 0):
  *   score_j = scale * q . k_j;  softcap > 0: softcap * tanh(score_j / softcap)
  *   out = sum_j exp(score_j - max) v_j / sum_j exp(score_j - max)
- * Scores, weights and sums are f32, products of 16-bit values on the matrix
- * cores.  The weights meet v as 16-bit values of the pool's type (half a step,
+ * Scores, weights and sums are f32 (capped scores to 2^-23 of the cap), products of
+ * 16-bit values on the matrix cores.  The weights meet v as 16-bit values of the pool's type (half a step,
  * 2^-8 or 2^-11 of a weight: as much as the rounding of a 16-bit output), or
  * as two such planes (no more than 2^-16 of a weight then) where the output is f32
  * or the request takes the form for few rows: at most 16 of them times query heads
