@@ -150,10 +150,10 @@ MI355X_API int mi355x_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_ar
  * Scores, weights and sums are f32 (capped scores to 2^-23 of the cap), products of
  * 16-bit values on the matrix cores.  The weights meet v as 16-bit values of the pool's type (half a step,
  * 2^-8 or 2^-11 of a weight: as much as the rounding of a 16-bit output), or
- * as two such planes (no more than 2^-16 of a weight then) where the output is f32
- * or the request takes the form for few rows: at most 16 of them times query heads
- * of a KV head, by max_added or, in a call of several requests, its own.  That form
- * with an f32 output has them to 2^-22.  F16 has steps of 2^-24 besides: weights
+ * as two such planes (no more than 2^-16 of a weight then) where the request takes
+ * the form for few rows: at most 16 of them times query heads of a KV head, by
+ * max_added or, in a call of several requests, its own.  With an f32 output they go in
+ * to 2^-22, in as many planes as that takes.  F16 has steps of 2^-24 besides: weights
  * are off by up to 2^-24 of the largest one among the 32 or 64 tokens that they are
  * taken with, and by more below 2^-40 of the row's largest.
  * A row that sees nothing gives zeros.  Tokens that a row does not see do not

@@ -198,13 +198,14 @@ struct Reference {
     __device__ __forceinline__ float base() const { return finite_base(m) - Num<TYPE>::kRaise; }
 };
 
-// A weight meets v as a sum of 16-bit planes.  Token form, where the matrix cores idle:
-// two, which leave 2^-16 (bf16) or 2^-22 (f16) of it, and three of bf16 for an f32
-// output (one request of 640 tokens 10.1 -> 10.2 us, 64 ragged ones 214).  Chunk form,
-// which the matrix and vector units bound: one for a 16-bit output, whose own rounding is as
-// large (errors against 64 bits 2.1e-3 of the norm, 1.65e-3 with f32 weights, in bf16),
-// and two for an f32 output (a third of bf16 takes 512 tokens on 4096 from 44 to 51 us,
-// a prompt of 4096 from 217 to 275).
+// A weight meets v as a sum of 16-bit planes.  For an f32 output as many as leave no
+// more than 2^-22 of it: two of f16, three of bf16, of which two leave 2^-16 (errors of up to
+// 2e-6 of the norm against 64 bits where f32 weights give 5e-7; the third takes a chunk of
+// 512 tokens on 4096 from 44 to 51 us, a prompt of 4096 from 217 to 275, single tokens
+// nothing).  For a 16-bit output one in the chunk form, which the matrix and vector units
+// bound, since the output's own rounding is as large (bf16: 2.1e-3 of the norm, 1.65e-3
+// with f32 weights), and two in the token form, where the matrix cores idle.
+constexpr int f32_planes(int type) { return type == MI355X_TYPE_BF16 ? 3 : 2; }
 
 // The planes of weight i.
 template <int TYPE, int PLANES>

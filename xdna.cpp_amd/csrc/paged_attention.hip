@@ -452,9 +452,7 @@ int launch_planes(mi355x_ctx *ctx, const AttnArgs &a) {
 
 template <int TYPE, int HD>
 int launch_token(mi355x_ctx *ctx, const AttnArgs &a) {
-    if constexpr (TYPE == MI355X_TYPE_BF16)
-        if (a.f32_out) return launch_planes<TYPE, HD, 3>(ctx, a);
-    return launch_planes<TYPE, HD, 2>(ctx, a);
+    return a.f32_out ? launch_planes<TYPE, HD, f32_planes(TYPE)>(ctx, a) : launch_planes<TYPE, HD, 2>(ctx, a);
 }
 
 // rows: the host's bound on a request's head rows.  Up to kTokenRows the token

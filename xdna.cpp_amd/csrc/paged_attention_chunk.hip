@@ -474,7 +474,9 @@ template <int TYPE, int HD>
 int launch_size(mi355x_ctx *ctx, const AttnArgs &a) {
     // the common path masks and takes the maximum before it scales, for which the scale has to be positive
     const bool cap = a.cap_out > 0.0f || !(a.scale2 > 0.0f);
-    if (a.f32_out) return cap ? launch_chunk<TYPE, HD, true, 2>(ctx, a) : launch_chunk<TYPE, HD, false, 2>(ctx, a);
+    constexpr int kPlanes = f32_planes(TYPE);
+    if (a.f32_out)
+        return cap ? launch_chunk<TYPE, HD, true, kPlanes>(ctx, a) : launch_chunk<TYPE, HD, false, kPlanes>(ctx, a);
     return cap ? launch_chunk<TYPE, HD, true, 1>(ctx, a) : launch_chunk<TYPE, HD, false, 1>(ctx, a);
 }
 
