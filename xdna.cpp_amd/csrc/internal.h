@@ -12,6 +12,7 @@
 
 #include "mi355x-attention.h"
 #include "mi355x-gemv.h"
+#include "mi355x-layer.h"
 
 struct mi355x_ctx {
     int device = 0;
@@ -196,6 +197,15 @@ int launch_kv_plan(mi355x_ctx *ctx, const mi355x_kv_plan_args &a);
 int launch_qk_norm_rope(mi355x_ctx *ctx, const mi355x_qk_norm_rope_args &a);
 int launch_paged_attention(mi355x_ctx *ctx, const mi355x_paged_attention_args &a);
 size_t paged_attention_workspace_bytes(const mi355x_ctx *ctx, int n_heads, int n_kv_heads, int head_dim);
+
+// The operators of mi355x-layer.h, with arguments that its entry points have
+// checked.
+int launch_norm_q8(mi355x_ctx *ctx, const mi355x_norm_q8_args &a);
+int launch_swiglu_q8(mi355x_ctx *ctx, const mi355x_swiglu_q8_args &a);
+int launch_matmul_q8(mi355x_ctx *ctx, const mi355x_matmul_q8_args &a);
+size_t matmul_q8_workspace_bytes(const mi355x_ctx *ctx);
+int launch_logprobs(mi355x_ctx *ctx, const mi355x_logprobs_args &a);
+size_t logprobs_workspace_bytes(const mi355x_ctx *ctx);
 
 // Resident workgroups per CU of `kernel` at this block size and LDS (cached).
 int occupancy(const void *kernel, int block_threads, size_t lds_bytes);

@@ -1,5 +1,6 @@
 """ctypes binding of libggml-mi355x.so (the C-ABI in include/mi355x-gemv.h and
-include/mi355x-attention.h).
+include/mi355x-attention.h,
+include/mi355x-layer.h).
 
 Python is only the harness language here: tests and bench.py drive the
 library through this module.  Loading fails loudly when the shared library is
@@ -91,6 +92,12 @@ _SIGNATURES = {
     "mi355x_qk_norm_rope": (_c.c_int, [_vp, _vp]),
     "mi355x_paged_attention": (_c.c_int, [_vp, _vp]),
     "mi355x_paged_attention_workspace": (_c.c_int, [_vp, _c.c_int, _c.c_int, _c.c_int, _c.POINTER(_c.c_size_t)]),
+    "mi355x_norm_q8": (_c.c_int, [_vp, _vp]),
+    "mi355x_swiglu_q8": (_c.c_int, [_vp, _vp]),
+    "mi355x_matmul_q8": (_c.c_int, [_vp, _vp]),
+    "mi355x_matmul_q8_workspace": (_c.c_int, [_vp, _c.POINTER(_c.c_size_t)]),
+    "mi355x_logprobs": (_c.c_int, [_vp, _vp]),
+    "mi355x_logprobs_workspace": (_c.c_int, [_vp, _c.POINTER(_c.c_size_t)]),
     "mi355x_time_gemv": (_c.c_int, [_vp, _c.c_int, _c.POINTER(_vp), _c.c_int, _c.c_int64, _c.c_int64, _vp,
                                     _vp, _c.c_int, _c.c_int, _c.POINTER(_c.c_double)]),
 }
@@ -137,6 +144,41 @@ class PagedAttentionArgs(_c.Structure):
                 ("scale", _c.c_float), ("softcap", _c.c_float), ("window", _c.c_int), ("causal", _c.c_int),
                 ("out", _vp), ("out_type", _c.c_int), ("out_stride", _c.c_int64), ("workspace", _vp),
                 ("workspace_bytes", _c.c_size_t)]
+
+
+# a layer's rows and products in 8 bits, and log probabilities (mi355x-layer.h)
+ROW_Q8_MAX, MATMUL_Q8_MAX_K, LOGPROBS_MAX_TOP = 65536, 131056, 64
+
+
+class NormQ8Args(_c.Structure):
+    """mi355x_norm_q8_args (pointers are device addresses)."""
+    _fields_ = [("n_rows", _c.c_int64), ("n", _c.c_int), ("type", _c.c_int), ("x", _vp), ("x_stride", _c.c_int64),
+                ("residual_type", _c.c_int), ("eps", _c.c_float), ("residual", _vp),
+                ("residual_stride", _c.c_int64), ("residual_out", _vp), ("residual_out_stride", _c.c_int64),
+                ("norm", _vp), ("q", _vp), ("q_stride", _c.c_int64), ("scales", _vp)]
+
+
+class SwigluQ8Args(_c.Structure):
+    """mi355x_swiglu_q8_args."""
+    _fields_ = [("n_rows", _c.c_int64), ("n", _c.c_int), ("type", _c.c_int), ("gate", _vp),
+                ("gate_stride", _c.c_int64), ("up", _vp), ("up_stride", _c.c_int64), ("q", _vp),
+                ("q_stride", _c.c_int64), ("scales", _vp)]
+
+
+class MatmulQ8Args(_c.Structure):
+    """mi355x_matmul_q8_args."""
+    _fields_ = [("n_rows", _c.c_int64), ("n_out", _c.c_int64), ("k", _c.c_int64), ("x", _vp),
+                ("x_stride", _c.c_int64), ("x_scales", _vp), ("w", _vp), ("w_stride", _c.c_int64),
+                ("w_scales", _vp), ("bias", _vp), ("out", _vp), ("out_type", _c.c_int), ("out_stride", _c.c_int64),
+                ("workspace", _vp), ("workspace_bytes", _c.c_size_t)]
+
+
+class LogprobsArgs(_c.Structure):
+    """mi355x_logprobs_args."""
+    _fields_ = [("n_rows", _c.c_int64), ("n_vocab", _c.c_int), ("type", _c.c_int), ("logits", _vp),
+                ("stride", _c.c_int64), ("scale", _c.c_float), ("n_tokens", _c.c_int), ("tokens", _vp),
+                ("token_logprobs", _vp), ("entropy", _vp), ("n_top", _c.c_int), ("top_tokens", _vp),
+                ("top_logprobs", _vp), ("workspace", _vp), ("workspace_bytes", _c.c_size_t)]
 
 
 class GemvJob(_c.Structure):
@@ -442,6 +484,34 @@ class Context:
         """Bytes of workspace that paged_attention needs with these heads."""
         n = ctypes.c_size_t()
         check(self.lib.mi355x_paged_attention_workspace(self.h, n_heads, n_kv_heads, head_dim, ctypes.byref(n)))
+        return n.value
+
+    def norm_q8(self, args: NormQ8Args) -> None:
+        """The residual's addition, the norm, and the rows in 8 bits."""
+        check(self.lib.mi355x_norm_q8(self.h, ctypes.byref(args)))
+
+    def swiglu_q8(self, args: SwigluQ8Args) -> None:
+        """silu(gate) * up, rows in 8 bits."""
+        check(self.lib.mi355x_swiglu_q8(self.h, ctypes.byref(args)))
+
+    def matmul_q8(self, args: MatmulQ8Args) -> None:
+        """Rows in 8 bits times a weight in 8 bits."""
+        check(self.lib.mi355x_matmul_q8(self.h, ctypes.byref(args)))
+
+    def matmul_q8_workspace(self) -> int:
+        """Bytes of workspace that matmul_q8 needs."""
+        n = ctypes.c_size_t()
+        check(self.lib.mi355x_matmul_q8_workspace(self.h, ctypes.byref(n)))
+        return n.value
+
+    def logprobs(self, args: LogprobsArgs) -> None:
+        """Log probabilities of given tokens, entropy and top tokens of logits."""
+        check(self.lib.mi355x_logprobs(self.h, ctypes.byref(args)))
+
+    def logprobs_workspace(self) -> int:
+        """Bytes of workspace that logprobs needs."""
+        n = ctypes.c_size_t()
+        check(self.lib.mi355x_logprobs_workspace(self.h, ctypes.byref(n)))
         return n.value
 
     def gemv(self, w: ResidentWeights, x: np.ndarray) -> np.ndarray:
