@@ -34,7 +34,8 @@ extern "C" {
  * A row of values t_0 .. t_n-1 is held as codes and a scale, t_i ~ scale * code_i:
  *   code_i = t_i * 127 / max_j |t_j|, rounded to nearest, ties to even, -127 .. 127
  *   scale  = max_j |t_j| / 127, rounded to f32 (infinite past f32's range)
- * The codes are those of the exact quotient.  A row of zeros has codes and scale
+ * The t_i, the product and the quotient are 64-bit numbers, so that a code is not
+ * off where its quotient lies next to a border.  A row of zeros has codes and scale
  * 0.  A row with a t_i that is infinite or NaN has codes 0 and the scale NaN, so
  * that its products are NaN. */
 

@@ -1,6 +1,4 @@
 """64-bit numpy forms of the operators of mi355x-layer.h."""
-from fractions import Fraction
-
 import numpy as np
 
 from paged_ref import HALF_STEP, decode, encode, storage  # noqa: F401  (what the tests use)
@@ -8,7 +6,7 @@ from paged_ref import HALF_STEP, decode, encode, storage  # noqa: F401  (what th
 
 def codes_of(t, loose=0.0):
     """(codes, scales in 64 bits, whether either neighbour may stand) of rows of 64-bit values, ties to even.
-    A quotient within 1e-9 of a border is settled with whole numbers; one within `loose` may go either way."""
+    A quotient within `loose` of a border may go either way."""
     t = np.asarray(t, np.float64)
     bad = ~np.isfinite(t).all(1)
     t = np.where(bad[:, None], 0.0, t)
@@ -16,9 +14,6 @@ def codes_of(t, loose=0.0):
     y = t * 127 / np.where(most > 0, most, 1)[:, None]
     c = np.rint(y)
     off = np.abs(np.abs(y - np.trunc(y)) - 0.5)
-    for r, i in zip(*np.nonzero(off < 1e-9)):
-        q = Fraction(t[r, i]) * 127 / Fraction(most[r]) if most[r] else Fraction(0)
-        c[r, i] = round(q)  # ties to even
     scale = most / 127
     scale[bad] = np.nan
     return c.astype(np.int8), scale, off < loose

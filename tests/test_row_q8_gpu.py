@@ -1,6 +1,6 @@
 """mi355x_norm_q8 and mi355x_swiglu_q8 against 64 bits.
 
-Codes are those of the exact quotients: equal, but that a gate's value has the
+Codes are those of the 64-bit quotients: equal, but that a gate's value has the
 64-bit rounding of an exponential (a few units of 2^-52 of a quotient of at most
 127, 1e-12 at most), so that a quotient this near to a border may go either way.
 Scales are rounded once: half a step of f32, and 1e-13 for the 64-bit sum, root

@@ -1,11 +1,11 @@
 // Rows in 8 bits: the residual's addition with the root-mean-square norm, and
 // the gated product, each with the largest magnitude of the row as its scale.
 //
-// Codes are the exact quotients' (t * 127 / max |t|, ties to even): the values t
-// are formed in 64 bits -- a product of two f32 numbers is exact there -- and a
-// quotient too near to a border for 64 bits is settled by the sign of
-// 254 |t| - (2 k + 1) max |t|, whose products a fused multiply-add leaves whole.
-// The norm's root multiplies a whole row, so it meets the scale alone.
+// Codes are rint(t * 127 / max |t|) in 64-bit arithmetic: the values t are formed
+// there (a product of two f32 numbers is exact in it), a multiplication by 127 /
+// max |t| gives the code, and one that lands near to a border is settled by the
+// division itself.  The norm's root multiplies a whole row, so it meets the scale
+// alone.
 #include "internal.h"
 #include "row_values.h"
 
@@ -33,15 +33,11 @@ struct RowArgs {
 };
 
 // The code of t in a row whose largest magnitude is `most` > 0; unit = 127 / most.
+// t * unit is within 2^-44 of the stated quotient.
 __device__ __forceinline__ int code_of(double t, double most, double unit) {
-    const double y = t * unit, r = rint(y), off = fabs(y - r);
-    if (off < 0.5 - 1e-9) return static_cast<int>(r);
-    const double a = fabs(t), k = floor(fabs(y)), b = 2.0 * k + 1.0;
-    // k and k + 1 lie around the quotient's magnitude
-    const double p = b * most, side = fma(254.0, a, -p) - fma(b, most, -p);
-    const int lower = static_cast<int>(k);
-    const int c = side > 0.0 || (side == 0.0 && (lower & 1)) ? lower + 1 : lower;
-    return t < 0.0 ? -c : c;
+    const double y = t * unit, r = rint(y);
+    if (fabs(y - r) < 0.5 - 1e-9) return static_cast<int>(r);
+    return static_cast<int>(rint(t * 127.0 / most));
 }
 
 // Sum and largest over the workgroup's threads, one after the other in `lds`.
