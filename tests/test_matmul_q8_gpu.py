@@ -126,6 +126,32 @@ def test_model_sizes(ctx, ws, M, N, K):
     go(ctx, ws, M, N, K, BF16, lo=-128)
 
 
+@pytest.mark.parametrize("K", [16, 96, 128, 144, 272, 400, 1104])
+@pytest.mark.parametrize("t,N", [(BF16, 4100), (F32, 4103), (F16, 4096)])
+def test_more_tiles_than_compute_units(ctx, ws, t, N, K):
+    """Tiles of 256 by 256, several a workgroup, the last ones over their neighbours."""
+    go(ctx, ws, 4900, N, K, t, bias=t == F16, opad=4, lo=-128)
+
+
+def test_strides_past_32_bit_offsets(ctx, ws):
+    """Rows so far apart that a tile's offsets would not fit 32 bits."""
+    M, N, K, far = 130, 70, 272, (1 << 23) + 16
+    c = Product(ctx, ws, M, N, K)
+    big = ctx.alloc(M * far)
+    try:
+        for r in range(M):
+            big.upload(c.x[r], r * far)
+            if r < N:
+                big.upload(c.w[r], r * far + 1024)
+        c.args.x, c.args.x_stride, c.args.w, c.args.w_stride = big.ptr, far, big.ptr + 1024, far
+        ctx.matmul_q8(c.args)
+        ctx.sync()
+        c.verify()
+    finally:
+        big.free()
+        c.free()
+
+
 def test_scales_that_are_not_finite(ctx, ws):
     """A row of codes 0 with the scale NaN gives NaN throughout, and no other row."""
     for M in (1, 20, 140):

@@ -2,12 +2,18 @@
 // integer matrix cores: sums of products of codes are exact in 32 bits (128 * 128
 // * 131056 < 2^31), so the order of the sum and the split of the work do not show.
 //
-// The weight is the products' left operand: a lane then holds consecutive channels
-// of one row of the output.
+// The weight is the products' left operand: a lane then holds four consecutive
+// channels of one row of the output.
+//
+// All operands travel to LDS directly (global_load_lds, whole 128-byte lines) in
+// pieces of 8 rows, eight lanes a row; such loads fill LDS in lane order, so the
+// 16-byte chunks of a row are permuted by the row's number, that the operands' reads
+// (16 rows, one chunk) do not meet in a bank.
 #include "far_parts.h"
 #include "internal.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace mi355x {
 namespace {
@@ -22,14 +28,44 @@ struct MatmulArgs {
     int *counters;  // 0 before and after a call
     float *ws;
     int m, n, k, out_type;
-    int wide;            // stores of four channels at once keep to their alignment
-    int m_tiles, n_tiles, splits, split_steps;
+    int m_tiles, n_tiles, splits, split_stages;
 };
 
-constexpr int kStepBytes = 64;  // of k that one matrix product takes
+constexpr int kStage = 128;  // bytes of k in a stage: two matrix products deep
 
 __device__ __forceinline__ i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+// At most N of this wavefront's loads (and stores) are under way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N >= 0 && N < 64, "");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
+}
+// The same, and all of its LDS reads are done.
+template <int N>
+__device__ __forceinline__ void wait_loads_and_reads() {
+    static_assert(N >= 0 && N < 64, "");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+}
+__device__ __forceinline__ void wait_reads() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Row `row` (0 .. 7 of the piece's half, 8 more for the second) and chunk of a piece
+// that a lane fills, and where an operand's lane finds its chunk again.
+__device__ __forceinline__ int piece_row(int half, int lane) { return 8 * half + (lane >> 3); }
+__device__ __forceinline__ int piece_chunk(int half, int lane) {
+    return 16 * ((lane & 7) ^ (piece_row(half, lane) >> 1));
+}
+__device__ __forceinline__ int operand_at(int half, int col, int quad) {
+    return 128 * col + 16 * ((4 * half + quad) ^ (col >> 1));
 }
 
 // One value of the product, in the stated order of roundings.
@@ -41,129 +77,155 @@ __device__ __forceinline__ float scaled(int sum, float ws, float xs, bool has_bi
     return v;
 }
 
-template <class T>
-__device__ __forceinline__ void store4(void *out, int64_t at, int left, bool wide, const float *v) {
-    typedef T T4 __attribute__((ext_vector_type(4)));
+template <class T, int N>
+__device__ __forceinline__ void store_some(void *out, int64_t at, int left, const float *v) {
+    typedef T TN __attribute__((ext_vector_type(N), aligned(sizeof(T))));
     T *p = static_cast<T *>(out) + at;
-    if (wide && left >= 4) {
-        *reinterpret_cast<T4 *>(p) = T4{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
+    if (left >= N) {
+        TN t;
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = static_cast<T>(v[i]);
+        *reinterpret_cast<TN *>(p) = t;
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < N; ++i)
             if (i < left) p[i] = static_cast<T>(v[i]);
     }
 }
 
-// Channels n .. n + 3 of row m from their sums.
-__device__ __forceinline__ void write4(const MatmulArgs &a, int m, int n, i32x4 sum) {
-    if (m >= a.m || n >= a.n) return;
-    const float xs = a.x_scales[m];
-    float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = min(n + i, a.n - 1);
-        v[i] = scaled(sum[i], a.w_scales[c], xs, a.bias != nullptr, a.bias ? a.bias[c] : 0.0f);
-    }
+// Channels n .. n + N - 1 of row m.
+template <int N>
+__device__ __forceinline__ void store_row(const MatmulArgs &a, int m, int n, const float *v) {
     const int64_t at = m * a.out_stride + n;
-    if (a.out_type == MI355X_TYPE_F32) store4<float>(a.out, at, a.n - n, a.wide, v);
-    else if (a.out_type == MI355X_TYPE_F16) store4<_Float16>(a.out, at, a.n - n, a.wide, v);
-    else store4<__bf16>(a.out, at, a.n - n, a.wide, v);
+    if (a.out_type == MI355X_TYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) store_some<float, 4>(a.out, at + i, a.n - n - i, v + i);
+    } else if (a.out_type == MI355X_TYPE_F16) {
+        store_some<_Float16, N>(a.out, at, a.n - n, v);
+    } else {
+        store_some<__bf16, N>(a.out, at, a.n - n, v);
+    }
 }
 
 // ---- few rows ------------------------------------------------------------------
 
-// A workgroup computes 16 * R channels of up to 16 * TM rows; its wavefronts share
-// out k and add their sums in LDS.
-constexpr int kFewWaves = 8;
+// A workgroup computes 16 * R channels of up to 16 * TM rows.  Its WAVES wavefronts
+// share out k, each with a ring of ST stages of its own, and add their sums in LDS.
+template <int TM, int R, int WAVES, int ST>
+struct FewShape {
+    static constexpr int kUnit = 2048 * (TM + R);
+    static constexpr int kRing = WAVES * ST * kUnit, kSums = WAVES * R * TM * 1024;
+    static constexpr int kLds = kRing > kSums ? kRing : kSums;
+};
 
-template <int TM, int R>
-__global__ __launch_bounds__(64 * kFewWaves) void matmul_few_kernel(MatmulArgs a) {
-    constexpr int U = TM >= 3 ? 2 : 4;  // steps whose operands are loaded together
-    __shared__ i32x4 part[kFewWaves][R * TM][64];
+template <int TM, int R, int WAVES, int ST>
+__global__ __launch_bounds__(64 * WAVES) void matmul_few_kernel(MatmulArgs a) {
+    typedef FewShape<TM, R, WAVES, ST> S;
+    constexpr int kBlocks = R + TM, kLoads = 2 * kBlocks;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, quad = lane >> 4;
     const int n0 = blockIdx.x * 16 * R, m0 = blockIdx.y * 16 * TM;
-    const int steps = (a.k + kStepBytes - 1) / kStepBytes;
-    const int s0 = steps * wave / kFewWaves, s1 = steps * (wave + 1) / kFewWaves;
-    const int8_t *w[R], *x[TM];
+    const int stages = (a.k + kStage - 1) / kStage;
+    const int s0 = stages * wave / WAVES, s1 = stages * (wave + 1) / WAVES;
+    const int8_t *src[kBlocks][2];
+    int chunk[2];
 #pragma unroll
-    for (int r = 0; r < R; ++r) w[r] = a.w + static_cast<int64_t>(min(n0 + 16 * r + col, a.n - 1)) * a.w_stride;
+    for (int i = 0; i < 2; ++i) {
+        chunk[i] = piece_chunk(i, lane);
 #pragma unroll
-    for (int t = 0; t < TM; ++t) x[t] = a.x + static_cast<int64_t>(min(m0 + 16 * t + col, a.m - 1)) * a.x_stride;
+        for (int b = 0; b < kBlocks; ++b) {
+            const int row = 16 * (b < R ? b : b - R) + piece_row(i, lane);
+            src[b][i] = (b < R ? a.w + min(n0 + row, a.n - 1) * a.w_stride : a.x + min(m0 + row, a.m - 1) * a.x_stride) +
+                        chunk[i];
+        }
+    }
+    uint8_t *mine = lds + wave * ST * S::kUnit;
+    auto load = [&](int s, int slot) {
+        const int k = kStage * s;
+        int at[2] = {k, k};
+        if (k + kStage > a.k)  // instead of chunks behind the rows' ends the stage's first
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (k + chunk[i] >= a.k) at[i] = k - chunk[i];
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                __builtin_amdgcn_global_load_lds(
+                    reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(
+                        reinterpret_cast<uintptr_t>(src[b][i] + at[i])),
+                    (__attribute__((address_space(3))) uint32_t *)(mine + slot * S::kUnit + 2048 * b + 1024 * i), 16, 0, 0);
+    };
     i32x4 c[R][TM];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int t = 0; t < TM; ++t) c[r][t] = i32x4{0, 0, 0, 0};
-    i32x4 wf[2][U][R], xf[2][U][TM];
-    auto load = [&](int b, int s) {
+    auto multiply = [&](int s, int slot) {
+        i32x4 f[2][kBlocks];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = kStepBytes * (s + u) + 16 * quad;
-            const bool in = s + u < s1 && k < a.k;
-            const int at = in ? k : 0;
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < R; ++r) wf[b][u][r] = *reinterpret_cast<const i32x4 *>(w[r] + at);
+            for (int b = 0; b < kBlocks; ++b)
+                f[h][b] = *reinterpret_cast<const i32x4 *>(mine + slot * S::kUnit + 2048 * b + operand_at(h, col, quad));
+        if (kStage * (s + 1) > a.k)
 #pragma unroll
-            for (int t = 0; t < TM; ++t) xf[b][u][t] = *reinterpret_cast<const i32x4 *>(x[t] + at);
-        }
+            for (int h = 0; h < 2; ++h)
+                if (kStage * s + 64 * h + 16 * quad >= a.k)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) f[h][r] = i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int t = 0; t < TM; ++t) c[r][t] = mfma(f[h][r], f[h][R + t], c[r][t]);
     };
-    auto multiply = [&](int b, int s) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = s + u < s1 && kStepBytes * (s + u) + 16 * quad < a.k;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                i32x4 v = wf[b][u][r];
-                if (!in) v = i32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int t = 0; t < TM; ++t) c[r][t] = mfma(v, xf[b][u][t], c[r][t]);
-            }
+    for (int i = 0; i < ST - 1; ++i)
+        if (s0 + i < s1) load(s0 + i, i);
+    int slot = 0;
+    for (int s = s0; s < s1; ++s) {
+        // the slot that is filled was read in the last step, whose products have its values
+        if (s + ST - 1 < s1) {
+            load(s + ST - 1, slot == 0 ? ST - 1 : slot - 1);
+            wait_loads<(ST - 1) * kLoads>();
+        } else {
+            wait_loads<0>();
         }
-    };
-    if (s0 < s1) {
-        load(0, s0);
-        for (int s = s0; s < s1; s += 2 * U) {
-            if (s + U < s1) load(1, s + U);
-            multiply(0, s);
-            if (s + U < s1) {
-                if (s + 2 * U < s1) load(0, s + 2 * U);
-                multiply(1, s + U);
-            }
-        }
+        asm volatile("" ::: "memory");
+        multiply(s, slot);
+        wait_reads();
+        asm volatile("" ::: "memory");
+        slot = slot + 1 == ST ? 0 : slot + 1;
     }
+    __syncthreads();
+    i32x4 *sums = reinterpret_cast<i32x4 *>(lds);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int t = 0; t < TM; ++t) part[wave][r * TM + t][lane] = c[r][t];
+        for (int t = 0; t < TM; ++t) sums[(wave * R * TM + r * TM + t) * 64 + lane] = c[r][t];
     __syncthreads();
-    for (int b = wave; b < R * TM; b += kFewWaves) {
-        i32x4 sum = part[0][b][lane];
+    for (int b = wave; b < R * TM; b += WAVES) {
+        i32x4 sum = sums[b * 64 + lane];
 #pragma unroll
-        for (int v = 1; v < kFewWaves; ++v) sum += part[v][b][lane];
-        write4(a, m0 + 16 * (b % TM) + col, n0 + 16 * (b / TM) + 4 * quad, sum);
+        for (int v = 1; v < WAVES; ++v) sum += sums[(v * R * TM + b) * 64 + lane];
+        const int m = m0 + 16 * (b % TM) + col, n = n0 + 16 * (b / TM) + 4 * quad;
+        if (m < a.m && n < a.n) {
+            const float xs = a.x_scales[m];
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int ch = min(n + i, a.n - 1);
+                v[i] = scaled(sum[i], a.w_scales[ch], xs, a.bias != nullptr, a.bias ? a.bias[ch] : 0.0f);
+            }
+            store_row<4>(a, m, n, v);
+        }
     }
 }
 
-// ---- many rows -------------------------------------------------------------------
-
-// A workgroup computes BM rows by BN channels from tiles in LDS.  Such tiles travel
-// there directly (global_load_lds), kStages - 1 steps ahead; a load fills 16 rows of
-// 64 bytes in lane order, four lanes a row, whose 16-byte chunks are permuted by the
-// row's number so that the operands' reads (16 rows, one chunk) do not meet in a bank.
-constexpr int kStages = 4;
-
-template <int BM, int BN, int WM, int WN>
-struct TileShape {
-    static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
-    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-    static constexpr int kBlocks = (BM + BN) / 16;       // of a stage, 1 KB each
-    static constexpr int kLoads = kBlocks / kWaves;      // of a wavefront and stage
-    static constexpr int kStageBytes = 1024 * kBlocks;
-    static constexpr int kLds = kStages * kStageBytes;
-    static constexpr int kPartInts = BM * BN;
-    static_assert(kBlocks % kWaves == 0, "every wavefront loads as many blocks");
-};
+// ---- tiles -------------------------------------------------------------------
 
 // The tile that workgroup `id` of `total` computes: each die (workgroups go round
 // the 8 dies) takes a run of them, rows first within bands of 8 row tiles, so that
@@ -181,9 +243,73 @@ __device__ __forceinline__ void tile_of(const MatmulArgs &a, int id, int total, 
     *mt = 8 * band + t - *nt * rows;
 }
 
-template <int BM, int BN, int WM, int WN>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const int8_t *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(p), 0, 0xFFFFFFFFu, kBufferWord3);
+}
+__device__ __forceinline__ void load_piece(__amdgpu_buffer_rsrc_t rows, uint8_t *dst, uint32_t at, uint32_t k) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (__attribute__((address_space(3))) void *)dst, 16, at, k, 0, 0);
+}
+
+// Channel of a wavefront that row `row` of its block `tn` of 16 stands for.  For a
+// 16-bit output two blocks share 32 channels so that a lane has 8 consecutive ones.
+__device__ __forceinline__ int channel_of(int row, int tn, bool pairs) {
+    return pairs ? 32 * (tn >> 1) + 8 * (row >> 2) + 4 * (tn & 1) + (row & 3) : 16 * tn + row;
+}
+
+// The outputs of a wavefront's sums: rows m + 16 j, channels from n on.
+template <int TM, int TN>
+__device__ __forceinline__ void write_tile(const MatmulArgs &a, int m, int n, const i32x4 (&c)[TN][TM], int quad) {
+    float ws[TN][4], bias[TN][4];
+    const bool pairs = a.out_type != MI355X_TYPE_F32, has_bias = a.bias != nullptr;
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int ch = min(n + channel_of(4 * quad + q, i, pairs), a.n - 1);
+            ws[i][q] = a.w_scales[ch];
+            bias[i][q] = has_bias ? a.bias[ch] : 0.0f;
+        }
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+        const int row = m + 16 * j;
+        if (row >= a.m) continue;
+        const float xs = a.x_scales[row];
+#pragma unroll
+        for (int i = 0; i < TN; i += 2) {
+            float v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                v[q] = scaled(c[i + q / 4][j][q % 4], ws[i + q / 4][q % 4], xs, has_bias, bias[i + q / 4][q % 4]);
+            if (pairs) {
+                const int ch = n + channel_of(4 * quad, i, true);
+                if (ch < a.n) store_row<8>(a, row, ch, v);
+            } else {
+                const int ch = n + channel_of(4 * quad, i, false);
+                if (ch < a.n) store_row<4>(a, row, ch, v);
+                if (ch + 16 < a.n) store_row<4>(a, row, ch + 16, v + 4);
+            }
+        }
+    }
+}
+
+// A workgroup of WM x WN wavefronts computes BM rows by BN channels from a ring of ST
+// stages.  One barrier a stage; operands are read half a stage ahead of their
+// products.  Where there are few tiles k is split, and the last workgroup of a tile
+// adds the others' sums to its own.
+template <int BM, int BN, int WM, int WN, int ST>
+struct TileShape {
+    static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+    static constexpr int kBlocks = (BM + BN) / 16;
+    static constexpr int kLoads = 2 * kBlocks / kWaves;  // pieces of a wavefront and stage
+    static constexpr int kStageBytes = 2048 * kBlocks;
+    static constexpr int kLds = ST * kStageBytes;
+    static_assert(2 * kBlocks % kWaves == 0 && TN % 2 == 0, "");
+};
+
+template <int BM, int BN, int WM, int WN, int ST>
 __global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a) {
-    typedef TileShape<BM, BN, WM, WN> S;
+    typedef TileShape<BM, BN, WM, WN, ST> S;
     constexpr int TM = S::TM, TN = S::TN;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -191,92 +317,269 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a)
     int mt, nt, split;
     tile_of(a, blockIdx.x, gridDim.x, &mt, &nt, &split);
     const int m0 = mt * BM, n0 = nt * BN;
-    const int steps = (a.k + kStepBytes - 1) / kStepBytes;
-    const int s0 = split * a.split_steps, s1 = min(steps, s0 + a.split_steps);
-
+    const int s0 = split * a.split_stages, s1 = min((a.k + kStage - 1) / kStage, s0 + a.split_stages);
+    const bool pairs = a.out_type != MI355X_TYPE_F32;
+    const __amdgpu_buffer_rsrc_t w_rows = rows_at(a.w + n0 * a.w_stride), x_rows = rows_at(a.x + m0 * a.x_stride);
     // blocks of a stage: BN / 16 of w, then BM / 16 of x
-    const int8_t *src[S::kLoads];
-    const int chunk = 16 * ((lane & 3) ^ (lane >> 4)), r = lane >> 2;
+    uint32_t at[S::kLoads];
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-        const int b = wave * S::kLoads + i;
-        if (b < BN / 16) {
-            // a wavefront's channels are dealt out so that a lane's are consecutive
-            const int wn = b / TN, tn = b % TN;
-            const int n = n0 + wn * 16 * TN + (r >> 2) * 4 * TN + 4 * tn + (r & 3);
-            src[i] = a.w + static_cast<int64_t>(min(n, a.n - 1)) * a.w_stride;
-        } else {
-            const int m = m0 + 16 * (b - BN / 16) + r;
-            src[i] = a.x + static_cast<int64_t>(min(m, a.m - 1)) * a.x_stride;
-        }
+        const int p = wave * S::kLoads + i, b = p >> 1, row = piece_row(p & 1, lane);
+        const uint32_t r = b < BN / 16 ? min(16 * TN * (b / TN) + channel_of(row, b % TN, pairs), a.n - 1 - n0)
+                                       : min(16 * (b - BN / 16) + row, a.m - 1 - m0);
+        at[i] = r * static_cast<uint32_t>(b < BN / 16 ? a.w_stride : a.x_stride) + piece_chunk(p & 1, lane);
     }
-    auto load = [&](int s) {
-        const int k = kStepBytes * s + chunk;
-        const int at = k < a.k ? k : 0;
-        uint8_t *dst = lds + (s - s0) % kStages * S::kStageBytes + 1024 * wave * S::kLoads;
+    auto load = [&](int s, int slot) {
+        const int k = kStage * s;
 #pragma unroll
-        for (int i = 0; i < S::kLoads; ++i)
-            __builtin_amdgcn_global_load_lds(
-                reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(reinterpret_cast<uintptr_t>(src[i] + at)),
-                (__attribute__((address_space(3))) uint32_t *)(dst + 1024 * i), 16, 0, 0);
+        for (int i = 0; i < S::kLoads; ++i) {
+            const int p = wave * S::kLoads + i;
+            uint32_t v = at[i];
+            if (k + kStage > a.k && k + piece_chunk(p & 1, lane) >= a.k) v -= piece_chunk(p & 1, lane);
+            if (p < BN / 8) load_piece(w_rows, lds + slot * S::kStageBytes + 1024 * p, v, k);
+            else load_piece(x_rows, lds + slot * S::kStageBytes + 1024 * p, v, k);
+        }
     };
-    i32x4 c[TN][TM];
+    const int wm = wave % WM, wn = wave / WM;
+    const int w_at = 2048 * wn * TN, x_at = 2048 * (BN / 16 + wm * TM);
+    i32x4 c[TN][TM], wf[2][TN], xf[2][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int j = 0; j < TM; ++j) c[i][j] = i32x4{0, 0, 0, 0};
-    const int wm = wave % WM, wn = wave / WM;
-    const int slot = 16 * (4 * col + (quad ^ (col >> 2)));
-    const int w_at = 1024 * wn * TN + slot, x_at = 1024 * (BN / 16 + wm * TM) + slot;
+    auto read = [&](int h, int s, int slot) {
+        const uint8_t *p = lds + slot * S::kStageBytes + operand_at(h, col, quad);
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i)
-        if (s0 + i < s1) load(s0 + i);
-    for (int s = s0; s < s1; ++s) {
-        // this wavefront's loads of stage s are done where only the later ones are left
-        if (s + kStages - 2 < s1) __builtin_amdgcn_s_waitcnt(0x0F70 | ((kStages - 2) * S::kLoads));
-        else __builtin_amdgcn_s_waitcnt(0x0F70);
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (s + kStages - 1 < s1) load(s + kStages - 1);
-        const uint8_t *stage = lds + (s - s0) % kStages * S::kStageBytes;
-        i32x4 wf[TN], xf[TM];
+        for (int i = 0; i < TN; ++i) wf[h][i] = *reinterpret_cast<const i32x4 *>(p + w_at + 2048 * i);
 #pragma unroll
-        for (int i = 0; i < TN; ++i) wf[i] = *reinterpret_cast<const i32x4 *>(stage + w_at + 1024 * i);
+        for (int j = 0; j < TM; ++j) xf[h][j] = *reinterpret_cast<const i32x4 *>(p + x_at + 2048 * j);
+        if (kStage * (s + 1) > a.k && kStage * s + 64 * h + 16 * quad >= a.k)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) xf[j] = *reinterpret_cast<const i32x4 *>(stage + x_at + 1024 * j);
-        if (kStepBytes * s + 16 * quad >= a.k)
-#pragma unroll
-            for (int i = 0; i < TN; ++i) wf[i] = i32x4{0, 0, 0, 0};
+            for (int i = 0; i < TN; ++i) wf[h][i] = i32x4{0, 0, 0, 0};
+    };
+    auto multiply = [&](int h) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < TM; ++j)
 #pragma unroll
-            for (int i = 0; i < TN; ++i) c[i][j] = mfma(wf[i], xf[j], c[i][j]);
+            for (int i = 0; i < TN; ++i) c[i][j] = mfma(wf[h][i], xf[h][j], c[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int i = 0; i < ST; ++i)
+        if (s0 + i < s1) load(s0 + i, i);
+    if (s0 + ST - 1 < s1) wait_loads<(ST - 1) * S::kLoads>();
+    else wait_loads<0>();
+    barrier();
+    read(0, s0, 0);
+    int slot = 0;
+    for (int s = s0; s < s1; ++s) {
+        const int next = slot + 1 == ST ? 0 : slot + 1;
+        read(1, s, slot);
+        multiply(0);
+        // stage s + 1 is there (up to s + ST - 1 have been asked for), and stage s has been read
+        if (s + ST - 1 < s1) wait_loads_and_reads<(ST - 2) * S::kLoads>();
+        else wait_loads_and_reads<0>();
+        barrier();
+        if (s + ST < s1) load(s + ST, slot);
+        if (s + 1 < s1) read(0, s + 1, next);
+        multiply(1);
+        slot = next;
     }
     if (a.splits > 1) {
         const FarParts far(a.ws);
         const int tile = mt * a.n_tiles + nt, tiles = a.m_tiles * a.n_tiles;
         const int mine = 4 * (wave * TM * TN * 64 + lane);
-        const int at = (split * tiles + tile) * S::kPartInts + mine;
+        const int to = (split * tiles + tile) * BM * BN + mine;
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
-            for (int j = 0; j < TM; ++j) far.store4(at + 256 * (i * TM + j), __builtin_bit_cast(f32x4, c[i][j]));
+            for (int j = 0; j < TM; ++j) far.store4(to + 256 * (i * TM + j), __builtin_bit_cast(f32x4, c[i][j]));
         if (!last_of(a.counters + tile, a.splits, reinterpret_cast<int *>(lds))) return;
         for (int p = 0; p < a.splits; ++p) {
             if (p == split) continue;
-            const int from = (p * tiles + tile) * S::kPartInts + mine;
+            const int from = (p * tiles + tile) * BM * BN + mine;
 #pragma unroll
             for (int i = 0; i < TN; ++i)
 #pragma unroll
                 for (int j = 0; j < TM; ++j) c[i][j] += __builtin_bit_cast(i32x4, far.load4(from + 256 * (i * TM + j)));
         }
     }
-    const int n = n0 + wn * 16 * TN + quad * 4 * TN, m = m0 + wm * 16 * TM + col;
+    write_tile<TM, TN>(a, m0 + wm * 16 * TM + col, n0 + wn * 16 * TN, c, quad);
+}
+
+// ---- large tiles -----------------------------------------------------------------
+
+// 256 rows by 256 channels, eight wavefronts of 128 by 64 in two groups of four, one
+// of each group on a SIMD.  A group's memory part (reads of a quarter of the next
+// products' operands, loads of a quarter of the stage after next) runs while the other
+// group multiplies; barriers swap them.  A stage is four such turns: with X0, X1 and W0,
+// W1 the halves of a wavefront's rows and channels, X0 W0, X0 W1, X1 W1, X1 W0.  Of the
+// two stages in LDS a quarter is free as soon as both groups have read it, so that loads
+// are under way for 7 turns.  The workgroup goes through several tiles; the first
+// stages of the next are loaded while a tile's outputs are written.
+constexpr int kLarge = 256;
+constexpr int kLargeThreads = 512;
+constexpr int kLargeStage = 2 * kLarge * kStage;
+constexpr int kLargeLds = 2 * kLargeStage;
+
+__global__ __launch_bounds__(kLargeThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void matmul_large_kernel(
+    MatmulArgs a) {
+    constexpr int TM = 8, TN = 4, HM = TM / 2, HN = TN / 2;  // blocks of 16 of a wavefront, and of a half of them
+    constexpr int kQuarter = 2;                              // loads of a wavefront
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const bool pairs = a.out_type != MI355X_TYPE_F32;
+    const int stages = (a.k + kStage - 1) / kStage;
+    // a wavefront loads one block of each quarter: of x the row half wave / 4, of w the
+    // channels of wavefront wave / 2
+    const int x_block = wave / HM * TM + wave % HM, w_block = wave / HN * TN + wave % HN;
+    uint32_t x_at[2], w_at[2];
+    int chunk[2];
 #pragma unroll
-    for (int j = 0; j < TM; ++j)
+    for (int i = 0; i < 2; ++i) {
+        chunk[i] = piece_chunk(i, lane);
+        const int row = piece_row(i, lane);
+        x_at[i] = row * static_cast<uint32_t>(a.x_stride) + chunk[i];
+        w_at[i] = channel_of(row, 0, pairs) * static_cast<uint32_t>(a.w_stride) + chunk[i];
+    }
+    const uint32_t x_half = 16 * HM * static_cast<uint32_t>(a.x_stride), w_half = 16 * HN * static_cast<uint32_t>(a.w_stride);
+    const int wm = wave & 1, wn = wave >> 1;
+    const int x_lds = 2048 * wm * TM, w_lds = 2048 * (16 + wn * TN);
+    const int operand[2] = {operand_at(0, col, quad), operand_at(1, col, quad)};
+    const int tiles = a.m_tiles * a.n_tiles;
+
+    __amdgpu_buffer_rsrc_t x_rows, w_rows;
+    int m0 = 0, n0 = 0;
+    // tiles of the last row and column end with the output, over their neighbours' outputs
+    auto begin = [&](int t) {
+        int mt, nt, split;
+        tile_of(a, t, tiles, &mt, &nt, &split);
+        m0 = min(mt * kLarge, a.m - kLarge);
+        n0 = min(nt * kLarge, a.n - kLarge);
+        x_rows = rows_at(a.x + (m0 + 16 * x_block) * a.x_stride);
+        w_rows = rows_at(a.w + (n0 + 16 * TN * (wave / HN) + channel_of(0, wave % HN, pairs)) * a.w_stride);
+    };
+    auto piece = [&](__amdgpu_buffer_rsrc_t rows, uint8_t *dst, const uint32_t *at, uint32_t off, int s) {
+        const int k = kStage * s;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) write4(a, m + 16 * j, n + 4 * i, c[i][j]);
+        for (int i = 0; i < 2; ++i) {
+            uint32_t v = at[i];
+            if (k + kStage > a.k && k + chunk[i] >= a.k) v -= chunk[i];  // the stage's first
+            load_piece(rows, dst + 1024 * i, v, k + off);
+        }
+    };
+    auto load_x = [&](int h, int s) {
+        piece(x_rows, lds + (s & 1) * kLargeStage + 2048 * (x_block + h * HM), x_at, h * x_half, s);
+    };
+    auto load_w = [&](int h, int s) {
+        piece(w_rows, lds + (s & 1) * kLargeStage + 2048 * (16 + w_block + h * HN), w_at, h * w_half, s);
+    };
+    auto load_first = [&]() {
+        load_x(0, 0);
+        load_w(0, 0);
+        load_w(1, 0);
+        load_x(1, 0);
+        if (stages > 1) {
+            load_x(0, 1);
+            load_w(0, 1);
+            load_w(1, 1);
+            load_x(1, 1);
+        }
+    };
+    i32x4 c[TN][TM], x0[2][HM], x1[2][HM], w0[2][HN], w1[2][HN];
+    auto read_x = [&](i32x4 (&f)[2][HM], int q, int h, int s) {
+#pragma unroll
+        for (int j = 0; j < HM; ++j)
+            f[q][j] = *reinterpret_cast<const i32x4 *>(lds + (s & 1) * kLargeStage + x_lds + 2048 * (h * HM + j) + operand[q]);
+    };
+    auto read_w = [&](i32x4 (&f)[2][HN], int h, int s) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < HN; ++i)
+                f[q][i] = *reinterpret_cast<const i32x4 *>(lds + (s & 1) * kLargeStage + w_lds + 2048 * (h * HN + i) + operand[q]);
+        if (kStage * (s + 1) > a.k)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                if (kStage * s + 64 * q + 16 * quad >= a.k)
+#pragma unroll
+                    for (int i = 0; i < HN; ++i) f[q][i] = i32x4{0, 0, 0, 0};
+    };
+    auto multiply = [&](i32x4 (&xf)[2][HM], i32x4 (&wf)[2][HN], int xh, int wh) {
+        wait_reads();
+        barrier();
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int j = 0; j < HM; ++j)
+#pragma unroll
+                for (int i = 0; i < HN; ++i)
+                    c[wh * HN + i][xh * HM + j] = mfma(wf[q][i], xf[q][j], c[wh * HN + i][xh * HM + j]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        barrier();
+    };
+    int t = blockIdx.x;
+    if (t >= tiles) return;
+    begin(t);
+    load_first();
+    wait_loads<0>();
+    for (;;) {
+        // here the first two stages are there for this wavefront's part
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) c[i][j] = i32x4{0, 0, 0, 0};
+        barrier();
+        if (wave >= 4) barrier();  // the second group is one part behind
+        read_x(x0, 0, 0, 0);
+        for (int s = 0; s < stages; ++s) {
+            const bool more = s + 2 < stages, next = s + 1 < stages;
+            read_x(x0, 1, 0, s);
+            read_w(w0, 0, s);
+            // W1 and X1 of this stage (asked for with it) are there: the next stage's are under way
+            if (s >= 2) {
+                if (next) wait_loads<4 * kQuarter>();
+                else wait_loads<0>();
+            }
+            multiply(x0, w0, 0, 0);
+            read_w(w1, 1, s);
+            read_x(x1, 0, 1, s);
+            if (more) {
+                load_x(0, s + 2);
+                load_w(0, s + 2);
+            }
+            multiply(x0, w1, 0, 1);
+            read_x(x1, 1, 1, s);
+            // X0 and W0 of the next stage
+            if (more) {
+                load_w(1, s + 2);
+                if (s >= 1) wait_loads<5 * kQuarter>();
+            } else if (next && s >= 1) {
+                wait_loads<2 * kQuarter>();
+            }
+            multiply(x1, w1, 1, 1);
+            if (next) read_x(x0, 0, 0, s + 1);
+            if (more) load_x(1, s + 2);
+            multiply(x1, w0, 1, 0);
+        }
+        if (wave < 4) barrier();  // both groups have read everything
+        const int m = m0 + wm * 16 * TM + col, n = n0 + wn * 16 * TN;
+        t += gridDim.x;
+        const bool last = t >= tiles;
+        if (!last) {
+            begin(t);
+            load_first();
+        }
+        write_tile<TM, TN>(a, m, n, c, quad);
+        if (last) return;
+        // of the operations so far only stores of outputs, the newest, may be under way
+        if (pairs) wait_loads<TM * TN / 2>();
+        else wait_loads<TM * TN>();
+    }
 }
 
 // ---- the choice ---------------------------------------------------------------
@@ -284,39 +587,84 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a)
 constexpr size_t kCounters = 4096;
 constexpr size_t kPartBytes = size_t(64) << 20;
 
-template <int TM, int R>
+template <int TM, int R, int WAVES, int ST>
 int launch_few(mi355x_ctx *ctx, const MatmulArgs &a) {
-    matmul_few_kernel<TM, R><<<(a.n + 16 * R - 1) / (16 * R), 64 * kFewWaves, 0, ctx->stream>>>(a);
+    const dim3 grid((a.n + 16 * R - 1) / (16 * R), (a.m + 16 * TM - 1) / (16 * TM));
+    matmul_few_kernel<TM, R, WAVES, ST><<<grid, 64 * WAVES, FewShape<TM, R, WAVES, ST>::kLds, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
     return MI355X_OK;
 }
 
-template <int BM, int BN, int WM, int WN>
-int launch_tiles(mi355x_ctx *ctx, MatmulArgs a) {
-    typedef TileShape<BM, BN, WM, WN> S;
-    static bool sized = false;  // the same for every device
-    if (!sized) {
-        MI355X_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(matmul_tile_kernel<BM, BN, WM, WN>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
-        sized = true;
-    }
+int stages_of(const MatmulArgs &a) { return (a.k + kStage - 1) / kStage; }
+
+template <int BM, int BN, int WM, int WN, int ST>
+int launch_tiles(mi355x_ctx *ctx, MatmulArgs a, int splits) {
+    typedef TileShape<BM, BN, WM, WN, ST> S;
     a.m_tiles = (a.m + BM - 1) / BM;
     a.n_tiles = (a.n + BN - 1) / BN;
-    const int64_t tiles = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
-    if (tiles >= (1 << 22))
-        return set_error(MI355X_EUNSUPPORTED,
-                         "mi355x_matmul_q8: " + std::to_string(tiles) + " tiles of the output, 2^22 or more");
-    const int steps = (a.k + kStepBytes - 1) / kStepBytes;
-    int64_t splits = 1;
-    if (tiles <= ctx->num_cus / 2)
-        splits = std::min<int64_t>({ctx->num_cus / tiles, steps / 16, int64_t(kPartBytes / (4 * S::kPartInts) / tiles)});
-    splits = std::max<int64_t>(splits, 1);
-    a.split_steps = static_cast<int>((steps + splits - 1) / splits);
-    a.splits = (steps + a.split_steps - 1) / a.split_steps;
-    matmul_tile_kernel<BM, BN, WM, WN>
-        <<<static_cast<unsigned>(tiles * a.splits), S::kThreads, S::kLds, ctx->stream>>>(a);
+    const int stages = stages_of(a);
+    a.split_stages = (stages + splits - 1) / splits;
+    a.splits = (stages + a.split_stages - 1) / a.split_stages;
+    matmul_tile_kernel<BM, BN, WM, WN, ST>
+        <<<static_cast<unsigned>(a.m_tiles * a.n_tiles * a.splits), S::kThreads, S::kLds, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
     return MI355X_OK;
+}
+
+int launch_large(mi355x_ctx *ctx, MatmulArgs a) {
+    a.m_tiles = (a.m + kLarge - 1) / kLarge;
+    a.n_tiles = (a.n + kLarge - 1) / kLarge;
+    const int groups = std::min(a.m_tiles * a.n_tiles, ctx->num_cus);
+    matmul_large_kernel<<<groups, kLargeThreads, kLargeLds, ctx->stream>>>(a);
+    MI355X_HIP(hipGetLastError());
+    return MI355X_OK;
+}
+
+// Tiles, and the time that a workgroup takes for a stage of k where it has a CU for
+// itself and where `per_cu` share one (us; from calls of 128 to 8192 rows).
+struct Form {
+    int bm, bn, per_cu, most_splits;
+    float alone, shared;
+};
+constexpr Form kForms[] = {
+    {64, 64, 2, 8, 0.37f, 0.55f},
+    {128, 128, 1, 8, 0.70f, 0.70f},
+    {256, 128, 1, 8, 1.08f, 1.08f},
+    {kLarge, kLarge, 1, 1, 1.65f, 1.65f},
+};
+
+// The form and the split of k with the least estimated time: the launch, rounds of
+// workgroups (three stages more for a tile's begin and end), and for a split the sums
+// that go out and come back.  us, estimated and measured, of the forms in order
+// (split): 512 x 4096, k 14336: 67 (1), 54 (2), 52 (4), 194; 67, 47, 49, 156.  256 x 8192,
+// k 8192: 41 (1), 37 (2), 44 (4), 115; 41, 32, 38, 92.  1024 x 4096, k 4096: 43, 29, 42, 62;
+// 40, 27, 38, 52.  512 x 17408, k 5120: 122, 94, 97, 75; 116, 97, 99, 70.  128 x 4096, k 4096:
+// 17 (2), 27 (4); 12, 18.
+struct Choice {
+    int form, splits;
+};
+Choice choose(const mi355x_ctx *ctx, const MatmulArgs &a) {
+    const int stages = stages_of(a);
+    Choice best{0, 1};
+    float least = 1e30f;
+    for (int f = 0; f < 4; ++f) {
+        const Form &g = kForms[f];
+        if (g.bm == kLarge && g.bn == kLarge && (a.m < kLarge || a.n < kLarge)) continue;
+        const int64_t tiles = static_cast<int64_t>((a.m + g.bm - 1) / g.bm) * ((a.n + g.bn - 1) / g.bn);
+        for (int s = 1; s <= g.most_splits && s <= stages; ++s) {
+            const int64_t groups = tiles * s, part_bytes = groups * g.bm * g.bn * 4;
+            if (s > 1 && (tiles > static_cast<int64_t>(kCounters / 4) || part_bytes > static_cast<int64_t>(kPartBytes))) break;
+            const float rounds = std::ceil(static_cast<float>(groups) / static_cast<float>(ctx->num_cus * g.per_cu));
+            float us = 4.0f + rounds * (groups <= ctx->num_cus ? g.alone : g.shared) *
+                                  static_cast<float>((stages + s - 1) / s + 3);
+            if (s > 1) us += 3.0f + 2.0f * static_cast<float>(part_bytes) / 6.0e6f;
+            if (us < least) {
+                least = us;
+                best = {f, s};
+            }
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -340,15 +688,24 @@ int launch_matmul_q8(mi355x_ctx *ctx, const mi355x_matmul_q8_args &u) {
     a.n = static_cast<int>(u.n_out);
     a.k = static_cast<int>(u.k);
     a.out_type = u.out_type;
-    const int64_t four = u.out_type == MI355X_TYPE_F32 ? 16 : 8;
-    a.wide = reinterpret_cast<uintptr_t>(u.out) % four == 0 && u.out_stride % 4 == 0;
-    if (a.m <= 16) return a.n > 8192 ? launch_few<1, 2>(ctx, a) : launch_few<1, 1>(ctx, a);
-    if (a.m <= 32) return launch_few<2, 2>(ctx, a);
-    if (a.m <= 48) return launch_few<3, 2>(ctx, a);
-    if (a.m <= 64) return launch_few<4, 2>(ctx, a);
-    const int64_t large = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + 255) / 256);
-    if (large >= ctx->num_cus) return launch_tiles<256, 256, 2, 4>(ctx, a);
-    return launch_tiles<128, 128, 2, 2>(ctx, a);
+    // the tile kernels form offsets of up to 256 rows in 32 bits, and a grid's second side has 16
+    const bool far = u.x_stride > (1 << 23) || u.w_stride > (1 << 23);
+    if (static_cast<int64_t>(a.m) * a.n >= int64_t(1) << 34)
+        return set_error(MI355X_EUNSUPPORTED, "mi355x_matmul_q8: 2^34 outputs or more");
+    if (far && a.m > 64 * 65535)
+        return set_error(MI355X_EUNSUPPORTED, "mi355x_matmul_q8: more than 64 * 65535 rows with strides past 2^23");
+    const bool many = a.n >= 32 * ctx->num_cus;
+    if (a.m <= 16) return many ? launch_few<1, 2, 4, 3>(ctx, a) : launch_few<1, 1, 4, 4>(ctx, a);
+    if (a.m <= 32) return many ? launch_few<2, 2, 4, 2>(ctx, a) : launch_few<2, 1, 8, 2>(ctx, a);
+    if (a.m <= 48 && many) return launch_few<3, 3, 2, 3>(ctx, a);
+    if ((a.m <= 64 && many) || far) return launch_few<4, 3, 2, 2>(ctx, a);
+    const Choice c = choose(ctx, a);
+    switch (c.form) {
+    case 0: return launch_tiles<64, 64, 4, 2, 4>(ctx, a, c.splits);
+    case 1: return launch_tiles<128, 128, 2, 4, 4>(ctx, a, c.splits);
+    case 2: return launch_tiles<256, 128, 2, 4, 3>(ctx, a, c.splits);
+    default: return launch_large(ctx, a);
+    }
 }
 
 }  // namespace mi355x
