@@ -50,23 +50,6 @@ struct LogitArgs {
 // The larger logit first, of equal ones the lower token.
 __device__ __forceinline__ bool before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
-__device__ __forceinline__ float wave_max(float v) {
-    // lanes that no move writes read -inf: the identity
-    const int none = __builtin_bit_cast(int, -INFINITY);
-    auto mov = [&](auto ctrl, auto mask) {
-        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(none, __builtin_bit_cast(int, v), decltype(ctrl)::value,
-                                                                     decltype(mask)::value, 0xF, false));
-    };
-    typedef std::integral_constant<int, 0xF> All;
-    v = fmaxf(v, mov(std::integral_constant<int, 0xB1>{}, All{}));
-    v = fmaxf(v, mov(std::integral_constant<int, 0x4E>{}, All{}));
-    v = fmaxf(v, mov(std::integral_constant<int, 0x141>{}, All{}));
-    v = fmaxf(v, mov(std::integral_constant<int, 0x140>{}, All{}));
-    v = fmaxf(v, mov(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{}));
-    v = fmaxf(v, mov(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{}));
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
-
 // A bound from below, at least -FLT_MAX and 2^-11 of itself or less off, of the n-th
 // largest of the 64 * N numbers that a wavefront's lanes hold: the 20 highest bits of
 // it, found one by one.

@@ -111,19 +111,21 @@ __device__ __forceinline__ void norm_values(const RowArgs &a, int64_t row, int i
     }
 }
 
+__device__ __forceinline__ double gated(float g, float u) {
+    const double d = g;
+    return d / (1.0 + exp(-d)) * static_cast<double>(u);
+}
+
 __device__ __forceinline__ void swiglu_values(const RowArgs &a, int64_t row, int i, double *t) {
     float g[8], u[8];
     load_as_float(row_at(a.x, a.type, row * a.x_stride), a.type, i, a.n, g);
     load_as_float(row_at(a.y, a.type, row * a.y_stride), a.type, i, a.n, u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const double d = g[j];
-        t[j] = d / (1.0 + exp(-d)) * static_cast<double>(u[j]);
-    }
+    for (int j = 0; j < 8; ++j) t[j] = gated(g[j], u[j]);
 }
 
-// A workgroup per row, the row's values formed twice: for the largest, and for
-// the codes.
+// Rows longer than a workgroup's registers: the values formed twice, for the largest
+// and for the codes.
 template <bool GATED>
 __global__ __launch_bounds__(64 * kMostWaves) void row_q8_kernel(RowArgs a) {
     __shared__ double lds[2][kMostWaves][2];
@@ -163,13 +165,329 @@ __global__ __launch_bounds__(64 * kMostWaves) void row_q8_kernel(RowArgs a) {
     }
 }
 
+// ---- rows held in registers ------------------------------------------------------
+
+// A thread has CHUNKS runs of 8 values, so rows of up to 8 * CHUNKS * threads values
+// are read once.
+constexpr int kMostChunks = 4;
+constexpr int kMostHeld = 8 * kMostChunks * 64 * kMostWaves;
+
+template <int TYPE, int CHUNKS>
+__device__ __forceinline__ void load_row(const void *p, int n, typename RowElem<TYPE>::Raw8 *r) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) r[c] = row_load8<TYPE>(p, 8 * (c * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)), n);
+}
+
+// Codes, a byte each, of t * unit with `unit` next to 127 / most: 1.5 * 2^23 is added in
+// the multiplication's own rounding, which leaves the nearest whole number in the low
+// bits.  A bit of *doubt is set for each product nearer than `error` to a border.
+__device__ __forceinline__ uint64_t pack_codes(const float *t, float unit, float error, uint32_t *doubt) {
+    constexpr float kWhole = 12582912.0f;
+    float z[8], worst = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        z[j] = fmaf(t[j], unit, kWhole);
+        worst = fmaxf(worst, fabsf(fmaf(t[j], unit, kWhole - z[j])));
+    }
+    uint32_t c[2];
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+        auto bits = [&](int j) { return __builtin_bit_cast(uint32_t, z[4 * d + j]); };
+        // the low bytes of two, and of two such pairs
+        const uint32_t lo = __builtin_amdgcn_perm(bits(1), bits(0), 0x0C0C0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(bits(3), bits(2), 0x0C0C0400u);
+        c[d] = lo | hi << 16;
+    }
+    *doubt = 0;
+    if (worst >= 0.5f - error)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *doubt |= fabsf(fmaf(t[j], unit, kWhole - z[j])) >= 0.5f - error ? 1u << j : 0u;
+    return c[0] | static_cast<uint64_t>(c[1]) << 32;
+}
+
+// The codes with those in doubt from exact(j).
+template <class F>
+__device__ __forceinline__ uint64_t settle_codes(uint64_t codes, uint32_t doubt, F exact) {
+    while (doubt) {
+        const int j = __builtin_ctz(doubt);
+        doubt &= doubt - 1;
+        const uint64_t code = static_cast<uint64_t>(exact(j) & 255) << (8 * j);
+        codes = (codes & ~(uint64_t(255) << (8 * j))) | code;
+    }
+    return codes;
+}
+
+// Value i of a row, read again.
+__device__ __forceinline__ float value_at(const void *p, int type, int64_t i) {
+    if (type == MI355X_TYPE_F32) return static_cast<const float *>(p)[i];
+    if (type == MI355X_TYPE_F16) return static_cast<float>(static_cast<const _Float16 *>(p)[i]);
+    return static_cast<float>(static_cast<const __bf16 *>(p)[i]);
+}
+
+// Largest magnitudes that leave f32's range neither way when 127 is divided by them.
+__device__ __forceinline__ bool in_range(double most) { return most > 0x1p-60 && most < 0x1p100; }
+
+template <int XT, int RT, int CHUNKS>
+__global__ __launch_bounds__(64 * kMostWaves) void norm_rows_kernel(RowArgs a) {
+    constexpr bool kResidual = RT >= 0;
+    constexpr int kRes = kResidual ? RT : MI355X_TYPE_F32;
+    typedef typename RowElem<kRes>::T ResT;
+    __shared__ double lds[2][kMostWaves][2];
+    const int first = 8 * threadIdx.x, step = 8 * blockDim.x;
+    float w[CHUNKS][8];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int i = first + c * step;
+        if (a.norm) {
+            const auto r = row_load8<MI355X_TYPE_F32>(a.norm, i, a.n);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[c][j] = r[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[c][j] = 1.0f;
+        }
+    }
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x, turn ^= 1) {
+        float h[CHUNKS][8];
+        {
+            typename RowElem<XT>::Raw8 x[CHUNKS];
+            typename RowElem<kRes>::Raw8 r[CHUNKS];
+            load_row<XT, CHUNKS>(row_at(a.x, XT, row * a.x_stride), a.n, x);
+            if (kResidual) load_row<kRes, CHUNKS>(row_at(a.y, kRes, row * a.y_stride), a.n, r);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    h[c][j] = static_cast<float>(x[c][j]);
+                    if (kResidual) {
+                        r[c][j] = static_cast<ResT>(h[c][j] + static_cast<float>(r[c][j]));
+                        h[c][j] = static_cast<float>(r[c][j]);
+                    }
+                }
+                if (kResidual && a.y_out)
+                    row_store8<kRes>(const_cast<void *>(row_at(a.y_out, kRes, row * a.y_out_stride)), first + c * step,
+                                     a.n, r[c]);
+            }
+        }
+        double sum = 0.0, most = 0.0;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const double d = h[c][j], t = d * static_cast<double>(w[c][j]);
+                sum = fma(d, d, sum);
+                sum = fma(t, 0.0, sum);  // NaN where t is not finite
+                most = fmax(most, fabs(t));
+            }
+        group_sum_max(&sum, &most, lds[turn]);
+        const bool bad = !(fabs(sum) <= 1.7976931348623157e308), zero = bad || most == 0.0;
+        const double unit = zero ? 0.0 : 127.0 / most;
+        if (threadIdx.x == 0) {
+            double scale = most / 127.0;
+            if (a.norm) scale = most / sqrt(sum / a.n + static_cast<double>(a.eps)) / 127.0;
+            a.scales[row] = bad ? __builtin_nanf("") : most == 0.0 ? 0.0f : static_cast<float>(scale);
+        }
+        int8_t *q = a.q + row * a.q_stride;
+        // h w and the unit are off by half a step each, 2^-23 of 127 together; outside f32's
+        // range every code is formed in 64 bits
+        const bool near = in_range(most);
+        const float unit32 = near && !bad ? static_cast<float>(unit) : 0.0f, error = near || zero ? 5e-5f : 1.0f;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int i = first + c * step;
+            if (i >= a.n) break;
+            float t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = near && !bad ? h[c][j] * w[c][j] : 0.0f;
+            uint32_t doubt;
+            uint64_t codes = pack_codes(t, unit32, error, &doubt);
+            codes = settle_codes(codes, doubt, [&](int j) {
+                if (i + j >= a.n) return 0;
+                float again;
+                if (kResidual && a.y_out) {
+                    again = value_at(a.y_out, kRes, row * a.y_out_stride + i + j);
+                } else {
+                    again = value_at(a.x, XT, row * a.x_stride + i + j);
+                    if (kResidual)
+                        again = static_cast<float>(static_cast<ResT>(again + value_at(a.y, kRes, row * a.y_stride + i + j)));
+                }
+                const double t = static_cast<double>(again) * (a.norm ? static_cast<double>(a.norm[i + j]) : 1.0);
+                return code_of(t, most, unit);
+            });
+            row_store_codes(q, i, a.n, static_cast<uint32_t>(codes), static_cast<uint32_t>(codes >> 32));
+        }
+    }
+}
+
+// The same in f32: the exponent -g log2 e as a sum of two numbers, so that 2^it is off
+// by 2 units of 2^-24 and not by |g| of them; the sum, its inverse and two products
+// make 8 at most.  A gate below -80 or a result past f32's range says nothing.
+constexpr float kGateError = 0x1p-20f;
+__device__ __forceinline__ float gated32(float g, float u) {
+    const float hi = g * -1.44269504088896341f;
+    const float lo = fmaf(g, -1.44269504088896341f, -hi) + g * -1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return g * __builtin_amdgcn_rcpf(1.0f + fmaf(e, lo * 0.693147181f, e)) * u;
+}
+
+template <int TYPE, int CHUNKS>
+__global__ __launch_bounds__(64 * kMostWaves) void swiglu_rows_kernel(RowArgs a) {
+    __shared__ double lds[kMostWaves][2];
+    __shared__ float tops[2][kMostWaves];
+    __shared__ unsigned long long largest[2];  // bits of a number that is not negative
+    const int first = 8 * threadIdx.x, step = 8 * blockDim.x, waves = (blockDim.x + 63) >> 6;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x, turn ^= 1) {
+        auto exact = [&](int i) {
+            if (i >= a.n) return 0.0;
+            return gated(value_at(a.x, TYPE, row * a.x_stride + i), value_at(a.y, TYPE, row * a.y_stride + i));
+        };
+        float t[CHUNKS][8], top = 0.0f, low = 0.0f, odd = 0.0f;
+        {
+            typename RowElem<TYPE>::Raw8 g[CHUNKS], u[CHUNKS];
+            load_row<TYPE, CHUNKS>(row_at(a.x, TYPE, row * a.x_stride), a.n, g);
+            load_row<TYPE, CHUNKS>(row_at(a.y, TYPE, row * a.y_stride), a.n, u);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float x = static_cast<float>(g[c][j]);
+                    t[c][j] = gated32(x, static_cast<float>(u[c][j]));
+                    low = fminf(low, x);
+                    top = fmaxf(top, fabsf(t[c][j]));
+                    odd = fmaf(t[c][j], 0.0f, odd);  // NaN where t is not finite
+                }
+        }
+        // the row's largest in f32, infinite where f32 will not do
+        const float wave_top = wave_max(low >= -80.0f && odd == 0.0f ? top : INFINITY);
+        if ((threadIdx.x & 63) == 0) tops[turn][threadIdx.x >> 6] = wave_top;
+        if (threadIdx.x == 0) largest[turn] = 0;
+        __syncthreads();
+        float all = 0.0f;
+        for (int w = 0; w < waves; ++w) all = fmaxf(all, tops[turn][w]);
+        uint64_t codes[CHUNKS];
+        uint32_t doubt[CHUNKS];
+        double most, unit;
+        if (in_range(all)) {
+            // the value or two of the row that its largest may be, in 64 bits
+            const float at_least = all * (1.0f - 4.0f * kGateError);
+            if (top >= at_least)
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) {
+                    uint32_t left = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) left |= fabsf(t[c][j]) >= at_least ? 1u << j : 0u;
+                    while (left) {
+                        const double x = fabs(exact(first + c * step + __builtin_ctz(left)));
+                        left &= left - 1;
+                        atomicMax(&largest[turn], __builtin_bit_cast(unsigned long long, x));
+                    }
+                }
+            // meanwhile the codes by the f32 one: both are off by kGateError at most
+            const float unit32 = 127.0f / all;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) codes[c] = pack_codes(t[c], unit32, 128.0f * 2.5f * kGateError, &doubt[c]);
+            __syncthreads();
+            most = __builtin_bit_cast(double, largest[turn]);
+            unit = 127.0 / most;
+            if (threadIdx.x == 0) a.scales[row] = static_cast<float>(most / 127.0);
+        } else {
+            double sum = most = 0.0;
+            for (int i = first; i < a.n; i += step)
+                for (int j = 0; j < 8; ++j) {
+                    const double x = exact(i + j);
+                    most = fmax(most, fabs(x));
+                    sum = fma(x, 0.0, sum);  // NaN where x is not finite
+                }
+            group_sum_max(&sum, &most, lds);
+            __syncthreads();  // lds
+            const bool bad = !(fabs(sum) <= 1.7976931348623157e308), zero = bad || most == 0.0;
+            unit = zero ? 0.0 : 127.0 / most;
+            if (threadIdx.x == 0) a.scales[row] = bad ? __builtin_nanf("") : static_cast<float>(most / 127.0);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                codes[c] = 0;
+                doubt[c] = zero ? 0 : 255;
+            }
+        }
+        int8_t *q = a.q + row * a.q_stride;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int i = first + c * step;
+            if (i >= a.n) break;
+            codes[c] = settle_codes(codes[c], doubt[c], [&](int j) { return code_of(exact(i + j), most, unit); });
+            row_store_codes(q, i, a.n, static_cast<uint32_t>(codes[c]), static_cast<uint32_t>(codes[c] >> 32));
+        }
+    }
+}
+
+// ---- launches ------------------------------------------------------------------
+
+// Threads, and runs of 8 values of each: as many threads as there are runs for few
+// rows, so that a row's latency is short (one row of 8192 4.2 us, with 4 runs a thread
+// 5.6); 256 or more with up to 4 runs each for many, so that fewer threads meet at a
+// row's barriers (8192 rows of 8192, one run a thread 117 us, 4 runs 91; without a
+// residual 105, 48; 4096 gated rows of 14336 96, 80; rows of 2048 25, 32).
+struct RowShape {
+    int threads, chunks;
+};
+RowShape row_shape(const mi355x_ctx *ctx, const RowArgs &a) {
+    const int runs = (a.n + 7) / 8, most = 64 * kMostWaves;
+    const int least = (runs + most - 1) / most;
+    const int wanted = a.n_rows >= 4 * ctx->num_cus ? 4 : a.n_rows >= ctx->num_cus ? 2 : 1;
+    int chunks = std::max(least, std::min(wanted, runs / 256));
+    chunks = chunks <= 1 ? 1 : chunks <= 2 ? 2 : 4;
+    return {std::min(most, ((runs + chunks - 1) / chunks + 63) / 64 * 64), chunks};
+}
+
+template <class F>
+int by_chunks(int chunks, F f) {
+    if (chunks == 1) return f(std::integral_constant<int, 1>{});
+    if (chunks == 2) return f(std::integral_constant<int, 2>{});
+    return f(std::integral_constant<int, 4>{});
+}
+
+unsigned row_groups(const RowArgs &a) { return static_cast<unsigned>(std::min<int64_t>(a.n_rows, 1 << 20)); }
+
 template <bool GATED>
-int launch_rows(mi355x_ctx *ctx, const RowArgs &a) {
-    const int threads = std::min(64 * kMostWaves, (a.n + 511) / 512 * 64);
-    const int64_t groups = std::min<int64_t>(a.n_rows, 1 << 20);
-    row_q8_kernel<GATED><<<static_cast<unsigned>(groups), threads, 0, ctx->stream>>>(a);
+int launch_long(mi355x_ctx *ctx, const RowArgs &a) {
+    row_q8_kernel<GATED><<<row_groups(a), 64 * kMostWaves, 0, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
     return MI355X_OK;
+}
+
+template <int XT, int RT>
+int launch_norm(mi355x_ctx *ctx, const RowArgs &a) {
+    const RowShape s = row_shape(ctx, a);
+    unsigned groups = row_groups(a);
+    if (s.chunks > 1) {  // workgroups keep the norm's weights over several rows (8192 rows of 8192: 91 us, 95 without)
+        const int64_t per = (a.n_rows + 8 * ctx->num_cus - 1) / (8 * ctx->num_cus);
+        groups = static_cast<unsigned>(std::min<int64_t>(groups, (a.n_rows + per - 1) / per));
+    }
+    return by_chunks(s.chunks, [&](auto c) {
+        norm_rows_kernel<XT, RT, decltype(c)::value><<<groups, s.threads, 0, ctx->stream>>>(a);
+        MI355X_HIP(hipGetLastError());
+        return MI355X_OK;
+    });
+}
+
+template <int XT>
+int launch_norm_of(mi355x_ctx *ctx, const RowArgs &a) {
+    if (!a.y) return launch_norm<XT, -1>(ctx, a);
+    if (a.residual_type == MI355X_TYPE_F32) return launch_norm<XT, MI355X_TYPE_F32>(ctx, a);
+    if (a.residual_type == MI355X_TYPE_F16) return launch_norm<XT, MI355X_TYPE_F16>(ctx, a);
+    return launch_norm<XT, MI355X_TYPE_BF16>(ctx, a);
+}
+
+template <int TYPE>
+int launch_swiglu(mi355x_ctx *ctx, const RowArgs &a) {
+    const RowShape s = row_shape(ctx, a);
+    return by_chunks(s.chunks, [&](auto c) {
+        swiglu_rows_kernel<TYPE, decltype(c)::value><<<row_groups(a), s.threads, 0, ctx->stream>>>(a);
+        MI355X_HIP(hipGetLastError());
+        return MI355X_OK;
+    });
 }
 
 }  // namespace
@@ -191,7 +509,10 @@ int launch_norm_q8(mi355x_ctx *ctx, const mi355x_norm_q8_args &u) {
     a.q = u.q;
     a.q_stride = u.q_stride;
     a.scales = u.scales;
-    return launch_rows<false>(ctx, a);
+    if (a.n > kMostHeld) return launch_long<false>(ctx, a);
+    if (a.type == MI355X_TYPE_F32) return launch_norm_of<MI355X_TYPE_F32>(ctx, a);
+    if (a.type == MI355X_TYPE_F16) return launch_norm_of<MI355X_TYPE_F16>(ctx, a);
+    return launch_norm_of<MI355X_TYPE_BF16>(ctx, a);
 }
 
 int launch_swiglu_q8(mi355x_ctx *ctx, const mi355x_swiglu_q8_args &u) {
@@ -206,7 +527,10 @@ int launch_swiglu_q8(mi355x_ctx *ctx, const mi355x_swiglu_q8_args &u) {
     a.q = u.q;
     a.q_stride = u.q_stride;
     a.scales = u.scales;
-    return launch_rows<true>(ctx, a);
+    if (a.n > kMostHeld) return launch_long<true>(ctx, a);
+    if (a.type == MI355X_TYPE_F32) return launch_swiglu<MI355X_TYPE_F32>(ctx, a);
+    if (a.type == MI355X_TYPE_F16) return launch_swiglu<MI355X_TYPE_F16>(ctx, a);
+    return launch_swiglu<MI355X_TYPE_BF16>(ctx, a);
 }
 
 }  // namespace mi355x

@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "device_common.h"
 #include "mi355x-attention.h"
 
@@ -106,6 +108,25 @@ __device__ __forceinline__ double wave_max64(double v) {
     v = fmax(v, dpp_mov64<0x142, 0xA>(v));
     v = fmax(v, dpp_mov64<0x143, 0xC>(v));
     return last_lane64(v);
+}
+
+// Largest over a wavefront whose lanes are all active (NaN does not count); the same in
+// every lane.
+__device__ __forceinline__ float wave_max(float v) {
+    // lanes that no move writes read -inf: the identity
+    const int none = __builtin_bit_cast(int, -INFINITY);
+    auto mov = [&](auto ctrl, auto mask) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(none, __builtin_bit_cast(int, v), decltype(ctrl)::value,
+                                                                     decltype(mask)::value, 0xF, false));
+    };
+    typedef std::integral_constant<int, 0xF> All;
+    v = fmaxf(v, mov(std::integral_constant<int, 0xB1>{}, All{}));
+    v = fmaxf(v, mov(std::integral_constant<int, 0x4E>{}, All{}));
+    v = fmaxf(v, mov(std::integral_constant<int, 0x141>{}, All{}));
+    v = fmaxf(v, mov(std::integral_constant<int, 0x140>{}, All{}));
+    v = fmaxf(v, mov(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{}));
+    v = fmaxf(v, mov(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{}));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 }  // namespace mi355x
