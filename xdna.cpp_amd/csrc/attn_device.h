@@ -38,7 +38,6 @@ struct AttnArgs {
 constexpr float kLog2e = 1.44269504088896341f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x2_a __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // The pool's 16-bit type: matrix products, roundings, the bits of its exponent

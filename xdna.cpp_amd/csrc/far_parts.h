@@ -9,6 +9,7 @@
 namespace mi355x {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_a __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_a __attribute__((ext_vector_type(4)));
 
 // Parts of a row's sums that travel between workgroups of one launch, whose dies'
@@ -26,6 +27,12 @@ struct FarParts {
     }
     __device__ __forceinline__ void store4(int at, f32x4 v) const {
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_a, v), rsrc, 4 * at, 0, kPastL2);
+    }
+    __device__ __forceinline__ void store2(int at, u32x2_a v) const {
+        __builtin_amdgcn_raw_buffer_store_b64(v, rsrc, 4 * at, 0, kPastL2);
+    }
+    __device__ __forceinline__ u32x2_a load2(int at) const {
+        return __builtin_bit_cast(u32x2_a, __builtin_amdgcn_raw_buffer_load_b64(rsrc, 4 * at, 0, kPastL2));
     }
     __device__ __forceinline__ float load(int at) const {
         return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, 4 * at, 0, kPastL2));

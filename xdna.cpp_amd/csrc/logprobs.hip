@@ -39,7 +39,7 @@ struct LogitArgs {
     const void *logits;
     int n_vocab, n_tokens, n_top;
     float scale;
-    int parts, part_len;  // of a row; part_len is a multiple of 8
+    int parts, part_len;  // of a row; part_len is a multiple of kStep
     const int32_t *tokens;
     float *token_logprobs, *entropy, *top_logprobs;
     int32_t *top_tokens;
@@ -47,31 +47,40 @@ struct LogitArgs {
     float *ws;
 };
 
-// The larger logit first, of equal ones the lower token.
-__device__ __forceinline__ bool before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
-
-// A bound from below, at least -FLT_MAX and 2^-11 of itself or less off, of the n-th
-// largest of the 64 * N numbers that a wavefront's lanes hold: the 20 highest bits of
-// it, found one by one.
-template <int N>
-__device__ __forceinline__ float nth_largest(const float *v, int n) {
-    uint32_t key[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, v[i] + 0.0f);  // no zero with a sign
-        key[i] = b & 0x80000000u ? ~b : b | 0x80000000u;               // in the order of the numbers
-    }
-    uint32_t found = 0;
-    for (int bit = 31; bit >= 12; --bit) {
-        const uint32_t tried = found | 1u << bit;
-        int above = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) above += __builtin_popcountll(__ballot(key[i] >= tried));
-        if (above >= n) found = tried;
-    }
-    const uint32_t b = found & 0x80000000u ? found & 0x7FFFFFFFu : ~found;
-    return fmaxf(__builtin_bit_cast(float, b), -FLT_MAX);  // below -inf lie NaN patterns
+// Numbers in the order of the logits (zeros have no sign), and of entries of a list:
+// the larger logit, of equal ones the lower token, has the larger one.
+__device__ __forceinline__ uint32_t rank_of(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float logit_of(uint32_t rank) {
+    return __builtin_bit_cast(float, rank & 0x80000000u ? rank & 0x7FFFFFFFu : ~rank);
+}
+__device__ __forceinline__ uint64_t entry_of(float x, int at) {
+    return static_cast<uint64_t>(rank_of(x)) << 32 | static_cast<uint32_t>(~at);
+}
+constexpr uint64_t kNoEntry = 0;  // below every entry
+
+// A bound from below, 2^-7 of itself or less off, of the n-th largest of the 64 * N
+// numbers that a wavefront's lanes hold: the 16 highest bits of its rank, found two by
+// two.
+template <int N>
+__device__ __forceinline__ uint32_t nth_largest(const uint32_t *rank, int n) {
+    uint32_t found = 0;
+    for (int bit = 30; bit >= 16; bit -= 2) {
+        int above[4];
+#pragma unroll
+        for (int t = 1; t < 4; ++t) {
+            above[t] = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) above[t] += __builtin_popcountll(__ballot(rank[i] >= (found | static_cast<uint32_t>(t) << bit)));
+        }
+        found |= (above[3] >= n ? 3u : above[2] >= n ? 2u : above[1] >= n ? 1u : 0u) << bit;
+    }
+    return found;
+}
+// The logit of such a bound, but at least -FLT_MAX (below -inf lie NaN patterns).
+__device__ __forceinline__ float bound_of(uint32_t rank) { return fmaxf(logit_of(rank), -FLT_MAX); }
 
 // Sums against the largest logit so far, `high` (0 stands for it while it is -inf).
 struct Sums {
@@ -94,10 +103,9 @@ struct Sums {
 };
 
 struct Lds {
-    float list[kList];
-    int list_at[kList];
-    float best[kList];
-    int best_at[kList];
+    uint64_t list[kList], best[kList];
+    uint64_t top[MI355X_LOGPROBS_MAX_TOP];  // the top tokens in order
+    int rank[64];
     float tops[2][kThreads];
     float sums[kWaves][2];
     int count, best_count, flag;
@@ -117,39 +125,51 @@ __device__ __forceinline__ void to_float(typename RowElem<TYPE>::Raw8 r, int i, 
 
 __device__ __forceinline__ void put(Lds &l, float x, int at) {
     const int p = atomicAdd(&l.count, 1);
-    if (p < kList) {
-        l.list[p] = x;
-        l.list_at[p] = at;
-    }
+    if (p < kList) l.list[p] = entry_of(x, at);
 }
 
-// The n top entries of the `count` ones in l.list that are not below `bound`, in
-// order, to l.best; how many there are.  Called by all threads, with the list
-// complete.
-__device__ __forceinline__ int order_list(Lds &l, int count, float bound, int n) {
-    const int tid = threadIdx.x;
-    if (tid == 0) l.best_count = 0;
-    __syncthreads();
-    for (int p = tid; p < count; p += kThreads)
-        if (l.list[p] >= bound) {
-            const int q = atomicAdd(&l.best_count, 1);
-            l.best[q] = l.list[p];
-            l.best_at[q] = l.list_at[p];
-        }
-    __syncthreads();
-    const int m = l.best_count;
-    for (int p = tid; p < m; p += kThreads) {
-        const float x = l.best[p];
-        const int at = l.best_at[p];
+// The n first of `m` entries, in order, to l.top.  Up to 64 entries: each wavefront
+// counts, for all of them, those of every kWaves-th that come before (l.rank is 0), and
+// some may be none.
+__device__ __forceinline__ int order(Lds &l, const uint64_t *list, int m, int n) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (m <= 64) {
+        const uint64_t x = lane < m ? list[lane] : kNoEntry;
+        const int real = __builtin_popcountll(__ballot(x != kNoEntry));
         int r = 0;
-        for (int q = 0; q < m; ++q) r += before(l.best[q], l.best_at[q], x, at);
-        if (r < n) {
-            l.list[r] = x;
-            l.list_at[r] = at;
+#pragma unroll 4
+        for (int q = wave; q < m; q += kWaves) r += list[q] > x;
+        if (lane < m && r) atomicAdd(&l.rank[lane], r);
+        __syncthreads();
+        if (tid < m && l.rank[tid] < n) l.top[l.rank[tid]] = x;
+        m = real;
+    } else {
+        for (int p = tid; p < m; p += kThreads) {
+            const uint64_t x = list[p];
+            int r = 0;
+#pragma unroll 8
+            for (int q = 0; q < m; ++q) r += list[q] > x;
+            if (r < n) l.top[r] = x;
         }
     }
     __syncthreads();
     return min(m, n);
+}
+
+// The n first of the `count` entries of l.list, none of which has a rank below `bound()`.
+// Called by all threads, with the list complete.
+template <class F>
+__device__ __forceinline__ int order_list(Lds &l, int count, int n, F bound) {
+    if (count <= 64) return order(l, l.list, count, n);
+    const uint32_t least = bound();
+    if (threadIdx.x == 0) l.best_count = 0;
+    __syncthreads();
+    for (int p = threadIdx.x; p < count; p += kThreads) {
+        const uint64_t x = l.list[p];
+        if (x != kNoEntry && x >> 32 >= least) l.best[atomicAdd(&l.best_count, 1)] = x;
+    }
+    __syncthreads();
+    return order(l, l.best, l.best_count, n);
 }
 
 // The same by n searches of the row.
@@ -158,41 +178,29 @@ __device__ int search(Lds &l, const void *row, int lo, int hi, int n) {
     typedef typename RowElem<TYPE>::T T;
     const T *p = static_cast<const T *>(row);
     const int tid = threadIdx.x;
-    float last = INFINITY;
-    int last_at = -1, r = 0;
+    uint64_t last = ~uint64_t(0);
+    int r = 0;
     for (; r < n; ++r) {
-        float x = -INFINITY;
-        int at = INT_MAX;
+        uint64_t x = kNoEntry;
         for (int i = lo + tid; i < hi; i += kThreads) {
             const float v = static_cast<float>(p[i]);
-            if (v > -INFINITY && before(last, last_at, v, i) && before(v, i, x, at)) {
-                x = v;
-                at = i;
-            }
+            const uint64_t e = entry_of(v, i);
+            if (v > -INFINITY && e < last && e > x) x = e;
         }
         __syncthreads();
         l.best[tid] = x;
-        l.best_at[tid] = at;
         __syncthreads();
-        for (int t = 0; t < kThreads; ++t)
-            if (before(l.best[t], l.best_at[t], x, at)) {
-                x = l.best[t];
-                at = l.best_at[t];
-            }
-        if (at == INT_MAX) break;
-        if (tid == 0) {
-            l.list[r] = x;
-            l.list_at[r] = at;
-        }
+        for (int t = 0; t < kThreads; ++t) x = l.best[t] > x ? l.best[t] : x;
+        if (x == kNoEntry) break;
+        if (tid == 0) l.top[r] = x;
         last = x;
-        last_at = at;
     }
     __syncthreads();
     return r;
 }
 
 // What a row's outputs are made of: its largest logit, the sums against it, and
-// `found` top tokens in l.list.
+// `found` top tokens in l.top.
 template <int TYPE>
 __device__ __forceinline__ void write_row(const LogitArgs &a, int64_t row, const Lds &l, float top, float s, float e,
                                           int found) {
@@ -212,8 +220,9 @@ __device__ __forceinline__ void write_row(const LogitArgs &a, int64_t row, const
     }
     for (int r = tid; r < a.n_top; r += kThreads) {
         const bool in = r < found && !bad;
-        a.top_tokens[row * a.n_top + r] = in ? l.list_at[r] : -1;
-        a.top_logprobs[row * a.n_top + r] = bad ? NAN : in ? a.scale * (l.list[r] - top) - log_total : -INFINITY;
+        a.top_tokens[row * a.n_top + r] = in ? static_cast<int>(~static_cast<uint32_t>(l.top[r])) : -1;
+        a.top_logprobs[row * a.n_top + r] =
+            bad ? NAN : in ? a.scale * (logit_of(static_cast<uint32_t>(l.top[r] >> 32)) - top) - log_total : -INFINITY;
     }
 }
 
@@ -233,22 +242,27 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
         Raw8 raw[kLoads];
         auto load = [&](int base) {
 #pragma unroll
-            for (int c = 0; c < kLoads; ++c) raw[c] = row_load8<TYPE>(logits, base + c * kStep + 8 * tid, hi);
+            for (int c = 0; c < kLoads; ++c)
+                if (base + c * kStep < hi) raw[c] = row_load8<TYPE>(logits, base + c * kStep + 8 * tid, hi);
         };
         load(lo);
         if (tid == 0) l.count = 0;
+        if (tid < 64) l.rank[tid] = 0;
         Sums sums;
         float top = -INFINITY, bound = FLT_MAX;
         int turn = 0, next = 0;  // the bound is formed in batch `next`
-        for (int batch = 0, base = lo; base < hi; base += kBatch, ++batch) {
+        auto step = [&](int batch, int base, auto whole) {
+            constexpr bool kWhole = decltype(whole)::value;  // the batch ends in the part
+            auto in = [&](int c) { return kWhole || base + c * kStep < hi; };
             float x[kLoads][8], most = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < kLoads; ++c) to_float<TYPE>(raw[c], base + c * kStep + 8 * tid, hi, x[c]);
-            if (base + kBatch < hi) load(base + kBatch);
-#pragma unroll
             for (int c = 0; c < kLoads; ++c)
+                if (in(c)) {
+                    to_float<TYPE>(raw[c], kWhole ? INT_MIN : base + c * kStep + 8 * tid, hi, x[c]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) most = fmaxf(most, x[c][j]);
+                    for (int j = 0; j < 8; ++j) most = fmaxf(most, x[c][j]);
+                }
+            if (kWhole) load(base + kBatch);
             top = fmaxf(top, most);
             if (batch == next) {
                 next = max(2, 4 * next);
@@ -258,21 +272,31 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
 #pragma unroll
                 for (int i = 0; i < kWaves; ++i) v[i] = l.tops[turn][64 * i + lane];
                 turn ^= 1;
-                if (n > 0) bound = nth_largest<kWaves>(v, n);
+                if (n > 0) {
+                    uint32_t ranks[kWaves];
+#pragma unroll
+                    for (int i = 0; i < kWaves; ++i) ranks[i] = rank_of(v[i]);
+                    bound = bound_of(nth_largest<kWaves>(ranks, n));
+                }
                 sums.raise(wave_max(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))), k);
             }
             sums.raise(most, k);
 #pragma unroll
             for (int c = 0; c < kLoads; ++c)
+                if (in(c))
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sums.add(x[c][j], k);
+                    for (int j = 0; j < 8; ++j) sums.add(x[c][j], k);
             if (most >= bound)
 #pragma unroll
                 for (int c = 0; c < kLoads; ++c)
+                    if (in(c))
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (x[c][j] >= bound) put(l, x[c][j], base + c * kStep + 8 * tid + j);
-        }
+                        for (int j = 0; j < 8; ++j)
+                            if (x[c][j] >= bound) put(l, x[c][j], base + c * kStep + 8 * tid + j);
+        };
+        int batch = 0, base = lo;
+        for (; base + kBatch <= hi; base += kBatch, ++batch) step(batch, base, std::true_type{});
+        if (base < hi) step(batch, base, std::false_type{});
         // the workgroup's sums, and the n-th largest of what its threads had
         l.tops[turn][tid] = top;
         __syncthreads();
@@ -288,8 +312,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
         }
         int found = 0, count = l.count;
         if (n > 0) {
-            bound = nth_largest<kWaves>(v, n);
+            auto last_bound = [&]() {
+                uint32_t ranks[kWaves];
+#pragma unroll
+                for (int i = 0; i < kWaves; ++i) ranks[i] = rank_of(v[i]);
+                return nth_largest<kWaves>(ranks, n);
+            };
             if (count > kList) {  // once more, with the bound that the whole row gives
+                bound = bound_of(last_bound());
                 __syncthreads();
                 if (tid == 0) l.count = 0;
                 __syncthreads();
@@ -300,7 +330,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
                 __syncthreads();
                 count = l.count;
             }
-            found = count > kList ? search<TYPE>(l, logits, lo, hi, n) : order_list(l, count, bound, n);
+            found = count > kList ? search<TYPE>(l, logits, lo, hi, n) : order_list(l, count, n, last_bound);
         } else {
             __syncthreads();
         }
@@ -316,16 +346,24 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
             const FarParts far(a.ws);
             const int at = static_cast<int>(item) * kPartFloats;
             if (tid == 0) far.store4(at, f32x4{all, s, e, 0.0f});
-            for (int r = tid; r < n; r += kThreads) {
-                far.store(at + 4 + r, r < found ? l.list[r] : -INFINITY);
-                far.store(at + 4 + MI355X_LOGPROBS_MAX_TOP + r,
-                          __builtin_bit_cast(float, r < found ? l.list_at[r] : -1));
-            }
+            for (int r = tid; r < n; r += kThreads)
+                far.store2(at + 4 + 2 * r, __builtin_bit_cast(u32x2_a, r < found ? l.top[r] : kNoEntry));
             if (last_of(a.counters + row, a.parts, &l.flag)) {
-                // the row's parts, one a lane
-                const int first = static_cast<int>(row) * a.parts;
-                f32x4 p = {-INFINITY, 0.0f, 0.0f, 0.0f};
+                const int first = static_cast<int>(row) * a.parts, total = a.parts * n;  // at most kList
+                f32x4 p = {-INFINITY, 0.0f, 0.0f, 0.0f};  // the row's parts, one a lane
                 if (lane < a.parts) p = far.load4((first + lane) * kPartFloats);
+                uint64_t entry[kList / kThreads];  // all on their way before one is waited for
+#pragma unroll
+                for (int i = 0; i < kList / kThreads; ++i) {
+                    const int j = min(i * kThreads + tid, total - 1), q = n > 0 ? j / n : 0;
+                    entry[i] = kNoEntry;
+                    if (i * kThreads < total)
+                        entry[i] = __builtin_bit_cast(uint64_t, far.load2((first + q) * kPartFloats + 4 + 2 * (j - q * n)));
+                }
+#pragma unroll
+                for (int i = 0; i < kList / kThreads; ++i)
+                    if (i * kThreads + tid < total) l.list[i * kThreads + tid] = entry[i];
+                if (tid < 64) l.rank[tid] = 0;
                 const float most = wave_max(p[0]);
                 Sums mine;
                 mine.high = mine.ref = p[0];  // (not used where it is -inf: the sums are 0)
@@ -333,21 +371,19 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
                 mine.e = p[2];
                 mine.raise(most, k);
                 const float ts = wave_sum(mine.s), te = wave_sum(mine.e);
-                if (n > 0) {
-                    const int total = a.parts * n;  // at most kList
-                    for (int j = tid; j < total; j += kThreads) {
-                        const int q = j / n, from = (first + q) * kPartFloats + 4 + j - q * n;
-                        l.list[j] = far.load(from);
-                        l.list_at[j] = __builtin_bit_cast(int, far.load(from + MI355X_LOGPROBS_MAX_TOP));
-                    }
-                    __syncthreads();
-                    float c[kList / 64];
+                __syncthreads();
+                if (n > 0)
+                    found = order_list(l, total, n, [&]() {
+                        // the n-th largest of the first few of each part
+                        const int few = min(n, kThreads / a.parts);
+                        uint32_t ranks[kWaves];
 #pragma unroll
-                    for (int i = 0; i < kList / 64; ++i)
-                        c[i] = 64 * i + lane < total ? l.list[64 * i + lane] : -INFINITY;
-                    bound = nth_largest<kList / 64>(c, n);
-                    found = order_list(l, total, bound, n);
-                }
+                        for (int i = 0; i < kWaves; ++i) {
+                            const int j = 64 * i + lane, q = j / few;
+                            ranks[i] = q < a.parts ? static_cast<uint32_t>(l.list[q * n + j - q * few] >> 32) : 0;
+                        }
+                        return nth_largest<kWaves>(ranks, n);
+                    });
                 write_row<TYPE>(a, row, l, most, ts, te, found);
             }
         }
@@ -389,7 +425,7 @@ int launch_logprobs(mi355x_ctx *ctx, const mi355x_logprobs_args &u) {
     int64_t parts = std::min<int64_t>(kMostItems / u.n_rows, (u.n_vocab + kBatch / 2 - 1) / (kBatch / 2));
     parts = std::min<int64_t>(parts, std::min(kMostParts, kList / std::max(u.n_top, 1)));
     parts = std::max<int64_t>(parts, 1);
-    a.part_len = static_cast<int>((u.n_vocab + 8 * parts - 1) / (8 * parts) * 8);
+    a.part_len = static_cast<int>((u.n_vocab + kStep * parts - 1) / (kStep * parts) * kStep);
     a.parts = static_cast<int>((u.n_vocab + a.part_len - 1) / a.part_len);
     if (u.type == MI355X_TYPE_F32) return launch_type<MI355X_TYPE_F32>(ctx, a);
     if (u.type == MI355X_TYPE_F16) return launch_type<MI355X_TYPE_F16>(ctx, a);
