@@ -11,6 +11,7 @@
 // (16 rows, one chunk) do not meet in a bank.
 #include "far_parts.h"
 #include "internal.h"
+#include "paged_index.h"
 
 #include <algorithm>
 #include <cmath>
@@ -29,6 +30,7 @@ struct MatmulArgs {
     float *ws;
     int m, n, k, out_type;
     int m_tiles, n_tiles, splits, split_stages;
+    FastDiv tiles, band, last_rows;  // m_tiles * n_tiles, 8 * n_tiles, m_tiles % 8 (or 8)
 };
 
 constexpr int kStage = 128;  // bytes of k in a stage: two matrix products deep
@@ -107,6 +109,18 @@ __device__ __forceinline__ void store_row(const MatmulArgs &a, int m, int n, con
     }
 }
 
+// Number n of a vector of `size` (the last one where it is behind it), from a uniform base.
+__device__ __forceinline__ float one_of(const float *p, int n, int size) {
+    const uint32_t at = 4u * static_cast<uint32_t>(min(n, size - 1));
+    return *reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(p) + at);
+}
+// Four of them from n on.
+__device__ __forceinline__ f32x4 four_of(const float *p, int n, int size) {
+    return f32x4{one_of(p, n, size), one_of(p, n + 1, size), one_of(p, n + 2, size), one_of(p, n + 3, size)};
+}
+// A bias's numbers are asked for without a branch, of the scales where there is none.
+__device__ __forceinline__ const float *bias_or_scales(const MatmulArgs &a) { return a.bias ? a.bias : a.w_scales; }
+
 // ---- few rows ------------------------------------------------------------------
 
 // A workgroup computes 16 * R channels of up to 16 * TM rows.  Its WAVES wavefronts
@@ -140,6 +154,10 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_few_kernel(MatmulArgs a) {
                         chunk[i];
         }
     }
+    // the scales of the wavefront's first block of outputs are asked for before the codes
+    const int m_first = m0 + 16 * (wave % TM) + col, n_first = n0 + 16 * (wave / TM) + 4 * quad;
+    float xs = one_of(a.x_scales, m_first, a.m);
+    f32x4 ws = four_of(a.w_scales, n_first, a.n), bias = four_of(bias_or_scales(a), n_first, a.n);
     uint8_t *mine = lds + wave * ST * S::kUnit;
     auto load = [&](int s, int slot) {
         const int k = kStage * s;
@@ -212,14 +230,15 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_few_kernel(MatmulArgs a) {
 #pragma unroll
         for (int v = 1; v < WAVES; ++v) sum += sums[(v * R * TM + b) * 64 + lane];
         const int m = m0 + 16 * (b % TM) + col, n = n0 + 16 * (b / TM) + 4 * quad;
+        if (b != wave) {
+            xs = one_of(a.x_scales, m, a.m);
+            ws = four_of(a.w_scales, n, a.n);
+            bias = four_of(bias_or_scales(a), n, a.n);
+        }
         if (m < a.m && n < a.n) {
-            const float xs = a.x_scales[m];
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int ch = min(n + i, a.n - 1);
-                v[i] = scaled(sum[i], a.w_scales[ch], xs, a.bias != nullptr, a.bias ? a.bias[ch] : 0.0f);
-            }
+            for (int i = 0; i < 4; ++i) v[i] = scaled(sum[i], ws[i], xs, a.bias != nullptr, bias[i]);
             store_row<4>(a, m, n, v);
         }
     }
@@ -233,14 +252,17 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_few_kernel(MatmulArgs a) {
 __device__ __forceinline__ void tile_of(const MatmulArgs &a, int id, int total, int *mt, int *nt, int *split) {
     const int die = id & 7, each = total >> 3, over = total & 7;
     int t = die * each + min(die, over) + (id >> 3);
-    const int tiles = a.m_tiles * a.n_tiles;
-    *split = t / tiles;
-    t -= *split * tiles;
-    const int band = t / (8 * a.n_tiles);
-    const int rows = min(8, a.m_tiles - 8 * band);
-    t -= 8 * band * a.n_tiles;
-    *nt = t / rows;
-    *mt = 8 * band + t - *nt * rows;
+    *split = divided(t, a.tiles);
+    t -= *split * static_cast<int>(a.tiles.d);
+    const int band = divided(t, a.band);
+    t -= band * static_cast<int>(a.band.d);
+    if (8 * band + 8 <= a.m_tiles) {
+        *nt = t >> 3;
+        *mt = 8 * band + (t & 7);
+    } else {
+        *nt = divided(t, a.last_rows);
+        *mt = 8 * band + t - *nt * static_cast<int>(a.last_rows.d);
+    }
 }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const int8_t *p) {
@@ -256,30 +278,39 @@ __device__ __forceinline__ int channel_of(int row, int tn, bool pairs) {
     return pairs ? 32 * (tn >> 1) + 8 * (row >> 2) + 4 * (tn & 1) + (row & 3) : 16 * tn + row;
 }
 
-// The outputs of a wavefront's sums: rows m + 16 j, channels from n on.
+// The scales of a wavefront's outputs: rows m + 16 j, channels from n on.
 template <int TM, int TN>
-__device__ __forceinline__ void write_tile(const MatmulArgs &a, int m, int n, const i32x4 (&c)[TN][TM], int quad) {
-    float ws[TN][4], bias[TN][4];
-    const bool pairs = a.out_type != MI355X_TYPE_F32, has_bias = a.bias != nullptr;
+struct TileScales {
+    f32x4 w[TN], bias[TN];
+    float x[TM];
+    __device__ __forceinline__ TileScales(const MatmulArgs &a, int m, int n, int quad) {
+        const bool pairs = a.out_type != MI355X_TYPE_F32;
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int ch = min(n + channel_of(4 * quad + q, i, pairs), a.n - 1);
-            ws[i][q] = a.w_scales[ch];
-            bias[i][q] = has_bias ? a.bias[ch] : 0.0f;
+        for (int i = 0; i < TN; ++i) {
+            const int ch = n + channel_of(4 * quad, i, pairs);
+            w[i] = four_of(a.w_scales, ch, a.n);
+            bias[i] = four_of(bias_or_scales(a), ch, a.n);
         }
+#pragma unroll
+        for (int j = 0; j < TM; ++j) x[j] = one_of(a.x_scales, m + 16 * j, a.m);
+    }
+};
+
+template <int TM, int TN>
+__device__ __forceinline__ void write_tile(const MatmulArgs &a, int m, int n, const i32x4 (&c)[TN][TM], int quad,
+                                           const TileScales<TM, TN> &scales) {
+    const bool pairs = a.out_type != MI355X_TYPE_F32, has_bias = a.bias != nullptr;
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
         const int row = m + 16 * j;
         if (row >= a.m) continue;
-        const float xs = a.x_scales[row];
 #pragma unroll
         for (int i = 0; i < TN; i += 2) {
             float v[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q)
-                v[q] = scaled(c[i + q / 4][j][q % 4], ws[i + q / 4][q % 4], xs, has_bias, bias[i + q / 4][q % 4]);
+                v[q] = scaled(c[i + q / 4][j][q % 4], scales.w[i + q / 4][q % 4], scales.x[j], has_bias,
+                              scales.bias[i + q / 4][q % 4]);
             if (pairs) {
                 const int ch = n + channel_of(4 * quad, i, true);
                 if (ch < a.n) store_row<8>(a, row, ch, v);
@@ -347,15 +378,12 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a)
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int j = 0; j < TM; ++j) c[i][j] = i32x4{0, 0, 0, 0};
-    auto read = [&](int h, int s, int slot) {
+    auto read = [&](int h, int slot) {
         const uint8_t *p = lds + slot * S::kStageBytes + operand_at(h, col, quad);
 #pragma unroll
         for (int i = 0; i < TN; ++i) wf[h][i] = *reinterpret_cast<const i32x4 *>(p + w_at + 2048 * i);
 #pragma unroll
         for (int j = 0; j < TM; ++j) xf[h][j] = *reinterpret_cast<const i32x4 *>(p + x_at + 2048 * j);
-        if (kStage * (s + 1) > a.k && kStage * s + 64 * h + 16 * quad >= a.k)
-#pragma unroll
-            for (int i = 0; i < TN; ++i) wf[h][i] = i32x4{0, 0, 0, 0};
     };
     auto multiply = [&](int h) {
         __builtin_amdgcn_sched_barrier(0);
@@ -368,23 +396,35 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a)
 #pragma unroll
     for (int i = 0; i < ST; ++i)
         if (s0 + i < s1) load(s0 + i, i);
-    if (s0 + ST - 1 < s1) wait_loads<(ST - 1) * S::kLoads>();
-    else wait_loads<0>();
+    const TileScales<TM, TN> scales(a, m0 + wm * 16 * TM + col, n0 + wn * 16 * TN, quad);
+    wait_loads<0>();
     barrier();
-    read(0, s0, 0);
+    // stages that k fills, then what is left of it
+    const int s_whole = min(s1, a.k / kStage);
+    if (s0 < s_whole) read(0, 0);
     int slot = 0;
-    for (int s = s0; s < s1; ++s) {
+    for (int s = s0; s < s_whole; ++s) {
         const int next = slot + 1 == ST ? 0 : slot + 1;
-        read(1, s, slot);
+        read(1, slot);
         multiply(0);
         // stage s + 1 is there (up to s + ST - 1 have been asked for), and stage s has been read
         if (s + ST - 1 < s1) wait_loads_and_reads<(ST - 2) * S::kLoads>();
         else wait_loads_and_reads<0>();
         barrier();
         if (s + ST < s1) load(s + ST, slot);
-        if (s + 1 < s1) read(0, s + 1, next);
+        if (s + 1 < s_whole) read(0, next);
         multiply(1);
         slot = next;
+    }
+    if (s_whole < s1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            read(h, slot);
+            if (kStage * s_whole + 64 * h + 16 * quad >= a.k)
+#pragma unroll
+                for (int i = 0; i < TN; ++i) wf[h][i] = i32x4{0, 0, 0, 0};
+            multiply(h);
+        }
     }
     if (a.splits > 1) {
         const FarParts far(a.ws);
@@ -405,7 +445,7 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a)
                 for (int j = 0; j < TM; ++j) c[i][j] += __builtin_bit_cast(i32x4, far.load4(from + 256 * (i * TM + j)));
         }
     }
-    write_tile<TM, TN>(a, m0 + wm * 16 * TM + col, n0 + wn * 16 * TN, c, quad);
+    write_tile<TM, TN>(a, m0 + wm * 16 * TM + col, n0 + wn * 16 * TN, c, quad, scales);
 }
 
 // ---- large tiles -----------------------------------------------------------------
@@ -574,7 +614,7 @@ __global__ __launch_bounds__(kLargeThreads) __attribute__((amdgpu_waves_per_eu(2
             begin(t);
             load_first();
         }
-        write_tile<TM, TN>(a, m, n, c, quad);
+        write_tile<TM, TN>(a, m, n, c, quad, TileScales<TM, TN>(a, m, n, quad));
         if (last) return;
         // of the operations so far only stores of outputs, the newest, may be under way
         if (pairs) wait_loads<TM * TN / 2>();
@@ -595,13 +635,21 @@ int launch_few(mi355x_ctx *ctx, const MatmulArgs &a) {
     return MI355X_OK;
 }
 
+// The output in tiles of bm rows and bn channels.
+void set_tiles(MatmulArgs &a, int bm, int bn) {
+    a.m_tiles = (a.m + bm - 1) / bm;
+    a.n_tiles = (a.n + bn - 1) / bn;
+    a.tiles = fast_div(static_cast<uint32_t>(a.m_tiles * a.n_tiles));
+    a.band = fast_div(static_cast<uint32_t>(8 * a.n_tiles));
+    a.last_rows = fast_div(static_cast<uint32_t>(a.m_tiles % 8 ? a.m_tiles % 8 : 8));
+}
+
 int stages_of(const MatmulArgs &a) { return (a.k + kStage - 1) / kStage; }
 
 template <int BM, int BN, int WM, int WN, int ST>
 int launch_tiles(mi355x_ctx *ctx, MatmulArgs a, int splits) {
     typedef TileShape<BM, BN, WM, WN, ST> S;
-    a.m_tiles = (a.m + BM - 1) / BM;
-    a.n_tiles = (a.n + BN - 1) / BN;
+    set_tiles(a, BM, BN);
     const int stages = stages_of(a);
     a.split_stages = (stages + splits - 1) / splits;
     a.splits = (stages + a.split_stages - 1) / a.split_stages;
@@ -612,8 +660,7 @@ int launch_tiles(mi355x_ctx *ctx, MatmulArgs a, int splits) {
 }
 
 int launch_large(mi355x_ctx *ctx, MatmulArgs a) {
-    a.m_tiles = (a.m + kLarge - 1) / kLarge;
-    a.n_tiles = (a.n + kLarge - 1) / kLarge;
+    set_tiles(a, kLarge, kLarge);
     const int groups = std::min(a.m_tiles * a.n_tiles, ctx->num_cus);
     matmul_large_kernel<<<groups, kLargeThreads, kLargeLds, ctx->stream>>>(a);
     MI355X_HIP(hipGetLastError());
