@@ -667,26 +667,27 @@ int launch_large(mi355x_ctx *ctx, MatmulArgs a) {
     return MI355X_OK;
 }
 
-// Tiles, and the time that a workgroup takes for a stage of k where it has a CU for
-// itself and where `per_cu` share one (us; from calls of 128 to 8192 rows).
+// Tiles, the time that a workgroup takes for a stage of k where it has a CU for itself
+// and where `per_cu` share one, and what the first and each later round of workgroups
+// takes besides (us).
 struct Form {
     int bm, bn, per_cu, most_splits;
-    float alone, shared;
+    float alone, shared, first, later;
 };
 constexpr Form kForms[] = {
-    {64, 64, 2, 8, 0.37f, 0.55f},
-    {128, 128, 1, 8, 0.70f, 0.70f},
-    {256, 128, 1, 8, 1.08f, 1.08f},
-    {kLarge, kLarge, 1, 1, 1.65f, 1.65f},
+    {64, 64, 2, 8, 0.29f, 0.53f, 0.5f, 0.5f},
+    {128, 128, 1, 8, 0.66f, 0.66f, 0.5f, 2.5f},
+    {256, 128, 1, 8, 0.96f, 0.96f, 0.5f, 7.0f},
+    {kLarge, kLarge, 1, 1, 1.60f, 1.60f, 6.4f, 6.4f},
 };
 
 // The form and the split of k with the least estimated time: the launch, rounds of
-// workgroups (three stages more for a tile's begin and end), and for a split the sums
-// that go out and come back.  us, estimated and measured, of the forms in order
-// (split): 512 x 4096, k 14336: 67 (1), 54 (2), 52 (4), 194; 67, 47, 49, 156.  256 x 8192,
-// k 8192: 41 (1), 37 (2), 44 (4), 115; 41, 32, 38, 92.  1024 x 4096, k 4096: 43, 29, 42, 62;
-// 40, 27, 38, 52.  512 x 17408, k 5120: 122, 94, 97, 75; 116, 97, 99, 70.  128 x 4096, k 4096:
-// 17 (2), 27 (4); 12, 18.
+// workgroups, and for a split the parts that a tile's last workgroup reads.  us,
+// estimated and measured, of the forms in order with their best split: 512 x 4096, k
+// 14336: 63 (1), 46 (2), 48 (4), 189; 62, 46, 49, 158.  256 x 8192, k 8192: 38 (1), 30
+// (2), 37 (4), 112; 39, 32, 36, 92.  1024 x 4096, k 4096: 38 (1), 25 (1), 28 (2), 61; 37, 25,
+// 31, 51.  201 x 2560, k 2048: 8 (1), 14 (1), 21 (2); 8, 13, 17.  90 x 2048, k 11008: 14
+// (4), 25 (5); 14, 21.  5000 x 5000, k 2048: 120, 92, 86, 67; 118, 93, 87, 65.
 struct Choice {
     int form, splits;
 };
@@ -698,13 +699,15 @@ Choice choose(const mi355x_ctx *ctx, const MatmulArgs &a) {
         const Form &g = kForms[f];
         if (g.bm == kLarge && g.bn == kLarge && (a.m < kLarge || a.n < kLarge)) continue;
         const int64_t tiles = static_cast<int64_t>((a.m + g.bm - 1) / g.bm) * ((a.n + g.bn - 1) / g.bn);
+        const int64_t tile_bytes = int64_t(4) * g.bm * g.bn;
         for (int s = 1; s <= g.most_splits && s <= stages; ++s) {
-            const int64_t groups = tiles * s, part_bytes = groups * g.bm * g.bn * 4;
-            if (s > 1 && (tiles > static_cast<int64_t>(kCounters / 4) || part_bytes > static_cast<int64_t>(kPartBytes))) break;
+            const int64_t groups = tiles * s;
+            if (s > 1 && (tiles > static_cast<int64_t>(kCounters / 4) || groups * tile_bytes > static_cast<int64_t>(kPartBytes)))
+                break;
             const float rounds = std::ceil(static_cast<float>(groups) / static_cast<float>(ctx->num_cus * g.per_cu));
-            float us = 4.0f + rounds * (groups <= ctx->num_cus ? g.alone : g.shared) *
-                                  static_cast<float>((stages + s - 1) / s + 3);
-            if (s > 1) us += 3.0f + 2.0f * static_cast<float>(part_bytes) / 6.0e6f;
+            float us = 3.2f + g.first + (rounds - 1.0f) * g.later +
+                       rounds * (groups <= ctx->num_cus ? g.alone : g.shared) * static_cast<float>((stages + s - 1) / s);
+            if (s > 1) us += 1.5f + static_cast<float>(s) * static_cast<float>(tile_bytes) / 32768.0f;
             if (us < least) {
                 least = us;
                 best = {f, s};
