@@ -95,10 +95,17 @@ struct Sums {
         }
         high = ref = to;
     }
-    __device__ __forceinline__ void add(float x, float k) {
-        const float t = (x - ref) * k, p = __builtin_amdgcn_exp2f(t);
-        s += p;                              // NaN where x is NaN or +inf
-        e = fmaf(p, fmaxf(t, -1000.0f), e);  // -inf adds nothing
+    // Eight logits, added to each other first, so that no long chain of roundings grows.
+    __device__ __forceinline__ void add8(const float *x, float k) {
+        float s8 = 0.0f, e8 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float t = (x[j] - ref) * k, p = __builtin_amdgcn_exp2f(t);
+            s8 += p;                               // NaN where x is NaN or +inf
+            e8 = fmaf(p, fmaxf(t, -1000.0f), e8);  // -inf adds nothing
+        }
+        s += s8;
+        e += e8;
     }
 };
 
@@ -283,9 +290,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
             sums.raise(most, k);
 #pragma unroll
             for (int c = 0; c < kLoads; ++c)
-                if (in(c))
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) sums.add(x[c][j], k);
+                if (in(c)) sums.add8(x[c], k);
             if (most >= bound)
 #pragma unroll
                 for (int c = 0; c < kLoads; ++c)
