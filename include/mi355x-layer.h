@@ -139,7 +139,7 @@ typedef struct mi355x_logprobs_args {
     int type;        /* logits: MI355X_TYPE_F32, _F16 or _BF16 */
     const void *logits;
     int64_t stride;
-    float scale;     /* 1 / temperature: finite, above 0 */
+    float scale;     /* 1 / temperature: 2^-100 .. 2^100 */
     int n_tokens;    /* of each row, 0 .. 65536 */
     const int32_t *tokens;  /* n_rows * n_tokens */
     float *token_logprobs;  /* n_rows * n_tokens */

@@ -138,3 +138,8 @@ def test_the_reference_rounds_ties_to_even():
     assert c.tolist() == [[127, 2, 2, 0, -2, 0]] and np.all(s == 3)
     c, s, _ = layer_ref.codes_of(np.array([[0.0, 0.0], [1.0, np.inf], [np.nan, 1.0]]))
     assert not c.any() and s[0] == 0 and np.isnan(s[1:]).all()
+
+
+def test_scales_past_their_limits(host):
+    for scale, want in [(2.0 ** 100, EHIP), (2.0 ** -100, EHIP), (2.0 ** 101, EINVAL), (2.0 ** -101, EINVAL)]:
+        assert rc(host, "mi355x_logprobs", logprobs(scale=scale)) == want

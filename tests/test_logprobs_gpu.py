@@ -252,3 +252,25 @@ def test_rows_far_apart(ctx, ws):
     finally:
         big.free()
         c.free()
+
+
+@pytest.mark.parametrize("V", [40, 2048, 9000, 40000])
+@pytest.mark.parametrize("scale", [1.0, 0.75])
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_rows_that_begin_with_the_lowest_value(ctx, ws, t, scale, V):
+    """Sums against the lowest value, which a logit far above it then replaces: the
+    difference's multiple passes f32's range."""
+    x = logits(3, V, 8)
+    low = float(decode(encode(np.full(1, np.finfo(np.float32).min if t == F32 else -3.3e38), t), t)[0])
+    x[0, :V // 2] = low
+    x[1, :V - 3] = low
+    x[2, ::2] = low
+    go(ctx, ws, x, t, scale=scale)
+    for r in range(3):
+        go(ctx, ws, x[r:r + 1], t, scale=scale)
+
+
+def test_scales_at_their_limits(ctx, ws):
+    x = logits(2, 5000, 9)
+    go(ctx, ws, x * 2.0 ** 100, F32, scale=2.0 ** -100)
+    go(ctx, ws, x * 2.0 ** -100, F32, scale=2.0 ** 100)

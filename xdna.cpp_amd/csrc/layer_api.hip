@@ -181,7 +181,8 @@ int mi355x_logprobs(mi355x_ctx *ctx, const mi355x_logprobs_args *args) {
     if (a.n_vocab < 1 || a.n_vocab > (1 << 30))
         return invalid(who, "n_vocab must be 1 to 2^30 (got " + std::to_string(a.n_vocab) + ")");
     if (int rc = check_type(who, "type", a.type)) return rc;
-    if (!(a.scale > 0.0f) || std::isinf(a.scale)) return invalid(who, "scale must be finite and above 0");
+    // (a multiple of it by log2 e, and quotients by it, stay in f32's range)
+    if (!(a.scale >= 0x1p-100f && a.scale <= 0x1p100f)) return invalid(who, "scale must be 2^-100 to 2^100");
     if (a.n_tokens < 0 || a.n_tokens > 65536) return invalid(who, "n_tokens must be 0 to 65536");
     if (a.n_top < 0 || a.n_top > MI355X_LOGPROBS_MAX_TOP)
         return invalid(who, "n_top must be 0 to " + std::to_string(MI355X_LOGPROBS_MAX_TOP) + " (got " +

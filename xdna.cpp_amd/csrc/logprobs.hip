@@ -89,7 +89,8 @@ struct Sums {
     __device__ __forceinline__ void raise(float to, float k) {
         if (!(to > high)) return;
         if (s != 0.0f) {
-            const float shift = (ref - to) * k, f = __builtin_amdgcn_exp2f(shift);
+            // (a row's first logits may be the type's lowest value: the product may be infinite)
+            const float shift = fmaxf((ref - to) * k, -1000.0f), f = __builtin_amdgcn_exp2f(shift);
             e = f * (e + shift * s);
             s *= f;
         }
@@ -217,19 +218,23 @@ __device__ __forceinline__ void write_row(const LogitArgs &a, int64_t row, const
     const float log_total = bad ? NAN : none ? 0.0f : logf(s);
     if (a.entropy && tid == 0)
         a.entropy[row] = bad ? NAN : none ? 0.0f : fmaf(-0.693147180559945309f, e / s, log_total);
+    // in 64 bits: the difference of two f32 logits may pass f32's range where its multiple does not
+    auto logprob = [&](float x) {
+        return static_cast<float>(static_cast<double>(a.scale) * (static_cast<double>(x) - top) - log_total);
+    };
     const T *logits = static_cast<const T *>(a.logits) + row * a.stride;
     for (int t = tid; t < a.n_tokens; t += kThreads) {
         const int token = a.tokens[row * a.n_tokens + t];
         const bool in = token >= 0 && token < a.n_vocab;
         const float x = in ? static_cast<float>(logits[token]) : 0.0f;
         a.token_logprobs[row * a.n_tokens + t] =
-            bad || !in ? NAN : x == -INFINITY ? x : a.scale * (x - top) - log_total;
+            bad || !in ? NAN : x == -INFINITY ? x : logprob(x);
     }
     for (int r = tid; r < a.n_top; r += kThreads) {
         const bool in = r < found && !bad;
         a.top_tokens[row * a.n_top + r] = in ? static_cast<int>(~static_cast<uint32_t>(l.top[r])) : -1;
         a.top_logprobs[row * a.n_top + r] =
-            bad ? NAN : in ? a.scale * (logit_of(static_cast<uint32_t>(l.top[r] >> 32)) - top) - log_total : -INFINITY;
+            bad ? NAN : in ? logprob(logit_of(static_cast<uint32_t>(l.top[r] >> 32))) : -INFINITY;
     }
 }
 
