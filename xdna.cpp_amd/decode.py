@@ -66,6 +66,10 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     lib.qd_set_wait.argtypes = [C.c_void_p, C.c_int]
     lib.qd_set_attention.restype = C.c_int
     lib.qd_set_attention.argtypes = [C.c_void_p, C.c_int]
+    lib.qd_set_logprobs.restype = C.c_int
+    lib.qd_set_logprobs.argtypes = [C.c_void_p, C.c_int]
+    lib.qd_last_logprobs.restype = C.c_int
+    lib.qd_last_logprobs.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]
     lib.qd_last_wait.restype = C.c_int
     lib.qd_last_wait.argtypes = [C.c_void_p]
     lib.qd_last_launches.restype = C.c_int64
@@ -206,6 +210,22 @@ class Model:
             raise RuntimeError(self.lib.qd_last_error().decode())
 
     PLUGIN_GROUPS_SERVER, PLUGIN_GROUPS_LAUNCH = 0, 1
+
+    def set_logprobs(self, n_top: int) -> None:
+        """With ATTENTION_GPU: log probabilities, entropies and the n_top most
+        likely tokens of every generated token, on the GPU (-1, default: none)."""
+        if self.lib.qd_set_logprobs(self.h, n_top) != 0:
+            raise RuntimeError(self.lib.qd_last_error().decode())
+
+    def last_logprobs(self, n: int, n_top: int = 0):
+        """Of the n tokens of the last generation: log probabilities, entropies,
+        top tokens and their log probabilities (n x n_top)."""
+        lp, ent = np.empty(n, np.float32), np.empty(n, np.float32)
+        top, top_lp = np.empty((n, n_top), np.int32), np.empty((n, n_top), np.float32)
+        if self.lib.qd_last_logprobs(self.h, n, lp.ctypes.data, ent.ctypes.data, n_top, top.ctypes.data,
+                                     top_lp.ctypes.data) != 0:
+            raise RuntimeError(self.lib.qd_last_error().decode())
+        return lp, ent, top, top_lp
 
     def set_plugin_groups(self, mode: int) -> None:
         """WAIT_PLUGIN: graph_compute runs a group as one launch

@@ -8,6 +8,7 @@
 #include "ggml-mi355x.h"
 #include "ggml_abi.h"
 #include "mi355x-attention.h"
+#include "mi355x-layer.h"
 #include "mi355x-gemv.h"
 
 #include <hip/hip_runtime_api.h>
@@ -220,6 +221,12 @@ struct qd_model {
     int variant = MI355X_VARIANT_AUTO;
     int last_wait = QD_WAIT_FENCE;  // the mode the last GPU decode used
     int attention = QD_ATTENTION_HOST;
+    int logprobs = -1;  // top tokens of each generated one; -1: no log probabilities
+    // of the last generation's tokens: top tokens (last_top of each, the first of them the
+    // token itself) with their log probabilities, and entropies
+    int last_top = -1;  // -1: it had none
+    std::vector<int32_t> last_top_tokens;
+    std::vector<float> last_top_logprobs, last_entropies;
 
     mi355x_server *server = nullptr;
     std::unique_ptr<PluginDecode> plugin;
@@ -578,6 +585,31 @@ int qd_set_attention(qd_model *m, int mode) {
     return 0;
 }
 
+int qd_set_logprobs(qd_model *m, int n_top) {
+    if (!m) return fail("qd_set_logprobs: null model");
+    if (n_top < -1 || n_top > MI355X_LOGPROBS_MAX_TOP || n_top > m->c.vocab)
+        return fail("qd_set_logprobs: n_top is not in -1 .. min(vocab, MI355X_LOGPROBS_MAX_TOP)");
+    m->logprobs = n_top;
+    return 0;
+}
+
+int qd_last_logprobs(const qd_model *m, int n, float *logprobs, float *entropies, int n_top, int32_t *top_tokens,
+                     float *top_logprobs) {
+    if (!m) return fail("qd_last_logprobs: null model");
+    if (n < 0 || m->last_top < 0 || static_cast<size_t>(n) != m->last_entropies.size() || n_top < 0 ||
+        n_top > m->last_top)
+        return fail("qd_last_logprobs: the last generation has no such log probabilities");
+    for (int i = 0; i < n; ++i) {
+        const int32_t *tokens = m->last_top_tokens.data() + static_cast<size_t>(i) * m->last_top;
+        const float *of = m->last_top_logprobs.data() + static_cast<size_t>(i) * m->last_top;
+        if (logprobs) logprobs[i] = of[0];
+        if (entropies) entropies[i] = m->last_entropies[i];
+        if (top_tokens) std::copy(tokens, tokens + n_top, top_tokens + static_cast<size_t>(i) * n_top);
+        if (top_logprobs) std::copy(of, of + n_top, top_logprobs + static_cast<size_t>(i) * n_top);
+    }
+    return 0;
+}
+
 int64_t qd_last_launches(const qd_model *m) { return m ? m->last_launches : 0; }
 
 int qd_last_wait(const qd_model *m) { return m ? m->last_wait : -1; }
@@ -749,6 +781,12 @@ struct GpuDecode {
     volatile int32_t *h_status = nullptr;  // of the pass's plan, which writes it there
     int32_t *status = nullptr;             // its device address
     std::string refused;                   // the error of a plan that does not fit
+    // with log probabilities: the top tokens, their log probabilities and the entropy, which
+    // the GPU writes to page-locked memory
+    int top = 0;
+    void *top_workspace = nullptr;
+    size_t top_workspace_bytes = 0;
+    float *h_top = nullptr, *d_top = nullptr;
     int n_pages = 0;
     int64_t launches = 0;
     double t_gpu = 0.0;
@@ -794,6 +832,17 @@ struct GpuDecode {
         const size_t R = static_cast<size_t>(rows), wide = static_cast<size_t>(std::max(2 * F, std::max(H, QD)));
         y_floats = std::max(R * wide, static_cast<size_t>(m->c.vocab));
         const size_t pool = static_cast<size_t>(n_pages) * QD_PAGE_TOKENS * KVD;  // values of one layer's keys
+        if (m->logprobs >= 0) {
+            top = std::max(1, m->logprobs);
+            void *dev = nullptr;
+            if (mi355x_logprobs_workspace(ctx, &top_workspace_bytes) != MI355X_OK ||
+                !alloc(&top_workspace, top_workspace_bytes) ||
+                mi355x_fill(ctx, top_workspace, 0, top_workspace_bytes) != MI355X_OK ||
+                !alloc_host(&h_top, 4 * (2 * static_cast<size_t>(top) + 1)) ||
+                mi355x_host_device_ptr(h_top, &dev) != MI355X_OK)
+                return -1;
+            d_top = static_cast<float *>(dev);
+        }
         if (mi355x_paged_attention_workspace(ctx, m->c.n_heads, m->c.n_kv_heads, hd, &workspace_bytes) != MI355X_OK)
             return -1;
         if (!alloc(&x, 4 * R * std::max(F, std::max(H, QD))) || !alloc(&y, 4 * y_floats) ||
@@ -933,8 +982,32 @@ struct GpuDecode {
         return mi355x_paged_attention(ctx, &a);
     }
 
-    // The pass of n tokens; with logits, those behind the last one.
-    int pass(const int32_t *tokens, int n, float *logits) {
+    const int32_t *top_tokens() const { return reinterpret_cast<const int32_t *>(h_top); }
+    const float *top_logprobs() const { return h_top + top; }
+    float entropy() const { return h_top[2 * top]; }
+
+    // Top tokens, log probabilities and entropy of the logits in y.
+    int read_top() {
+        mi355x_logprobs_args a{};
+        a.n_rows = 1;
+        a.n_vocab = m->c.vocab;
+        a.type = MI355X_TYPE_F32;
+        a.logits = y;
+        a.stride = m->c.vocab;
+        a.scale = 1.0f;
+        a.entropy = d_top + 2 * top;
+        a.n_top = top;
+        a.top_tokens = reinterpret_cast<int32_t *>(d_top);
+        a.top_logprobs = d_top + top;
+        a.workspace = top_workspace;
+        a.workspace_bytes = top_workspace_bytes;
+        if (mi355x_logprobs(ctx, &a) != MI355X_OK) return -1;
+        return wait();
+    }
+
+    // The pass of n tokens; with `want`, its last one's logits (in logits) or, with log
+    // probabilities, what read_top leaves.
+    int pass(const int32_t *tokens, int n, bool want, float *logits) {
         const int64_t width = QD + 2 * KVD;
         std::vector<float> h(static_cast<size_t>(n) * H);
         for (int i = 0; i < n; ++i)
@@ -982,11 +1055,16 @@ struct GpuDecode {
             t_gpu += now() - t0;
             residual();
         }
-        if (!logits) return 0;
+        if (!want) return 0;
         rmsnorm(h.data() + static_cast<size_t>(n - 1) * H, m->out_norm.data(), hx, H, m->c.norm_eps);
         t0 = now();
-        if (upload(H) || product(7 * L, x, y, 0, 1) || download(m->c.vocab)) return -1;
+        if (upload(H) || product(7 * L, x, y, 0, 1) || (top ? read_top() : read_logits(logits))) return -1;
         t_gpu += now() - t0;
+        return 0;
+    }
+
+    int read_logits(float *logits) {
+        if (download(m->c.vocab)) return -1;
         std::memcpy(logits, hy, static_cast<size_t>(m->c.vocab) * 4);
         return 0;
     }
@@ -999,22 +1077,40 @@ int generate_gpu_attention(qd_model *m, const int32_t *prompt, int n_prompt, int
     auto failed = [&] { return fail("qd_generate: " + (d.refused.empty() ? mi355x_last_error() : d.refused)); };
     if (d.init()) return failed();
     std::vector<float> logits(static_cast<size_t>(m->c.vocab));
+    std::vector<int32_t> top_tokens;
+    std::vector<float> top_logprobs, entropies;
+    int32_t tok = 0;
+    auto take = [&](int i) {  // the token that the last pass picks
+        if (d.top) {
+            top_tokens.insert(top_tokens.end(), d.top_tokens(), d.top_tokens() + d.top);
+            top_logprobs.insert(top_logprobs.end(), d.top_logprobs(), d.top_logprobs() + d.top);
+            entropies.push_back(d.entropy());
+            // logits without a largest one (NaN) have no top token
+            out_tokens[i] = tok = std::max(d.top_tokens()[0], 0);
+        } else {
+            out_tokens[i] = tok = argmax(logits.data(), m->c.vocab);
+        }
+    };
     const double t_start = now();
     for (int at = 0; at < n_prompt; at += QD_CHUNK_ROWS) {
         const int n = std::min(QD_CHUNK_ROWS, n_prompt - at);
-        if (d.pass(prompt + at, n, at + n == n_prompt && n_gen > 0 ? logits.data() : nullptr)) return failed();
+        if (d.pass(prompt + at, n, at + n == n_prompt && n_gen > 0, logits.data())) return failed();
     }
-    int32_t tok = 0;
-    if (n_gen > 0) out_tokens[0] = tok = argmax(logits.data(), m->c.vocab);
+    if (n_gen > 0) take(0);
     const double t_gen0 = now();
     d.t_gpu = 0.0;
     d.launches = 0;
     for (int i = 1; i < n_gen; ++i) {
-        if (d.pass(&tok, 1, logits.data())) return failed();
-        out_tokens[i] = tok = argmax(logits.data(), m->c.vocab);
+        if (d.pass(&tok, 1, true, logits.data())) return failed();
+        take(i);
     }
     const double t_end = now();
+    if (n_gen > 0 && d.top && d.read_logits(logits.data())) return failed();
     if (n_gen > 0) m->last_logits = logits;
+    m->last_top = d.top ? d.top : -1;
+    m->last_top_tokens = std::move(top_tokens);
+    m->last_top_logprobs = std::move(top_logprobs);
+    m->last_entropies = std::move(entropies);
     m->last_launches = d.launches;
     m->last_wait = m->wait_mode == QD_WAIT_STREAM ? QD_WAIT_STREAM : QD_WAIT_FENCE;
     if (timings) {
@@ -1034,6 +1130,12 @@ int qd_generate(qd_model *m, int backend, qd_gemv_fn cpu_gemv, void *user, const
         return fail("qd_generate: bad arguments");
     if (backend == 0 && !m->ctx) return fail("qd_generate: qd_attach_gpu first");
     if (backend == 1 && !cpu_gemv) return fail("qd_generate: no CPU GEMV");
+    if (m->logprobs >= 0 && (backend != 0 || m->attention != QD_ATTENTION_GPU))
+        return fail("qd_generate: log probabilities need attention on the GPU");
+    m->last_top = -1;  // none yet
+    m->last_top_tokens.clear();
+    m->last_top_logprobs.clear();
+    m->last_entropies.clear();
     if (backend == 0 && m->attention == QD_ATTENTION_GPU) {
         omp_set_num_threads(m->threads);
         return generate_gpu_attention(m, prompt, n_prompt, n_gen, out_tokens, timings);

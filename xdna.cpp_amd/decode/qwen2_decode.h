@@ -144,6 +144,18 @@ QD_API int qd_last_wait(const qd_model *m);
 #define QD_PAGE_TOKENS 64
 #define QD_CHUNK_ROWS 512
 QD_API int qd_set_attention(qd_model *m, int mode);
+/* Log probabilities of the generated tokens, with attention on the GPU
+ * (qd_generate fails otherwise): n_top -1 (default) none, 0 ..
+ * MI355X_LOGPROBS_MAX_TOP: mi355x_logprobs on the logits where the vocabulary
+ * GEMV leaves them, with the entropy and n_top most likely tokens.  The greedy
+ * token is then the GPU's first top token, and logits come to the host for the
+ * last token alone. */
+QD_API int qd_set_logprobs(qd_model *m, int n_top);
+/* Of the n = n_gen tokens of the last qd_generate: their log probabilities, the
+ * entropies, and n * n_top tokens and log probabilities (each may be NULL).  n_top: up
+ * to the one that was set, or 1 for 0. */
+QD_API int qd_last_logprobs(const qd_model *m, int n, float *logprobs, float *entropies, int n_top,
+                            int32_t *top_tokens, float *top_logprobs);
 /* Kernel variant of the GPU GEMVs (MI355X_OPT_VARIANT of mi355x-gemv.h):
  * MI355X_VARIANT_GGML_Q8 gives ggml-cpu's Q8_0-activation arithmetic. */
 QD_API int qd_set_variant(qd_model *m, int variant);
