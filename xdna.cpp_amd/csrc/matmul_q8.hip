@@ -393,11 +393,13 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a)
             for (int i = 0; i < TN; ++i) c[i][j] = mfma(wf[h][i], xf[h][j], c[i][j]);
         __builtin_amdgcn_sched_barrier(0);
     };
+    const TileScales<TM, TN> scales(a, m0 + wm * 16 * TM + col, n0 + wn * 16 * TN, quad);
 #pragma unroll
     for (int i = 0; i < ST; ++i)
         if (s0 + i < s1) load(s0 + i, i);
-    const TileScales<TM, TN> scales(a, m0 + wm * 16 * TM + col, n0 + wn * 16 * TN, quad);
-    wait_loads<0>();
+    // the first stage is there
+    if (s0 + ST <= s1) wait_loads<(ST - 1) * S::kLoads>();
+    else wait_loads<0>();
     barrier();
     // stages that k fills, then what is left of it
     const int s_whole = min(s1, a.k / kStage);
@@ -668,46 +670,56 @@ int launch_large(mi355x_ctx *ctx, MatmulArgs a) {
 }
 
 // Tiles, the time that a workgroup takes for a stage of k where it has a CU for itself
-// and where `per_cu` share one, and what the first and each later round of workgroups
-// takes besides (us).
+// and where `per_cu` share one (of one row of tiles: weights come from memory, and not
+// from an L2), and what the first and each later round of workgroups takes besides (us).
 struct Form {
     int bm, bn, per_cu, most_splits;
-    float alone, shared, first, later;
+    float alone, shared, alone_one_row, shared_one_row, first, later;
 };
 constexpr Form kForms[] = {
-    {64, 64, 2, 8, 0.29f, 0.53f, 0.5f, 0.5f},
-    {128, 128, 1, 8, 0.66f, 0.66f, 0.5f, 2.5f},
-    {256, 128, 1, 8, 0.96f, 0.96f, 0.5f, 7.0f},
-    {kLarge, kLarge, 1, 1, 1.60f, 1.60f, 6.4f, 6.4f},
+    {64, 64, 2, 8, 0.29f, 0.53f, 0.31f, 0.65f, 0.5f, 0.5f},
+    {64, 128, 1, 8, 0.47f, 0.47f, 0.57f, 0.57f, 0.5f, 0.5f},
+    {128, 128, 1, 8, 0.66f, 0.66f, 0.66f, 0.66f, 0.5f, 2.5f},
+    {256, 128, 1, 8, 0.96f, 0.96f, 0.96f, 0.96f, 0.5f, 7.0f},
+    {kLarge, kLarge, 1, 1, 1.60f, 1.60f, 1.60f, 1.60f, 6.4f, 6.4f},
 };
 
 // The form and the split of k with the least estimated time: the launch, rounds of
-// workgroups, and for a split the parts that a tile's last workgroup reads.  us,
-// estimated and measured, of the forms in order with their best split: 512 x 4096, k
-// 14336: 63 (1), 46 (2), 48 (4), 189; 62, 46, 49, 158.  256 x 8192, k 8192: 38 (1), 30
-// (2), 37 (4), 112; 39, 32, 36, 92.  1024 x 4096, k 4096: 38 (1), 25 (1), 28 (2), 61; 37, 25,
-// 31, 51.  201 x 2560, k 2048: 8 (1), 14 (1), 21 (2); 8, 13, 17.  90 x 2048, k 11008: 14
-// (4), 25 (5); 14, 21.  5000 x 5000, k 2048: 120, 92, 86, 67; 118, 93, 87, 65.
+// workgroups, and for a split the parts that a tile's last workgroup reads; operands
+// come from memory at 4.4 TB/s at most.  us measured, of the forms in order with their
+// best split in parentheses: 37 x 17408, k 5120: 28 (2), 26.6 (1).  64 x 28672, k 4096: 30
+// (1), 30 (1).  64 x 2048, k 11008: 12.7 (6), 15 (8).  201 x 2560, k 2048: 8 (1), 9 (1), 12 (3),
+// 17 (2).  200 x 22016, k 2048: 31, 30, 28, 22 (1).  300 x 5120, k 5120: 26 (1), 23 (1), 21 (2),
+// 30 (2), 64.  256 x 8192, k 8192: 39 (1), 33 (1), 31 (2), 36 (4), 92.  512 x 4096, k 14336:
+// 63 (1), 52 (1), 44 (2), 46 (4), 154.  1024 x 4096, k 4096: 37, 33, 25 (1), 31 (2), 51.  512 x
+// 22016, k 2048: 54, 59, 43, 43, 33.  5000 x 5000, k 2048: 105, 106, 85, 82, 65.  Of these the
+// least is chosen in each, and elsewhere one within 10% of the least.
 struct Choice {
     int form, splits;
 };
 Choice choose(const mi355x_ctx *ctx, const MatmulArgs &a) {
     const int stages = stages_of(a);
+    const float from_memory = static_cast<float>(a.m + a.n) * static_cast<float>(a.k) / 4.4e6f;
     Choice best{0, 1};
     float least = 1e30f;
-    for (int f = 0; f < 4; ++f) {
+    for (int f = 0; f < 5; ++f) {
         const Form &g = kForms[f];
         if (g.bm == kLarge && g.bn == kLarge && (a.m < kLarge || a.n < kLarge)) continue;
         const int64_t tiles = static_cast<int64_t>((a.m + g.bm - 1) / g.bm) * ((a.n + g.bn - 1) / g.bn);
         const int64_t tile_bytes = int64_t(4) * g.bm * g.bn;
         for (int s = 1; s <= g.most_splits && s <= stages; ++s) {
             const int64_t groups = tiles * s;
-            if (s > 1 && (tiles > static_cast<int64_t>(kCounters / 4) || groups * tile_bytes > static_cast<int64_t>(kPartBytes)))
+            // (parts in more than one round did not gain: 37 x 17408, k 5120 in 5 parts 31 us, whole 27)
+            if (s > 1 && (groups > ctx->num_cus * g.per_cu || tiles > static_cast<int64_t>(kCounters / 4) ||
+                          groups * tile_bytes > static_cast<int64_t>(kPartBytes)))
                 break;
             const float rounds = std::ceil(static_cast<float>(groups) / static_cast<float>(ctx->num_cus * g.per_cu));
-            float us = 3.2f + g.first + (rounds - 1.0f) * g.later +
-                       rounds * (groups <= ctx->num_cus ? g.alone : g.shared) * static_cast<float>((stages + s - 1) / s);
+            const bool alone = groups <= ctx->num_cus, one_row = a.m <= g.bm;
+            float us = (rounds - 1.0f) * g.later +
+                       rounds * (one_row ? alone ? g.alone_one_row : g.shared_one_row : alone ? g.alone : g.shared) *
+                           static_cast<float>((stages + s - 1) / s);
             if (s > 1) us += 1.5f + static_cast<float>(s) * static_cast<float>(tile_bytes) / 32768.0f;
+            us = 3.2f + g.first + std::max(us, from_memory);
             if (us < least) {
                 least = us;
                 best = {f, s};
@@ -744,16 +756,22 @@ int launch_matmul_q8(mi355x_ctx *ctx, const mi355x_matmul_q8_args &u) {
         return set_error(MI355X_EUNSUPPORTED, "mi355x_matmul_q8: 2^34 outputs or more");
     if (far && a.m > 64 * 65535)
         return set_error(MI355X_EUNSUPPORTED, "mi355x_matmul_q8: more than 64 * 65535 rows with strides past 2^23");
+    // Up to 32 rows have the weight in flight in each wavefront by itself; blocks of 32
+    // channels where that fills the CUs, else of 16 so that more workgroups share the work
+    // (16, then 32 channels; us: one row of 2048, k 11008 7.6, 10.4; of 8192, k 8192 12.9, 12.9;
+    // of 22016, k 2048 11.6, 10.1; 32 rows of 2048, k 2048 3.5, 4.0; of 22016 20, 12).  The tiles
+    // take more: 32 rows of 2048, k 2048 7.0, of 22016 13.9; 17 of 28672, k 4096 27.6, here
+    // 24.5; 37 rows 28.6, here (48 channels, 48 rows) 31.3.
     const bool many = a.n >= 32 * ctx->num_cus;
     if (a.m <= 16) return many ? launch_few<1, 2, 4, 3>(ctx, a) : launch_few<1, 1, 4, 4>(ctx, a);
     if (a.m <= 32) return many ? launch_few<2, 2, 4, 2>(ctx, a) : launch_few<2, 1, 8, 2>(ctx, a);
-    if (a.m <= 48 && many) return launch_few<3, 3, 2, 3>(ctx, a);
-    if ((a.m <= 64 && many) || far) return launch_few<4, 3, 2, 2>(ctx, a);
+    if (far) return launch_few<4, 3, 2, 2>(ctx, a);
     const Choice c = choose(ctx, a);
     switch (c.form) {
     case 0: return launch_tiles<64, 64, 4, 2, 4>(ctx, a, c.splits);
-    case 1: return launch_tiles<128, 128, 2, 4, 4>(ctx, a, c.splits);
-    case 2: return launch_tiles<256, 128, 2, 4, 3>(ctx, a, c.splits);
+    case 1: return launch_tiles<64, 128, 2, 4, 4>(ctx, a, c.splits);
+    case 2: return launch_tiles<128, 128, 2, 4, 4>(ctx, a, c.splits);
+    case 3: return launch_tiles<256, 128, 2, 4, 3>(ctx, a, c.splits);
     default: return launch_large(ctx, a);
     }
 }
