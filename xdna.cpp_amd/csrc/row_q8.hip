@@ -111,9 +111,30 @@ __device__ __forceinline__ void norm_values(const RowArgs &a, int64_t row, int i
     }
 }
 
+// e^x in 64 bits: 2^k times a polynomial on +-(log 2) / 2, of which 4e-18 is left out.  Its
+// loop is unrolled where it is a kernel's work, and else not, so that its numbers do not
+// take up the registers of the values (4096 gated rows of 14336: 90 us with them).
+__constant__ double kInverses[14] = {0.0,     1.0,     1.0 / 2, 1.0 / 3,  1.0 / 4,  1.0 / 5,  1.0 / 6,
+                                     1.0 / 7, 1.0 / 8, 1.0 / 9, 1.0 / 10, 1.0 / 11, 1.0 / 12, 1.0 / 13};
+template <bool UNROLLED>
+__device__ __forceinline__ double exp64(double x) {
+    x = fmin(fmax(x, -800.0), 800.0);  // 0 and infinity
+    const double k = rint(x * 1.4426950408889634), r = fma(k, -2.3190468138462996e-17, fma(k, -0.6931471805599453, x));
+    double p = 1.0;
+    if (UNROLLED) {
+#pragma unroll
+        for (int n = 13; n > 0; --n) p = fma(p, r * (1.0 / n), 1.0);
+    } else {
+#pragma unroll 1
+        for (int n = 13; n > 0; --n) p = fma(p, r * kInverses[n], 1.0);
+    }
+    return ldexp(p, static_cast<int>(k));
+}
+
+template <bool UNROLLED>
 __device__ __forceinline__ double gated(float g, float u) {
     const double d = g;
-    return d / (1.0 + exp(-d)) * static_cast<double>(u);
+    return d / (1.0 + exp64<UNROLLED>(-d)) * static_cast<double>(u);
 }
 
 __device__ __forceinline__ void swiglu_values(const RowArgs &a, int64_t row, int i, double *t) {
@@ -121,7 +142,7 @@ __device__ __forceinline__ void swiglu_values(const RowArgs &a, int64_t row, int
     load_as_float(row_at(a.x, a.type, row * a.x_stride), a.type, i, a.n, g);
     load_as_float(row_at(a.y, a.type, row * a.y_stride), a.type, i, a.n, u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = gated(g[j], u[j]);
+    for (int j = 0; j < 8; ++j) t[j] = gated<true>(g[j], u[j]);
 }
 
 // Rows longer than a workgroup's registers: the values formed twice, for the largest
@@ -180,14 +201,19 @@ __device__ __forceinline__ void load_row(const void *p, int n, typename RowElem<
 
 // Codes, a byte each, of t * unit with `unit` next to 127 / most: 1.5 * 2^23 is added in
 // the multiplication's own rounding, which leaves the nearest whole number in the low
-// bits.  A bit of *doubt is set for each product nearer than `error` to a border.
-__device__ __forceinline__ uint64_t pack_codes(const float *t, float unit, float error, uint32_t *doubt) {
+// bits.  A bit of *doubt is set for each product nearer than error + slope |t| to a border.
+template <bool SLOPE>
+__device__ __forceinline__ uint64_t pack_codes(const float *t, float unit, float error, float slope, uint32_t *doubt) {
     constexpr float kWhole = 12582912.0f;
     float z[8], worst = 0.0f;
+    auto off = [&](int j) {
+        const float d = fabsf(fmaf(t[j], unit, kWhole - z[j]));
+        return SLOPE ? fmaf(fabsf(t[j]), slope, d) : d;
+    };
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         z[j] = fmaf(t[j], unit, kWhole);
-        worst = fmaxf(worst, fabsf(fmaf(t[j], unit, kWhole - z[j])));
+        worst = fmaxf(worst, off(j));
     }
     uint32_t c[2];
 #pragma unroll
@@ -201,7 +227,7 @@ __device__ __forceinline__ uint64_t pack_codes(const float *t, float unit, float
     *doubt = 0;
     if (worst >= 0.5f - error)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) *doubt |= fabsf(fmaf(t[j], unit, kWhole - z[j])) >= 0.5f - error ? 1u << j : 0u;
+        for (int j = 0; j < 8; ++j) *doubt |= off(j) >= 0.5f - error ? 1u << j : 0u;
     return c[0] | static_cast<uint64_t>(c[1]) << 32;
 }
 
@@ -301,7 +327,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void norm_rows_kernel(RowArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) t[j] = near && !bad ? h[c][j] * w[c][j] : 0.0f;
             uint32_t doubt;
-            uint64_t codes = pack_codes(t, unit32, error, &doubt);
+            uint64_t codes = pack_codes<false>(t, unit32, error, 0.0f, &doubt);
             codes = settle_codes(codes, doubt, [&](int j) {
                 if (i + j >= a.n) return 0;
                 float again;
@@ -320,15 +346,13 @@ __global__ __launch_bounds__(64 * kMostWaves) void norm_rows_kernel(RowArgs a) {
     }
 }
 
-// The same in f32: the exponent -g log2 e as a sum of two numbers, so that 2^it is off
-// by 2 units of 2^-24 and not by |g| of them; the sum, its inverse and two products
-// make 8 at most.  A gate below -80 or a result past f32's range says nothing.
-constexpr float kGateError = 0x1p-20f;
+// The same in f32.  In units of 2^-24, 2^it is off by 1.22 |g| (the exponent -g log2 e and
+// its constant) and 2, which for g > 0 the sum with 1 makes less of; the sum, its inverse
+// and two products add 5: 17 units of t where g >= -8.  Below, 0.05 units of u are more than
+// (7 + 1.22 |g|) of t, and than t itself where 2^it or its inverse has left f32's range.
+constexpr float kGateError = 20 * 0x1p-24f, kFarGateError = 0.05f * 0x1p-24f;
 __device__ __forceinline__ float gated32(float g, float u) {
-    const float hi = g * -1.44269504088896341f;
-    const float lo = fmaf(g, -1.44269504088896341f, -hi) + g * -1.92596299e-8f;
-    const float e = __builtin_amdgcn_exp2f(hi);
-    return g * __builtin_amdgcn_rcpf(1.0f + fmaf(e, lo * 0.693147181f, e)) * u;
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f)) * u;
 }
 
 template <int TYPE, int CHUNKS>
@@ -339,11 +363,12 @@ __global__ __launch_bounds__(64 * kMostWaves) void swiglu_rows_kernel(RowArgs a)
     const int first = 8 * threadIdx.x, step = 8 * blockDim.x, waves = (blockDim.x + 63) >> 6;
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x, turn ^= 1) {
+        auto place = [&](int b) { return first + (b >> 3) * step + (b & 7); };  // in the row, of a thread's value b
         auto exact = [&](int i) {
             if (i >= a.n) return 0.0;
-            return gated(value_at(a.x, TYPE, row * a.x_stride + i), value_at(a.y, TYPE, row * a.y_stride + i));
+            return gated<false>(value_at(a.x, TYPE, row * a.x_stride + i), value_at(a.y, TYPE, row * a.y_stride + i));
         };
-        float t[CHUNKS][8], top = 0.0f, low = 0.0f, odd = 0.0f;
+        float t[CHUNKS][8], top = 0.0f, wide = 0.0f;
         {
             typename RowElem<TYPE>::Raw8 g[CHUNKS], u[CHUNKS];
             load_row<TYPE, CHUNKS>(row_at(a.x, TYPE, row * a.x_stride), a.n, g);
@@ -352,47 +377,62 @@ __global__ __launch_bounds__(64 * kMostWaves) void swiglu_rows_kernel(RowArgs a)
             for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float x = static_cast<float>(g[c][j]);
-                    t[c][j] = gated32(x, static_cast<float>(u[c][j]));
-                    low = fminf(low, x);
-                    top = fmaxf(top, fabsf(t[c][j]));
-                    odd = fmaf(t[c][j], 0.0f, odd);  // NaN where t is not finite
+                    const float y = static_cast<float>(u[c][j]);
+                    t[c][j] = gated32(static_cast<float>(g[c][j]), y);
+                    top = __builtin_elementwise_maximum(top, fabsf(t[c][j]));  // NaN stays
+                    wide = fmaxf(wide, fabsf(y));
                 }
         }
         // the row's largest in f32, infinite where f32 will not do
-        const float wave_top = wave_max(low >= -80.0f && odd == 0.0f ? top : INFINITY);
+        const float wave_top = wave_max(top == top ? top : INFINITY);
         if ((threadIdx.x & 63) == 0) tops[turn][threadIdx.x >> 6] = wave_top;
         if (threadIdx.x == 0) largest[turn] = 0;
         __syncthreads();
         float all = 0.0f;
         for (int w = 0; w < waves; ++w) all = fmaxf(all, tops[turn][w]);
         uint64_t codes[CHUNKS];
-        uint32_t doubt[CHUNKS];
+        uint32_t doubt = 0;  // a bit for each of the thread's values
         double most, unit;
-        if (in_range(all)) {
-            // the value or two of the row that its largest may be, in 64 bits
+        bool quick = in_range(all);
+        if (quick) {
+            // The value or two of the row that its largest may be, in 64 bits.  A thread with
+            // a u so large that t may be off by more than kGateError of the largest takes all of
+            // its values, and has all codes in doubt.
             const float at_least = all * (1.0f - 4.0f * kGateError);
-            if (top >= at_least)
+            const bool far = wide > 256.0f * all;
+            if (top >= at_least || far) {
+                uint32_t left = 0;
 #pragma unroll
-                for (int c = 0; c < CHUNKS; ++c) {
-                    uint32_t left = 0;
+                for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) left |= fabsf(t[c][j]) >= at_least ? 1u << j : 0u;
-                    while (left) {
-                        const double x = fabs(exact(first + c * step + __builtin_ctz(left)));
-                        left &= left - 1;
-                        atomicMax(&largest[turn], __builtin_bit_cast(unsigned long long, x));
-                    }
+                    for (int j = 0; j < 8; ++j) left |= fabsf(t[c][j]) >= at_least ? 1u << (8 * c + j) : 0u;
+                if (far) left = ~0u;
+                for (; left; left &= left - 1) {
+                    const int b = __builtin_ctz(left);
+                    if (b >= 8 * CHUNKS) break;
+                    const double x = fabs(exact(place(b)));
+                    atomicMax(&largest[turn], __builtin_bit_cast(unsigned long long, x));
                 }
-            // meanwhile the codes by the f32 one: both are off by kGateError at most
+            }
+            // meanwhile the codes by the f32 one: both are off by kGateError, the quotient by 5
+            // units of 2^-24
             const float unit32 = 127.0f / all;
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) codes[c] = pack_codes(t[c], unit32, 128.0f * 2.5f * kGateError, &doubt[c]);
+            for (int c = 0; c < CHUNKS; ++c) {
+                uint32_t d;
+                codes[c] = pack_codes<true>(t[c], unit32, fmaf(kFarGateError * wide, unit32, 1e-6f),
+                                            (2.0f * kGateError + 8 * 0x1p-24f) * unit32, &d);
+                doubt |= d << (8 * c);
+            }
+            if (far) doubt = ~0u;
             __syncthreads();
             most = __builtin_bit_cast(double, largest[turn]);
             unit = 127.0 / most;
-            if (threadIdx.x == 0) a.scales[row] = static_cast<float>(most / 127.0);
-        } else {
+            // (the largest in f32 may be one of such a thread's)
+            quick = fabs(most - all) <= all * (1.25 * kGateError);
+            if (quick && threadIdx.x == 0) a.scales[row] = static_cast<float>(most / 127.0);
+        }
+        if (!quick) {
             double sum = most = 0.0;
             for (int i = first; i < a.n; i += step)
                 for (int j = 0; j < 8; ++j) {
@@ -406,18 +446,18 @@ __global__ __launch_bounds__(64 * kMostWaves) void swiglu_rows_kernel(RowArgs a)
             unit = zero ? 0.0 : 127.0 / most;
             if (threadIdx.x == 0) a.scales[row] = bad ? __builtin_nanf("") : static_cast<float>(most / 127.0);
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                codes[c] = 0;
-                doubt[c] = zero ? 0 : 255;
-            }
+            for (int c = 0; c < CHUNKS; ++c) codes[c] = 0;
+            doubt = zero ? 0 : ~0u;
         }
         int8_t *q = a.q + row * a.q_stride;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const int i = first + c * step;
-            if (i >= a.n) break;
-            codes[c] = settle_codes(codes[c], doubt[c], [&](int j) { return code_of(exact(i + j), most, unit); });
-            row_store_codes(q, i, a.n, static_cast<uint32_t>(codes[c]), static_cast<uint32_t>(codes[c] >> 32));
+        for (int c = 0; c < CHUNKS; ++c)
+            if (first + c * step < a.n)
+                row_store_codes(q, first + c * step, a.n, static_cast<uint32_t>(codes[c]), static_cast<uint32_t>(codes[c] >> 32));
+        // codes in doubt once more
+        for (; doubt; doubt &= doubt - 1) {
+            const int b = __builtin_ctz(doubt), i = place(b);
+            if (b < 8 * CHUNKS && i < a.n) q[i] = static_cast<int8_t>(code_of(exact(i), most, unit));
         }
     }
 }
