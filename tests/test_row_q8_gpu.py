@@ -278,3 +278,19 @@ def test_rows_far_apart(ctx):
     finally:
         far.free()
         c.free()
+
+
+@pytest.mark.parametrize("n", [64, 2048, 9000, 20000])
+def test_swiglu_closed_gates_that_large_factors_meet(ctx, n):
+    """A few of them among ordinary values: products that are next to nothing, about as large
+    as the rest, the row's largest, and of gates whose exponential leaves f32's range."""
+    rng = np.random.default_rng([n, 3])
+    g, u = rng.standard_normal((8, n)), rng.standard_normal((8, n))
+    at = rng.integers(0, n, 5)
+    for r, (gate, factor) in enumerate([(-30, 1e12), (-30, 1e14), (-60, 1e25), (-86, 1e37), (-95, 3e38), (-9, 2e3),
+                                        (-1e4, 3e38), (-20, 300)]):
+        g[r, at] = gate * rng.uniform(0.99, 1.01, 5)
+        u[r, at] = factor * rng.uniform(0.5, 1, 5)
+    swiglu_case(ctx, 8, n, F32, g=g, u=u)
+    swiglu_case(ctx, 8, n, BF16, g=g, u=u)
+    swiglu_case(ctx, 8, n, F16, g=np.clip(g, -6e4, 6e4), u=np.clip(u, -6e4, 6e4))

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void row_q8_kernel(RowArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (!zero) c[j >> 2] |= (static_cast<uint32_t>(code_of(t[j], most, unit)) & 255u) << (8 * (j & 3));
-            row_store_codes(a.q + row * a.q_stride, i, a.n, c[0], c[1]);
+            row_store_codes(a.q + row * a.q_stride, i, a.n, static_cast<uint64_t>(c[1]) << 32 | c[0]);
         }
     }
 }
@@ -193,10 +193,21 @@ __global__ __launch_bounds__(64 * kMostWaves) void row_q8_kernel(RowArgs a) {
 constexpr int kMostChunks = 4;
 constexpr int kMostHeld = 8 * kMostChunks * 64 * kMostWaves;
 
+// Whether all threads' runs number c lie in the row, which the whole workgroup asks at once.
+__device__ __forceinline__ bool all_in(int c, int n) { return 8 * (c + 1) * static_cast<int>(blockDim.x) <= n; }
+
 template <int TYPE, int CHUNKS>
 __device__ __forceinline__ void load_row(const void *p, int n, typename RowElem<TYPE>::Raw8 *r) {
+    const int first = 8 * threadIdx.x, step = 8 * blockDim.x;
+    if (CHUNKS == 1) {
+        r[0] = row_load8<TYPE>(p, first, n);
+        return;
+    }
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) r[c] = row_load8<TYPE>(p, 8 * (c * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)), n);
+    for (int c = 0; c < CHUNKS; ++c) r[c] = row_load8_near<TYPE>(p, first + c * step, n);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+        if (!all_in(c, n)) row_end(r[c], first + c * step, n);
 }
 
 // Codes, a byte each, of t * unit with `unit` next to 127 / most: 1.5 * 2^23 is added in
@@ -260,18 +271,14 @@ __global__ __launch_bounds__(64 * kMostWaves) void norm_rows_kernel(RowArgs a) {
     typedef typename RowElem<kRes>::T ResT;
     __shared__ double lds[2][kMostWaves][2];
     const int first = 8 * threadIdx.x, step = 8 * blockDim.x;
-    float w[CHUNKS][8];
+    typename RowElem<MI355X_TYPE_F32>::Raw8 w[CHUNKS];
+    if (a.norm) {
+        load_row<MI355X_TYPE_F32, CHUNKS>(a.norm, a.n, w);
+    } else {
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        const int i = first + c * step;
-        if (a.norm) {
-            const auto r = row_load8<MI355X_TYPE_F32>(a.norm, i, a.n);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[c][j] = r[j];
-        } else {
+        for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[c][j] = 1.0f;
-        }
     }
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x, turn ^= 1) {
@@ -341,7 +348,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void norm_rows_kernel(RowArgs a) {
                 const double t = static_cast<double>(again) * (a.norm ? static_cast<double>(a.norm[i + j]) : 1.0);
                 return code_of(t, most, unit);
             });
-            row_store_codes(q, i, a.n, static_cast<uint32_t>(codes), static_cast<uint32_t>(codes >> 32));
+            row_store_codes(q, i, a.n, codes);
         }
     }
 }
@@ -452,8 +459,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void swiglu_rows_kernel(RowArgs a)
         int8_t *q = a.q + row * a.q_stride;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
-            if (first + c * step < a.n)
-                row_store_codes(q, first + c * step, a.n, static_cast<uint32_t>(codes[c]), static_cast<uint32_t>(codes[c] >> 32));
+            row_store_codes(q, first + c * step, a.n, codes[c]);
         // codes in doubt once more
         for (; doubt; doubt &= doubt - 1) {
             const int b = __builtin_ctz(doubt), i = place(b);

@@ -46,6 +46,26 @@ __device__ __forceinline__ typename RowElem<TYPE>::Raw8 row_load8(const void *ro
     return r;
 }
 
+// Values 1 .. 7 of eight, and a zero.
+template <class R>
+__device__ __forceinline__ R shifted(R r) {
+    return __builtin_shufflevector(r, R{}, 1, 2, 3, 4, 5, 6, 7, 8);
+}
+
+// The same without a branch, of a row of 8 or more: a run that the row ends in is taken from
+// the row's last eight, as row_end then has to put right.
+template <int TYPE>
+__device__ __forceinline__ typename RowElem<TYPE>::Raw8 row_load8_near(const void *row, int i, int n) {
+    typedef typename RowElem<TYPE>::T T;
+    return *reinterpret_cast<const typename RowElem<TYPE>::Raw8 *>(static_cast<const T *>(row) + min(i, n - 8));
+}
+template <class R>
+__device__ __forceinline__ void row_end(R &r, int i, int n) {
+#pragma unroll 1
+    for (int k = min(i + 8 - n, 8); k > 0; --k) r = shifted(r);
+}
+
+// (The tail's loops are not unrolled: their conditions would take a kernel's scalar registers.)
 template <int TYPE>
 __device__ __forceinline__ void row_store8(void *row, int i, int n, typename RowElem<TYPE>::Raw8 r) {
     typedef typename RowElem<TYPE>::T T;
@@ -54,22 +74,20 @@ __device__ __forceinline__ void row_store8(void *row, int i, int n, typename Row
     if (i + 8 <= n) {
         *reinterpret_cast<R *>(p) = r;
     } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j < n) p[j] = r[j];
+#pragma unroll 1
+        for (int j = 0; i + j < n; ++j, r = shifted(r)) p[j] = r[0];
     }
 }
 
 // Eight codes, a byte each, to codes i .. i + 7 of a row of n.
-__device__ __forceinline__ void row_store_codes(int8_t *row, int i, int n, uint32_t lo, uint32_t hi) {
-    typedef uint32_t U2 __attribute__((ext_vector_type(2), aligned(1)));
+__device__ __forceinline__ void row_store_codes(int8_t *row, int i, int n, uint64_t codes) {
+    typedef uint64_t U8 __attribute__((aligned(1)));
     int8_t *p = row + i;
     if (i + 8 <= n) {
-        *reinterpret_cast<U2 *>(p) = U2{lo, hi};
+        *reinterpret_cast<U8 *>(p) = codes;
     } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i + j < n) p[j] = static_cast<int8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+#pragma unroll 1
+        for (int j = 0; i + j < n; ++j, codes >>= 8) p[j] = static_cast<int8_t>(codes);
     }
 }
 
