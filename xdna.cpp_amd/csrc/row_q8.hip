@@ -111,38 +111,20 @@ __device__ __forceinline__ void norm_values(const RowArgs &a, int64_t row, int i
     }
 }
 
-// e^x in 64 bits: 2^k times a polynomial on +-(log 2) / 2, of which 4e-18 is left out.  Its
-// loop is unrolled where it is a kernel's work, and else not, so that its numbers do not
-// take up the registers of the values (4096 gated rows of 14336: 90 us with them).
-__constant__ double kInverses[14] = {0.0,     1.0,     1.0 / 2, 1.0 / 3,  1.0 / 4,  1.0 / 5,  1.0 / 6,
-                                     1.0 / 7, 1.0 / 8, 1.0 / 9, 1.0 / 10, 1.0 / 11, 1.0 / 12, 1.0 / 13};
-template <bool UNROLLED>
-__device__ __forceinline__ double exp64(double x) {
-    x = fmin(fmax(x, -800.0), 800.0);  // 0 and infinity
-    const double k = rint(x * 1.4426950408889634), r = fma(k, -2.3190468138462996e-17, fma(k, -0.6931471805599453, x));
-    double p = 1.0;
-    if (UNROLLED) {
-#pragma unroll
-        for (int n = 13; n > 0; --n) p = fma(p, r * (1.0 / n), 1.0);
-    } else {
-#pragma unroll 1
-        for (int n = 13; n > 0; --n) p = fma(p, r * kInverses[n], 1.0);
-    }
-    return ldexp(p, static_cast<int>(k));
-}
-
-template <bool UNROLLED>
 __device__ __forceinline__ double gated(float g, float u) {
     const double d = g;
-    return d / (1.0 + exp64<UNROLLED>(-d)) * static_cast<double>(u);
+    return d / (1.0 + exp(-d)) * static_cast<double>(u);
 }
+// For single values: a function of its own, so that the exponential's numbers do not take up
+// the registers of a kernel's values (4096 gated rows of 14336: 90 us with them).
+__device__ __attribute__((noinline)) double gated_value(float g, float u) { return gated(g, u); }
 
 __device__ __forceinline__ void swiglu_values(const RowArgs &a, int64_t row, int i, double *t) {
     float g[8], u[8];
     load_as_float(row_at(a.x, a.type, row * a.x_stride), a.type, i, a.n, g);
     load_as_float(row_at(a.y, a.type, row * a.y_stride), a.type, i, a.n, u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = gated<true>(g[j], u[j]);
+    for (int j = 0; j < 8; ++j) t[j] = gated(g[j], u[j]);
 }
 
 // Rows longer than a workgroup's registers: the values formed twice, for the largest
@@ -373,7 +355,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void swiglu_rows_kernel(RowArgs a)
         auto place = [&](int b) { return first + (b >> 3) * step + (b & 7); };  // in the row, of a thread's value b
         auto exact = [&](int i) {
             if (i >= a.n) return 0.0;
-            return gated<false>(value_at(a.x, TYPE, row * a.x_stride + i), value_at(a.y, TYPE, row * a.y_stride + i));
+            return gated_value(value_at(a.x, TYPE, row * a.x_stride + i), value_at(a.y, TYPE, row * a.y_stride + i));
         };
         float t[CHUNKS][8], top = 0.0f, wide = 0.0f;
         {
