@@ -170,6 +170,11 @@ __global__ __launch_bounds__(64 * kMostWaves) void row_q8_kernel(RowArgs a) {
 
 // ---- rows held in registers ------------------------------------------------------
 
+// One pass: a row is read once, its sum of squares and its largest magnitude meet in one
+// reduction over the workgroup, and codes leave from registers.  Bound by memory: the norm
+// of 8192 rows of 8192 in bf16 with its residual, 470 MB, takes 91 us (5.2 TB/s, as a copy);
+// gates of 4096 x 14336 in bf16, 294 MB, 63 us (4.7 TB/s; besides memory some 20 vector
+// operations and two of a quarter's rate a value).  One row: what a launch takes, 4 and 5 us.
 // A thread has CHUNKS runs of 8 values, so rows of up to 8 * CHUNKS * threads values
 // are read once.
 constexpr int kMostChunks = 4;
@@ -454,17 +459,19 @@ __global__ __launch_bounds__(64 * kMostWaves) void swiglu_rows_kernel(RowArgs a)
 
 // Threads, and runs of 8 values of each: as many threads as there are runs for few
 // rows, so that a row's latency is short (one row of 8192 4.2 us, with 4 runs a thread
-// 5.6); 256 or more with up to 4 runs each for many, so that fewer threads meet at a
-// row's barriers (8192 rows of 8192, one run a thread 117 us, 4 runs 91; without a
-// residual 105, 48; 4096 gated rows of 14336 96, 80; rows of 2048 25, 32).
+// 4.9); for many rows up to 4 runs each, so that fewer threads meet at a row's barriers,
+// while 256 threads are left, or 128 where a value is much work (300 rows of 8192, one, two
+// and four runs a thread 8.9, 7.9, 9.1; 8192 rows of 8192 116, 94, 91; without a residual
+// 94, 56, 45; rows of 2048 26, 27, 31; 4096 gated rows of 14336 76, 76, 63; 8192 of 2048 25,
+// 21, 21).
 struct RowShape {
     int threads, chunks;
 };
-RowShape row_shape(const mi355x_ctx *ctx, const RowArgs &a) {
+RowShape row_shape(const mi355x_ctx *ctx, const RowArgs &a, int fewest) {
     const int runs = (a.n + 7) / 8, most = 64 * kMostWaves;
     const int least = (runs + most - 1) / most;
     const int wanted = a.n_rows >= 4 * ctx->num_cus ? 4 : a.n_rows >= ctx->num_cus ? 2 : 1;
-    int chunks = std::max(least, std::min(wanted, runs / 256));
+    int chunks = std::max(least, std::min(wanted, runs / fewest));
     chunks = chunks <= 1 ? 1 : chunks <= 2 ? 2 : 4;
     return {std::min(most, ((runs + chunks - 1) / chunks + 63) / 64 * 64), chunks};
 }
@@ -487,7 +494,7 @@ int launch_long(mi355x_ctx *ctx, const RowArgs &a) {
 
 template <int XT, int RT>
 int launch_norm(mi355x_ctx *ctx, const RowArgs &a) {
-    const RowShape s = row_shape(ctx, a);
+    const RowShape s = row_shape(ctx, a, 256);
     unsigned groups = row_groups(a);
     if (s.chunks > 1) {  // workgroups keep the norm's weights over several rows (8192 rows of 8192: 91 us, 95 without)
         const int64_t per = (a.n_rows + 8 * ctx->num_cus - 1) / (8 * ctx->num_cus);
@@ -510,7 +517,7 @@ int launch_norm_of(mi355x_ctx *ctx, const RowArgs &a) {
 
 template <int TYPE>
 int launch_swiglu(mi355x_ctx *ctx, const RowArgs &a) {
-    const RowShape s = row_shape(ctx, a);
+    const RowShape s = row_shape(ctx, a, 128);
     return by_chunks(s.chunks, [&](auto c) {
         swiglu_rows_kernel<TYPE, decltype(c)::value><<<row_groups(a), s.threads, 0, ctx->stream>>>(a);
         MI355X_HIP(hipGetLastError());
