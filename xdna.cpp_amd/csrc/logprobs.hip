@@ -14,6 +14,7 @@
 // made again with the last bound, and failing that the row is searched n times.
 #include "far_parts.h"
 #include "internal.h"
+#include "paged_index.h"
 #include "row_values.h"
 
 #include <algorithm>
@@ -33,6 +34,9 @@ constexpr int kMostParts = 64;
 constexpr int kMostItems = 1024;                  // parts of a call's rows
 constexpr int kPartFloats = 4 + 2 * MI355X_LOGPROBS_MAX_TOP;
 constexpr size_t kCounterBytes = 4 * kMostItems;
+// Top tokens up to which the bound is formed of 64 numbers, each the largest of a lane's
+// logits in the four wavefronts, and not of all 256: fewer steps, a few more entries.
+constexpr int kFewTop = 32;
 
 struct LogitArgs {
     int64_t n_rows, stride;
@@ -40,6 +44,7 @@ struct LogitArgs {
     int n_vocab, n_tokens, n_top;
     float scale;
     int parts, part_len;  // of a row; part_len is a multiple of kStep
+    FastDiv by_top;       // n_top, or 1
     const int32_t *tokens;
     float *token_logprobs, *entropy, *top_logprobs;
     int32_t *top_tokens;
@@ -284,13 +289,19 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
 #pragma unroll
                 for (int i = 0; i < kWaves; ++i) v[i] = l.tops[turn][64 * i + lane];
                 turn ^= 1;
+                const float of_lane = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
                 if (n > 0) {
                     uint32_t ranks[kWaves];
+                    if (n <= kFewTop) {
+                        ranks[0] = rank_of(of_lane);
+                        bound = bound_of(nth_largest<1>(ranks, n));
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < kWaves; ++i) ranks[i] = rank_of(v[i]);
-                    bound = bound_of(nth_largest<kWaves>(ranks, n));
+                        for (int i = 0; i < kWaves; ++i) ranks[i] = rank_of(v[i]);
+                        bound = bound_of(nth_largest<kWaves>(ranks, n));
+                    }
                 }
-                sums.raise(wave_max(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))), k);
+                sums.raise(wave_max(of_lane), k);
             }
             sums.raise(most, k);
 #pragma unroll
@@ -365,7 +376,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
                 uint64_t entry[kList / kThreads];  // all on their way before one is waited for
 #pragma unroll
                 for (int i = 0; i < kList / kThreads; ++i) {
-                    const int j = min(i * kThreads + tid, total - 1), q = n > 0 ? j / n : 0;
+                    const int j = min(i * kThreads + tid, total - 1), q = divided(j, a.by_top);
                     entry[i] = kNoEntry;
                     if (i * kThreads < total)
                         entry[i] = __builtin_bit_cast(uint64_t, far.load2((first + q) * kPartFloats + 4 + 2 * (j - q * n)));
@@ -384,9 +395,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
                 __syncthreads();
                 if (n > 0)
                     found = order_list(l, total, n, [&]() {
-                        // the n-th largest of the first few of each part
-                        const int few = min(n, kThreads / a.parts);
+                        // the n-th largest of the first of each part, or of its first few
                         uint32_t ranks[kWaves];
+                        if (2 * n <= a.parts + 8) {
+                            ranks[0] = lane < a.parts ? static_cast<uint32_t>(l.list[lane * n] >> 32) : 0;
+                            return nth_largest<1>(ranks, n);
+                        }
+                        const int few = min(n, kThreads / a.parts);
 #pragma unroll
                         for (int i = 0; i < kWaves; ++i) {
                             const int j = 64 * i + lane, q = j / few;
@@ -423,6 +438,7 @@ int launch_logprobs(mi355x_ctx *ctx, const mi355x_logprobs_args &u) {
     a.n_vocab = u.n_vocab;
     a.n_tokens = u.n_tokens;
     a.n_top = u.n_top;
+    a.by_top = fast_div(static_cast<uint32_t>(std::max(u.n_top, 1)));
     a.scale = u.scale;
     a.tokens = u.tokens;
     a.token_logprobs = u.token_logprobs;
