@@ -89,7 +89,8 @@ MI355X_API int mi355x_swiglu_q8(mi355x_ctx *ctx, const mi355x_swiglu_q8_args *ar
  * may be -128); it is rounded to f32, multiplied and added to in f32 in this
  * order, and rounded once to out_type.  x, w: 16-byte aligned, rows of a multiple
  * of 16 codes, strides multiples of 16.  The result does not depend on how the
- * work is split.
+ * work is split.  MI355X_EUNSUPPORTED: 2^34 outputs or more, and more than 64 *
+ * 65535 rows where a stride passes 2^23.
  *
  * workspace: mi355x_matmul_q8_workspace bytes, 16-byte aligned.  Zero it once,
  * before its first call (mi355x_fill): it begins with counters that every call

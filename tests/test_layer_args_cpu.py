@@ -143,3 +143,14 @@ def test_the_reference_rounds_ties_to_even():
 def test_scales_past_their_limits(host):
     for scale, want in [(2.0 ** 100, EHIP), (2.0 ** -100, EHIP), (2.0 ** 101, EINVAL), (2.0 ** -101, EINVAL)]:
         assert rc(host, "mi355x_logprobs", logprobs(scale=scale)) == want
+
+
+def test_products_too_large(host):
+    wide = dict(out_stride=2 ** 24)
+    for over, want in [
+            (dict(wide, n_rows=1024, n_out=2 ** 24), mi355x.EUNSUPPORTED), (dict(wide, n_rows=1023, n_out=2 ** 24), EHIP),
+            (dict(n_rows=64 * 65535 + 1, x_stride=2 ** 23 + 16), mi355x.EUNSUPPORTED),
+            (dict(n_rows=64 * 65535 + 1, w_stride=2 ** 23 + 16), mi355x.EUNSUPPORTED),
+            (dict(n_rows=64 * 65535, x_stride=2 ** 23 + 16), EHIP),
+            (dict(n_rows=64 * 65535 + 1, x_stride=2 ** 23), EHIP)]:
+        assert rc(host, "mi355x_matmul_q8", matmul(**over)) == want

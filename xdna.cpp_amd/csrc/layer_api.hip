@@ -151,6 +151,11 @@ int mi355x_matmul_q8(mi355x_ctx *ctx, const mi355x_matmul_q8_args *args) {
     if (int rc = check_rows_at(who, "w", a.w, 16, a.n_out, a.w_stride, a.k)) return rc;
     if (a.x_stride % 16 != 0 || a.w_stride % 16 != 0)
         return invalid(who, "x_stride and w_stride must be multiples of 16");
+    if (a.n_rows * a.n_out >= int64_t(1) << 34)
+        return set_error(MI355X_EUNSUPPORTED, std::string(who) + ": 2^34 outputs or more");
+    // (a grid's second side has 16 bits)
+    if (a.n_rows > 64 * 65535 && (a.x_stride > (1 << 23) || a.w_stride > (1 << 23)))
+        return set_error(MI355X_EUNSUPPORTED, std::string(who) + ": more than 64 * 65535 rows with a stride past 2^23");
     if (int rc = check_vector(who, "x_scales", a.x_scales)) return rc;
     if (int rc = check_vector(who, "w_scales", a.w_scales)) return rc;
     if (a.bias)

@@ -758,12 +758,8 @@ int launch_matmul_q8(mi355x_ctx *ctx, const mi355x_matmul_q8_args &u) {
     a.n = static_cast<int>(u.n_out);
     a.k = static_cast<int>(u.k);
     a.out_type = u.out_type;
-    // the tile kernels form offsets of up to 256 rows in 32 bits, and a grid's second side has 16
+    // the tile kernels form offsets of up to 256 rows in 32 bits
     const bool far = u.x_stride > (1 << 23) || u.w_stride > (1 << 23);
-    if (static_cast<int64_t>(a.m) * a.n >= int64_t(1) << 34)
-        return set_error(MI355X_EUNSUPPORTED, "mi355x_matmul_q8: 2^34 outputs or more");
-    if (far && a.m > 64 * 65535)
-        return set_error(MI355X_EUNSUPPORTED, "mi355x_matmul_q8: more than 64 * 65535 rows with strides past 2^23");
     // Up to 32 rows have the weight in flight in each wavefront by itself; blocks of 32
     // channels where that fills the CUs, else of 16 so that more workgroups share the work
     // (16, then 32 channels; us: one row of 2048, k 11008 7.6, 10.4; of 8192, k 8192 12.9, 12.9;
