@@ -274,3 +274,9 @@ def test_scales_at_their_limits(ctx, ws):
     x = logits(2, 5000, 9)
     go(ctx, ws, x * 2.0 ** 100, F32, scale=2.0 ** -100)
     go(ctx, ws, x * 2.0 ** -100, F32, scale=2.0 ** 100)
+
+
+def test_more_rows_than_workgroups(ctx, ws):
+    T = (1 << 20) + 77
+    rng = np.random.default_rng(T)
+    go(ctx, ws, 3 * rng.standard_normal((T, 9)), F16, top=2)

@@ -294,3 +294,29 @@ def test_swiglu_closed_gates_that_large_factors_meet(ctx, n):
     swiglu_case(ctx, 8, n, F32, g=g, u=u)
     swiglu_case(ctx, 8, n, BF16, g=g, u=u)
     swiglu_case(ctx, 8, n, F16, g=np.clip(g, -6e4, 6e4), u=np.clip(u, -6e4, 6e4))
+
+
+@pytest.mark.parametrize("T", [256, 1025, 2500])
+@pytest.mark.parametrize("n", [2048, 2059, 4099, 6000])
+def test_many_rows_of_several_runs_a_thread(ctx, T, n):
+    """Workgroups that go through several rows, and rows that end inside a thread's runs."""
+    norm_case(ctx, T, n, BF16, BF16)
+    norm_case(ctx, T, n, F16, F32, alias="residual", pad=1)
+    norm_case(ctx, T, n, BF16, BF16, norm=False, alias="x")
+    swiglu_case(ctx, T, n, BF16, halves=True)
+    swiglu_case(ctx, T, n, F32, pad=3, shift=1)
+
+
+def test_infinities_among_many_rows(ctx):
+    """Rows that are not finite, or zero, between others that the same workgroup computes."""
+    x = values(2100, 4100, 5)
+    x[::7, 4099], x[1::7, 0], x[2::7] = np.inf, np.nan, 0
+    norm_case(ctx, 2100, 4100, F32, F32, x=x, res=np.zeros_like(x))
+    norm_case(ctx, 2100, 4100, BF16, x=x)
+    g, u = values(2100, 4100, 6, False), x
+    swiglu_case(ctx, 2100, 4100, F32, g=g, u=u)
+
+
+def test_more_rows_than_workgroups(ctx):
+    norm_case(ctx, (1 << 20) + 77, 9, BF16, BF16)
+    swiglu_case(ctx, (1 << 20) + 77, 9, BF16)
