@@ -206,3 +206,11 @@ def test_rows_far_apart(ctx, ws):
     finally:
         big.free()
         c.free()
+
+
+@pytest.mark.parametrize("M", [33, 47, 64, 100, 150])
+@pytest.mark.parametrize("N,K", [(17411, 1040), (22016, 144), (20011, 16), (5121, 17408), (8195, 4112)])
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_few_rows_of_many_channels(ctx, ws, M, N, K, t):
+    """Tiles whose weights come from memory, whole and in parts."""
+    go(ctx, ws, M, N, K, t, bias=M % 2 == 1)
