@@ -15,7 +15,7 @@
 //
 // Many rows, a workgroup each, are bound by memory: 2048 rows of 151936 in bf16, 622 MB,
 // take 112 us (5.6 TB/s), with 5 top tokens 116, 20 128, 64 153.  One row in f32, 38 parts:
-// 5.9 us, most of it a launch and a join, with 20 top tokens 10.2.
+// 5.9 us, most of it a launch and a join, with 20 top tokens 10.2; 64 rows 12.6 and 19.8.
 #include "far_parts.h"
 #include "internal.h"
 #include "paged_index.h"
@@ -37,7 +37,8 @@ constexpr int kList = 1024;
 constexpr int kMostParts = 64;
 constexpr int kMostItems = 1024;                  // parts of a call's rows
 constexpr int kPartFloats = 4 + 2 * MI355X_LOGPROBS_MAX_TOP;
-constexpr size_t kCounterBytes = 4 * kMostItems;
+constexpr int kCounterStep = 32;                  // ints from one row's counter to the next: a cache line
+constexpr size_t kCounterBytes = size_t(4) * kCounterStep * (kMostItems / 2);  // rows of two parts or more
 // Top tokens up to which the bound is formed of 64 numbers, each the largest of a lane's
 // logits in the four wavefronts, and not of all 256: fewer steps, a few more entries.
 constexpr int kFewTop = 32;
@@ -373,7 +374,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogitArgs a) {
             if (tid == 0) far.store4(at, f32x4{all, s, e, 0.0f});
             for (int r = tid; r < n; r += kThreads)
                 far.store2(at + 4 + 2 * r, __builtin_bit_cast(u32x2_a, r < found ? l.top[r] : kNoEntry));
-            if (last_of(a.counters + row, a.parts, &l.flag)) {
+            if (last_of(a.counters + kCounterStep * row, a.parts, &l.flag)) {
                 const int first = static_cast<int>(row) * a.parts, total = a.parts * n;  // at most kList
                 f32x4 p = {-INFINITY, 0.0f, 0.0f, 0.0f};  // the row's parts, one a lane
                 if (lane < a.parts) p = far.load4((first + lane) * kPartFloats);
@@ -451,10 +452,13 @@ int launch_logprobs(mi355x_ctx *ctx, const mi355x_logprobs_args &u) {
     a.top_tokens = u.top_tokens;
     a.counters = static_cast<int *>(u.workspace);
     a.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(u.workspace) + kCounterBytes);
-    // few rows are cut into parts of half a batch or more, so that a part is one round of loads
-    // (one row of 151936 with 20 top tokens in parts of 4096 10.2 us, of 8192 11.6; more parts
-    // than kMostItems did not gain: 64 rows 26.7)
-    int64_t parts = std::min<int64_t>(kMostItems / u.n_rows, (u.n_vocab + kBatch / 2 - 1) / (kBatch / 2));
+    // Few rows are cut into parts of half a batch or more, so that a part is one round of loads
+    // (one row of 151936 with 20 top tokens in parts of 4096 10.2 us, of 8192 11.6), as many
+    // as 4 workgroups a CU, or 3 with 32 bits, of which twice as much is under way (3, 4 and 8 a
+    // CU: 64 rows of 151936 in f32 19.8, 24.7, 27.6, in bf16 17.5, 16.8, 20.3; 400 of 50000 in f32
+    // 22, 32; 300 of 151936 in bf16 39, 35, 42).
+    const int items = std::min(kMostItems, (u.type == MI355X_TYPE_F32 ? 3 : 4) * ctx->num_cus);
+    int64_t parts = std::min<int64_t>(items / u.n_rows, (u.n_vocab + kBatch / 2 - 1) / (kBatch / 2));
     parts = std::min<int64_t>(parts, std::min(kMostParts, kList / std::max(u.n_top, 1)));
     parts = std::max<int64_t>(parts, 1);
     a.part_len = static_cast<int>((u.n_vocab + kStep * parts - 1) / (kStep * parts) * kStep);
