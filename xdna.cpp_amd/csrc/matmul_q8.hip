@@ -21,6 +21,8 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+constexpr int kCounterStep = 32;  // ints from one tile's counter to the next: a cache line
+
 struct MatmulArgs {
     int64_t x_stride, w_stride, out_stride;
     const int8_t *x, *w;
@@ -443,7 +445,7 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a)
         for (int i = 0; i < TN; ++i)
 #pragma unroll
             for (int j = 0; j < TM; ++j) far.store4(to + 256 * (i * TM + j), __builtin_bit_cast(f32x4, c[i][j]));
-        if (!last_of(a.counters + tile, a.splits, reinterpret_cast<int *>(lds))) return;
+        if (!last_of(a.counters + kCounterStep * tile, a.splits, reinterpret_cast<int *>(lds))) return;
         for (int p = 0; p < a.splits; ++p) {
             if (p == split) continue;
             const int from = (p * tiles + tile) * BM * BN + mine;
@@ -634,7 +636,7 @@ __global__ __launch_bounds__(kLargeThreads) __attribute__((amdgpu_waves_per_eu(2
 
 // ---- the choice ---------------------------------------------------------------
 
-constexpr size_t kCounters = 4096;
+constexpr size_t kCounters = size_t(4) * kCounterStep * 1024;
 constexpr size_t kPartBytes = size_t(64) << 20;
 
 template <int TM, int R, int WAVES, int ST>
@@ -718,7 +720,7 @@ Choice choose(const mi355x_ctx *ctx, const MatmulArgs &a) {
         for (int s = 1; s <= g.most_splits && s <= stages; ++s) {
             const int64_t groups = tiles * s;
             // (parts in more than one round did not gain: 37 x 17408, k 5120 in 5 parts 31 us, whole 27)
-            if (s > 1 && (groups > ctx->num_cus * g.per_cu || tiles > static_cast<int64_t>(kCounters / 4) ||
+            if (s > 1 && (groups > ctx->num_cus * g.per_cu || tiles > static_cast<int64_t>(kCounters / (4 * kCounterStep)) ||
                           groups * tile_bytes > static_cast<int64_t>(kPartBytes)))
                 break;
             const float rounds = std::ceil(static_cast<float>(groups) / static_cast<float>(ctx->num_cus * g.per_cu));
