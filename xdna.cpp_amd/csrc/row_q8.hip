@@ -194,7 +194,7 @@ __device__ __forceinline__ void load_row(const void *p, int n, typename RowElem<
     for (int c = 0; c < CHUNKS; ++c) r[c] = row_load8_near<TYPE>(p, first + c * step, n);
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
-        if (!all_in(c, n)) row_end(r[c], first + c * step, n);
+        if (!all_in(c, n)) row_end<TYPE>(r[c], first + c * step, n);
 }
 
 // Codes, a byte each, of t * unit with `unit` next to 127 / most: 1.5 * 2^23 is added in

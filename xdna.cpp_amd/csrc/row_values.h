@@ -59,8 +59,8 @@ __device__ __forceinline__ typename RowElem<TYPE>::Raw8 row_load8_near(const voi
     typedef typename RowElem<TYPE>::T T;
     return *reinterpret_cast<const typename RowElem<TYPE>::Raw8 *>(static_cast<const T *>(row) + min(i, n - 8));
 }
-template <class R>
-__device__ __forceinline__ void row_end(R &r, int i, int n) {
+template <int TYPE>
+__device__ __forceinline__ void row_end(typename RowElem<TYPE>::Raw8 &r, int i, int n) {
 #pragma unroll 1
     for (int k = min(i + 8 - n, 8); k > 0; --k) r = shifted(r);
 }
