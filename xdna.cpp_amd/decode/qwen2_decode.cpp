@@ -223,7 +223,7 @@ struct qd_model {
     int attention = QD_ATTENTION_HOST;
     int logprobs = -1;  // top tokens of each generated one; -1: no log probabilities
     // of the last generation's tokens: top tokens (last_top of each, the first of them the
-    // token itself) with their log probabilities, and entropies
+    // token itself, or -1 where there is none) with their log probabilities, and entropies
     int last_top = -1;  // -1: it had none
     std::vector<int32_t> last_top_tokens;
     std::vector<float> last_top_logprobs, last_entropies;
@@ -1085,24 +1085,26 @@ int generate_gpu_attention(qd_model *m, const int32_t *prompt, int n_prompt, int
             top_tokens.insert(top_tokens.end(), d.top_tokens(), d.top_tokens() + d.top);
             top_logprobs.insert(top_logprobs.end(), d.top_logprobs(), d.top_logprobs() + d.top);
             entropies.push_back(d.entropy());
-            // logits without a largest one (NaN) have no top token
-            out_tokens[i] = tok = std::max(d.top_tokens()[0], 0);
-        } else {
-            out_tokens[i] = tok = argmax(logits.data(), m->c.vocab);
+            tok = d.top_tokens()[0];
         }
+        if (!d.top || tok < 0) {  // -1: NaN or +inf among the logits, or -inf alone
+            if (d.top && d.read_logits(logits.data())) return -1;
+            tok = argmax(logits.data(), m->c.vocab);
+        }
+        out_tokens[i] = tok;
+        return 0;
     };
     const double t_start = now();
     for (int at = 0; at < n_prompt; at += QD_CHUNK_ROWS) {
         const int n = std::min(QD_CHUNK_ROWS, n_prompt - at);
         if (d.pass(prompt + at, n, at + n == n_prompt && n_gen > 0, logits.data())) return failed();
     }
-    if (n_gen > 0) take(0);
+    if (n_gen > 0 && take(0)) return failed();
     const double t_gen0 = now();
     d.t_gpu = 0.0;
     d.launches = 0;
     for (int i = 1; i < n_gen; ++i) {
-        if (d.pass(&tok, 1, true, logits.data())) return failed();
-        take(i);
+        if (d.pass(&tok, 1, true, logits.data()) || take(i)) return failed();
     }
     const double t_end = now();
     if (n_gen > 0 && d.top && d.read_logits(logits.data())) return failed();

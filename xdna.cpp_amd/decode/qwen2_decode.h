@@ -149,7 +149,10 @@ QD_API int qd_set_attention(qd_model *m, int mode);
  * MI355X_LOGPROBS_MAX_TOP: mi355x_logprobs on the logits where the vocabulary
  * GEMV leaves them, with the entropy and n_top most likely tokens.  The greedy
  * token is then the GPU's first top token, and logits come to the host for the
- * last token alone. */
+ * last token alone, and where there is no top token (NaN or +inf among them, or
+ * -inf alone): the token is then the one that n_top -1 gives, with the log
+ * probability, entropy and top tokens that mi355x_logprobs states (NaN or -inf,
+ * and -1). */
 QD_API int qd_set_logprobs(qd_model *m, int n_top);
 /* Of the n = n_gen tokens of the last qd_generate: their log probabilities, the
  * entropies, and n * n_top tokens and log probabilities (each may be NULL).  n_top: up
