@@ -43,9 +43,13 @@ extern "C" {
  *   h_i = x_i + residual_i, in f32, rounded to residual_type (without a residual
  *         h_i = x_i as it is); stored in residual_out where one is given
  *   t_i = h_i * norm_i / sqrt(mean_j(h_j^2) + eps)
- * The mean is summed in 64 bits.  Without norm t_i = h_i: rows are only put in 8
- * bits, and eps is not used.  residual_out may be residual or x (same type and
- * stride as that). */
+ * The mean is summed in 64 bits.  The root, which a whole row has in common, meets the
+ * scale alone: codes are those of the products h_i * norm_i (64-bit numbers, exact), so
+ * that a tie of theirs is a tie whatever the root rounds to.  Without norm t_i = h_i:
+ * rows are only put in 8 bits, and eps is not used (it is checked all the same).  So a
+ * weight of 16 or 32 bits, its channels as rows, becomes the w and w_scales of
+ * mi355x_matmul_q8.  residual_out may be residual or x (same type and stride as
+ * that). */
 #define MI355X_ROW_Q8_MAX 65536
 typedef struct mi355x_norm_q8_args {
     int64_t n_rows;       /* at most 2^31 - 1 */
