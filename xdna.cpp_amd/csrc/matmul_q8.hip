@@ -11,10 +11,10 @@
 // (16 rows, one chunk) do not meet in a bank.
 #include "far_parts.h"
 #include "internal.h"
+#include "matmul_q8_forms.h"
 #include "paged_index.h"
 
 #include <algorithm>
-#include <cmath>
 
 namespace mi355x {
 namespace {
@@ -35,7 +35,7 @@ struct MatmulArgs {
     FastDiv tiles, band, last_rows;  // m_tiles * n_tiles, 8 * n_tiles, m_tiles % 8 (or 8)
 };
 
-constexpr int kStage = 128;  // bytes of k in a stage: two matrix products deep
+constexpr int kStage = kMatmulStage;  // bytes of k in a stage: two matrix products deep
 
 __device__ __forceinline__ i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
@@ -634,10 +634,10 @@ __global__ __launch_bounds__(kLargeThreads) __attribute__((amdgpu_waves_per_eu(2
     }
 }
 
-// ---- the choice ---------------------------------------------------------------
+// ---- launches ------------------------------------------------------------------
 
-constexpr size_t kCounters = size_t(4) * kCounterStep * 1024;
-constexpr size_t kPartBytes = size_t(64) << 20;
+constexpr size_t kCounters = size_t(4) * kCounterStep * kMatmulSplitTiles;
+constexpr size_t kPartBytes = size_t(kMatmulPartBytes);
 
 template <int TM, int R, int WAVES, int ST>
 int launch_few(mi355x_ctx *ctx, const MatmulArgs &a) {
@@ -679,66 +679,6 @@ int launch_large(mi355x_ctx *ctx, MatmulArgs a) {
     return MI355X_OK;
 }
 
-// Tiles, the time that a workgroup takes for a stage of k where it has a CU for itself
-// and where `per_cu` share one (of one row of tiles: weights come from memory, and not
-// from an L2), and what the first and each later round of workgroups takes besides (us).
-struct Form {
-    int bm, bn, per_cu, most_splits;
-    float alone, shared, alone_one_row, shared_one_row, first, later;
-};
-constexpr Form kForms[] = {
-    {64, 64, 2, 8, 0.29f, 0.53f, 0.31f, 0.65f, 0.5f, 0.5f},
-    {64, 128, 1, 8, 0.47f, 0.47f, 0.57f, 0.57f, 0.5f, 0.5f},
-    {128, 128, 1, 8, 0.66f, 0.66f, 0.66f, 0.66f, 0.5f, 2.5f},
-    {256, 128, 1, 8, 0.96f, 0.96f, 0.96f, 0.96f, 0.5f, 7.0f},
-    {kLarge, kLarge, 1, 1, 1.60f, 1.60f, 1.60f, 1.60f, 6.4f, 6.4f},
-};
-
-// The form and the split of k with the least estimated time: the launch, rounds of
-// workgroups, and for a split the parts that a tile's last workgroup reads; operands
-// come from memory at 4.4 TB/s at most.  us measured, of the forms in order with their
-// best split in parentheses: 37 x 17408, k 5120: 28 (2), 26.6 (1).  64 x 28672, k 4096: 30
-// (1), 30 (1).  64 x 2048, k 11008: 12.7 (6), 15 (8).  201 x 2560, k 2048: 8 (1), 9 (1), 12 (3),
-// 17 (2).  200 x 22016, k 2048: 31, 30, 28, 22 (1).  300 x 5120, k 5120: 26 (1), 23 (1), 21 (2),
-// 30 (2), 64.  256 x 8192, k 8192: 39 (1), 33 (1), 31 (2), 36 (4), 92.  512 x 4096, k 14336:
-// 63 (1), 52 (1), 44 (2), 46 (4), 154.  1024 x 4096, k 4096: 37, 33, 25 (1), 31 (2), 51.  512 x
-// 22016, k 2048: 54, 59, 43, 43, 33.  5000 x 5000, k 2048: 105, 106, 85, 82, 65.  Of these the
-// least is chosen in each, and elsewhere one within 10% of the least.
-struct Choice {
-    int form, splits;
-};
-Choice choose(const mi355x_ctx *ctx, const MatmulArgs &a) {
-    const int stages = stages_of(a);
-    const float from_memory = static_cast<float>(a.m + a.n) * static_cast<float>(a.k) / 4.4e6f;
-    Choice best{0, 1};
-    float least = 1e30f;
-    for (int f = 0; f < 5; ++f) {
-        const Form &g = kForms[f];
-        if (g.bm == kLarge && g.bn == kLarge && (a.m < kLarge || a.n < kLarge)) continue;
-        const int64_t tiles = static_cast<int64_t>((a.m + g.bm - 1) / g.bm) * ((a.n + g.bn - 1) / g.bn);
-        const int64_t tile_bytes = int64_t(4) * g.bm * g.bn;
-        for (int s = 1; s <= g.most_splits && s <= stages; ++s) {
-            const int64_t groups = tiles * s;
-            // (parts in more than one round did not gain: 37 x 17408, k 5120 in 5 parts 31 us, whole 27)
-            if (s > 1 && (groups > ctx->num_cus * g.per_cu || tiles > static_cast<int64_t>(kCounters / (4 * kCounterStep)) ||
-                          groups * tile_bytes > static_cast<int64_t>(kPartBytes)))
-                break;
-            const float rounds = std::ceil(static_cast<float>(groups) / static_cast<float>(ctx->num_cus * g.per_cu));
-            const bool alone = groups <= ctx->num_cus, one_row = a.m <= g.bm;
-            float us = (rounds - 1.0f) * g.later +
-                       rounds * (one_row ? alone ? g.alone_one_row : g.shared_one_row : alone ? g.alone : g.shared) *
-                           static_cast<float>((stages + s - 1) / s);
-            if (s > 1) us += 1.5f + static_cast<float>(s) * static_cast<float>(tile_bytes) / 32768.0f;
-            us = 3.2f + g.first + std::max(us, from_memory);
-            if (us < least) {
-                least = us;
-                best = {f, s};
-            }
-        }
-    }
-    return best;
-}
-
 }  // namespace
 
 size_t matmul_q8_workspace_bytes(const mi355x_ctx *) { return kCounters + kPartBytes; }
@@ -760,26 +700,20 @@ int launch_matmul_q8(mi355x_ctx *ctx, const mi355x_matmul_q8_args &u) {
     a.n = static_cast<int>(u.n_out);
     a.k = static_cast<int>(u.k);
     a.out_type = u.out_type;
-    // the tile kernels form offsets of up to 256 rows in 32 bits
-    const bool far = u.x_stride > (1 << 23) || u.w_stride > (1 << 23);
-    // Up to 32 rows have the weight in flight in each wavefront by itself; blocks of 32
-    // channels where that fills the CUs, else of 16 so that more workgroups share the work
-    // (16, then 32 channels; us: one row of 2048, k 11008 7.6, 10.4; of 8192, k 8192 12.9, 12.9;
-    // of 22016, k 2048 11.6, 10.1; 32 rows of 2048, k 2048 3.5, 4.0; of 22016 20, 12).  The tiles
-    // take more: 32 rows of 2048, k 2048 7.0, of 22016 13.9; 17 of 28672, k 4096 27.6, here
-    // 24.5; 37 rows 28.6, here (48 channels, 48 rows) 31.3.
-    const bool many = a.n >= 32 * ctx->num_cus;
-    if (a.m <= 16) return many ? launch_few<1, 2, 4, 3>(ctx, a) : launch_few<1, 1, 4, 4>(ctx, a);
-    if (a.m <= 32) return many ? launch_few<2, 2, 4, 2>(ctx, a) : launch_few<2, 1, 8, 2>(ctx, a);
-    if (far) return launch_few<4, 3, 2, 2>(ctx, a);
-    const Choice c = choose(ctx, a);
+    const MatmulChoice c = choose_matmul(ctx->num_cus, a.m, a.n, a.k, u.x_stride, u.w_stride);
     switch (c.form) {
-    case 0: return launch_tiles<64, 64, 4, 2, 4>(ctx, a, c.splits);
-    case 1: return launch_tiles<64, 128, 2, 4, 4>(ctx, a, c.splits);
-    case 2: return launch_tiles<128, 128, 2, 4, 4>(ctx, a, c.splits);
-    case 3: return launch_tiles<256, 128, 2, 4, 3>(ctx, a, c.splits);
-    default: return launch_large(ctx, a);
+    case MatmulForm::kFew16: return launch_few<1, 1, 4, 4>(ctx, a);
+    case MatmulForm::kFew16Wide: return launch_few<1, 2, 4, 3>(ctx, a);
+    case MatmulForm::kFew32: return launch_few<2, 1, 8, 2>(ctx, a);
+    case MatmulForm::kFew32Wide: return launch_few<2, 2, 4, 2>(ctx, a);
+    case MatmulForm::kFar: return launch_few<4, 3, 2, 2>(ctx, a);
+    case MatmulForm::k64x64: return launch_tiles<64, 64, 4, 2, 4>(ctx, a, c.splits);
+    case MatmulForm::k64x128: return launch_tiles<64, 128, 2, 4, 4>(ctx, a, c.splits);
+    case MatmulForm::k128x128: return launch_tiles<128, 128, 2, 4, 4>(ctx, a, c.splits);
+    case MatmulForm::k256x128: return launch_tiles<256, 128, 2, 4, 3>(ctx, a, c.splits);
+    case MatmulForm::k256x256: return launch_large(ctx, a);
     }
+    return set_error(MI355X_EINVAL, "mi355x_matmul_q8: no form");
 }
 
 }  // namespace mi355x
