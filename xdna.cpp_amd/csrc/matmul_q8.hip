@@ -127,9 +127,12 @@ __device__ __forceinline__ const float *bias_or_scales(const MatmulArgs &a) { re
 
 // A workgroup computes 16 * R channels of up to 16 * TM rows.  Its WAVES wavefronts
 // share out k, each with a ring of ST stages of its own, and add their sums in LDS, so
-// that no wavefront waits for another while weights stream.  Bound by memory: one row of
-// 22016 channels, k 2048, 45 MB, 8.7 us (5.2 TB/s); of 151936 52 us (6.0); 32 rows of 28672,
-// k 4096 26.7 us.
+// that no wavefront waits for another while weights stream.  Bound by memory, with weights
+// taken in turn from 1.1 GB of them: one row of 22016 channels, k 2048, 45 MB, 10.2 us (4.4
+// TB/s); of 151936 52 us (6.0); 32 rows of 28672, k 4096 26.7 us (4.5).  One weight over and
+// over, which the last-level cache holds where it is below 256 MB: 7.6, 48, 19.1.  Not so
+// for few channels: one row of 2048, k 11008 7.4 us (3.0 TB/s; 5.5), as 128 workgroups leave half
+// of the CUs without one.
 template <int TM, int R, int WAVES, int ST>
 struct FewShape {
     static constexpr int kUnit = 2048 * (TM + R);
@@ -331,10 +334,13 @@ __device__ __forceinline__ void write_tile(const MatmulArgs &a, int m, int n, co
 // A workgroup of WM x WN wavefronts computes BM rows by BN channels from a ring of ST
 // stages.  One barrier a stage; operands are read half a stage ahead of their
 // products.  Where there are few tiles k is split, and the last workgroup of a tile
-// adds the others' sums to its own.  What bounds it is what a CU gets from its L2: each
-// stage brings BM + BN rows for BM * BN products, at about 48 GB/s a CU (12.3 TB/s in all)
-// however many stages are under way.  512 x 4096, k 14336, 128 x 128 in 2 parts: 43 us, 1.4
-// Pop/s, 531 MB from L2, of which parts and their join are 5 us.
+// adds the others' sums to its own.  Most of the time goes to operands on their way from
+// L2 to LDS: each stage brings BM + BN rows for BM * BN products, at about 48 GB/s a CU
+// (12.3 TB/s in all) however many stages are under way.  That is what this loop gets and no
+// limit of L2: the same loads without products run at 12 to 18 TB/s.  512 x 4096, k 14336,
+// 128 x 128 in 2 parts: 41 us with one weight over and over, 45 with weights in turn from
+// memory (1.4 Pop/s), 531 MB from L2; parts and their join are 5 us.  Rows 128, 256 and 384 bytes
+// further apart, which spreads a stage's lines over other channels of L2: 41, 44.
 template <int BM, int BN, int WM, int WN, int ST>
 struct TileShape {
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
@@ -468,8 +474,9 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_tile_kernel(MatmulArgs a)
 // two stages in LDS a quarter is free as soon as both groups have read it, so that loads
 // are under way for 7 turns.  The workgroup goes through several tiles; the first
 // stages of the next are loaded while a tile's outputs are written.  8192 x 8192, k 8192:
-// 430 us, 2.56 Pop/s (torch's library product 440; products alone 262), the matrix cores
-// busy 58% of the time, 10.6 TB/s from L2.
+// 426 us, 2.58 Pop/s, with weights in turn 441, 2.49 (torch's library product 440 to 465;
+// products alone, without loads, 262), the matrix cores busy 58% of the time, 10.6 TB/s from
+// L2.
 constexpr int kLarge = 256;
 constexpr int kLargeThreads = 512;
 constexpr int kLargeStage = 2 * kLarge * kStage;

@@ -174,7 +174,8 @@ __global__ __launch_bounds__(64 * kMostWaves) void row_q8_kernel(RowArgs a) {
 // reduction over the workgroup, and codes leave from registers.  Bound by memory: the norm
 // of 8192 rows of 8192 in bf16 with its residual, 470 MB, takes 91 us (5.2 TB/s, as a copy);
 // gates of 4096 x 14336 in bf16, 294 MB, 63 us (4.7 TB/s; besides memory some 20 vector
-// operations and two of a quarter's rate a value).  One row: what a launch takes, 4 and 5 us.
+// operations and two of a quarter's rate a value; rows of zeros, and others that f32 will not
+// do for, are formed in 64 bits: 191).  One row: what a launch takes, 4 and 5 us.
 // A thread has CHUNKS runs of 8 values, so rows of up to 8 * CHUNKS * threads values
 // are read once.
 constexpr int kMostChunks = 4;
