@@ -134,8 +134,9 @@ MI355X_API int mi355x_matmul_q8_workspace(mi355x_ctx *ctx, size_t *bytes);
  * top token: where fewer than n_top others are left, -1 and -inf stand in their
  * place.  A row of -inf alone has -inf for every token, and the entropy 0.  A row
  * with NaN or +inf has NaN for everything, and -1 for every top token.  Tokens that are
- * not allowed are best given -inf: where more than 1024 logits equal the last top token's
- * (a finite lowest value on all but a few), the row is read n_top times.
+ * not allowed are best given -inf: where more than 1024 logits above -inf are as large as
+ * the last top token's less 2^-7 of its size (a finite lowest value on all but a few, or a
+ * common offset of a hundred times their spread), the row is read n_top times.
  *
  * workspace: mi355x_logprobs_workspace bytes, under the same rules as that of
  * mi355x_matmul_q8. */

@@ -12,7 +12,8 @@
 // when four times as many logits have been seen, so that about n log4 of the row's
 // length get there.  A list that overflows (rows that ascend, many equal logits) is
 // made again with the last bound, and failing that the row is searched n times: more than
-// 1024 logits that equal the last top token's, as where all but a few have one finite value.
+// 1024 logits that are no smaller than the last top token's less 2^-7 of its size (what the
+// bound is off by), as where all but a few have one finite value.
 // That is right and slow: 2048 rows of 151936 in bf16 with 5, 20 and 64 top tokens 3.7, 11.9
 // and 35 ms, one row 47, 160 and 606 us.  Masks of -inf are no candidates (119 us, and 14).
 //
